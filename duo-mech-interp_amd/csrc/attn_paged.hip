@@ -1,0 +1,769 @@
+// Gated causal grouped attention of T new tokens per row over a paged KV cache in bf16 or 4 bits.
+//
+//   token t of row b sits at position p = pos[b] + t; q' = rope_p(q rsqrt(mean q^2 + eps) (1 + w)), and per query head
+//   out = sum_j softmax_j(q' . k_j scale) v_j * sigmoid(gate) over the cached keys j <= p (HF:656-698 with a cache; WGSL
+//   attention, engine/kernels_qwen35.js:73-123). The new tokens' keys are in the pages already.
+//
+// A block takes 16 NR query rows (row r = t G + head of the group, G = Hq / Hkv) of one kv head against one run of the
+// row's keys; its four waves take 32 keys each in turn. Both products run with the keys on the matrix core's row side:
+//   S^T [keys x rows]  = K Q^T   A: 16 keys of K as they lie in the page, B: Q from LDS
+//   O^T [dims x rows] += V^T P^T A: V^T formed in registers, B: the exponentials, which S^T's layout hands over as they
+//                                are (lane: row l % 16, keys 4 (l / 16) + r of two 16-key tiles)
+// so that no score or probability crosses lanes except for a row's maximum (two exchanges) and, at the end, its sum.
+// Q is held as bf16 hi + lo parts (two products): the scores carry fp32 q to 2^-17. The exponentials are rounded to bf16
+// (one rounding of 2^-9 per weight, with the value's scale already in it); sums, maxima and accumulators are fp32.
+//
+// 4 bits: a code n enters the products as a small whole number that bf16 holds exactly, 128 + n for keys and 16 + n for
+// values: its bits or-ed into the mantissa of 128 (of 16), 7 or 8 operations for 8 values with no conversion. The
+// offsets leave again exactly: the keys' products start from -136 sum(Q) of the group, the values' by the sum of the
+// rounded weights times -24. Scales apply outside the codes: a key's to its group's partial score (fp32), a value's to the
+// exponential before its rounding.
+//
+// A row's keys are dealt over S blocks in runs of whole 128-key rounds by the row's own length, read on the device: the
+// grid is sized by the table's capacity, the work by what is cached. With S > 1 the blocks leave (max, sum, acc) and a
+// second kernel merges them; blocks whose run is empty leave nothing and are not read.
+#include "paged_kv.h"
+
+namespace q35 {
+
+struct PagedAttnArgs {
+  const void *q, *gate;
+  int64_t qb, qt, qh, gb, gt, gh;  // strides of q and gate, in elements
+  const float *qw, *cos_t, *sin_t;
+  float eps, scale;
+  int rot, q_f32, out_f32;
+  PagedTable pt;
+  const int32_t *pos, *lens;
+  const void *kp, *vp;
+  const __bf16 *ks, *vs;
+  void* out;
+  float *part, *ml;  // S > 1: O [B][Hkv][T G][S][256], (max, sum) [B][Hkv][T G][S][2]
+  int T, Hkv, G, S, RB;
+};
+
+typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
+
+constexpr int kRound = 128;     // keys per round of the four waves
+constexpr int kORow = kPgD + 4; // LDS row of a wave's result
+
+// Keys that token t of row b sees: 0 .. n - 1. 0 for a token that is not there.
+__device__ __forceinline__ int keys_seen(const PagedAttnArgs& p, int64_t pos, int len, int t) {
+  const int64_t at = pos + t;
+  return t < len && at >= 0 && at < p.pt.capacity() ? (int)at + 1 : 0;
+}
+// Keys of row b's run over S blocks, from the keys its last token sees: a multiple of a round.
+__device__ __forceinline__ int run_keys(int n, int S) {
+  const int rounds = (n + kRound - 1) / kRound;
+  return (rounds + S - 1) / S * kRound;
+}
+
+template <bool I4> struct KTile;
+template <> struct KTile<true> {
+  u32x4 c[2];  // codes: dword 2 g + u
+  u32x4 s[2];  // scales of keys 4 a + r: four bf16 each
+};
+template <> struct KTile<false> {
+  bf16x8 c[8];
+};
+template <bool I4> struct VTile;
+template <> struct VTile<true> {
+  u32x2 c[4];  // key 4 a + r: 16 bits per group
+  u32x4 s[2];
+};
+template <> struct VTile<false> {
+  u32x4 c[4][2];  // key 4 a + r: dims 8 c .. and 128 + 8 c ..
+};
+
+__device__ __forceinline__ bf16x8 as_bf16x8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  const u32x4 r = {a, b, c, d};
+  return __builtin_bit_cast(bf16x8, r);
+}
+__device__ __forceinline__ float scale_of(const u32x4 (&s)[2], int r, int g) {
+  const uint32_t w = s[r >> 1][2 * (r & 1) + (g >> 1)];
+  return g & 1 ? bf16hi(w) : bf16lo(w);
+}
+
+template <bool I4, int NR>
+__global__ __launch_bounds__(256, NR == 1 ? 2 : 1) void paged_attn_kernel(PagedAttnArgs p) {
+  constexpr int ROWS = 16 * NR, QF = 8 * 64;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 15, a = lane >> 4;
+  const int s = blockIdx.x, kvh = blockIdx.y % p.Hkv, rb = blockIdx.y / p.Hkv, b = blockIdx.z;
+  const int R = p.T * p.G, r0 = rb * ROWS;
+
+  constexpr int kQBytes = NR * 2 * QF * 16, kOBytes = 4 * ROWS * kORow * 4;
+  __shared__ __attribute__((aligned(16))) char lds[kQBytes > kOBytes ? kQBytes : kOBytes];
+  __shared__ float qsum[NR][kPgNG][16];
+  __shared__ float mls[4][ROWS][2];
+  bf16x8* qf = reinterpret_cast<bf16x8*>(lds);  // [NR][hi, lo][8 steps][64 lanes]
+  float* ob = reinterpret_cast<float*>(lds);    // [4 waves][ROWS][kORow], once Q has been used
+
+  const int64_t pos = p.pos[b];
+  const int len = p.lens ? min(max(p.lens[b], 0), p.T) : p.T;
+  // the row's keys: those of its last token that is there (a later one sees more)
+  int n_row = 0;
+  if (len > 0) n_row = (int)min((int64_t)max(pos + len, (int64_t)0), p.pt.capacity());
+  const int t0 = r0 / p.G, t1 = min(r0 + ROWS, R) - 1 < 0 ? 0 : (min(r0 + ROWS, R) - 1) / p.G;
+  // what this block's rows see at most and at least
+  int n_max = 0;
+  if (t0 < len) n_max = (int)min(max(pos + min(t1, len - 1) + 1, (int64_t)0), p.pt.capacity());
+  const int run = run_keys(n_row, p.S);
+  const int k0 = s * run, k1 = min(k0 + run, n_max);
+  const bool work = k0 < k1;
+  if (!work && p.S > 1) return;  // the merge does not read empty runs' slots
+
+  int seen[NR];
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    const int r = r0 + 16 * i + c;
+    seen[i] = r < R ? keys_seen(p, pos, len, r / p.G) : 0;
+  }
+  // rows that are not there are not stored: let them see what the others do, so that they ask for no mask
+  const int n_min = keys_seen(p, pos, len, t0);
+#pragma unroll
+  for (int i = 0; i < NR; ++i)
+    if (r0 + 16 * i + c >= R) seen[i] = n_max;
+
+  f32x4 acc[NR][16];
+  float corr[I4 ? NR : 1][kPgNG];  // -24 times the sum of a group's weights, over this lane's keys
+  float m_run[NR], l_run[NR];
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[i][e] = zero4();
+    m_run[i] = -INFINITY;
+    l_run[i] = 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < (I4 ? NR : 1); ++i)
+#pragma unroll
+    for (int g = 0; g < kPgNG; ++g) corr[i][g] = 0.f;
+
+  if (work) {
+    // ---- Q: norm, rotation, scale log2(e) and the split into hi + lo, one wave per row, into LDS as B operands
+    const int half = p.rot >> 1, d0 = 4 * lane;
+#pragma unroll 1
+    for (int i = wave; i < ROWS; i += 4) {
+      const int r = r0 + i, t = r / p.G, h = kvh * p.G + r - t * p.G;
+      f32x4 x = zero4();
+      if (r < R && t < len && pos + t >= 0 && pos + t < p.pt.capacity()) {
+        const int64_t o = b * p.qb + t * p.qt + h * p.qh;
+        const bool turns = d0 < p.rot;
+        const int pd = !turns ? d0 : d0 < half ? d0 + half : d0 - half;
+        f32x4 px;
+        if (p.q_f32) {
+          x = load_quad<float>((const float*)p.q + o + d0);
+          px = load_quad<float>((const float*)p.q + o + pd);
+        } else {
+          x = load_quad<__bf16>((const __bf16*)p.q + o + d0);
+          px = load_quad<__bf16>((const __bf16*)p.q + o + pd);
+        }
+        if (p.qw) {
+          const f32x4 wx = load_quad<float>(p.qw + d0), wp = load_quad<float>(p.qw + pd);
+          const float ss = wave_sum(x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]);
+          const float rr = rsqrtf(ss * (1.f / kPgD) + p.eps);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] = x[e] * rr * (1.f + wx[e]);
+            px[e] = px[e] * rr * (1.f + wp[e]);
+          }
+        }
+        if (turns) {
+          const int j = d0 < half ? d0 : d0 - half;
+          const f32x4 co = load_quad<float>(p.cos_t + (pos + t) * half + j);
+          const f32x4 si = load_quad<float>(p.sin_t + (pos + t) * half + j);
+          const float sg = d0 < half ? -1.f : 1.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = x[e] * co[e] + sg * px[e] * si[e];
+        }
+      }
+      const int ti = i >> 4, col = i & 15;
+      __bf16* qe = reinterpret_cast<__bf16*>(qf + (size_t)ti * 2 * QF);
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bf16_hl hl = bf16_split(x[e] * (p.scale * 1.4426950408889634f));
+        // 4 bits: dim 64 g + 16 a + 8 u + j is step 2 g + u of lane group a, and a dword's nibbles leave it in pairs
+        // (j, j + 4). bf16: dim 32 step + 8 a + j in order.
+        const int d = d0 + e, j = d & 7;
+        const int step = I4 ? 2 * (d >> 6) + ((d >> 3) & 1) : d >> 5;
+        const int ga = I4 ? (d >> 4) & 3 : (d >> 3) & 3;
+        const int el = I4 ? 2 * (j & 3) + (j >> 2) : j;
+        const int o = (step * 64 + 16 * ga + col) * 8 + el;
+        qe[o] = hl.hi;
+        qe[QF * 8 + o] = hl.lo;
+        sum += (float)hl.hi + (float)hl.lo;
+      }
+      if constexpr (I4) {
+        sum = add_xor4_quads(add_xor<2>(add_xor<1>(sum)));
+        sum = add_xor<8>(sum);
+        // takes the offset of the codes out again
+        if ((lane & 15) == 0) qsum[ti][lane >> 4][col] = -136.f * sum;
+      }
+    }
+    __syncthreads();
+
+    const int n_last = n_max - 1, pmask = (1 << p.pt.shift) - 1;
+    // 16 keys from key0 on: the page (that of the last key for a tile past it, whose keys are masked) and the row in it.
+    // Bases are scalar, a lane's part of the address 32 bits.
+    struct Tile {
+      size_t slot;
+      bool ok;
+    };
+    auto tile_at = [&](int key0) -> Tile {
+      const int page = p.pt.page_uniform(b, min(key0, n_last) >> p.pt.shift);
+      return {(((size_t)max(page, 0) * p.Hkv + kvh) << p.pt.shift) + (key0 & pmask), page >= 0};
+    };
+    const uint32_t k_off = I4 ? 128 * c + 32 * a : 512 * c + 16 * a, s_off = 32 * a;
+    const uint32_t v_off = I4 ? 128 * 4 * a + 8 * c : 16 * c;
+    auto k_load = [&](const Tile& t, KTile<I4>& k) {
+      const char* src = (const char*)p.kp + t.slot * (I4 ? 128 : 512);
+      if constexpr (I4) {
+        k.c[0] = *reinterpret_cast<const u32x4*>(src + k_off);
+        k.c[1] = *reinterpret_cast<const u32x4*>(src + (k_off + 16));
+        const char* sc = (const char*)p.ks + t.slot * 8;
+        k.s[0] = *reinterpret_cast<const u32x4*>(sc + s_off);
+        k.s[1] = *reinterpret_cast<const u32x4*>(sc + (s_off + 16));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) k.c[i] = *reinterpret_cast<const bf16x8*>(src + (k_off + 64 * i));
+      }
+    };
+    auto v_load = [&](const Tile& t, VTile<I4>& v, int key0) {
+      const char* src = (const char*)p.vp + t.slot * (I4 ? 128 : 512);
+      if constexpr (I4) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v.c[r] = *reinterpret_cast<const u32x2*>(src + (v_off + 128 * r));
+        const char* sc = (const char*)p.vs + t.slot * 8;
+        v.s[0] = *reinterpret_cast<const u32x4*>(sc + s_off);
+        v.s[1] = *reinterpret_cast<const u32x4*>(sc + (s_off + 16));
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          // rows past the last key may hold anything, and 0 times infinity is NaN: read the last key's row instead
+          const uint32_t row = max(min(4 * a + r, n_last - key0), 0);
+          v.c[r][0] = *reinterpret_cast<const u32x4*>(src + (v_off + 512 * row));
+          v.c[r][1] = *reinterpret_cast<const u32x4*>(src + (v_off + 512 * row + 256));
+        }
+      }
+    };
+
+    KTile<I4> kt[2];
+    VTile<I4> vt[2];
+    bool okv[2];
+    int key = k0 + 32 * wave;
+    if (key < k1) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const Tile t = tile_at(key + 16 * u);
+        okv[u] = t.ok;
+        k_load(t, kt[u]);
+        v_load(t, vt[u], key + 16 * u);
+      }
+    }
+    while (key < k1) {
+      const int next = key + kRound;
+      const bool more = next < k1;
+      Tile nt[2];
+      if (more) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) nt[u] = tile_at(next + 16 * u);
+      }
+      // ---- scores, two tiles of 16 keys against each 16 rows
+      f32x4 sc[2][NR];
+      if constexpr (I4) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < NR; ++i) sc[u][i] = zero4();
+#pragma unroll
+        for (int g = 0; g < kPgNG; ++g) {
+          bf16x8 ka[2][2];  // [tile][u]
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              const uint32_t x = kt[u].c[g >> 1][2 * (g & 1) + w];
+              ka[u][w] = as_bf16x8((x & 0x000F000Fu) | 0x43004300u, ((x >> 4) & 0x000F000Fu) | 0x43004300u,
+                                   ((x >> 8) & 0x000F000Fu) | 0x43004300u, ((x >> 12) & 0x000F000Fu) | 0x43004300u);
+            }
+#pragma unroll
+          for (int i = 0; i < NR; ++i) {
+            const bf16x8* qi = qf + (size_t)i * 2 * QF + 2 * g * 64 + lane;
+            const bf16x8 h0 = qi[0], h1 = qi[64], l0 = qi[QF], l1 = qi[QF + 64];
+            const float z = qsum[i][g][c];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              f32x4 d = {z, z, z, z};
+              d = mfma16(ka[u][0], h0, d);
+              d = mfma16(ka[u][1], h1, d);
+              d = mfma16(ka[u][0], l0, d);
+              d = mfma16(ka[u][1], l1, d);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) sc[u][i][r] += scale_of(kt[u].s, r, g) * d[r];
+            }
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < NR; ++i) sc[u][i] = zero4();
+#pragma unroll
+        for (int st = 0; st < 8; ++st)
+#pragma unroll
+          for (int i = 0; i < NR; ++i) {
+            const bf16x8* qi = qf + (size_t)i * 2 * QF + st * 64 + lane;
+            const bf16x8 hi = qi[0], lo = qi[QF];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              sc[u][i] = mfma16(kt[u].c[st], hi, sc[u][i]);
+              sc[u][i] = mfma16(kt[u].c[st], lo, sc[u][i]);
+            }
+            if (st & 1) __builtin_amdgcn_sched_barrier(0);
+          }
+      }
+      if (more) {
+        k_load(nt[0], kt[0]);
+        k_load(nt[1], kt[1]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      // ---- masks, only where some row does not see every key of the two tiles
+      const bool masked = key + 32 > n_min || !okv[0] || !okv[1];
+      if (masked) {
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (key + 16 * u + 4 * a + r >= seen[i] || !okv[u]) sc[u][i][r] = -INFINITY;
+      }
+      // ---- running maximum (with a slack of 2^8 before the accumulators are rescaled) and the exponentials
+      float pr[NR][8];
+      bool up = false;
+      float mx[NR];
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) m = fmaxf(m, sc[u][i][r]);
+        lane_pair q = lane_swap<16>(m);
+        m = max_xor32(fmaxf(q.a, q.b));
+        mx[i] = m;
+        up |= m > m_run[i] + 8.f || (m_run[i] == -INFINITY && m > -INFINITY);
+      }
+      if (__builtin_amdgcn_ballot_w64(up) != 0) {
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+          const float mn = fmaxf(m_run[i], mx[i]);
+          const float f = m_run[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[i] - mn);
+          m_run[i] = mn;
+          l_run[i] *= f;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][e][r] *= f;
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          if constexpr (I4) {
+#pragma unroll
+            for (int g = 0; g < kPgNG; ++g) corr[i][g] *= f;
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        const float ms = m_run[i] == -INFINITY ? 0.f : m_run[i];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float e = __builtin_amdgcn_exp2f(sc[u][i][r] - ms);
+            pr[i][4 * u + r] = e;
+            l_run[i] += e;
+          }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      // ---- P V
+      if constexpr (I4) {
+        const bf16x2 m24 = {(__bf16)-24.f, (__bf16)-24.f};
+#pragma unroll
+        for (int g = 0; g < kPgNG; ++g) {
+          float sv[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) sv[k] = scale_of(vt[k >> 2].s, k & 3, g);
+          bf16x8 pg[NR];
+#pragma unroll
+          for (int i = 0; i < NR; ++i) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              float w = pr[i][k] * sv[k];
+              // a masked key weighs nothing, whatever its scale is
+              if (masked && pr[i][k] == 0.f) w = 0.f;
+              pg[i][k] = (__bf16)w;
+            }
+          }
+          uint32_t x[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            x[k] = __builtin_amdgcn_perm(vt[k >> 1].c[2 * (k & 1) + 1][g >> 1], vt[k >> 1].c[2 * (k & 1)][g >> 1],
+                                         g & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t y[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              y[k] = ((e == 0 ? x[k] << 3 : x[k] >> (4 * e - 3)) & 0x00780078u) | 0x41804180u;
+            const bf16x8 va = as_bf16x8(y[0], y[1], y[2], y[3]);
+#pragma unroll
+            for (int i = 0; i < NR; ++i) acc[i][4 * g + e] = mfma16(va, pg[i], acc[i][4 * g + e]);
+          }
+#pragma unroll
+          for (int i = 0; i < NR; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const bf16x2 w = {pg[i][2 * k], pg[i][2 * k + 1]};
+              corr[i][g] = __builtin_amdgcn_fdot2_f32_bf16(w, m24, corr[i][g], false);
+            }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+        bf16x8 pg[NR];
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) pg[i][k] = (__bf16)pr[i][k];
+        bool odd = false;
+        if (masked) {
+          // a value that is not finite must not meet a weight of 0 in a product
+          uint32_t any = 0;
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+              for (int w = 0; w < 2; ++w)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  const uint32_t x = vt[u].c[r][w][k];
+                  any |= ((x & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
+                }
+          odd = __builtin_amdgcn_ballot_w64(any != 0) != 0;
+        }
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int hl = 0; hl < 2; ++hl) {
+              const int e = 8 * w + 2 * k + hl;  // dim 128 w + 8 c + 2 k + hl
+              uint32_t y[4];
+#pragma unroll
+              for (int n = 0; n < 4; ++n)
+                y[n] = __builtin_amdgcn_perm(vt[n >> 1].c[2 * (n & 1) + 1][w][k], vt[n >> 1].c[2 * (n & 1)][w][k],
+                                             hl ? 0x07060302u : 0x05040100u);
+              if (odd) {
+                // the finite values as ever; the others by whether any weight meets one: +inf, -inf or both (NaN)
+                uint32_t up[4], dn[4];
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                  up[n] = dn[n] = 0;
+#pragma unroll
+                  for (int j = 0; j < 2; ++j) {
+                    const uint32_t v = (y[n] >> (16 * j)) & 0xFFFFu, one = 0x3F80u << (16 * j);
+                    if ((v & 0x7F80u) == 0x7F80u) {
+                      if (v != 0xFF80u) up[n] |= one;
+                      if (v != 0x7F80u) dn[n] |= one;
+                      y[n] &= ~(0xFFFFu << (16 * j));
+                    }
+                  }
+                }
+#pragma unroll
+                for (int i = 0; i < NR; ++i) {
+                  bf16x8 on;
+#pragma unroll
+                  for (int n = 0; n < 8; ++n) on[n] = (__bf16)(pr[i][n] != 0.f ? 1.f : 0.f);
+                  const f32x4 cu = mfma16(as_bf16x8(up[0], up[1], up[2], up[3]), on, zero4());
+                  const f32x4 cd = mfma16(as_bf16x8(dn[0], dn[1], dn[2], dn[3]), on, zero4());
+#pragma unroll
+                  for (int r = 0; r < 4; ++r) {
+                    if (cu[r] > 0.f) acc[i][e][r] += INFINITY;
+                    if (cd[r] > 0.f) acc[i][e][r] -= INFINITY;
+                  }
+                }
+              }
+              const bf16x8 va = as_bf16x8(y[0], y[1], y[2], y[3]);
+#pragma unroll
+              for (int i = 0; i < NR; ++i) acc[i][e] = mfma16(va, pg[i], acc[i][e]);
+            }
+      }
+      if (more) {
+        v_load(nt[0], vt[0], next);
+        v_load(nt[1], vt[1], next + 16);
+        okv[0] = nt[0].ok;
+        okv[1] = nt[1].ok;
+      }
+      key = next;
+    }
+  }
+  __syncthreads();  // Q has been used: its LDS takes the waves' results
+
+  // ---- each wave's rows (those that are there) into LDS, dims in order
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    float l = l_run[i];
+    lane_pair q = lane_swap<16>(l);
+    l = add_xor<32>(q.a + q.b);
+    if constexpr (I4) {
+#pragma unroll
+      for (int g = 0; g < kPgNG; ++g) {
+        q = lane_swap<16>(corr[i][g]);
+        corr[i][g] = add_xor<32>(q.a + q.b);
+      }
+    }
+    if (r0 + 16 * i + c < R) {
+      float* o = ob + ((size_t)wave * ROWS + 16 * i + c) * kORow;
+      if constexpr (I4) {
+#pragma unroll
+        for (int g = 0; g < kPgNG; ++g)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            f32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = acc[i][4 * g + e][r] + corr[i][g];
+            *reinterpret_cast<f32x4*>(o + 64 * g + 16 * a + 4 * r) = v;
+          }
+      } else {
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            f32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = acc[i][4 * w + e][r];
+            *reinterpret_cast<f32x4*>(o + 128 * (w >> 1) + 8 * (4 * a + r) + 4 * (w & 1)) = v;
+          }
+      }
+      if (a == 0) {
+        mls[wave][16 * i + c][0] = m_run[i];
+        mls[wave][16 * i + c][1] = l;
+      }
+    }
+  }
+  __syncthreads();
+  // ---- the four waves joined, one wave per row: the result, or the run's partial
+  const int d0 = 4 * lane;
+#pragma unroll 1
+  for (int i = wave; i < ROWS && r0 + i < R; i += 4) {
+    const int r = r0 + i, t = r / p.G, h = kvh * p.G + r - t * p.G;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) M = fmaxf(M, mls[w][i][0]);
+    float L = 0.f;
+    f32x4 O = zero4();
+    if (M > -INFINITY) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        if (mls[w][i][0] == -INFINITY) continue;  // nothing seen (its sums may still hold a NaN: they count)
+        const float f = __builtin_amdgcn_exp2f(mls[w][i][0] - M);
+        L += mls[w][i][1] * f;
+        const f32x4 v = *reinterpret_cast<const f32x4*>(ob + ((size_t)w * ROWS + i) * kORow + d0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) O[e] += v[e] * f;
+      }
+    }
+    if (p.S > 1) {
+      const size_t slot = (((size_t)b * p.Hkv + kvh) * R + r) * p.S + s;
+      *reinterpret_cast<f32x4*>(p.part + slot * kPgD + d0) = O;
+      if (lane < 2) p.ml[2 * slot + lane] = lane ? L : M;
+    } else {
+      const int64_t oi = (((int64_t)b * p.T + t) * p.Hkv * p.G + h) * kPgD + d0;
+      f32x4 g = {INFINITY, INFINITY, INFINITY, INFINITY};
+      if (p.gate) {
+        const int64_t go = b * p.gb + t * p.gt + h * p.gh + d0;
+        g = p.q_f32 ? load_quad<float>((const float*)p.gate + go) : load_quad<__bf16>((const __bf16*)p.gate + go);
+      }
+      f32x4 v = zero4();
+      if (L != 0.f && keys_seen(p, pos, len, t) > 0) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = O[e] / L * (p.gate ? sigmoidf_(g[e]) : 1.f);
+      }
+      if (p.out_f32) {
+        *reinterpret_cast<f32x4*>((float*)p.out + oi) = v;
+      } else {
+        bf16x4 w = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+        *reinterpret_cast<bf16x4*>((__bf16*)p.out + oi) = w;
+      }
+    }
+  }
+}
+
+// The runs of one query row joined: block = (row, kv head) x batch row, wave w folds runs w, w + 4, ..., eight runs'
+// loads in flight.
+__global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs p) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d0 = 4 * lane;
+  const int kvh = blockIdx.x % p.Hkv, r = blockIdx.x / p.Hkv, b = blockIdx.y;
+  const int R = p.T * p.G, t = r / p.G, h = kvh * p.G + r - t * p.G;
+  const int64_t pos = p.pos[b];
+  const int len = p.lens ? min(max(p.lens[b], 0), p.T) : p.T;
+  const int seen = keys_seen(p, pos, len, t);
+  f32x4 g = zero4();
+  if (p.gate) {
+    const int64_t go = b * p.gb + t * p.gt + h * p.gh + d0;
+    g = p.q_f32 ? load_quad<float>((const float*)p.gate + go) : load_quad<__bf16>((const __bf16*)p.gate + go);
+  }
+  int n_row = 0;
+  if (len > 0) n_row = (int)min(max(pos + len, (int64_t)0), p.pt.capacity());
+  const int run = run_keys(n_row, p.S);
+  // runs that hold keys this row sees (its block wrote them: the block's rows see at least as much)
+  const int n = seen > 0 ? (seen + run - 1) / run : 0;
+  const size_t base = (((size_t)b * p.Hkv + kvh) * R + r) * p.S;
+  float M = -INFINITY, L = 0.f;
+  f32x4 O = zero4();
+  for (int s0 = wave; s0 < n; s0 += 32) {
+    f32x4 v[8];
+    float m[8], l[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const size_t s = base + min(s0 + 4 * u, n - 1);
+      v[u] = *reinterpret_cast<const f32x4*>(p.part + s * kPgD + d0);
+      m[u] = p.ml[2 * s];
+      l[u] = p.ml[2 * s + 1];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (s0 + 4 * u >= n || m[u] == -INFINITY) continue;
+      const float mn = fmaxf(M, m[u]);
+      const float c0 = __builtin_amdgcn_exp2f(M - mn), c1 = __builtin_amdgcn_exp2f(m[u] - mn);
+      L = L * c0 + l[u] * c1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) O[e] = O[e] * c0 + v[u][e] * c1;
+      M = mn;
+    }
+  }
+  __shared__ float gm[4], gl[4];
+  __shared__ f32x4 go[4][64];
+  if (lane == 0) {
+    gm[wave] = M;
+    gl[wave] = L;
+  }
+  go[wave][lane] = O;
+  __syncthreads();
+  if (wave) return;
+  float Mx = fmaxf(fmaxf(gm[0], gm[1]), fmaxf(gm[2], gm[3]));
+  L = 0.f;
+  O = zero4();
+  if (Mx > -INFINITY) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if (gm[w] == -INFINITY) continue;
+      const float f = __builtin_amdgcn_exp2f(gm[w] - Mx);
+      L += gl[w] * f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) O[e] += go[w][lane][e] * f;
+    }
+  }
+  f32x4 v = zero4();
+  if (L != 0.f) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = O[e] / L * (p.gate ? sigmoidf_(g[e]) : 1.f);
+  }
+  const int64_t oi = (((int64_t)b * p.T + t) * p.Hkv * p.G + h) * kPgD + d0;
+  if (p.out_f32) {
+    *reinterpret_cast<f32x4*>((float*)p.out + oi) = v;
+  } else {
+    bf16x4 w = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+    *reinterpret_cast<bf16x4*>((__bf16*)p.out + oi) = w;
+  }
+}
+
+// Query rows per block (in 16s) and runs per row: enough blocks for two per CU (one with 32 rows, whose registers leave
+// room for no more), each run at least one round long.
+struct PagedPlan {
+  int NR, RB, S;
+};
+static PagedPlan paged_plan(int64_t B, int64_t T, int64_t Hkv, int64_t G, int64_t capacity, int64_t splits) {
+  const int64_t R = T * G;
+  const int NR = R <= 16 ? 1 : 2;
+  const int64_t RB = (R + 16 * NR - 1) / (16 * NR), base = B * Hkv * RB;
+  const int64_t most = (capacity + kRound - 1) / kRound;
+  int64_t S = splits;
+  if (S <= 0) S = ((NR == 1 ? 512 : 256) + base - 1) / base;
+  if (S > most) S = most;
+  if (S > 1024) S = 1024;
+  if (S < 1) S = 1;
+  return {NR, (int)RB, (int)S};
+}
+
+}  // namespace q35
+
+extern "C" size_t q35_gated_attn_paged_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                                                       int64_t n_blocks, int64_t page_size, int64_t splits) {
+  using namespace q35;
+  if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || D != kPgD || Hq % Hkv || n_blocks <= 0 || page_size <= 0 ||
+      B > 65535 || T > (1 << 24) || Hq > 4096 || n_blocks > (1 << 26) || page_size > 1024)
+    return 0;
+  const PagedPlan pl = paged_plan(B, T, Hkv, Hq / Hkv, n_blocks * page_size, splits);
+  if (pl.S == 1) return 256;
+  return (size_t)B * T * Hq * pl.S * (kPgD + 2) * sizeof(float);
+}
+
+extern "C" int q35_gated_attn_paged(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* gate,
+                                    int64_t g_sb, int64_t g_st, int64_t g_sh, int dtype, const float* q_norm_w,
+                                    float eps, const float* cos, const float* sin, int64_t rot, const void* k_pages,
+                                    const void* v_pages, const void* k_scale, const void* v_scale, int fmt,
+                                    int64_t n_pages, int64_t page_size, const int32_t* table, int64_t ld_table,
+                                    int64_t n_blocks, const int32_t* pos, const int32_t* lens, void* out,
+                                    int out_dtype, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                                    float scale, int64_t splits, void* workspace, size_t workspace_bytes,
+                                    q35_stream_t stream) {
+  using namespace q35;
+  int shift = 0;
+  int chk = paged_check(k_pages, v_pages, k_scale, v_scale, fmt, table, ld_table, n_blocks, n_pages, page_size, pos, B,
+                        T, Hkv, D, &shift);
+  if (chk == Q35_OK) chk = view_check(q, dtype, q_sb, q_st, q_sh);
+  if (chk == Q35_OK && gate) chk = view_check(gate, dtype, g_sb, g_st, g_sh);
+  if (chk != Q35_OK) return chk;
+  if (!out || Hq <= 0 || Hq % Hkv || rot < 0 || rot > D || (rot & 1) || (rot > 0 && (!cos || !sin))) return Q35_EINVAL;
+  if (out_dtype != Q35_BF16 && out_dtype != Q35_F32) return Q35_EUNSUPPORTED;
+  if (rot % 8 || (uintptr_t)q_norm_w & 15 || (rot > 0 && ((uintptr_t)cos | (uintptr_t)sin) & 15) ||
+      (uintptr_t)out & 15)
+    return Q35_EUNSUPPORTED;
+  const int64_t G = Hq / Hkv;
+  if (Hq > 4096 || T * G > (1 << 24)) return Q35_EUNSUPPORTED;
+  const PagedPlan pl = paged_plan(B, T, Hkv, G, n_blocks * page_size, splits);
+  if (Hkv * pl.RB > 65535 || T * Hq > 0x7fffffff) return Q35_EUNSUPPORTED;
+  const size_t rows = (size_t)B * T * Hq * pl.S;
+  if (pl.S > 1 && (!workspace || workspace_bytes < rows * (kPgD + 2) * sizeof(float) || (uintptr_t)workspace & 15))
+    return Q35_EWORKSPACE;
+  PagedAttnArgs a{};
+  a.q = q;
+  a.gate = gate;
+  a.qb = q_sb, a.qt = q_st, a.qh = q_sh, a.gb = g_sb, a.gt = g_st, a.gh = g_sh;
+  a.qw = q_norm_w, a.cos_t = cos, a.sin_t = sin;
+  a.eps = eps, a.scale = scale;
+  a.rot = (int)rot, a.q_f32 = dtype == Q35_F32, a.out_f32 = out_dtype == Q35_F32;
+  a.pt = {table, ld_table, (int)n_blocks, (int)n_pages, shift};
+  a.pos = pos, a.lens = lens;
+  a.kp = k_pages, a.vp = v_pages, a.ks = (const __bf16*)k_scale, a.vs = (const __bf16*)v_scale;
+  a.out = out;
+  a.part = (float*)workspace;
+  a.ml = a.part ? a.part + rows * kPgD : nullptr;
+  a.T = (int)T, a.Hkv = (int)Hkv, a.G = (int)G, a.S = pl.S, a.RB = pl.RB;
+  const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const dim3 grid(pl.S, (unsigned)(Hkv * pl.RB), (unsigned)B), block(256);
+#define Q35_PAGED(I4, NR) hipLaunchKernelGGL((paged_attn_kernel<I4, NR>), grid, block, 0, st, a)
+  if (fmt == Q35_BF16) {
+    if (pl.NR == 1) Q35_PAGED(false, 1); else Q35_PAGED(false, 2);
+  } else {
+    if (pl.NR == 1) Q35_PAGED(true, 1); else Q35_PAGED(true, 2);
+  }
+#undef Q35_PAGED
+  if (pl.S > 1)
+    hipLaunchKernelGGL(paged_attn_merge_kernel, dim3((unsigned)(T * Hq), (unsigned)B), block, 0, st, a);
+  return hipGetLastError() == hipSuccess ? Q35_OK : Q35_ELAUNCH;
+}

@@ -25,9 +25,11 @@ EXPORTS = [
     "q35_add_rmsnorm", "q35_argmax_rows", "q35_gemv_norm", "q35_gemm_q8", "q35_gemm_q8_split",
     "q35_add_rmsnorm_split", "q35_gated_rmsnorm_split", "q35_gemm_q8_bf16",
     "q35_gdn_decode_sliced", "q35_gemv_norm_conv", "q35_gemv_gated_norm", "q35_gdn_chunk_prefill_conv",
+    "q35_paged_kv_append", "q35_paged_kv_rows", "q35_gated_attn_paged_workspace_bytes", "q35_gated_attn_paged",
+    "q35_verify_drafts_workspace_bytes", "q35_verify_drafts",
 ]
 
-Q35_F32, Q35_BF16, Q35_I8, Q35_I8_G128 = 0, 1, 2, 3
+Q35_F32, Q35_BF16, Q35_I8, Q35_I8_G128, Q35_I4_G64 = 0, 1, 2, 3, 4
 Q35_ESCRATCH = 5
 ABI_VERSION = 14  # the signatures below; q35_abi_version() of the loaded library must match
 
@@ -86,6 +88,14 @@ _SIGS = {
     "q35_gdn_decode_sliced": ([P, I64, P, P, I64, I64, P, F32, P, I64, I64, I64, P], I32),
     "q35_gemv_norm_conv": ([P, P, P, I64, P, F32, P, I32, P, P, I64, I64, I64, I64, P, P, P, I64, I64, P], I32),
     "q35_gemv_gated_norm": ([P, I64, P, I64, P, P, F32, P, I32, P, P, I64, I64, I64, I64, I32, P], I32),
+    "q35_paged_kv_append": ([P, I64, I64, I64, P, I64, I64, I64, I32, P, F32, P, P, I64, P, I64, I64, P, P, P, P, P, P,
+                             I32, I64, I64, I64, I64, I64, I64, P], I32),
+    "q35_paged_kv_rows": ([P, P, P, P, I32, I64, I64, P, I64, I64, P, P, P, P, I64, I64, I64, I64, P], I32),
+    "q35_gated_attn_paged_workspace_bytes": ([I64, I64, I64, I64, I64, I64, I64, I64], SZ),
+    "q35_gated_attn_paged": ([P, I64, I64, I64, P, I64, I64, I64, I32, P, F32, P, P, I64, P, P, P, P, I32, I64, I64, P,
+                              I64, I64, P, P, P, I32, I64, I64, I64, I64, I64, F32, I64, P, SZ, P], I32),
+    "q35_verify_drafts_workspace_bytes": ([I64, I64, I64], SZ),
+    "q35_verify_drafts": ([P, I64, I64, P, I64, P, I64, I64, P, I64, P, P, F32, P, P, I64, I64, I64, P, SZ, P], I32),
 }
 
 

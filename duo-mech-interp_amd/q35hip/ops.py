@@ -9,15 +9,17 @@ tests/engine_ref.py):
   gated_attention_decode      <- the same for one token over a KV cache (WGSL engine/kernels_qwen35.js:73-123)
   residual_steer_add_         <- layers[12] forward hook (tests/engine_ref.py:49-53), WGSL resAdd
                                  (engine/kernels.js:190-203)
+  paged_kv_append_, gated_attention_paged  <- the same attention over a paged cache in bf16 or 4 bits
 Every op runs on the current HIP stream of its inputs' device; inputs are validated here (device, dtype, layout,
 shape) and a bad call raises RuntimeError. CPU tensors raise: there is no CPU path in the product.
 """
 import math
+from typing import NamedTuple, Optional
 
 import torch
 
 from . import _lib
-from ._lib import Q35_BF16, Q35_F32, Q35_I8, Q35_I8_G128, Q35Error, check
+from ._lib import Q35_BF16, Q35_F32, Q35_I4_G64, Q35_I8, Q35_I8_G128, Q35Error, check
 
 _DT = {torch.float32: Q35_F32, torch.bfloat16: Q35_BF16}
 
@@ -29,6 +31,15 @@ def _ptr(t):
 def _stream(t):
     # the handle of t's device's current stream, without a Stream object around it (0.1 us against 2.0 a call)
     return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def _launch(fn, t, *args):
+    """fn(*args) with t's device current (a kernel is launched on the current device)."""
+    d = t.get_device()
+    if d == torch._C._cuda_getDevice():
+        return fn(*args)
+    with torch.cuda.device(d):
+        return fn(*args)
 
 
 def _require(cond, msg):
@@ -110,6 +121,16 @@ _LIB.define("gemv_gated_norm_(Tensor o, Tensor z, Tensor norm_w, Tensor? head_sc
 _LIB.define("attn_prep(Tensor y, Tensor q_norm_w, Tensor k_norm_w, float eps, Tensor cos, Tensor sin, Tensor pos, "
             "Tensor(a!) k_cache, Tensor(b!) v_cache, int Hq, int Hkv, bool want_kv) "
             "-> (Tensor, Tensor, Tensor, Tensor)")
+_LIB.define("paged_kv_append_(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor(c!)? k_scale, "
+            "Tensor(d!)? v_scale, Tensor table, Tensor pos, Tensor? lens, Tensor cos, Tensor sin, Tensor? k_norm_w, "
+            "float eps) -> ()")
+_LIB.define("paged_kv_rows(Tensor k_pages, Tensor v_pages, Tensor? k_scale, Tensor? v_scale, Tensor table, Tensor pos, "
+            "Tensor? lens, int T) -> (Tensor, Tensor)")
+_LIB.define("gated_attn_paged(Tensor q, Tensor? gate, Tensor k_pages, Tensor v_pages, Tensor? k_scale, "
+            "Tensor? v_scale, Tensor table, Tensor pos, Tensor? lens, Tensor cos, Tensor sin, Tensor? q_norm_w, "
+            "float eps, float scale, int splits, bool f32_out) -> Tensor")
+_LIB.define("verify_drafts(Tensor logits, Tensor draft_ids, Tensor? draft_probs, Tensor u, Tensor? lens, "
+            "Tensor? temperatures, float temperature) -> (Tensor, Tensor)")
 
 
 # ---------------------------------------------------------------- gated delta rule
@@ -332,6 +353,131 @@ def _attn_prefill_cached_proj_impl(y, q_norm_w, k_norm_w, eps, k_cache, v_cache,
                                               _stream(y))
     check(st, "q35_gated_attn_prefill_cached_proj")
     return out
+
+
+# ---------------------------------------------------------------- paged KV cache
+def _heads_view(x, what):
+    """A [B, T, H, 256] fp32 or bf16 view (rows of 256 dense, anything else strided): its strides of B, T and H."""
+    _require(x.dim() == 4 and x.shape[3] == 256 and x.stride(3) == 1 and x.dtype in _DT,
+             f"{what}: [B, T, heads, 256] fp32 or bf16 with dense rows")
+    return x.stride()[:3]
+
+
+def _pages_check(k_pages, v_pages, k_scale, v_scale, table, pos, lens, B):
+    """The format, n_pages, Hkv and page size of a paged cache; its table, positions and lengths checked for B rows."""
+    _on_gpu(k_pages, v_pages, k_scale, v_scale, pos, lens)
+    _require(table.device == k_pages.device and table.dtype == torch.int32 and table.dim() == 2 and table.shape[0] == B
+             and table.stride(1) == 1, "table: [B, blocks] int32 with dense rows, on the pages' device")
+    _require(pos.dtype == torch.int32 and tuple(pos.shape) == (B,), "pos: [B] int32")
+    _require(lens is None or (lens.dtype == torch.int32 and tuple(lens.shape) == (B,)), "lens: [B] int32")
+    _require(k_pages.dim() == 4 and v_pages.shape == k_pages.shape and v_pages.dtype == k_pages.dtype,
+             "pages: k and v alike, [pages, Hkv, page size, ...]")
+    n, Hkv, ps, w = k_pages.shape
+    if k_pages.dtype == torch.bfloat16:
+        _require(w == 256, "bf16 pages: [pages, Hkv, page size, 256]")
+        return Q35_BF16, n, Hkv, ps
+    _require(k_pages.dtype == torch.uint8 and w == 128, "4-bit pages: [pages, Hkv, page size, 128] uint8")
+    for s in (k_scale, v_scale):
+        _require(s is not None and s.dtype == torch.bfloat16 and tuple(s.shape) == (n, Hkv, ps, 4),
+                 "4-bit pages: k_scale, v_scale [pages, Hkv, page size, 4] bf16")
+    return Q35_I4_G64, n, Hkv, ps
+
+
+def _paged_kv_append_impl(k, v, k_pages, v_pages, k_scale, v_scale, table, pos, lens, cos, sin, k_norm_w, eps):
+    _on_gpu(cos, sin, k_norm_w)
+    _require(k.device == k_pages.device and v.device == k.device and cos.device == k.device,
+             "k, v, the tables and the pages must be on one device")
+    ks, vs = _heads_view(k, "k"), _heads_view(v, "v")
+    B, T, Hkv, D = k.shape
+    fmt, n, H, ps = _pages_check(k_pages, v_pages, k_scale, v_scale, table, pos, lens, B)
+    _require(v.shape == k.shape and v.dtype == k.dtype and H == Hkv, "k, v: alike, with the pages' heads")
+    _require(k_norm_w is None or (k_norm_w.dtype == torch.float32 and k_norm_w.numel() == D
+                                  and k_norm_w.device == k.device), "k_norm_w: [256] fp32")
+    rot = _tables_check(cos, sin, table.shape[1] * ps)
+    if k.numel() == 0:
+        return
+    st = _launch(_lib.lib().q35_paged_kv_append, k, _ptr(k), *ks, _ptr(v), *vs, _DT[k.dtype], _ptr(k_norm_w), float(eps), _ptr(cos),
+                                        _ptr(sin), rot, _ptr(table), table.stride(0), table.shape[1], _ptr(pos),
+                                        _ptr(lens), _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale), fmt, n,
+                                        ps, B, T, Hkv, D, _stream(k))
+    check(st, "q35_paged_kv_append")
+
+
+def _paged_kv_rows_impl(k_pages, v_pages, k_scale, v_scale, table, pos, lens, T):
+    B = table.shape[0]
+    fmt, n, Hkv, ps = _pages_check(k_pages, v_pages, k_scale, v_scale, table, pos, lens, B)
+    k = torch.empty(B, Hkv, T, 256, dtype=torch.bfloat16, device=k_pages.device)
+    v = torch.empty_like(k)
+    if k.numel() == 0:
+        return k, v
+    st = _launch(_lib.lib().q35_paged_kv_rows, k_pages, _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale), fmt, n, ps,
+                                      _ptr(table), table.stride(0), table.shape[1], _ptr(pos), _ptr(lens), _ptr(k),
+                                      _ptr(v), B, T, Hkv, 256, _stream(k_pages))
+    check(st, "q35_paged_kv_rows")
+    return k, v
+
+
+def _attn_paged_impl(q, gate, k_pages, v_pages, k_scale, v_scale, table, pos, lens, cos, sin, q_norm_w, eps, scale,
+                     splits, f32_out):
+    _on_gpu(cos, sin, q_norm_w)
+    _require(q.device == k_pages.device and cos.device == q.device, "q, the tables and the pages must be on one device")
+    qs = _heads_view(q, "q")
+    B, T, Hq, D = q.shape
+    fmt, n, Hkv, ps = _pages_check(k_pages, v_pages, k_scale, v_scale, table, pos, lens, B)
+    gs = (0, 0, 0)
+    if gate is not None:
+        gs = _heads_view(gate, "gate")
+        _require(gate.shape == q.shape and gate.dtype == q.dtype and gate.device == q.device, "gate: like q")
+    _require(q_norm_w is None or (q_norm_w.dtype == torch.float32 and q_norm_w.numel() == D
+                                  and q_norm_w.device == q.device), "q_norm_w: [256] fp32")
+    rot = _tables_check(cos, sin, table.shape[1] * ps)
+    out = torch.empty(B, T, Hq * D, dtype=torch.float32 if f32_out else torch.bfloat16, device=q.device)
+    if out.numel() == 0:
+        return out
+    L = _lib.lib()
+    nbytes = L.q35_gated_attn_paged_workspace_bytes(B, T, Hq, Hkv, D, table.shape[1], ps, splits)
+    _require(nbytes > 0, "unsupported attention shape")
+    ws = _workspace(nbytes, q.device)
+    st = _launch(L.q35_gated_attn_paged, q, _ptr(q), *qs, _ptr(gate), *gs, _DT[q.dtype], _ptr(q_norm_w), float(eps), _ptr(cos),
+                                _ptr(sin), rot, _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale), fmt, n, ps,
+                                _ptr(table), table.stride(0), table.shape[1], _ptr(pos), _ptr(lens), _ptr(out),
+                                _DT[out.dtype], B, T, Hq, Hkv, D, float(scale), int(splits), _ptr(ws), ws.numel(),
+                                _stream(q))
+    check(st, "q35_gated_attn_paged")
+    return out
+
+
+def _verify_drafts_impl(logits, draft_ids, draft_probs, u, lens, temperatures, temperature):
+    _on_gpu(lens, temperatures)
+    for t in (logits, draft_ids, draft_probs, u, lens, temperatures):
+        _require(t is None or (t.is_cuda and t.device == logits.device),
+                 "inputs must be HIP device tensors on one device (there is no CPU fallback)")
+    _require(logits.dtype == torch.float32 and logits.dim() == 3 and logits.stride(2) == 1,
+             "logits: [B, K + 1, V] fp32 with dense rows")
+    B, K, V = logits.shape[0], logits.shape[1] - 1, logits.shape[2]
+    _require(K >= 0 and tuple(draft_ids.shape) == (B, K) and draft_ids.dtype == torch.int32
+             and (K <= 1 or draft_ids.stride(1) == 1), "draft_ids: [B, K] int32 with dense rows")
+    _require(tuple(u.shape) == (B, K + 1) and u.dtype == torch.float32 and (K == 0 or u.stride(1) == 1),
+             "u: [B, K + 1] fp32 with dense rows")
+    _require(draft_probs is None or (tuple(draft_probs.shape) == (B, K, V) and draft_probs.dtype == torch.float32
+                                     and draft_probs.stride(2) == 1), "draft_probs: [B, K, V] fp32 with dense rows")
+    _require(lens is None or (lens.dtype == torch.int32 and tuple(lens.shape) == (B,)), "lens: [B] int32")
+    _require(temperatures is None or (temperatures.dtype == torch.float32 and tuple(temperatures.shape) == (B,)),
+             "temperature: a number of at least 0 or [B] fp32")
+    L = _lib.lib()
+    n = torch.empty(B, dtype=torch.int32, device=logits.device)
+    tokens = torch.empty(B, K + 1, dtype=torch.int32, device=logits.device)
+    if B == 0:
+        return n, tokens
+    nbytes = L.q35_verify_drafts_workspace_bytes(B, K, V)
+    _require(nbytes > 0, f"unsupported draft shape (B={B}, K={K}, V={V})")
+    ws = _workspace(nbytes, logits.device)
+    ps = draft_probs.stride()[:2] if draft_probs is not None else (0, 0)
+    st = _launch(L.q35_verify_drafts, logits, _ptr(logits), logits.stride(0), logits.stride(1), _ptr(draft_ids), draft_ids.stride(0),
+                             _ptr(draft_probs), *ps, _ptr(u), u.stride(0), _ptr(lens), _ptr(temperatures),
+                             float(temperature), _ptr(n), _ptr(tokens), B, K, V, _ptr(ws), ws.numel(), _stream(logits))
+    check(st, "q35_verify_drafts")
+    return n, tokens
 
 
 def _resid_add_impl(x, vecs, vec_of_row):
@@ -752,7 +898,9 @@ for _name, _impl in [("gdn_recurrent", _gdn_recurrent_impl), ("gdn_decode_step_"
                      ("gemv_norm_", _gemv_norm_impl), ("gdn_decode_sliced_", _gdn_decode_sliced_impl),
                      ("gemv_norm_argmax_", _gemv_norm_argmax_impl),
                      ("gdn_chunk_prefill_conv_", _gdn_chunk_prefill_conv_impl),
-                     ("gemv_norm_conv_", _gemv_norm_conv_impl), ("gemv_gated_norm_", _gemv_gated_norm_impl)]:
+                     ("gemv_norm_conv_", _gemv_norm_conv_impl), ("gemv_gated_norm_", _gemv_gated_norm_impl),
+                     ("paged_kv_append_", _paged_kv_append_impl), ("paged_kv_rows", _paged_kv_rows_impl),
+                     ("gated_attn_paged", _attn_paged_impl), ("verify_drafts", _verify_drafts_impl)]:
     _LIB.impl(_name, _impl, "CUDA")
     _LIB.impl(_name, _no_cpu(_name), "CPU")
 
@@ -829,6 +977,18 @@ def _meta_attn_prep(y, q_norm_w, k_norm_w, eps, cos, sin, pos, k_cache, v_cache,
     return q, gate, k, torch.empty_like(k)
 
 
+def _meta_paged_kv_rows(k_pages, v_pages, k_scale, v_scale, table, pos, lens, T):
+    k = k_pages.new_empty(table.shape[0], k_pages.shape[1], T, 256, dtype=torch.bfloat16)
+    return k, torch.empty_like(k)
+
+
+_LIB.impl("paged_kv_append_", lambda k, v, kp, vp, ks, vs, tb, pos, lens, cos, sin, w, eps: None, "Meta")
+_LIB.impl("paged_kv_rows", _meta_paged_kv_rows, "Meta")
+_LIB.impl("gated_attn_paged", lambda q, g, kp, vp, ks, vs, tb, pos, lens, cos, sin, w, eps, scale, splits, f32_out:
+          q.new_empty(q.shape[0], q.shape[1], q.shape[2] * q.shape[3],
+                      dtype=torch.float32 if f32_out else torch.bfloat16), "Meta")
+_LIB.impl("verify_drafts", lambda x, ids, q, u, lens, ts, t:
+          (ids.new_empty(ids.shape[0]), ids.new_empty(ids.shape[0], ids.shape[1] + 1)), "Meta")
 _LIB.impl("gdn_conv", _meta_gdn_conv, "Meta")
 _LIB.impl("attn_prep", _meta_attn_prep, "Meta")
 
@@ -1119,6 +1279,80 @@ def argmax_rows(x, out=None):
         out = torch.empty(x.shape[0], dtype=torch.int32, device=x.device)
     torch.ops.q35.argmax_rows_(x, out)
     return out
+
+
+class KVPages(NamedTuple):
+    """A paged KV cache: k, v [pages, Hkv, page size, 256] bf16; or 4 bits, k, v [pages, Hkv, page size, 128] uint8 with
+    k_scale, v_scale [pages, Hkv, page size, 4] bf16 (one scale per group of 64 dims, two codes a byte; include/q35hip.h
+    states which value each code stands for). The functions below take any such sequence of four."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: Optional[torch.Tensor] = None
+    v_scale: Optional[torch.Tensor] = None
+
+
+def kv_pages(num_pages, num_kv_heads, page_size, device, fmt="bf16"):
+    """An empty paged cache of num_pages pages of page_size tokens (a power of two of 16 .. 1024), fmt "bf16" (1 KB a
+    token and head) or "int4" (272 bytes)."""
+    if fmt not in ("bf16", "int4"):
+        raise ValueError(f"kv_pages: fmt must be 'bf16' or 'int4', not {fmt!r}")
+    if page_size not in (16, 32, 64, 128, 256, 512, 1024):
+        raise ValueError("kv_pages: page_size must be a power of two of 16 .. 1024")
+    shape = (num_pages, num_kv_heads, page_size)
+    if fmt == "bf16":
+        return KVPages(*(torch.zeros(*shape, 256, dtype=torch.bfloat16, device=device) for _ in range(2)))
+    return KVPages(*(torch.zeros(*shape, 128, dtype=torch.uint8, device=device) for _ in range(2)),
+                   *(torch.zeros(*shape, 4, dtype=torch.bfloat16, device=device) for _ in range(2)))
+
+
+def paged_kv_append_(k, v, pages, table, pos, cos, sin, *, lens=None, k_norm_w=None, eps=1e-6):
+    """The call's keys and values into a paged cache (pages, see KVPages), in place: k, v [B, T, Hkv, 256] fp32 or bf16,
+    e.g. columns of a fused projection output (rows dense, anything else strided); the keys normed with (1 + k_norm_w)
+    when it is given and rotated at their positions (cos, sin: [P, rot / 2] fp32, P at least the table's capacity).
+    table: [B, blocks] int32, row b's page of each block of page-size tokens; token t of row b goes to position
+    pos[b] + t, t < lens[b] ([B] int32; None: all T). Tokens past lens, past the capacity or on a table entry that names
+    no page are not written. Two rows of one call must not share a page they write to."""
+    torch.ops.q35.paged_kv_append_(k, v, *_four(pages), table, pos, lens, cos, sin, k_norm_w, float(eps))
+
+
+def paged_kv_rows(pages, table, pos, T, *, lens=None):
+    """Rows pos[b] .. pos[b] + T - 1 of each sequence read back from its pages: (k, v) [B, Hkv, T, 256] bf16, the layout
+    of the dense caches (with pos 0 and T a multiple of 64 the caches of gated_attention_prefill_cached); zeros past
+    lens, past the table and where a table entry names no page."""
+    return torch.ops.q35.paged_kv_rows(*_four(pages), table, pos, lens, int(T))
+
+
+def gated_attention_paged(q, gate, pages, table, pos, cos, sin, *, lens=None, q_norm_w=None, eps=1e-6, scale=None,
+                          splits=0, out_dtype=torch.bfloat16):
+    """Gated causal grouped attention of T tokens per row over a paged cache that holds them (paged_kv_append_ first):
+    token t < lens[b] of row b sits at position pos[b] + t and attends to keys 0 .. pos[b] + t. q and gate
+    [B, T, Hq, 256] fp32 or bf16 (strided views welcome; gate None: no gate), q normed with (1 + q_norm_w) when it is
+    given and rotated at its position. T = 1 is the decode step, a few tokens the check of drafts, many a chunk of a
+    prompt; Hq / Hkv any ratio. Returns [B, T, Hq * 256] in out_dtype (bf16 or fp32), zeros for tokens past lens or the
+    table's capacity. splits: over how many blocks a row's keys are dealt (0: by the sizes)."""
+    _require(out_dtype in (torch.bfloat16, torch.float32), "out_dtype: bf16 or fp32")
+    return torch.ops.q35.gated_attn_paged(q, gate, *_four(pages), table, pos, lens, cos, sin, q_norm_w, float(eps),
+                                          q.shape[-1] ** -0.5 if scale is None else float(scale), int(splits),
+                                          out_dtype == torch.float32)
+
+
+def _four(pages):
+    _require(len(pages) in (2, 4), "pages: (k, v) or (k, v, k_scale, v_scale)")
+    return pages if len(pages) == 4 else (*pages, None, None)
+
+
+def verify_drafts(logits, draft_ids, u, *, draft_probs=None, lens=None, temperature=1.0):
+    """Drafted tokens kept or refused against the target's probabilities, and one token drawn behind the kept ones (the
+    sampling form of argmax_rows for a step over several tokens; with K = 0 it draws one token per row). logits:
+    [B, K + 1, V] fp32, position i behind i drafts; draft_ids: [B, K] int32; u: [B, K + 1] fp32 random numbers in
+    [0, 1), u[:, i] for draft i and u[:, K] for the drawn token; draft_probs: [B, K, V] fp32, what each draft was drawn
+    from (None: drafts held for certain, e.g. from a lookup); lens: [B] int32 drafts of each row (None: K); temperature:
+    a number or [B] fp32, 0 the argmax. With p = softmax(logits / temperature), draft x_i is kept while
+    u_i q_i(x_i) < p_i(x_i); the drawn token comes from max(p - q, 0) at the first refusal, or from p behind the last
+    draft: the lowest index whose running sum exceeds u[:, K] of the whole. The kept drafts and the drawn token are then
+    distributed as draws from p. Returns (n_accept [B] int32, tokens [B, K + 1] int32: kept drafts, drawn token, -1)."""
+    ts, t = (temperature, 0.0) if torch.is_tensor(temperature) else (None, float(temperature))
+    return torch.ops.q35.verify_drafts(logits, draft_ids, draft_probs, u, lens, ts, t)
 
 
 def add_rmsnorm_(x, y, w, eps=1e-6, split=False):

@@ -53,6 +53,10 @@
  *   q35_add_rmsnorm_split,   counterpart in the reference's interface: a layout between the producers and the
  *   q35_gated_rmsnorm_split  GEMM)
  *   q35_argmax_rows          engine/kernels.js:260-283 `argmax` (greedy token of each row, engine/model.js:494-497)
+ *   q35_paged_kv_append,     q35_attn_prep's keys and values, and the attention over them, on a paged cache in bf16 or
+ *   q35_gated_attn_paged     4 bits (HF:656-701 and engine/kernels_qwen35.js:18-123 over another cache)
+ *   q35_paged_kv_rows,       no counterpart (a sequence's pages as rows of a dense cache; drafted tokens against the
+ *   q35_verify_drafts        target's probabilities, the sampling form of `argmax`)
  */
 #ifndef Q35HIP_H
 #define Q35HIP_H
@@ -78,8 +82,8 @@ enum q35_status {
 
 /* Weight formats of the GEMV / GEMM entry points: Q35_I8 is int8 with one fp32 scale per output row (w_scale [N]);
  * Q35_I8_G128 is the engine's q8 format, int8 with one fp32 scale per group of 128 consecutive inputs of a row
- * (w_scale [N, K / 128] row-major; engine/kernels.js:1-5, :15-47). */
-enum q35_dtype { Q35_F32 = 0, Q35_BF16 = 1, Q35_I8 = 2, Q35_I8_G128 = 3 };
+ * (w_scale [N, K / 128] row-major; engine/kernels.js:1-5, :15-47). Q35_I4_G64 is a format of paged KV caches. */
+enum q35_dtype { Q35_F32 = 0, Q35_BF16 = 1, Q35_I8 = 2, Q35_I8_G128 = 3, Q35_I4_G64 = 4 };
 
 /* One neuron push of the MLP hook (engine/model.js:8, :412-423): neuron -1 applies to every neuron of the layer;
  * mode 0 adds vals[row], mode 1 multiplies by it; row = min(m / T, 3) for input row m of a call with T tokens per
@@ -518,6 +522,86 @@ int q35_swiglu_push(const float* gu, float* a, int64_t M, int64_t I, const q35_p
  */
 int q35_argmax_rows(const float* x, int64_t ldx, int64_t rows, int64_t n, int32_t* idx, float* val,
                     q35_stream_t stream);
+
+/*
+ * Paged KV caches. k_pages, v_pages: [n_pages, Hkv, page_size, ...], page_size a power of two of 16 .. 1024, D = 256,
+ * 16-byte aligned. table: [B, ld_table] int32 on the device, entry j < n_blocks of row b the page of its tokens
+ * j page_size .. (j + 1) page_size - 1; the same page may not be appended to by two rows of one call. pos: [B] int32 on
+ * the device, the position of each row's first token of the call; lens: [B] int32 on the device, how many of the call's T
+ * tokens row b has (clamped to 0 .. T), or NULL for T. Token t of row b sits at pos[b] + t. A token that is not there
+ * (t >= lens[b], or a position outside 0 .. n_blocks page_size - 1) is not written and attends to nothing. A table entry
+ * outside 0 .. n_pages - 1 names no page: nothing is written there, and its keys are not attended to.
+ *   fmt Q35_BF16:   rows of 256 bf16; k_scale, v_scale not read
+ *   fmt Q35_I4_G64: 128 bytes a row of two 4-bit codes each, and k_scale, v_scale [n_pages, Hkv, page_size, 4] bf16, one
+ *     scale per group of 64 dims: s = bf16(max |x| / 7), code = 8 + clamp(rint(x / s), -7, 7), standing for
+ *     (code - 8) s; formed in 64 bits. A group that holds a value that is not finite gets the scale NaN. Nibbles (low
+ *     first) of a key row: dim 64 g + 16 a + 8 u + j at nibble 64 a + 16 g + 8 u + j (g, a < 4, u < 2, j < 8); of a
+ *     value row: dim 64 g + 4 c + e at nibble 16 c + 4 g + e (g, e < 4, c < 16).
+ *
+ * q35_paged_kv_append: the call's keys and values into the pages. k, v: [B, T, Hkv, D] in dtype (Q35_F32 or Q35_BF16)
+ * with strides sb, st, sh in elements (multiples of 4; quads aligned to 16 bytes, 8 for bf16), e.g. columns of a fused
+ * projection output; k_norm_w: [D] fp32 or NULL: the keys' RMS norm with (1 + w), eps; cos, sin: [P, rot / 2] fp32 by
+ * position, P >= n_blocks page_size; rot a multiple of 8. With bf16 pages the rows are bitwise those of q35_attn_prep.
+ * Replaces HF:667-680 and the cache part of engine/kernels_qwen35.js:18-69 `attnPrep`.
+ */
+int q35_paged_kv_append(const void* k, int64_t k_sb, int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb,
+                        int64_t v_st, int64_t v_sh, int dtype, const float* k_norm_w, float eps, const float* cos,
+                        const float* sin, int64_t rot, const int32_t* table, int64_t ld_table, int64_t n_blocks,
+                        const int32_t* pos, const int32_t* lens, void* k_pages, void* v_pages, void* k_scale,
+                        void* v_scale, int fmt, int64_t n_pages, int64_t page_size, int64_t B, int64_t T, int64_t Hkv,
+                        int64_t D, q35_stream_t stream);
+
+/*
+ * Rows of a paged cache read back as values, in the layout of a dense cache: k_out, v_out [B, Hkv, T, D] bf16, row t of
+ * sequence b the token at position pos[b] + t, zeros where there is none. 4-bit rows are (code - 8) s rounded to bf16.
+ */
+int q35_paged_kv_rows(const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale, int fmt,
+                      int64_t n_pages, int64_t page_size, const int32_t* table, int64_t ld_table, int64_t n_blocks,
+                      const int32_t* pos, const int32_t* lens, void* k_out, void* v_out, int64_t B, int64_t T,
+                      int64_t Hkv, int64_t D, q35_stream_t stream);
+
+/*
+ * Gated causal grouped attention of the call's T tokens per row over a paged cache that already holds them (T = 1 the
+ * decode step, a few the check of drafted tokens, many a chunk of a prompt): token t attends to cache keys
+ * 0 .. pos[b] + t. HF:656-698 over a cache; engine/kernels_qwen35.js:73-123.
+ *   q: [B, T, Hq, D] in dtype (Q35_F32 or Q35_BF16) with strides sb, st, sh, not rotated; normed here with
+ *   (1 + q_norm_w) when q_norm_w [D] is not NULL, and rotated at its position; gate: like q, or NULL for none;
+ *   out: [B, T, Hq * D] in out_dtype (16-byte aligned), zeros for tokens that are not there or see no key.
+ *   Hq a multiple of Hkv (any ratio). splits <= 0 lets the library choose over how many blocks a row's keys are dealt
+ *   (at most one per 128 keys of capacity). Needs q35_gated_attn_paged_workspace_bytes(...) bytes of workspace, 16-byte
+ *   aligned; calls that share one workspace must not overlap.
+ */
+size_t q35_gated_attn_paged_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t n_blocks,
+                                            int64_t page_size, int64_t splits);
+int q35_gated_attn_paged(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* gate, int64_t g_sb,
+                         int64_t g_st, int64_t g_sh, int dtype, const float* q_norm_w, float eps, const float* cos,
+                         const float* sin, int64_t rot, const void* k_pages, const void* v_pages, const void* k_scale,
+                         const void* v_scale, int fmt, int64_t n_pages, int64_t page_size, const int32_t* table,
+                         int64_t ld_table, int64_t n_blocks, const int32_t* pos, const int32_t* lens, void* out,
+                         int out_dtype, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, float scale,
+                         int64_t splits, void* workspace, size_t workspace_bytes, q35_stream_t stream);
+
+/*
+ * Drafted tokens kept or refused against the target's probabilities, and one token drawn behind the kept ones.
+ *   logits: [B, K + 1, V] fp32 (strides l_sb, l_sp): position i the target's logits behind i drafts
+ *   draft_ids: [B, K] int32 (row stride d_sb); draft_probs: [B, K, V] fp32 (strides p_sb, p_sp), the probabilities each
+ *   draft was drawn from, or NULL for drafts held for certain (q = 1 at the draft)
+ *   u: [B, K + 1] fp32 in [0, 1) (row stride u_sb): u[b, i] for draft i, u[b, K] for the drawn token
+ *   lens: [B] int32, the drafts of each row (clamped to 0 .. K), or NULL for K
+ *   temperatures: [B] fp32 on the device, or NULL for `temperature` on every row; 0 is the argmax (lowest index)
+ * With p_i = softmax(logits[b, i] / temperature): draft i is kept while u[b, i] q_i(x_i) < p_i(x_i); behind the first
+ * refusal n the token is drawn from max(p_n - q_n, 0) (from p_n should that be nothing), behind the last draft from
+ * p_n: the lowest index whose running sum exceeds u[b, K] times the whole. Formed in 64 bits. n_accept: [B] int32;
+ * tokens: [B, K + 1] int32, the kept drafts, the drawn token, then -1. A NaN logit counts as -inf; a row with no logit
+ * above -inf keeps no draft and gives token 0; a draft outside 0 .. V - 1 is refused. K <= 255, B (K + 1) <= 65535.
+ * Needs q35_verify_drafts_workspace_bytes(B, K, V) bytes of workspace, 16-byte aligned.
+ */
+size_t q35_verify_drafts_workspace_bytes(int64_t B, int64_t K, int64_t V);
+int q35_verify_drafts(const float* logits, int64_t l_sb, int64_t l_sp, const int32_t* draft_ids, int64_t d_sb,
+                      const float* draft_probs, int64_t p_sb, int64_t p_sp, const float* u, int64_t u_sb,
+                      const int32_t* lens, const float* temperatures, float temperature, int32_t* n_accept,
+                      int32_t* tokens, int64_t B, int64_t K, int64_t V, void* workspace, size_t workspace_bytes,
+                      q35_stream_t stream);
 
 #ifdef __cplusplus
 }
