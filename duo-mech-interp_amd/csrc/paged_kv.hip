@@ -4,7 +4,7 @@
 // position p = pos[b] + t (HF:667-680; WGSL attnPrep, engine/kernels_qwen35.js:18-69, on pages). One wave per row of 256
 // values, four dims a lane: the row's sum of squares is one wave sum, a group of 64 dims one row of 16 lanes.
 //   bf16 pages: the arithmetic of attn_prep_kernel (fp32, then one rounding), bit for bit the rows it writes.
-//   4-bit pages: per group s = bf16(max |x| / 7), code = 8 + clamp(rint(x / s), -7, 7). A code is a rounding decision, so
+//   4-bit pages: per group s = bf16(fp32(max |x| / 7)), code = 8 + clamp(rint(x / s), -7, 7). A code is a rounding decision, so
 //   norm, rotation and quotient are formed in 64 bits: which code a value gets then depends on the inputs alone and not on
 //   the order of a sum (in 32 bits about one value in 10^6 falls on the other side). fp64 multiply-adds run at the fp32
 //   rate here. A group that holds a value that is not finite gets the scale NaN: it reads back as NaN.
@@ -54,7 +54,10 @@ __device__ __forceinline__ uint32_t quantize_quad(const double (&x)[4], __bf16* 
   const double bad = (x[0] - x[0]) + (x[1] - x[1]) + (x[2] - x[2]) + (x[3] - x[3]);
   if (!(bad == 0.0)) m = INFINITY;
   m = row16_max64(m);
-  const __bf16 sb = (__bf16)(float)(m / 7.0);
+  // rounded to fp32, then to bf16: one of the two alone would give some groups near a tie another scale
+  float s32 = (float)(m / 7.0);
+  asm volatile("" : "+v"(s32));
+  const __bf16 sb = (__bf16)s32;
   const double s = (double)(float)sb;
   uint32_t q = 0;
   if (s > 0.0 && s < INFINITY) {

@@ -9,10 +9,12 @@
 // in 64 bits (a flat distribution over 150 K tokens puts one draw in a hundred on the wrong side in 32); fp64
 // multiply-adds run at the fp32 rate here. Temperature 0 is the argmax (lowest index, NaN never wins).
 //
-// Three launches, each spread over the vocabulary in chunks of 4096: chunk maxima and sums of every position that a row
-// has; then each block of a row folds those of all its positions, finds n (every block the same, from the same numbers in
-// the same order) and sums its chunk of r; then one block per row finds the chunk and the token. Nothing depends on the
-// order in which blocks run.
+// Spread over the vocabulary in chunks of 4096. verify_stats_kernel leaves each chunk's maximum and sum, without the
+// weight of the position's own draft: what is left of p behind a refused certain draft is then a sum of its own and not a
+// difference. verify_draw_kernel, one block per row, folds the chunks of all positions, finds n, the chunk in which the
+// random number falls and the token in it. A refusal with draft probabilities needs the sums of max(p - q, 0), which
+// depend on n: verify_mass_kernel between the two forms them (every block of a row finds the same n, from the same numbers
+// in the same order). Nothing depends on the order in which blocks run.
 #include "q35_common.h"
 #include "q35hip.h"
 
@@ -22,14 +24,9 @@ constexpr int kVChunk = 4096, kVPer = kVChunk / 256;
 constexpr int kVMaxK = 255;
 
 struct VStat {
-  double sum;  // of exp((x - max) / temperature)
-  float max;
+  double sum;  // of exp((x - max) / temperature), without the draft's
+  float max;   // over all values
   int idx;     // lowest index of the maximum
-};
-struct VRow {
-  double inv_z;
-  float max;
-  int n, idx, refused;
 };
 struct VerifyArgs {
   const float* x;
@@ -45,8 +42,7 @@ struct VerifyArgs {
   float temp;
   int K, V, C;
   VStat* st;
-  double* mass;  // [B][C][2]: sums of r behind a refusal (left) and of p
-  VRow* row;
+  double* mass;  // [B][C], with draft probabilities: sums of max(p_n - q_n, 0) behind a refusal
   int32_t *n_out, *tokens;
 };
 
@@ -58,9 +54,39 @@ __device__ __forceinline__ double v_inv_temp(const VerifyArgs& p, int b) {
   const float t = p.temps ? p.temps[b] : p.temp;
   return t > 0.f ? 1.0 / (double)t : 0.0;
 }
+// The position's draft when it is a token, else -1
+__device__ __forceinline__ int v_draft(const VerifyArgs& p, int b, int i, int len) {
+  if (i >= len) return -1;
+  const int id = p.ids[b * p.idb + i];
+  return id >= 0 && id < p.V ? id : -1;
+}
+
+// e^t for t <= 0 to 2e-14 relative: t = n ln 2 + r with |r| <= ln 2 / 2 (ln 2 in two parts, the first with trailing zeros,
+// so that n times it is exact), the Taylor series of e^r to r^11 (the rest is below r^12 / 12! = 6e-15). 17 operations of
+// 64 bits against about 45 of the library's full-range exp: the chunk sums of 160 positions of 151,936 tokens 40.6 -> 34.9 us.
+__device__ __forceinline__ double exp_neg(double t) {
+  t = fmax(t, -800.0);  // 0 from there on, also for -inf
+  const double n = __builtin_rint(t * 1.4426950408889634);
+  double r = __builtin_fma(-n, 0x1.62e42fefa0000p-1, t);
+  r = __builtin_fma(-n, 0x1.cf79abc9e3b3ap-40, r);
+  double e = 1.0 / 39916800.0;
+  e = __builtin_fma(e, r, 1.0 / 3628800.0);
+  e = __builtin_fma(e, r, 1.0 / 362880.0);
+  e = __builtin_fma(e, r, 1.0 / 40320.0);
+  e = __builtin_fma(e, r, 1.0 / 5040.0);
+  e = __builtin_fma(e, r, 1.0 / 720.0);
+  e = __builtin_fma(e, r, 1.0 / 120.0);
+  e = __builtin_fma(e, r, 1.0 / 24.0);
+  e = __builtin_fma(e, r, 1.0 / 6.0);
+  e = __builtin_fma(e, r, 0.5);
+  e = __builtin_fma(e, r, 1.0);
+  e = __builtin_fma(e, r, 1.0);
+  return __builtin_ldexp(e, (int)n);
+}
 // exp((x - m) / T): 1 at the maximum (also an infinite one), 0 for NaN
 __device__ __forceinline__ double v_weight(float x, float m, double inv_t) {
-  return x == m ? 1.0 : x < m ? exp(((double)x - (double)m) * inv_t) : 0.0;
+  const double e = exp_neg(((double)x - (double)m) * inv_t);
+  return x == m ? 1.0 : x < m ? e : 0.0;
 }
 
 __device__ __forceinline__ double wave_sum_f64(double v) {
@@ -79,7 +105,7 @@ __device__ __forceinline__ int wave_min_i32(int v) {
   return v;
 }
 
-// This thread's values of a chunk: element 4 (tid + 256 u) + e; -inf past the end.
+// This thread's values of a chunk: element 4 (tid + 256 u) + e; `fill` past the end.
 __device__ __forceinline__ void v_load_chunk(const float* row, int base, int V, int tid, float (&x)[kVPer],
                                              float fill) {
   if (base + kVChunk <= V && ((uintptr_t)row & 15) == 0) {
@@ -99,14 +125,17 @@ __device__ __forceinline__ void v_load_chunk(const float* row, int base, int V, 
       }
   }
 }
+__device__ __forceinline__ int v_index(int base, int tid, int k) { return base + 4 * (tid + 256 * (k >> 2)) + (k & 3); }
 
 __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int c = blockIdx.x, b = blockIdx.y / (p.K + 1), i = blockIdx.y % (p.K + 1);
-  if (i > v_len(p, b)) return;
+  const int c = blockIdx.x, b = blockIdx.y / (p.K + 1), i = blockIdx.y % (p.K + 1), base = c * kVChunk;
+  const int len = v_len(p, b);
+  if (i > len) return;
   const double inv_t = v_inv_temp(p, b);
+  const int draft = v_draft(p, b, i, len);
   float x[kVPer];
-  v_load_chunk(p.x + b * p.xb + i * p.xp, c * kVChunk, p.V, tid, x, -INFINITY);
+  v_load_chunk(p.x + b * p.xb + i * p.xp, base, p.V, tid, x, -INFINITY);
   __shared__ float sm[4];
   __shared__ int si[4];
   __shared__ double ss[4];
@@ -121,14 +150,17 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs p) {
   double s = 0.0;
   if (inv_t > 0.0) {
 #pragma unroll
-    for (int k = 0; k < kVPer; ++k) s += v_weight(x[k], m, inv_t);
+    for (int k = 0; k < kVPer; ++k) {
+      const double w = v_weight(x[k], m, inv_t);
+      s += v_index(base, tid, k) == draft ? 0.0 : w;
+    }
+    s = wave_sum_f64(s);
   } else {
 #pragma unroll
     for (int k = kVPer - 1; k >= 0; --k)
-      if (x[k] == m) idx = c * kVChunk + 4 * (tid + 256 * (k >> 2)) + (k & 3);
+      if (x[k] == m) idx = v_index(base, tid, k);
+    idx = wave_min_i32(idx);
   }
-  s = wave_sum_f64(s);
-  idx = wave_min_i32(idx);
   if (lane == 0) {
     ss[wave] = s;
     si[wave] = idx;
@@ -140,20 +172,21 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs p) {
   }
 }
 
-// r at one value: behind a refusal (left) and without one
-__device__ __forceinline__ double v_left(double w, float q, bool has_q, bool is_draft) {
-  return fmax(w - (has_q ? (double)q : is_draft ? 1.0 : 0.0), 0.0);
-}
-
-__global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs p) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int c = blockIdx.x, b = blockIdx.y, len = v_len(p, b);
-  const double inv_t = v_inv_temp(p, b);
-  __shared__ double iz[kVMaxK + 1];
-  __shared__ float mx[kVMaxK + 1];
-  __shared__ int ix[kVMaxK + 1], keep[kVMaxK + 1];
-  for (int i = wave; i <= len; i += 4) {
+// The chunks of each position of row b folded, one wave per position in turn: the maximum, its index, 1 / sum, and
+// whether the draft is kept. Returns n once every thread has them.
+struct VFold {
+  double inv_z[kVMaxK + 1];
+  float max[kVMaxK + 1];
+  int idx[kVMaxK + 1], keep[kVMaxK + 1];
+};
+__device__ __forceinline__ int v_fold(const VerifyArgs& p, int b, int len, double inv_t, int lane, int wave, int waves,
+                                      VFold& f) {
+  for (int i = wave; i <= len; i += waves) {
     const VStat* st = p.st + ((size_t)b * (p.K + 1) + i) * p.C;
+    const int draft = v_draft(p, b, i, len);
+    const float xd = draft >= 0 ? p.x[b * p.xb + i * p.xp + draft] : -INFINITY;
+    const double q = draft >= 0 && p.q ? (double)p.q[b * p.qb + i * p.qp + draft] : 1.0;
+    const float u = i < len ? p.u[b * p.ub + i] : 0.f;
     float M = -INFINITY;
     for (int k = lane; k < p.C; k += 64) M = fmaxf(M, st[k].max);
     M = wave_max_f32(M);
@@ -166,113 +199,128 @@ __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs p) {
     }
     z = wave_sum_f64(z);
     idx = wave_min_i32(idx);
-    int ok = 0;
-    if (i < len) {
-      const int id = p.ids[b * p.idb + i];
-      if (id >= 0 && id < p.V && M > -INFINITY) {
-        const double pr = inv_t > 0.0 ? v_weight(p.x[b * p.xb + i * p.xp + id], M, inv_t) / z : id == idx ? 1.0 : 0.0;
-        const double q = p.q ? (double)p.q[b * p.qb + i * p.qp + id] : 1.0;
-        ok = (double)p.u[b * p.ub + i] * q < pr;
-      }
-    }
+    const double wd = draft >= 0 && M > -INFINITY ? v_weight(xd, M, inv_t) : 0.0;
+    z += wd;
     if (lane == 0) {
-      iz[i] = 1.0 / z;
-      mx[i] = M;
-      ix[i] = idx;
-      keep[i] = ok;
+      const double pr = inv_t > 0.0 ? wd / z : draft == idx ? 1.0 : 0.0;
+      f.inv_z[i] = 1.0 / z;
+      f.max[i] = M;
+      f.idx[i] = idx;
+      f.keep[i] = draft >= 0 && M > -INFINITY && (double)u * q < pr;
     }
   }
   __syncthreads();
   int n = 0;
-  while (n < len && keep[n]) ++n;
-  const bool refused = n < len;
-  const float M = mx[n];
-  const double inv_z = iz[n];
-  if (c == 0 && tid == 0) {
-    const VRow r = {inv_z, M, n, M > -INFINITY ? ix[n] : 0, refused};
-    p.row[b] = r;
-  }
-  if (!(inv_t > 0.0) || !(M > -INFINITY)) return;
-  float x[kVPer], q[kVPer];
-  v_load_chunk(p.x + b * p.xb + n * p.xp, c * kVChunk, p.V, tid, x, -INFINITY);
-  const bool has_q = refused && p.q;
-  if (has_q) v_load_chunk(p.q + b * p.qb + n * p.qp, c * kVChunk, p.V, tid, q, 0.f);
-  const int draft = refused && !p.q ? p.ids[b * p.idb + n] : -1;
-  double sl = 0.0, sp = 0.0;
-#pragma unroll
-  for (int k = 0; k < kVPer; ++k) {
-    const double w = v_weight(x[k], M, inv_t) * inv_z;
-    sp += w;
-    sl += v_left(w, has_q ? q[k] : 0.f, has_q, c * kVChunk + 4 * (tid + 256 * (k >> 2)) + (k & 3) == draft);
-  }
-  sl = wave_sum_f64(sl);
-  sp = wave_sum_f64(sp);
-  __shared__ double s2[4][2];
-  if (lane == 0) {
-    s2[wave][0] = sl;
-    s2[wave][1] = sp;
-  }
-  __syncthreads();
-  if (tid < 2) p.mass[((size_t)b * p.C + c) * 2 + tid] = s2[0][tid] + s2[1][tid] + s2[2][tid] + s2[3][tid];
+  while (n < len && f.keep[n]) ++n;
+  return n;
 }
 
-__global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x;
-  const VRow r = p.row[b];
+__global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs p) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int c = blockIdx.x, b = blockIdx.y, len = v_len(p, b), base = c * kVChunk;
   const double inv_t = v_inv_temp(p, b);
-  __shared__ double pre[256];
-  __shared__ double s_target;
+  if (!(inv_t > 0.0) || len == 0) return;
+  __shared__ VFold f;
+  const int n = v_fold(p, b, len, inv_t, lane, wave, 4, f);
+  const float M = f.max[n];
+  if (n == len || !(M > -INFINITY)) return;  // nothing was refused: the draw takes the chunks' own sums
+  const double inv_z = f.inv_z[n];
+  float x[kVPer], q[kVPer];
+  v_load_chunk(p.x + b * p.xb + n * p.xp, base, p.V, tid, x, -INFINITY);
+  v_load_chunk(p.q + b * p.qb + n * p.qp, base, p.V, tid, q, 0.f);
+  double s = 0.0;
+#pragma unroll
+  for (int k = 0; k < kVPer; ++k) s += fmax(v_weight(x[k], M, inv_t) * inv_z - (double)q[k], 0.0);
+  s = wave_sum_f64(s);
+  __shared__ double ss[4];
+  if (lane == 0) ss[wave] = s;
+  __syncthreads();
+  if (tid == 0) p.mass[(size_t)b * p.C + c] = ss[0] + ss[1] + ss[2] + ss[3];
+}
+
+__global__ __launch_bounds__(1024) void verify_draw_kernel(VerifyArgs p) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x;
+  const int len = v_len(p, b);
+  const double inv_t = v_inv_temp(p, b);
+  __shared__ VFold f;
+  __shared__ double pre[16], s_target;
   __shared__ int s_chunk, s_kind, s_token, s_last;
-  int token = r.idx;
-  if (inv_t > 0.0 && r.max > -INFINITY) {
-    const double* ms = p.mass + (size_t)b * p.C * 2;
-    if (tid == 0) {
-      // sums over the chunks in order; what is left behind a refusal may be nothing (q = p to the last bit): then p
-      double tot = 0.0, all = 0.0;
-      for (int k = 0; k < p.C; ++k) {
-        tot += ms[2 * k];
-        all += ms[2 * k + 1];
+  const float us = p.u[b * p.ub + p.K];
+  const int n = v_fold(p, b, len, inv_t, lane, wave, 16, f);
+  const float M = f.max[n];
+  const bool refused = n < len;
+  const int draft = v_draft(p, b, n, len);
+  int token = M > -INFINITY ? f.idx[n] : 0;
+  if (inv_t > 0.0 && M > -INFINITY) {
+    const double inv_z = f.inv_z[n];
+    const VStat* st = p.st + ((size_t)b * (p.K + 1) + n) * p.C;
+    // Weight of chunk k: kind 0 max(p - q, 0), kind 1 p without the draft, kind 2 p
+    auto weight = [&](int k, int kind) -> double {
+      if (kind == 0) return p.mass[(size_t)b * p.C + k];
+      const VStat s = st[k];
+      double w = s.max > -INFINITY ? s.sum * v_weight(s.max, M, inv_t) : 0.0;
+      if (kind == 2 && draft >= 0 && k == draft / kVChunk) w += v_weight(p.x[b * p.xb + n * p.xp + draft], M, inv_t);
+      return w * inv_z;
+    };
+    if (wave == 0) {
+      int kind = !refused ? 2 : p.q ? 0 : 1;
+      double tot = 0.0;
+      for (int k0 = 0; k0 < p.C; k0 += 64) tot += wave_sum_f64(k0 + lane < p.C ? weight(k0 + lane, kind) : 0.0);
+      if (!(tot > 0.0)) {  // nothing is left behind the refusal (q = p to the last bit): p itself
+        kind = 2;
+        tot = 0.0;
+        for (int k0 = 0; k0 < p.C; k0 += 64) tot += wave_sum_f64(k0 + lane < p.C ? weight(k0 + lane, kind) : 0.0);
       }
-      const int kind = r.refused && tot > 0.0 ? 0 : 1;
-      const double target = (double)p.u[b * p.ub + p.K] * (kind ? all : tot);
-      double run = 0.0;
+      const double target = (double)us * tot;
+      double run = 0.0, before = 0.0;
       int chunk = -1, last = 0;
-      for (int k = 0; k < p.C; ++k) {
-        const double m = ms[2 * k + kind];
-        if (m > 0.0) last = k;
-        if (chunk < 0) {
-          if (run + m > target) chunk = k;
-          else run += m;
+      for (int k0 = 0; k0 < p.C && chunk < 0; k0 += 64) {
+        const double w = k0 + lane < p.C ? weight(k0 + lane, kind) : 0.0;
+        double inc = w;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const double v = __shfl_up(inc, o);
+          if (lane >= o) inc += v;
         }
+        const unsigned long long over = __builtin_amdgcn_ballot_w64(w > 0.0 && run + inc > target);
+        const unsigned long long some = __builtin_amdgcn_ballot_w64(w > 0.0);
+        if (some) last = k0 + 63 - __builtin_clzll(some);
+        if (over) {
+          const int l = __builtin_ctzll(over);
+          chunk = k0 + l;
+          before = run + __shfl(inc - w, l);
+        }
+        run += __shfl(inc, 63);
       }
-      if (chunk < 0) {
-        chunk = last;
-        run = 0.0;
-        s_target = INFINITY;  // none of them: its last value with weight
-      } else {
-        s_target = target - run;
+      if (lane == 0) {
+        s_chunk = chunk >= 0 ? chunk : last;
+        s_target = chunk >= 0 ? target - before : INFINITY;  // in no chunk: the last token with weight
+        s_kind = kind;
+        s_token = 0x7fffffff;
+        s_last = 0;
       }
-      s_chunk = chunk;
-      s_kind = kind;
-      s_token = 0x7fffffff;
-      s_last = 0;
     }
     __syncthreads();
-    const int base = s_chunk * kVChunk + tid * kVPer;
-    const bool left = s_kind == 0, has_q = left && p.q;
-    const int draft = left && !p.q ? p.ids[b * p.idb + r.n] : -1;
-    const float* xr = p.x + b * p.xb + r.n * p.xp;
-    const float* qr = has_q ? p.q + b * p.qb + r.n * p.qp : nullptr;
-    double w[kVPer], sum = 0.0;
+    constexpr int PER = kVChunk / 1024;
+    const int base = s_chunk * kVChunk + tid * PER, kind = s_kind;
+    const float* xr = p.x + b * p.xb + n * p.xp;
+    const float* qr = kind == 0 ? p.q + b * p.qb + n * p.qp : nullptr;
+    double w[PER], sum = 0.0;
     int last = -1;
+    float xv[PER], qv[PER];
 #pragma unroll
-    for (int k = 0; k < kVPer; ++k) {
-      const int i = base + k;
-      double v = i < p.V ? v_weight(xr[i], r.max, inv_t) * r.inv_z : 0.0;
-      if (left && i < p.V) v = v_left(v, has_q ? qr[i] : 0.f, has_q, i == draft);
+    for (int k = 0; k < PER; ++k) {
+      xv[k] = base + k < p.V ? xr[base + k] : -INFINITY;
+      qv[k] = kind == 0 && base + k < p.V ? qr[base + k] : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      double v = v_weight(xv[k], M, inv_t) * inv_z;
+      if (kind == 0) v = fmax(v - (double)qv[k], 0.0);
+      if (kind == 1 && base + k == draft) v = 0.0;
       w[k] = v;
       sum += v;
-      if (v > 0.0) last = i;
+      if (v > 0.0) last = base + k;
     }
     // sums before this thread's values: a scan within the wave, then over the waves
     double inc = sum;
@@ -288,7 +336,7 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
     const double target = s_target;
     int hit = 0x7fffffff;
 #pragma unroll
-    for (int k = 0; k < kVPer; ++k) {
+    for (int k = 0; k < PER; ++k) {
       run += w[k];
       if (run > target && w[k] > 0.0) hit = min(hit, base + k);
     }
@@ -297,9 +345,9 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs p) {
     __syncthreads();
     token = s_token != 0x7fffffff ? s_token : s_last;
   }
-  if (tid == 0) p.n_out[b] = r.n;
-  for (int i = tid; i <= p.K; i += 256)
-    p.tokens[(size_t)b * (p.K + 1) + i] = i < r.n ? p.ids[b * p.idb + i] : i == r.n ? token : -1;
+  if (tid == 0) p.n_out[b] = n;
+  for (int i = tid; i <= p.K; i += 1024)
+    p.tokens[(size_t)b * (p.K + 1) + i] = i < n ? p.ids[b * p.idb + i] : i == n ? token : -1;
 }
 
 static int64_t v_chunks(int64_t V) { return (V + kVChunk - 1) / kVChunk; }
@@ -310,7 +358,7 @@ extern "C" size_t q35_verify_drafts_workspace_bytes(int64_t B, int64_t K, int64_
   using namespace q35;
   if (B <= 0 || K < 0 || V <= 0 || B > 65535 || K > kVMaxK || V > 0x7fff0000 || B * (K + 1) > 65535) return 0;
   const size_t C = v_chunks(V);
-  return (size_t)B * (K + 1) * C * sizeof(VStat) + (size_t)B * C * 2 * sizeof(double) + (size_t)B * sizeof(VRow);
+  return (size_t)B * (K + 1) * C * sizeof(VStat) + (size_t)B * C * sizeof(double);
 }
 
 extern "C" int q35_verify_drafts(const float* logits, int64_t l_sb, int64_t l_sp, const int32_t* draft_ids, int64_t d_sb,
@@ -330,12 +378,11 @@ extern "C" int q35_verify_drafts(const float* logits, int64_t l_sb, int64_t l_sp
   const int C = (int)v_chunks(V);
   VStat* st = (VStat*)workspace;
   double* mass = (double*)(st + (size_t)B * (K + 1) * C);
-  VRow* row = (VRow*)(mass + (size_t)B * C * 2);
   const VerifyArgs a{logits, l_sb, l_sp, draft_ids, d_sb, K > 0 ? draft_probs : nullptr, p_sb, p_sp, u, u_sb, lens,
-                     temperatures, temperature, (int)K, (int)V, C, st, mass, row, n_accept, tokens};
+                     temperatures, temperature, (int)K, (int)V, C, st, mass, n_accept, tokens};
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(verify_stats_kernel, dim3(C, (unsigned)(B * (K + 1))), dim3(256), 0, s, a);
-  hipLaunchKernelGGL(verify_mass_kernel, dim3(C, (unsigned)B), dim3(256), 0, s, a);
-  hipLaunchKernelGGL(verify_draw_kernel, dim3((unsigned)B), dim3(256), 0, s, a);
+  if (a.q) hipLaunchKernelGGL(verify_mass_kernel, dim3(C, (unsigned)B), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(verify_draw_kernel, dim3((unsigned)B), dim3(1024), 0, s, a);
   return hipGetLastError() == hipSuccess ? Q35_OK : Q35_ELAUNCH;
 }

@@ -533,7 +533,7 @@ int q35_argmax_rows(const float* x, int64_t ldx, int64_t rows, int64_t n, int32_
  * outside 0 .. n_pages - 1 names no page: nothing is written there, and its keys are not attended to.
  *   fmt Q35_BF16:   rows of 256 bf16; k_scale, v_scale not read
  *   fmt Q35_I4_G64: 128 bytes a row of two 4-bit codes each, and k_scale, v_scale [n_pages, Hkv, page_size, 4] bf16, one
- *     scale per group of 64 dims: s = bf16(max |x| / 7), code = 8 + clamp(rint(x / s), -7, 7), standing for
+ *     scale per group of 64 dims: s = bf16(fp32(max |x| / 7)), code = 8 + clamp(rint(x / s), -7, 7), standing for
  *     (code - 8) s; formed in 64 bits. A group that holds a value that is not finite gets the scale NaN. Nibbles (low
  *     first) of a key row: dim 64 g + 16 a + 8 u + j at nibble 64 a + 16 g + 8 u + j (g, a < 4, u < 2, j < 8); of a
  *     value row: dim 64 g + 4 c + e at nibble 16 c + 4 g + e (g, e < 4, c < 16).

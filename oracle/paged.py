@@ -1,6 +1,6 @@
 """Paged KV cache, attention over it and the check of drafted tokens, on the CPU in 64 bits (test infrastructure only).
 
-  quantize_rows / row_values   the 4-bit row format: one bf16 scale s = bf16(max |x| / 7) per group of 64 dims, codes
+  quantize_rows / row_values   the 4-bit row format: one bf16 scale s = bf16(fp32(max |x| / 7)) per group of 64 dims, codes
                                8 + clamp(rint(x / s), -7, 7), standing for (code - 8) s
   pack_rows / unpack_rows      the order of the codes in a row's 128 bytes (include/q35hip.h)
   paged_append                 k norm with (1 + w), rotation, and the writes through the block table
@@ -34,7 +34,7 @@ def quantize_rows(x):
     """x [..., 256] -> codes [..., 256] (uint8, dims in order), scales [..., 4] bf16."""
     g = x.double().unflatten(-1, (D // GROUP, GROUP))
     finite = torch.isfinite(g).all(-1)
-    s = (torch.where(finite[..., None], g, 0.0).abs().amax(-1) / 7).to(torch.bfloat16)
+    s = (torch.where(finite[..., None], g, 0.0).abs().amax(-1) / 7).float().to(torch.bfloat16)
     sd = s.double()[..., None]
     n = torch.where((sd > 0) & finite[..., None], g / sd, 0.0).round().clamp(-7, 7)
     s = torch.where(finite, s, torch.tensor(math.nan, dtype=torch.bfloat16))

@@ -167,6 +167,23 @@ def test_append_ties_zeros_and_values_that_are_not_finite(fmt):
         assert torch.equal(rows[0, 0, 0, :64].cpu().float(), torch.round(d["y"][0, 0, -256:-192] / 1.5) * 1.5)
 
 
+def test_append_scales_near_a_tie():
+    """Among 65,536 groups of normed and rotated keys some scales lie so near the middle of two bf16 numbers that fp32 puts
+    them onto it: rounded to fp32 and then to bf16, as stated, and not straight to bf16."""
+    d = make("int4", 1, 4096, 4, 4, 256, [4096], seed=2)
+    want, g = oracle_append(d), to(d, device())
+    _, _, k, _ = columns(d["y"], 4, 4)
+    at = torch.arange(4096)
+    x = paged._norm(k, d["kw"], 1e-6)[0]
+    x = paged.apply_partial_rope(x, d["cos"][at].double(), d["sin"][at].double())
+    m = x.unflatten(-1, (4, 64)).abs().amax(-1) / 7
+    near = m.float()
+    assert int(((near.view(torch.int32) & 0xFFFF) == 0x8000).logical_and(near.double() != m).sum()) >= 1
+    announce("paged append int4, scales near a tie")
+    append(g)
+    same_pages("int4", g["pages"], want)
+
+
 @pytest.mark.parametrize("fmt", ["bf16", "int4"])
 def test_append_leaves_everything_else_alone(fmt):
     """Tokens past lens, at positions below 0 or past the table, and on entries that name no page are not written."""
