@@ -10,14 +10,17 @@
 //   O^T [dims x rows] += V^T P^T A: V^T formed in registers, B: the exponentials, which S^T's layout hands over as they
 //                                are (lane: row l % 16, keys 4 (l / 16) + r of two 16-key tiles)
 // so that no score or probability crosses lanes except for a row's maximum (two exchanges) and, at the end, its sum.
-// Q is held as bf16 hi + lo parts (two products): the scores carry fp32 q to 2^-17. The exponentials are rounded to bf16
-// (one rounding of 2^-9 per weight, with the value's scale already in it); sums, maxima and accumulators are fp32.
+// The exponentials are rounded to bf16 (one rounding of 2^-9 per weight, with the value's scale already in it); sums, maxima
+// and accumulators are fp32. Against bf16 keys Q is held as bf16 hi + lo parts (two products, 2^-17 of q); against 4-bit
+// codes as fp16, each row scaled by a power of two to a largest value of 16 to 32 (2^-12 of q).
 //
-// 4 bits: a code n enters the products as a small whole number that bf16 holds exactly, 128 + n for keys and 16 + n for
-// values: its bits or-ed into the mantissa of 128 (of 16), 7 or 8 operations for 8 values with no conversion. The
-// offsets leave again exactly: the keys' products start from -136 sum(Q) of the group, the values' by the sum of the
-// rounded weights times -24. Scales apply outside the codes: a key's to its group's partial score (fp32), a value's to the
-// exponential before its rounding.
+// 4 bits: a code n enters the products as a small whole number that the operand type holds exactly, its bits or-ed into the
+// mantissa of a power of two: keys 1024 + n and, from the nibble above, 1024 + 16 n in fp16 (Q / 16 against it), 5
+// operations for 8 values; values 16 + n in bf16 (fp16 would not hold weight times scale). The offsets leave again: the
+// keys' products start from minus the offsets' part of the sum, formed from the same rounded Q; the values' by the sum of
+// the rounded weights times -24. Scales apply outside the codes: a key's to its group's partial score (fp32), a value's
+// to the exponential before its rounding. What bounds the 4-bit form is the vector ALU's issue (every round unpacks 64 K
+// values' nibbles), so masks and constants are kept where one v_and_or_b32 takes both.
 //
 // A row's keys are dealt over S blocks in runs of whole 128-key rounds by the row's own length, read on the device: the
 // grid is sized by the table's capacity, the work by what is cached. With S > 1 the blocks leave (max, sum, acc) and a
@@ -42,6 +45,8 @@ struct PagedAttnArgs {
 };
 
 typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
+typedef __attribute__((__vector_size__(8 * sizeof(_Float16)))) _Float16 f16x8;
+typedef __attribute__((__vector_size__(2 * sizeof(float)))) float f32x2;
 
 constexpr int kRound = 128;     // keys per round of the four waves
 constexpr int kORow = kPgD + 4; // LDS row of a wave's result
@@ -83,27 +88,48 @@ __device__ __forceinline__ float scale_of(const u32x4 (&s)[2], int r, int g) {
   return g & 1 ? bf16hi(w) : bf16lo(w);
 }
 
+__device__ __forceinline__ float wave_max(float v) {
+  v = fmaxf(v, lane_dpp<0xB1>(v));
+  v = fmaxf(v, lane_dpp<0x4E>(v));
+  v = fmaxf(v, lane_dpp<0x141>(v));
+  v = fmaxf(v, lane_dpp<0x140>(v));
+  const lane_pair q = lane_swap<16>(v);
+  return max_xor32(fmaxf(q.a, q.b));
+}
+__device__ __forceinline__ f32x4 mfma16h(const u32x4& a, const f16x8& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), b, c, 0, 0, 0);
+}
+__device__ __forceinline__ uint32_t cvt2(float a, float b) {
+  const f32x2 v = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+}
+__device__ __forceinline__ int32_t load_uniform(const int32_t* p) {
+  typedef const __attribute__((address_space(4))) int32_t* cptr;
+  return *(cptr)(uintptr_t)p;
+}
+
 template <bool I4, int NR>
-__global__ __launch_bounds__(256, NR == 1 ? 2 : 1) void paged_attn_kernel(PagedAttnArgs p) {
-  constexpr int ROWS = 16 * NR, QF = 8 * 64;
+__global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(PagedAttnArgs p) {
+  constexpr int ROWS = 16 * NR, QP = I4 ? 1 : 2, QF = 8 * 64;  // parts of Q, 16-byte operands of one
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, a = lane >> 4;
   const int s = blockIdx.x, kvh = blockIdx.y % p.Hkv, rb = blockIdx.y / p.Hkv, b = blockIdx.z;
   const int R = p.T * p.G, r0 = rb * ROWS;
 
-  constexpr int kQBytes = NR * 2 * QF * 16, kOBytes = 4 * ROWS * kORow * 4;
+  constexpr int kQBytes = NR * QP * QF * 16, kOBytes = 4 * 16 * kORow * 4;
   __shared__ __attribute__((aligned(16))) char lds[kQBytes > kOBytes ? kQBytes : kOBytes];
-  __shared__ float qsum[NR][kPgNG][16];
-  __shared__ float mls[4][ROWS][2];
-  bf16x8* qf = reinterpret_cast<bf16x8*>(lds);  // [NR][hi, lo][8 steps][64 lanes]
-  float* ob = reinterpret_cast<float*>(lds);    // [4 waves][ROWS][kORow], once Q has been used
+  __shared__ float qoff[NR][kPgNG][16];  // what the codes' offsets add to a group's product, negated
+  __shared__ float qfac[ROWS];           // the power of two taken out of a row of Q
+  __shared__ float mls[4][16][2];
+  u32x4* qf = reinterpret_cast<u32x4*>(lds);  // [NR][hi, lo][8 steps][64 lanes]
+  float* ob = reinterpret_cast<float*>(lds);  // [4 waves][16][kORow], once Q has been used
 
-  const int64_t pos = p.pos[b];
-  const int len = p.lens ? min(max(p.lens[b], 0), p.T) : p.T;
+  const int64_t pos = load_uniform(p.pos + b);
+  const int len = p.lens ? min(max(load_uniform(p.lens + b), 0), p.T) : p.T;
   // the row's keys: those of its last token that is there (a later one sees more)
   int n_row = 0;
-  if (len > 0) n_row = (int)min((int64_t)max(pos + len, (int64_t)0), p.pt.capacity());
-  const int t0 = r0 / p.G, t1 = min(r0 + ROWS, R) - 1 < 0 ? 0 : (min(r0 + ROWS, R) - 1) / p.G;
+  if (len > 0) n_row = (int)min(max(pos + len, (int64_t)0), p.pt.capacity());
+  const int t0 = r0 / p.G, t1 = (min(r0 + ROWS, R) - 1) / p.G;
   // what this block's rows see at most and at least
   int n_max = 0;
   if (t0 < len) n_max = (int)min(max(pos + min(t1, len - 1) + 1, (int64_t)0), p.pt.capacity());
@@ -112,35 +138,97 @@ __global__ __launch_bounds__(256, NR == 1 ? 2 : 1) void paged_attn_kernel(PagedA
   const bool work = k0 < k1;
   if (!work && p.S > 1) return;  // the merge does not read empty runs' slots
 
-  int seen[NR];
+  const int n_min = keys_seen(p, pos, len, t0), n_last = n_max - 1, pmask = (1 << p.pt.shift) - 1;
+  // 16 keys from key0 on: the page (that of the last key for a tile past it, whose keys are masked) and the row in it.
+  // Bases are scalar, a lane's part of the address 32 bits.
+  struct Tile {
+    size_t slot;
+    bool ok;
+  };
+  auto tile_at = [&](int key0) -> Tile {
+    const int page = p.pt.page_uniform(b, min(key0, n_last) >> p.pt.shift);
+    return {(((size_t)max(page, 0) * p.Hkv + kvh) << p.pt.shift) + (key0 & pmask), page >= 0};
+  };
+  const uint32_t k_off = I4 ? 128 * c + 32 * a : 512 * c + 16 * a, s_off = 32 * a;
+  const uint32_t v_off = I4 ? 128 * 4 * a + 8 * c : 16 * c;
+  // With 32 rows the values are loaded behind the round's scores and the keys' scales behind its values: at two waves per
+  // SIMD there are 256 registers, 136 of them accumulators.
+  constexpr bool kLate = I4 && NR == 2;
+  // (the empty asm keeps a base in scalar registers: folded with a lane's offset it would take two vector ones)
+  auto base_of = [](const void* pages, size_t bytes) {
+    const char* src = (const char*)pages + bytes;
+    asm("" : "+s"(src));
+    return src;
+  };
+  auto ks_load = [&](const Tile& t, KTile<I4>& k) {
+    if constexpr (I4) {
+      const char* sc = base_of(p.ks, t.slot * 8);
+      k.s[0] = *reinterpret_cast<const u32x4*>(sc + s_off);
+      k.s[1] = *reinterpret_cast<const u32x4*>(sc + (s_off + 16));
+    }
+  };
+  auto k_load = [&](const Tile& t, KTile<I4>& k) {
+    const char* src = base_of(p.kp, t.slot * (I4 ? 128 : 512));
+    if constexpr (I4) {
+      k.c[0] = *reinterpret_cast<const u32x4*>(src + k_off);
+      k.c[1] = *reinterpret_cast<const u32x4*>(src + (k_off + 16));
+      if constexpr (!kLate) ks_load(t, k);
+    } else {
 #pragma unroll
-  for (int i = 0; i < NR; ++i) {
-    const int r = r0 + 16 * i + c;
-    seen[i] = r < R ? keys_seen(p, pos, len, r / p.G) : 0;
-  }
-  // rows that are not there are not stored: let them see what the others do, so that they ask for no mask
-  const int n_min = keys_seen(p, pos, len, t0);
+      for (int i = 0; i < 8; ++i) k.c[i] = *reinterpret_cast<const bf16x8*>(src + (k_off + 64 * i));
+    }
+  };
+  auto v_load = [&](const Tile& t, VTile<I4>& v, int key0) {
+    const char* src = base_of(p.vp, t.slot * (I4 ? 128 : 512));
+    if constexpr (I4) {
 #pragma unroll
-  for (int i = 0; i < NR; ++i)
-    if (r0 + 16 * i + c >= R) seen[i] = n_max;
+      for (int r = 0; r < 4; ++r) v.c[r] = *reinterpret_cast<const u32x2*>(src + (v_off + 128 * r));
+      const char* sc = base_of(p.vs, t.slot * 8);
+      v.s[0] = *reinterpret_cast<const u32x4*>(sc + s_off);
+      v.s[1] = *reinterpret_cast<const u32x4*>(sc + (s_off + 16));
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        // rows past the last key may hold anything, and 0 times infinity is NaN: read the last key's row instead
+        const uint32_t row = max(min(4 * a + r, n_last - key0), 0);
+        v.c[r][0] = *reinterpret_cast<const u32x4*>(src + (v_off + 512 * row));
+        v.c[r][1] = *reinterpret_cast<const u32x4*>(src + (v_off + 512 * row + 256));
+      }
+    }
+  };
 
-  f32x4 acc[NR][16];
-  float corr[I4 ? NR : 1][kPgNG];  // -24 times the sum of a group's weights, over this lane's keys
-  float m_run[NR], l_run[NR];
+  // ---- the first round's tiles, in flight while Q is prepared. The next round's tiles are loaded while this one's are
+  // used, and their pages a round earlier still. A wave's last round loads its own tiles once more (from the cache) rather
+  // than nothing: with no branch around the loads every wait counts how many of them may stay in flight.
+  KTile<I4> kt[2];
+  VTile<I4> vt[2];
+  Tile vtile[2] = {{0, true}, {0, true}};
+  bool okv[2] = {true, true};
+  int key = k0 + 32 * wave, next = key;
+  Tile nt[2] = {{0, true}, {0, true}};
+  if (key < k1) {
 #pragma unroll
-  for (int i = 0; i < NR; ++i) {
+    for (int u = 0; u < 2; ++u) nt[u] = tile_at(key + 16 * u);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) acc[i][e] = zero4();
-    m_run[i] = -INFINITY;
-    l_run[i] = 0.f;
+    for (int u = 0; u < 2; ++u) {
+      okv[u] = nt[u].ok;
+      k_load(nt[u], kt[u]);
+      if constexpr (kLate) ks_load(nt[u], kt[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if constexpr (kLate) vtile[u] = nt[u];
+      else v_load(nt[u], vt[u], key + 16 * u);
+    }
+    if (key + kRound < k1) next = key + kRound;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) nt[u] = tile_at(next + 16 * u);
   }
-#pragma unroll
-  for (int i = 0; i < (I4 ? NR : 1); ++i)
-#pragma unroll
-    for (int g = 0; g < kPgNG; ++g) corr[i][g] = 0.f;
+  __builtin_amdgcn_sched_barrier(0);
 
+  // ---- Q: norm, rotation, scale log2(e), the split into hi + lo or the power of two, into LDS as B operands; one wave
+  // per row
   if (work) {
-    // ---- Q: norm, rotation, scale log2(e) and the split into hi + lo, one wave per row, into LDS as B operands
     const int half = p.rot >> 1, d0 = 4 * lane;
 #pragma unroll 1
     for (int i = wave; i < ROWS; i += 4) {
@@ -150,7 +238,7 @@ __global__ __launch_bounds__(256, NR == 1 ? 2 : 1) void paged_attn_kernel(PagedA
         const int64_t o = b * p.qb + t * p.qt + h * p.qh;
         const bool turns = d0 < p.rot;
         const int pd = !turns ? d0 : d0 < half ? d0 + half : d0 - half;
-        f32x4 px;
+        f32x4 px, wx = zero4(), wp = zero4(), co = zero4(), si = zero4();
         if (p.q_f32) {
           x = load_quad<float>((const float*)p.q + o + d0);
           px = load_quad<float>((const float*)p.q + o + pd);
@@ -159,7 +247,15 @@ __global__ __launch_bounds__(256, NR == 1 ? 2 : 1) void paged_attn_kernel(PagedA
           px = load_quad<__bf16>((const __bf16*)p.q + o + pd);
         }
         if (p.qw) {
-          const f32x4 wx = load_quad<float>(p.qw + d0), wp = load_quad<float>(p.qw + pd);
+          wx = load_quad<float>(p.qw + d0);
+          wp = load_quad<float>(p.qw + pd);
+        }
+        if (turns) {
+          const int j = d0 < half ? d0 : d0 - half;
+          co = load_quad<float>(p.cos_t + (pos + t) * half + j);
+          si = load_quad<float>(p.sin_t + (pos + t) * half + j);
+        }
+        if (p.qw) {
           const float ss = wave_sum(x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]);
           const float rr = rsqrtf(ss * (1.f / kPgD) + p.eps);
 #pragma unroll
@@ -169,350 +265,346 @@ __global__ __launch_bounds__(256, NR == 1 ? 2 : 1) void paged_attn_kernel(PagedA
           }
         }
         if (turns) {
-          const int j = d0 < half ? d0 : d0 - half;
-          const f32x4 co = load_quad<float>(p.cos_t + (pos + t) * half + j);
-          const f32x4 si = load_quad<float>(p.sin_t + (pos + t) * half + j);
           const float sg = d0 < half ? -1.f : 1.f;
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[e] = x[e] * co[e] + sg * px[e] * si[e];
         }
       }
       const int ti = i >> 4, col = i & 15;
-      __bf16* qe = reinterpret_cast<__bf16*>(qf + (size_t)ti * 2 * QF);
-      float sum = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bf16_hl hl = bf16_split(x[e] * (p.scale * 1.4426950408889634f));
-        // 4 bits: dim 64 g + 16 a + 8 u + j is step 2 g + u of lane group a, and a dword's nibbles leave it in pairs
-        // (j, j + 4). bf16: dim 32 step + 8 a + j in order.
-        const int d = d0 + e, j = d & 7;
-        const int step = I4 ? 2 * (d >> 6) + ((d >> 3) & 1) : d >> 5;
-        const int ga = I4 ? (d >> 4) & 3 : (d >> 3) & 3;
-        const int el = I4 ? 2 * (j & 3) + (j >> 2) : j;
-        const int o = (step * 64 + 16 * ga + col) * 8 + el;
-        qe[o] = hl.hi;
-        qe[QF * 8 + o] = hl.lo;
-        sum += (float)hl.hi + (float)hl.lo;
-      }
+      for (int e = 0; e < 4; ++e) x[e] *= p.scale * 1.4426950408889634f;
       if constexpr (I4) {
-        sum = add_xor4_quads(add_xor<2>(add_xor<1>(sum)));
-        sum = add_xor<8>(sum);
-        // takes the offset of the codes out again
-        if ((lane & 15) == 0) qsum[ti][lane >> 4][col] = -136.f * sum;
+        // dim 64 g + 16 a + 8 u + j is step 2 g + u of lane group a; a dword's nibbles leave it in pairs (j, j + 4), those
+        // of odd j times 16
+        const int ex = __builtin_amdgcn_frexp_expf(
+            wave_max(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])))));
+        _Float16* qe = reinterpret_cast<_Float16*>(qf + (size_t)ti * QF);
+        const int base = ((2 * (lane >> 4) + ((lane >> 1) & 1)) * 64 + 16 * ((lane >> 2) & 3) + col) * 8 + (lane & 1);
+        float off = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const _Float16 hq = (_Float16)ldexpf(x[e], 5 - ex - 4 * (e & 1));
+          qe[base + 2 * e] = hq;
+          off -= (e & 1 ? 1152.f : 1032.f) * (float)hq;
+        }
+        off = add_xor4_quads(add_xor<2>(add_xor<1>(off)));
+        off = add_xor<8>(off);
+        if ((lane & 15) == 0) qoff[ti][lane >> 4][col] = off;
+        if (lane == 0) qfac[i] = ldexpf(1.f, ex - 5);
+      } else {
+        // dim 32 step + 8 a + j in order
+        __bf16* qe = reinterpret_cast<__bf16*>(qf + (size_t)ti * 2 * QF);
+        const int o = ((lane >> 3) * 64 + 16 * ((lane >> 1) & 3) + col) * 8 + 4 * (lane & 1);
+        bf16x4 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bf16_hl hl = bf16_split(x[e]);
+          hi[e] = hl.hi;
+          lo[e] = hl.lo;
+        }
+        *reinterpret_cast<bf16x4*>(qe + o) = hi;
+        *reinterpret_cast<bf16x4*>(qe + QF * 8 + o) = lo;
+        if (lane == 0) qfac[i] = 1.f;
       }
     }
-    __syncthreads();
+  }
 
-    const int n_last = n_max - 1, pmask = (1 << p.pt.shift) - 1;
-    // 16 keys from key0 on: the page (that of the last key for a tile past it, whose keys are masked) and the row in it.
-    // Bases are scalar, a lane's part of the address 32 bits.
-    struct Tile {
-      size_t slot;
-      bool ok;
-    };
-    auto tile_at = [&](int key0) -> Tile {
-      const int page = p.pt.page_uniform(b, min(key0, n_last) >> p.pt.shift);
-      return {(((size_t)max(page, 0) * p.Hkv + kvh) << p.pt.shift) + (key0 & pmask), page >= 0};
-    };
-    const uint32_t k_off = I4 ? 128 * c + 32 * a : 512 * c + 16 * a, s_off = 32 * a;
-    const uint32_t v_off = I4 ? 128 * 4 * a + 8 * c : 16 * c;
-    auto k_load = [&](const Tile& t, KTile<I4>& k) {
-      const char* src = (const char*)p.kp + t.slot * (I4 ? 128 : 512);
-      if constexpr (I4) {
-        k.c[0] = *reinterpret_cast<const u32x4*>(src + k_off);
-        k.c[1] = *reinterpret_cast<const u32x4*>(src + (k_off + 16));
-        const char* sc = (const char*)p.ks + t.slot * 8;
-        k.s[0] = *reinterpret_cast<const u32x4*>(sc + s_off);
-        k.s[1] = *reinterpret_cast<const u32x4*>(sc + (s_off + 16));
-      } else {
+  int seen[NR];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) k.c[i] = *reinterpret_cast<const bf16x8*>(src + (k_off + 64 * i));
-      }
-    };
-    auto v_load = [&](const Tile& t, VTile<I4>& v, int key0) {
-      const char* src = (const char*)p.vp + t.slot * (I4 ? 128 : 512);
-      if constexpr (I4) {
+  for (int i = 0; i < NR; ++i) {
+    // rows that are not there are not stored: let them see what the others do, so that they ask for no mask
+    const int r = r0 + 16 * i + c;
+    seen[i] = r < R ? keys_seen(p, pos, len, r / p.G) : n_max;
+  }
+  f32x4 acc[NR][16];
+  float corr[NR][kPgNG];  // 4 bits: -24 times the sum of a group's weights, over this lane's keys
+  float m_run[NR], l_run[NR], fac[NR];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v.c[r] = *reinterpret_cast<const u32x2*>(src + (v_off + 128 * r));
-        const char* sc = (const char*)p.vs + t.slot * 8;
-        v.s[0] = *reinterpret_cast<const u32x4*>(sc + s_off);
-        v.s[1] = *reinterpret_cast<const u32x4*>(sc + (s_off + 16));
-      } else {
+  for (int i = 0; i < NR; ++i) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          // rows past the last key may hold anything, and 0 times infinity is NaN: read the last key's row instead
-          const uint32_t row = max(min(4 * a + r, n_last - key0), 0);
-          v.c[r][0] = *reinterpret_cast<const u32x4*>(src + (v_off + 512 * row));
-          v.c[r][1] = *reinterpret_cast<const u32x4*>(src + (v_off + 512 * row + 256));
-        }
-      }
-    };
+    for (int e = 0; e < 16; ++e) acc[i][e] = zero4();
+#pragma unroll
+    for (int g = 0; g < kPgNG; ++g) corr[i][g] = 0.f;
+    m_run[i] = -INFINITY;
+    l_run[i] = 0.f;
+  }
+  // constants of the unpacking: the masks in scalar, the or-ed values in vector registers (one v_and_or_b32 takes both)
+  uint32_t mk0 = 0x000F000Fu, mk1 = 0x00F000F0u, mv = 0x00780078u, ck = 0x64006400u, cv = 0x41804180u;
+  asm("" : "+s"(mk0), "+s"(mk1), "+s"(mv), "+v"(ck), "+v"(cv));
+  lds_barrier();
+#pragma unroll
+  for (int i = 0; i < NR; ++i) fac[i] = qfac[16 * i + c];
 
-    KTile<I4> kt[2];
-    VTile<I4> vt[2];
-    bool okv[2];
-    int key = k0 + 32 * wave;
-    if (key < k1) {
+  while (key < k1) {
+    // ---- scores, two tiles of 16 keys against each 16 rows
+    f32x4 sc[2][NR];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const Tile t = tile_at(key + 16 * u);
-        okv[u] = t.ok;
-        k_load(t, kt[u]);
-        v_load(t, vt[u], key + 16 * u);
-      }
-    }
-    while (key < k1) {
-      const int next = key + kRound;
-      const bool more = next < k1;
-      Tile nt[2];
-      if (more) {
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) nt[u] = tile_at(next + 16 * u);
-      }
-      // ---- scores, two tiles of 16 keys against each 16 rows
-      f32x4 sc[2][NR];
-      if constexpr (I4) {
+      for (int i = 0; i < NR; ++i) sc[u][i] = zero4();
+    if constexpr (I4) {
+#pragma unroll
+      for (int g = 0; g < kPgNG; ++g) {
+        u32x4 ka[2][2];  // [tile][u]
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int i = 0; i < NR; ++i) sc[u][i] = zero4();
-#pragma unroll
-        for (int g = 0; g < kPgNG; ++g) {
-          bf16x8 ka[2][2];  // [tile][u]
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              const uint32_t x = kt[u].c[g >> 1][2 * (g & 1) + w];
-              ka[u][w] = as_bf16x8((x & 0x000F000Fu) | 0x43004300u, ((x >> 4) & 0x000F000Fu) | 0x43004300u,
-                                   ((x >> 8) & 0x000F000Fu) | 0x43004300u, ((x >> 12) & 0x000F000Fu) | 0x43004300u);
-            }
-#pragma unroll
-          for (int i = 0; i < NR; ++i) {
-            const bf16x8* qi = qf + (size_t)i * 2 * QF + 2 * g * 64 + lane;
-            const bf16x8 h0 = qi[0], h1 = qi[64], l0 = qi[QF], l1 = qi[QF + 64];
-            const float z = qsum[i][g][c];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              f32x4 d = {z, z, z, z};
-              d = mfma16(ka[u][0], h0, d);
-              d = mfma16(ka[u][1], h1, d);
-              d = mfma16(ka[u][0], l0, d);
-              d = mfma16(ka[u][1], l1, d);
-#pragma unroll
-              for (int r = 0; r < 4; ++r) sc[u][i][r] += scale_of(kt[u].s, r, g) * d[r];
-            }
+          for (int w = 0; w < 2; ++w) {
+            const uint32_t x = kt[u].c[g >> 1][2 * (g & 1) + w], y = x >> 8;
+            ka[u][w] = u32x4{(x & mk0) | ck, (x & mk1) | ck, (y & mk0) | ck, (y & mk1) | ck};
           }
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      } else {
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int i = 0; i < NR; ++i) sc[u][i] = zero4();
-#pragma unroll
-        for (int st = 0; st < 8; ++st)
-#pragma unroll
-          for (int i = 0; i < NR; ++i) {
-            const bf16x8* qi = qf + (size_t)i * 2 * QF + st * 64 + lane;
-            const bf16x8 hi = qi[0], lo = qi[QF];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              sc[u][i] = mfma16(kt[u].c[st], hi, sc[u][i]);
-              sc[u][i] = mfma16(kt[u].c[st], lo, sc[u][i]);
-            }
-            if (st & 1) __builtin_amdgcn_sched_barrier(0);
-          }
-      }
-      if (more) {
-        k_load(nt[0], kt[0]);
-        k_load(nt[1], kt[1]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      // ---- masks, only where some row does not see every key of the two tiles
-      const bool masked = key + 32 > n_min || !okv[0] || !okv[1];
-      if (masked) {
-#pragma unroll
-        for (int i = 0; i < NR; ++i)
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (key + 16 * u + 4 * a + r >= seen[i] || !okv[u]) sc[u][i][r] = -INFINITY;
-      }
-      // ---- running maximum (with a slack of 2^8 before the accumulators are rescaled) and the exponentials
-      float pr[NR][8];
-      bool up = false;
-      float mx[NR];
-#pragma unroll
-      for (int i = 0; i < NR; ++i) {
-        float m = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) m = fmaxf(m, sc[u][i][r]);
-        lane_pair q = lane_swap<16>(m);
-        m = max_xor32(fmaxf(q.a, q.b));
-        mx[i] = m;
-        up |= m > m_run[i] + 8.f || (m_run[i] == -INFINITY && m > -INFINITY);
-      }
-      if (__builtin_amdgcn_ballot_w64(up) != 0) {
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
-          const float mn = fmaxf(m_run[i], mx[i]);
-          const float f = m_run[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[i] - mn);
-          m_run[i] = mn;
-          l_run[i] *= f;
+          const u32x4* qi = qf + (size_t)i * QF + 2 * g * 64 + lane;
+          const f16x8 h0 = __builtin_bit_cast(f16x8, qi[0]), h1 = __builtin_bit_cast(f16x8, qi[64]);
+          const float z = qoff[i][g][c];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
+          for (int u = 0; u < 2; ++u) {
+            f32x4 d = {z, z, z, z};
+            d = mfma16h(ka[u][0], h0, d);
+            d = mfma16h(ka[u][1], h1, d);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[i][e][r] *= f;
-            __builtin_amdgcn_sched_barrier(0);
-          }
-          if constexpr (I4) {
-#pragma unroll
-            for (int g = 0; g < kPgNG; ++g) corr[i][g] *= f;
+            for (int r = 0; r < 4; ++r) sc[u][i][r] += scale_of(kt[u].s, r, g) * d[r];
           }
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
+    } else {
 #pragma unroll
-      for (int i = 0; i < NR; ++i) {
-        const float ms = m_run[i] == -INFINITY ? 0.f : m_run[i];
+      for (int st = 0; st < 8; ++st)
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+          const u32x4* qi = qf + (size_t)i * 2 * QF + st * 64 + lane;
+          const bf16x8 hi = __builtin_bit_cast(bf16x8, qi[0]), lo = __builtin_bit_cast(bf16x8, qi[QF]);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            sc[u][i] = mfma16(kt[u].c[st], hi, sc[u][i]);
+            sc[u][i] = mfma16(kt[u].c[st], lo, sc[u][i]);
+          }
+          if (st & 1) __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    if constexpr (kLate) {
+      v_load(vtile[0], vt[0], key);
+      v_load(vtile[1], vt[1], key + 16);
+    }
+    k_load(nt[0], kt[0]);
+    k_load(nt[1], kt[1]);
+    const int after = next + kRound < k1 ? next + kRound : next;
+    const Tile nn[2] = {tile_at(after), tile_at(after + 16)};
+    __builtin_amdgcn_sched_barrier(0);
+    // ---- masks, only where some row does not see every key of the two tiles
+    const bool masked = key + 32 > n_min || !okv[0] || !okv[1];
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < NR; ++i)
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float e = __builtin_amdgcn_exp2f(sc[u][i][r] - ms);
-            pr[i][4 * u + r] = e;
-            l_run[i] += e;
-          }
+          for (int r = 0; r < 4; ++r)
+            if (key + 16 * u + 4 * a + r >= seen[i] || !okv[u]) sc[u][i][r] = -INFINITY;
+    }
+    // ---- running maximum (with a slack of 2^8 before the accumulators are rescaled) and the exponentials
+    float pr[NR][8], mx[NR];
+    bool up = false;
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      float m = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) m = fmaxf(m, sc[u][i][r]);
+      const lane_pair q = lane_swap<16>(m);
+      m = max_xor32(fmaxf(q.a, q.b)) * fac[i];
+      mx[i] = m;
+      up |= m > m_run[i] + 8.f || (m_run[i] == -INFINITY && m > -INFINITY);
+    }
+    if (__builtin_amdgcn_ballot_w64(up) != 0) {
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        const float mn = fmaxf(m_run[i], mx[i]);
+        const float f = m_run[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[i] - mn);
+        m_run[i] = mn;
+        l_run[i] *= f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[i][e][r] *= f;
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (I4) {
+#pragma unroll
+          for (int g = 0; g < kPgNG; ++g) corr[i][g] *= f;
+        }
       }
-      __builtin_amdgcn_sched_barrier(0);
-      // ---- P V
-      if constexpr (I4) {
-        const bf16x2 m24 = {(__bf16)-24.f, (__bf16)-24.f};
+    }
 #pragma unroll
-        for (int g = 0; g < kPgNG; ++g) {
-          float sv[8];
+    for (int i = 0; i < NR; ++i) {
+      const float ms = m_run[i] == -INFINITY ? 0.f : m_run[i];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) sv[k] = scale_of(vt[k >> 2].s, k & 3, g);
-          bf16x8 pg[NR];
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int i = 0; i < NR; ++i) {
+        for (int r = 0; r < 4; ++r) {
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][i][r], fac[i], -ms));
+          pr[i][4 * u + r] = e;
+          l_run[i] += e;
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    // ---- P V
+    if constexpr (I4) {
+      bool odd = false;  // a scale that is not finite, next to a weight of 0
+      if (masked) {
+        uint32_t any = 0;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              float w = pr[i][k] * sv[k];
-              // a masked key weighs nothing, whatever its scale is
-              if (masked && pr[i][k] == 0.f) w = 0.f;
-              pg[i][k] = (__bf16)w;
-            }
-          }
-          uint32_t x[4];
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            x[k] = __builtin_amdgcn_perm(vt[k >> 1].c[2 * (k & 1) + 1][g >> 1], vt[k >> 1].c[2 * (k & 1)][g >> 1],
-                                         g & 1 ? 0x07060302u : 0x05040100u);
+          for (int w = 0; w < 2; ++w)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t y[4];
+            for (int k = 0; k < 4; ++k) any |= ((vt[u].s[w][k] & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
+        odd = __builtin_amdgcn_ballot_w64(any != 0) != 0;
+      }
+      const bf16x2 m24 = {(__bf16)-24.f, (__bf16)-24.f};
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              y[k] = ((e == 0 ? x[k] << 3 : x[k] >> (4 * e - 3)) & 0x00780078u) | 0x41804180u;
-            const bf16x8 va = as_bf16x8(y[0], y[1], y[2], y[3]);
+      for (int g = 0; g < kPgNG; ++g) {
+        float w[NR][8];
 #pragma unroll
-            for (int i = 0; i < NR; ++i) acc[i][4 * g + e] = mfma16(va, pg[i], acc[i][4 * g + e]);
-          }
+        for (int k = 0; k < 8; ++k) {
+          const float sv = scale_of(vt[k >> 2].s, k & 3, g);
+#pragma unroll
+          for (int i = 0; i < NR; ++i) w[i][k] = pr[i][k] * sv;
+        }
+        if (odd) {
+          // a key that a row does not see weighs nothing there, whatever its scale is
 #pragma unroll
           for (int i = 0; i < NR; ++i)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const bf16x2 w = {pg[i][2 * k], pg[i][2 * k + 1]};
-              corr[i][g] = __builtin_amdgcn_fdot2_f32_bf16(w, m24, corr[i][g], false);
-            }
-          __builtin_amdgcn_sched_barrier(0);
+            for (int k = 0; k < 8; ++k)
+              if (pr[i][k] == 0.f) w[i][k] = 0.f;
         }
-      } else {
         bf16x8 pg[NR];
 #pragma unroll
-        for (int i = 0; i < NR; ++i)
+        for (int i = 0; i < NR; ++i) {
+          u32x4 pw;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) pg[i][k] = (__bf16)pr[i][k];
-        bool odd = false;
-        if (masked) {
-          // a value that is not finite must not meet a weight of 0 in a product
-          uint32_t any = 0;
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-              for (int w = 0; w < 2; ++w)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  const uint32_t x = vt[u].c[r][w][k];
-                  any |= ((x & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
-                }
-          odd = __builtin_amdgcn_ballot_w64(any != 0) != 0;
+          for (int k = 0; k < 4; ++k) {
+            pw[k] = cvt2(w[i][2 * k], w[i][2 * k + 1]);
+            corr[i][g] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, (uint32_t)pw[k]), m24, corr[i][g], false);
+          }
+          pg[i] = __builtin_bit_cast(bf16x8, pw);
         }
+        uint32_t x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          x[k] = __builtin_amdgcn_perm(vt[k >> 1].c[2 * (k & 1) + 1][g >> 1], vt[k >> 1].c[2 * (k & 1)][g >> 1],
+                                       g & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          u32x4 y;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) y[k] = ((e == 0 ? x[k] << 3 : x[k] >> (4 * e - 3)) & mv) | cv;
+          const bf16x8 va = __builtin_bit_cast(bf16x8, y);
+#pragma unroll
+          for (int i = 0; i < NR; ++i) acc[i][4 * g + e] = mfma16(va, pg[i], acc[i][4 * g + e]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+      bf16x8 pg[NR];
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        u32x4 pw;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) pw[k] = cvt2(pr[i][2 * k], pr[i][2 * k + 1]);
+        pg[i] = __builtin_bit_cast(bf16x8, pw);
+      }
+      bool odd = false;  // a value that is not finite, next to a weight of 0
+      if (masked) {
+        uint32_t any = 0;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) any |= ((vt[u].c[r][w][k] & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
+        odd = __builtin_amdgcn_ballot_w64(any != 0) != 0;
+      }
+      if (odd) {
+        // What is not finite must not meet a weight of 0 in a product: it is taken out of the values here and added by
+        // whether any weight meets it, +inf, -inf or both (NaN)
 #pragma unroll
         for (int w = 0; w < 2; ++w)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
 #pragma unroll
             for (int hl = 0; hl < 2; ++hl) {
-              const int e = 8 * w + 2 * k + hl;  // dim 128 w + 8 c + 2 k + hl
-              uint32_t y[4];
+              u32x4 up4 = {0, 0, 0, 0}, dn4 = {0, 0, 0, 0};
 #pragma unroll
-              for (int n = 0; n < 4; ++n)
-                y[n] = __builtin_amdgcn_perm(vt[n >> 1].c[2 * (n & 1) + 1][w][k], vt[n >> 1].c[2 * (n & 1)][w][k],
-                                             hl ? 0x07060302u : 0x05040100u);
-              if (odd) {
-                // the finite values as ever; the others by whether any weight meets one: +inf, -inf or both (NaN)
-                uint32_t up[4], dn[4];
+              for (int j = 0; j < 8; ++j) {
+                const uint32_t word = vt[j >> 2].c[j & 3][w][k];
+                const uint32_t v = (word >> (16 * hl)) & 0xFFFFu, one = 0x3F80u << (16 * (j & 1));
+                const bool bad = (v & 0x7F80u) == 0x7F80u;
+                up4[j >> 1] |= bad && v != 0xFF80u ? one : 0u;
+                dn4[j >> 1] |= bad && v != 0x7F80u ? one : 0u;
+                vt[j >> 2].c[j & 3][w][k] = bad ? word & ~(0xFFFFu << (16 * hl)) : word;
+              }
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                  up[n] = dn[n] = 0;
+              for (int i = 0; i < NR; ++i) {
+                u32x4 on;
 #pragma unroll
-                  for (int j = 0; j < 2; ++j) {
-                    const uint32_t v = (y[n] >> (16 * j)) & 0xFFFFu, one = 0x3F80u << (16 * j);
-                    if ((v & 0x7F80u) == 0x7F80u) {
-                      if (v != 0xFF80u) up[n] |= one;
-                      if (v != 0x7F80u) dn[n] |= one;
-                      y[n] &= ~(0xFFFFu << (16 * j));
-                    }
-                  }
-                }
+                for (int n = 0; n < 4; ++n)
+                  on[n] = (pr[i][2 * n] != 0.f ? 0x3F80u : 0u) | (pr[i][2 * n + 1] != 0.f ? 0x3F800000u : 0u);
+                const f32x4 cu = mfma16(__builtin_bit_cast(bf16x8, up4), __builtin_bit_cast(bf16x8, on), zero4());
+                const f32x4 cd = mfma16(__builtin_bit_cast(bf16x8, dn4), __builtin_bit_cast(bf16x8, on), zero4());
+                const int e = 8 * w + 2 * k + hl;
 #pragma unroll
-                for (int i = 0; i < NR; ++i) {
-                  bf16x8 on;
-#pragma unroll
-                  for (int n = 0; n < 8; ++n) on[n] = (__bf16)(pr[i][n] != 0.f ? 1.f : 0.f);
-                  const f32x4 cu = mfma16(as_bf16x8(up[0], up[1], up[2], up[3]), on, zero4());
-                  const f32x4 cd = mfma16(as_bf16x8(dn[0], dn[1], dn[2], dn[3]), on, zero4());
-#pragma unroll
-                  for (int r = 0; r < 4; ++r) {
-                    if (cu[r] > 0.f) acc[i][e][r] += INFINITY;
-                    if (cd[r] > 0.f) acc[i][e][r] -= INFINITY;
-                  }
+                for (int r = 0; r < 4; ++r) {
+                  if (cu[r] > 0.f) acc[i][e][r] += INFINITY;
+                  if (cd[r] > 0.f) acc[i][e][r] -= INFINITY;
                 }
               }
-              const bf16x8 va = as_bf16x8(y[0], y[1], y[2], y[3]);
-#pragma unroll
-              for (int i = 0; i < NR; ++i) acc[i][e] = mfma16(va, pg[i], acc[i][e]);
+              __builtin_amdgcn_sched_barrier(0);
             }
       }
-      if (more) {
-        v_load(nt[0], vt[0], next);
-        v_load(nt[1], vt[1], next + 16);
-        okv[0] = nt[0].ok;
-        okv[1] = nt[1].ok;
-      }
-      key = next;
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+#pragma unroll
+          for (int hl = 0; hl < 2; ++hl) {
+            const int e = 8 * w + 2 * k + hl;  // dim 128 w + 8 c + 2 k + hl
+            u32x4 y;
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+              y[n] = __builtin_amdgcn_perm(vt[n >> 1].c[2 * (n & 1) + 1][w][k], vt[n >> 1].c[2 * (n & 1)][w][k],
+                                           hl ? 0x07060302u : 0x05040100u);
+            const bf16x8 va = __builtin_bit_cast(bf16x8, y);
+#pragma unroll
+            for (int i = 0; i < NR; ++i) acc[i][e] = mfma16(va, pg[i], acc[i][e]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
     }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if constexpr (kLate) {
+        vtile[u] = nt[u];
+        ks_load(nt[u], kt[u]);
+      } else {
+        v_load(nt[u], vt[u], next + 16 * u);
+      }
+      okv[u] = nt[u].ok;
+      nt[u] = nn[u];
+    }
+    key += kRound;
+    next = after;
   }
-  __syncthreads();  // Q has been used: its LDS takes the waves' results
 
-  // ---- each wave's rows (those that are there) into LDS, dims in order
+  // ---- 16 rows at a time: each wave's rows (those that are there) into LDS, dims in order, then the four waves joined, one
+  // wave per row: the result, or the run's partial
+  const int d0 = 4 * lane;
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
     float l = l_run[i];
@@ -525,8 +617,9 @@ __global__ __launch_bounds__(256, NR == 1 ? 2 : 1) void paged_attn_kernel(PagedA
         corr[i][g] = add_xor<32>(q.a + q.b);
       }
     }
+    lds_barrier();  // Q, or the rows before these, have been used
     if (r0 + 16 * i + c < R) {
-      float* o = ob + ((size_t)wave * ROWS + 16 * i + c) * kORow;
+      float* o = ob + ((size_t)wave * 16 + c) * kORow;
       if constexpr (I4) {
 #pragma unroll
         for (int g = 0; g < kPgNG; ++g)
@@ -549,54 +642,52 @@ __global__ __launch_bounds__(256, NR == 1 ? 2 : 1) void paged_attn_kernel(PagedA
           }
       }
       if (a == 0) {
-        mls[wave][16 * i + c][0] = m_run[i];
-        mls[wave][16 * i + c][1] = l;
+        mls[wave][c][0] = m_run[i];
+        mls[wave][c][1] = l;
       }
     }
-  }
-  __syncthreads();
-  // ---- the four waves joined, one wave per row: the result, or the run's partial
-  const int d0 = 4 * lane;
+    lds_barrier();
 #pragma unroll 1
-  for (int i = wave; i < ROWS && r0 + i < R; i += 4) {
-    const int r = r0 + i, t = r / p.G, h = kvh * p.G + r - t * p.G;
-    float M = -INFINITY;
+    for (int j = wave; j < 16 && r0 + 16 * i + j < R; j += 4) {
+      const int r = r0 + 16 * i + j, t = r / p.G, h = kvh * p.G + r - t * p.G;
+      float M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, mls[w][i][0]);
-    float L = 0.f;
-    f32x4 O = zero4();
-    if (M > -INFINITY) {
+      for (int w = 0; w < 4; ++w) M = fmaxf(M, mls[w][j][0]);
+      float L = 0.f;
+      f32x4 O = zero4();
+      if (M > -INFINITY) {
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        if (mls[w][i][0] == -INFINITY) continue;  // nothing seen (its sums may still hold a NaN: they count)
-        const float f = __builtin_amdgcn_exp2f(mls[w][i][0] - M);
-        L += mls[w][i][1] * f;
-        const f32x4 v = *reinterpret_cast<const f32x4*>(ob + ((size_t)w * ROWS + i) * kORow + d0);
+        for (int w = 0; w < 4; ++w) {
+          if (mls[w][j][0] == -INFINITY) continue;  // nothing seen
+          const float f = __builtin_amdgcn_exp2f(mls[w][j][0] - M);
+          L += mls[w][j][1] * f;
+          const f32x4 v = *reinterpret_cast<const f32x4*>(ob + ((size_t)w * 16 + j) * kORow + d0);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) O[e] += v[e] * f;
+          for (int e = 0; e < 4; ++e) O[e] += v[e] * f;
+        }
       }
-    }
-    if (p.S > 1) {
-      const size_t slot = (((size_t)b * p.Hkv + kvh) * R + r) * p.S + s;
-      *reinterpret_cast<f32x4*>(p.part + slot * kPgD + d0) = O;
-      if (lane < 2) p.ml[2 * slot + lane] = lane ? L : M;
-    } else {
-      const int64_t oi = (((int64_t)b * p.T + t) * p.Hkv * p.G + h) * kPgD + d0;
-      f32x4 g = {INFINITY, INFINITY, INFINITY, INFINITY};
-      if (p.gate) {
-        const int64_t go = b * p.gb + t * p.gt + h * p.gh + d0;
-        g = p.q_f32 ? load_quad<float>((const float*)p.gate + go) : load_quad<__bf16>((const __bf16*)p.gate + go);
-      }
-      f32x4 v = zero4();
-      if (L != 0.f && keys_seen(p, pos, len, t) > 0) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = O[e] / L * (p.gate ? sigmoidf_(g[e]) : 1.f);
-      }
-      if (p.out_f32) {
-        *reinterpret_cast<f32x4*>((float*)p.out + oi) = v;
+      if (p.S > 1) {
+        const size_t slot = (((size_t)b * p.Hkv + kvh) * R + r) * p.S + s;
+        *reinterpret_cast<f32x4*>(p.part + slot * kPgD + d0) = O;
+        if (lane < 2) p.ml[2 * slot + lane] = lane ? L : M;
       } else {
-        bf16x4 w = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
-        *reinterpret_cast<bf16x4*>((__bf16*)p.out + oi) = w;
+        const int64_t oi = (((int64_t)b * p.T + t) * p.Hkv * p.G + h) * kPgD + d0;
+        f32x4 g = zero4();
+        if (p.gate) {
+          const int64_t go = b * p.gb + t * p.gt + h * p.gh + d0;
+          g = p.q_f32 ? load_quad<float>((const float*)p.gate + go) : load_quad<__bf16>((const __bf16*)p.gate + go);
+        }
+        f32x4 v = zero4();
+        if (L != 0.f && keys_seen(p, pos, len, t) > 0) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = O[e] / L * (p.gate ? sigmoidf_(g[e]) : 1.f);
+        }
+        if (p.out_f32) {
+          *reinterpret_cast<f32x4*>((float*)p.out + oi) = v;
+        } else {
+          bf16x4 w = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+          *reinterpret_cast<bf16x4*>((__bf16*)p.out + oi) = w;
+        }
       }
     }
   }
@@ -681,8 +772,7 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs p) 
   }
 }
 
-// Query rows per block (in 16s) and runs per row: enough blocks for two per CU (one with 32 rows, whose registers leave
-// room for no more), each run at least one round long.
+// Query rows per block (in 16s) and runs per row: enough blocks for two per CU, each run at least one round long.
 struct PagedPlan {
   int NR, RB, S;
 };
@@ -692,7 +782,7 @@ static PagedPlan paged_plan(int64_t B, int64_t T, int64_t Hkv, int64_t G, int64_
   const int64_t RB = (R + 16 * NR - 1) / (16 * NR), base = B * Hkv * RB;
   const int64_t most = (capacity + kRound - 1) / kRound;
   int64_t S = splits;
-  if (S <= 0) S = ((NR == 1 ? 512 : 256) + base - 1) / base;
+  if (S <= 0) S = (512 + base - 1) / base;
   if (S > most) S = most;
   if (S > 1024) S = 1024;
   if (S < 1) S = 1;

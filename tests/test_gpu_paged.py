@@ -3,8 +3,9 @@
 Bounds. Append: bf16 rows within one rounding (2^-8 relative) of the 64-bit values plus the fp32 arithmetic in front of it
 (2^-18 of the row's largest value); 4-bit codes and scales equal. Attention, per output value, with w the softmax weights:
   2^-8 sum w |v|            each weight rounded to bf16 once
-  2 d sum w |v|             scores off by d = 2^-15 sum |q k| scale: q as bf16 hi + lo (2^-17), fp32 norm, rotation and sums;
-                            a weight's numerator and the sum of all both move
+  2 d sum w |v|             scores off by d sum |q k| scale, a weight's numerator and the sum of all both moving: fp32 norm,
+                            rotation and sums (2^-16) and q's own rounding, bf16 hi + lo (2^-17) against bf16 keys, so
+                            d = 2^-15; against 4-bit codes fp16 (half a step is 2^-12 of q), so d = 2^-12 + 2^-15
   2^-16 sum w |v|           exponentials, sums and divisions in fp32
   (n / 32 + 16) 2^-19 sum w s   fp32 sums over n keys of offset codes (at most 31 s each, in n / 32 products per wave)
   2^-8 |out| (2^-23 for fp32)   the output's own rounding, with 2^-20 |out| of the gate
@@ -68,7 +69,8 @@ def check_attention(d, out, gated=True, **kw):
                                                        d["cos"], d["sin"], d["lens"], d["qw"], spread=True, **kw)
     n = d["table"].shape[1] * d["pages"][0].shape[2]
     last = 2.0 ** -8 if out.dtype == torch.bfloat16 else 2.0 ** -23
-    bound = (2.0 ** -8 + 2 * 2.0 ** -15 * prod + 2.0 ** -16) * amp + (n / 32 + 16) * 2.0 ** -19 * step \
+    q_off = 2.0 ** -15 + (2.0 ** -12 if d["fmt"] == "int4" else 0)
+    bound = (2.0 ** -8 + 2 * q_off * prod + 2.0 ** -16) * amp + (n / 32 + 16) * 2.0 ** -19 * step \
         + (last + 2.0 ** -20) * ref.abs() * (1 + 2.0 ** -7) + 1e-30
     err = (out.double().cpu() - ref).abs()
     worst = float((err / bound).max())
