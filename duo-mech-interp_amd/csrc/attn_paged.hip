@@ -197,6 +197,43 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
     }
   };
 
+  // ---- Q's rows, one wave each: row i of the block (i = wave, wave + 4, ...) is token r / G, head r % G of the group. The
+  // first row's loads go out ahead of the tiles': loads return in order.
+  struct QRow {
+    f32x4 x, px, co, si;
+    bool there;
+  };
+  const int half = p.rot >> 1, d0 = 4 * lane;
+  const bool turns = d0 < p.rot;
+  const int pd = !turns ? d0 : d0 < half ? d0 + half : d0 - half, pj = d0 < half ? d0 : d0 - half;
+  auto q_load = [&](int i) -> QRow {
+    QRow w = {zero4(), zero4(), zero4(), zero4(), false};
+    const int r = r0 + i, t = r / p.G, h = kvh * p.G + r - t * p.G;
+    w.there = i < ROWS && r < R && keys_seen(p, pos, len, t) > 0;
+    if (w.there) {
+      const int64_t o = b * p.qb + t * p.qt + h * p.qh;
+      if (p.q_f32) {
+        w.x = load_quad<float>((const float*)p.q + o + d0);
+        w.px = load_quad<float>((const float*)p.q + o + pd);
+      } else {
+        w.x = load_quad<__bf16>((const __bf16*)p.q + o + d0);
+        w.px = load_quad<__bf16>((const __bf16*)p.q + o + pd);
+      }
+      if (turns) {
+        w.co = load_quad<float>(p.cos_t + (pos + t) * half + pj);
+        w.si = load_quad<float>(p.sin_t + (pos + t) * half + pj);
+      }
+    }
+    return w;
+  };
+  f32x4 wx = zero4(), wp = zero4();
+  if (p.qw) {
+    wx = load_quad<float>(p.qw + d0);
+    wp = load_quad<float>(p.qw + pd);
+  }
+  QRow row = q_load(wave);
+  __builtin_amdgcn_sched_barrier(0);
+
   // ---- the first round's tiles, in flight while Q is prepared. The next round's tiles are loaded while this one's are
   // used, and their pages a round earlier still. A wave's last round loads its own tiles once more (from the cache) rather
   // than nothing: with no branch around the loads every wait counts how many of them may stay in flight.
@@ -226,48 +263,24 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
   }
   __builtin_amdgcn_sched_barrier(0);
 
-  // ---- Q: norm, rotation, scale log2(e), the split into hi + lo or the power of two, into LDS as B operands; one wave
-  // per row
+  // ---- Q: norm, rotation, scale log2(e), the split into hi + lo or the power of two, into LDS as B operands
   if (work) {
-    const int half = p.rot >> 1, d0 = 4 * lane;
 #pragma unroll 1
     for (int i = wave; i < ROWS; i += 4) {
-      const int r = r0 + i, t = r / p.G, h = kvh * p.G + r - t * p.G;
-      f32x4 x = zero4();
-      if (r < R && t < len && pos + t >= 0 && pos + t < p.pt.capacity()) {
-        const int64_t o = b * p.qb + t * p.qt + h * p.qh;
-        const bool turns = d0 < p.rot;
-        const int pd = !turns ? d0 : d0 < half ? d0 + half : d0 - half;
-        f32x4 px, wx = zero4(), wp = zero4(), co = zero4(), si = zero4();
-        if (p.q_f32) {
-          x = load_quad<float>((const float*)p.q + o + d0);
-          px = load_quad<float>((const float*)p.q + o + pd);
-        } else {
-          x = load_quad<__bf16>((const __bf16*)p.q + o + d0);
-          px = load_quad<__bf16>((const __bf16*)p.q + o + pd);
-        }
-        if (p.qw) {
-          wx = load_quad<float>(p.qw + d0);
-          wp = load_quad<float>(p.qw + pd);
-        }
-        if (turns) {
-          const int j = d0 < half ? d0 : d0 - half;
-          co = load_quad<float>(p.cos_t + (pos + t) * half + j);
-          si = load_quad<float>(p.sin_t + (pos + t) * half + j);
-        }
+      const QRow cur = row;
+      row = q_load(i + 4);
+      f32x4 x = cur.x;
+      if (cur.there) {
+        float rr = 1.f;
         if (p.qw) {
           const float ss = wave_sum(x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]);
-          const float rr = rsqrtf(ss * (1.f / kPgD) + p.eps);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[e] = x[e] * rr * (1.f + wx[e]);
-            px[e] = px[e] * rr * (1.f + wp[e]);
-          }
+          rr = rsqrtf(ss * (1.f / kPgD) + p.eps);
         }
-        if (turns) {
-          const float sg = d0 < half ? -1.f : 1.f;
+        const float sg = d0 < half ? -1.f : 1.f;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = x[e] * co[e] + sg * px[e] * si[e];
+        for (int e = 0; e < 4; ++e) {
+          x[e] = x[e] * rr * (1.f + wx[e]);
+          if (turns) x[e] = x[e] * cur.co[e] + sg * (cur.px[e] * rr * (1.f + wp[e])) * cur.si[e];
         }
       }
       const int ti = i >> 4, col = i & 15;
@@ -276,8 +289,10 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
       if constexpr (I4) {
         // dim 64 g + 16 a + 8 u + j is step 2 g + u of lane group a; a dword's nibbles leave it in pairs (j, j + 4), those
         // of odd j times 16
-        const int ex = __builtin_amdgcn_frexp_expf(
-            wave_max(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])))));
+        int ex = 0;
+        if (cur.there)
+          ex = __builtin_amdgcn_frexp_expf(
+              wave_max(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])))));
         _Float16* qe = reinterpret_cast<_Float16*>(qf + (size_t)ti * QF);
         const int base = ((2 * (lane >> 4) + ((lane >> 1) & 1)) * 64 + 16 * ((lane >> 2) & 3) + col) * 8 + (lane & 1);
         float off = 0.f;
@@ -334,6 +349,19 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
   lds_barrier();
 #pragma unroll
   for (int i = 0; i < NR; ++i) fac[i] = qfac[16 * i + c];
+  // 16 rows against codes: Q's operands and the offsets stay in registers
+  constexpr bool kQReg = I4 && NR == 1;
+  u32x4 qreg[kQReg ? 8 : 1];
+  f32x4 zreg[kQReg ? kPgNG : 1];
+  if constexpr (kQReg) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) qreg[k] = qf[64 * k + lane];
+#pragma unroll
+    for (int g = 0; g < kPgNG; ++g) {
+      const float z = qoff[0][g][c];
+      zreg[g] = f32x4{z, z, z, z};
+    }
+  }
 
   while (key < k1) {
     // ---- scores, two tiles of 16 keys against each 16 rows
@@ -355,19 +383,28 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
           }
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
-          const u32x4* qi = qf + (size_t)i * QF + 2 * g * 64 + lane;
-          const f16x8 h0 = __builtin_bit_cast(f16x8, qi[0]), h1 = __builtin_bit_cast(f16x8, qi[64]);
-          const float z = qoff[i][g][c];
+          f16x8 h0, h1;
+          f32x4 z;
+          if constexpr (kQReg) {
+            h0 = __builtin_bit_cast(f16x8, qreg[2 * g]);
+            h1 = __builtin_bit_cast(f16x8, qreg[2 * g + 1]);
+            z = zreg[g];
+          } else {
+            const u32x4* qi = qf + (size_t)i * QF + 2 * g * 64 + lane;
+            h0 = __builtin_bit_cast(f16x8, qi[0]);
+            h1 = __builtin_bit_cast(f16x8, qi[64]);
+            const float z1 = qoff[i][g][c];
+            z = f32x4{z1, z1, z1, z1};
+          }
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            f32x4 d = {z, z, z, z};
-            d = mfma16h(ka[u][0], h0, d);
+            f32x4 d = mfma16h(ka[u][0], h0, z);
             d = mfma16h(ka[u][1], h1, d);
 #pragma unroll
             for (int r = 0; r < 4; ++r) sc[u][i][r] += scale_of(kt[u].s, r, g) * d[r];
           }
         }
-        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (NR > 1) __builtin_amdgcn_sched_barrier(0);
       }
     } else {
 #pragma unroll
@@ -507,7 +544,7 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
 #pragma unroll
           for (int i = 0; i < NR; ++i) acc[i][4 * g + e] = mfma16(va, pg[i], acc[i][4 * g + e]);
         }
-        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (NR > 1) __builtin_amdgcn_sched_barrier(0);
       }
     } else {
       bf16x8 pg[NR];
@@ -604,7 +641,6 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
 
   // ---- 16 rows at a time: each wave's rows (those that are there) into LDS, dims in order, then the four waves joined, one
   // wave per row: the result, or the run's partial
-  const int d0 = 4 * lane;
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
     float l = l_run[i];
@@ -699,14 +735,9 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs p) 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d0 = 4 * lane;
   const int kvh = blockIdx.x % p.Hkv, r = blockIdx.x / p.Hkv, b = blockIdx.y;
   const int R = p.T * p.G, t = r / p.G, h = kvh * p.G + r - t * p.G;
-  const int64_t pos = p.pos[b];
-  const int len = p.lens ? min(max(p.lens[b], 0), p.T) : p.T;
+  const int64_t pos = load_uniform(p.pos + b);
+  const int len = p.lens ? min(max(load_uniform(p.lens + b), 0), p.T) : p.T;
   const int seen = keys_seen(p, pos, len, t);
-  f32x4 g = zero4();
-  if (p.gate) {
-    const int64_t go = b * p.gb + t * p.gt + h * p.gh + d0;
-    g = p.q_f32 ? load_quad<float>((const float*)p.gate + go) : load_quad<__bf16>((const __bf16*)p.gate + go);
-  }
   int n_row = 0;
   if (len > 0) n_row = (int)min(max(pos + len, (int64_t)0), p.pt.capacity());
   const int run = run_keys(n_row, p.S);
@@ -715,16 +746,27 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs p) 
   const size_t base = (((size_t)b * p.Hkv + kvh) * R + r) * p.S;
   float M = -INFINITY, L = 0.f;
   f32x4 O = zero4();
-  for (int s0 = wave; s0 < n; s0 += 32) {
-    f32x4 v[8];
-    float m[8], l[8];
+  // the first eight runs are loaded without knowing n (slots of the workspace, whatever they hold), the gate with them
+  f32x4 pv[8];
+  float m[8], l[8];
+  auto load = [&](int s0) {
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
-      const size_t s = base + min(s0 + 4 * u, n - 1);
-      v[u] = *reinterpret_cast<const f32x4*>(p.part + s * kPgD + d0);
+      const size_t s = base + min(s0 + 4 * u, p.S - 1);
+      pv[u] = *reinterpret_cast<const f32x4*>(p.part + s * kPgD + d0);
       m[u] = p.ml[2 * s];
       l[u] = p.ml[2 * s + 1];
     }
+  };
+  load(wave);
+  f32x4 g = zero4();
+  if (p.gate) {
+    const int64_t go = b * p.gb + t * p.gt + h * p.gh + d0;
+    g = p.q_f32 ? load_quad<float>((const float*)p.gate + go) : load_quad<__bf16>((const __bf16*)p.gate + go);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  for (int s0 = wave; s0 < n; s0 += 32) {
+    if (s0 != wave) load(s0);
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       if (s0 + 4 * u >= n || m[u] == -INFINITY) continue;
@@ -732,7 +774,7 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs p) 
       const float c0 = __builtin_amdgcn_exp2f(M - mn), c1 = __builtin_amdgcn_exp2f(m[u] - mn);
       L = L * c0 + l[u] * c1;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) O[e] = O[e] * c0 + v[u][e] * c1;
+      for (int e = 0; e < 4; ++e) O[e] = O[e] * c0 + pv[u][e] * c1;
       M = mn;
     }
   }
@@ -772,7 +814,8 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs p) 
   }
 }
 
-// Query rows per block (in 16s) and runs per row: enough blocks for two per CU, each run at least one round long.
+// Query rows per block (in 16s) and runs per row: two blocks per CU, but one where that leaves a block no more than two
+// rounds (three rows of 8192 4-bit keys: 64 runs 17.2 us, 32 runs 15.3, 16 runs 18.8).
 struct PagedPlan {
   int NR, RB, S;
 };
@@ -782,7 +825,10 @@ static PagedPlan paged_plan(int64_t B, int64_t T, int64_t Hkv, int64_t G, int64_
   const int64_t RB = (R + 16 * NR - 1) / (16 * NR), base = B * Hkv * RB;
   const int64_t most = (capacity + kRound - 1) / kRound;
   int64_t S = splits;
-  if (S <= 0) S = (512 + base - 1) / base;
+  if (S <= 0) {
+    S = (512 + base - 1) / base;
+    if (most <= 2 * S) S = (256 + base - 1) / base;
+  }
   if (S > most) S = most;
   if (S > 1024) S = 1024;
   if (S < 1) S = 1;

@@ -13,6 +13,7 @@ tests/engine_ref.py):
 Every op runs on the current HIP stream of its inputs' device; inputs are validated here (device, dtype, layout,
 shape) and a bad call raises RuntimeError. CPU tensors raise: there is no CPU path in the product.
 """
+import functools
 import math
 from typing import NamedTuple, Optional
 
@@ -356,126 +357,172 @@ def _attn_prefill_cached_proj_impl(y, q_norm_w, k_norm_w, eps, k_cache, v_cache,
 
 
 # ---------------------------------------------------------------- paged KV cache
+# A decode step makes these calls eagerly for every layer, so their checks are plain comparisons in one pass each.
 def _heads_view(x, what):
     """A [B, T, H, 256] fp32 or bf16 view (rows of 256 dense, anything else strided): its strides of B, T and H."""
-    _require(x.dim() == 4 and x.shape[3] == 256 and x.stride(3) == 1 and x.dtype in _DT,
-             f"{what}: [B, T, heads, 256] fp32 or bf16 with dense rows")
-    return x.stride()[:3]
+    if not x.is_cuda:
+        raise Q35Error("q35hip: inputs must be HIP device tensors (there is no CPU fallback)")
+    s = x.stride()
+    if len(s) != 4 or s[3] != 1 or x.shape[3] != 256 or x.dtype not in _DT:
+        raise Q35Error(f"q35hip: {what}: [B, T, heads, 256] fp32 or bf16 with dense rows")
+    return s[0], s[1], s[2]
 
 
-def _pages_check(k_pages, v_pages, k_scale, v_scale, table, pos, lens, B):
-    """The format, n_pages, Hkv and page size of a paged cache; its table, positions and lengths checked for B rows."""
-    _on_gpu(k_pages, v_pages, k_scale, v_scale, pos, lens)
-    _require(table.device == k_pages.device and table.dtype == torch.int32 and table.dim() == 2 and table.shape[0] == B
-             and table.stride(1) == 1, "table: [B, blocks] int32 with dense rows, on the pages' device")
-    _require(pos.dtype == torch.int32 and tuple(pos.shape) == (B,), "pos: [B] int32")
-    _require(lens is None or (lens.dtype == torch.int32 and tuple(lens.shape) == (B,)), "lens: [B] int32")
-    _require(k_pages.dim() == 4 and v_pages.shape == k_pages.shape and v_pages.dtype == k_pages.dtype,
-             "pages: k and v alike, [pages, Hkv, page size, ...]")
-    n, Hkv, ps, w = k_pages.shape
-    if k_pages.dtype == torch.bfloat16:
-        _require(w == 256, "bf16 pages: [pages, Hkv, page size, 256]")
+def _dense_on(d, *ts):
+    """Whether every tensor is dense and on device d."""
+    for t in ts:
+        if t is not None and not (t.get_device() == d and t.is_contiguous()):
+            if not t.is_cuda:
+                raise Q35Error("q35hip: inputs must be HIP device tensors (there is no CPU fallback)")
+            return False
+    return True
+
+
+def _pages_check(d, k_pages, v_pages, k_scale, v_scale, table, pos, lens, B):
+    """The format, n_pages, Hkv and page size of a paged cache on device d; its table, positions and lengths checked for
+    B rows."""
+    if not _dense_on(d, k_pages, v_pages, k_scale, v_scale, pos, lens):
+        raise Q35Error("q35hip: pages, pos and lens must be contiguous and on one device with the other inputs")
+    i32 = torch.int32
+    if table.get_device() != d or table.dtype != i32 or table.dim() != 2 or table.shape[0] != B or table.stride(1) != 1:
+        raise Q35Error("q35hip: table: [B, blocks] int32 with dense rows, on the pages' device")
+    if pos.dtype != i32 or pos.shape != (B,) or (lens is not None and (lens.dtype != i32 or lens.shape != (B,))):
+        raise Q35Error("q35hip: pos, lens: [B] int32")
+    shape, dt = k_pages.shape, k_pages.dtype
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype != dt:
+        raise Q35Error("q35hip: pages: k and v alike, [pages, Hkv, page size, ...]")
+    n, Hkv, ps, w = shape
+    if dt == torch.bfloat16:
+        if w != 256:
+            raise Q35Error("q35hip: bf16 pages: [pages, Hkv, page size, 256]")
         return Q35_BF16, n, Hkv, ps
-    _require(k_pages.dtype == torch.uint8 and w == 128, "4-bit pages: [pages, Hkv, page size, 128] uint8")
+    if dt != torch.uint8 or w != 128:
+        raise Q35Error("q35hip: 4-bit pages: [pages, Hkv, page size, 128] uint8")
     for s in (k_scale, v_scale):
-        _require(s is not None and s.dtype == torch.bfloat16 and tuple(s.shape) == (n, Hkv, ps, 4),
-                 "4-bit pages: k_scale, v_scale [pages, Hkv, page size, 4] bf16")
+        if s is None or s.dtype != torch.bfloat16 or s.shape != (n, Hkv, ps, 4):
+            raise Q35Error("q35hip: 4-bit pages: k_scale, v_scale [pages, Hkv, page size, 4] bf16")
     return Q35_I4_G64, n, Hkv, ps
 
 
+def _rope_check(d, cos, sin, norm_w, rows):
+    """rot of cos / sin tables of at least `rows` rows; norm_w None or [256] fp32."""
+    f32 = torch.float32
+    if not _dense_on(d, cos, sin, norm_w):
+        raise Q35Error("q35hip: cos, sin and the norm weight must be contiguous and on one device with the other inputs")
+    shape = cos.shape
+    if cos.dtype != f32 or sin.dtype != f32 or len(shape) != 2 or sin.shape != shape or \
+            (norm_w is not None and (norm_w.dtype != f32 or norm_w.shape != (256,))):
+        raise Q35Error("q35hip: cos, sin: [P, rot / 2] fp32; norm weight: [256] fp32")
+    if shape[0] < rows and shape[1]:
+        raise Q35Error(f"q35hip: cos/sin tables need {rows} rows")
+    return 2 * shape[1]
+
+
 def _paged_kv_append_impl(k, v, k_pages, v_pages, k_scale, v_scale, table, pos, lens, cos, sin, k_norm_w, eps):
-    _on_gpu(cos, sin, k_norm_w)
-    _require(k.device == k_pages.device and v.device == k.device and cos.device == k.device,
-             "k, v, the tables and the pages must be on one device")
-    ks, vs = _heads_view(k, "k"), _heads_view(v, "v")
+    kb, kt, kh = _heads_view(k, "k")
+    vb, vt, vh = _heads_view(v, "v")
     B, T, Hkv, D = k.shape
-    fmt, n, H, ps = _pages_check(k_pages, v_pages, k_scale, v_scale, table, pos, lens, B)
-    _require(v.shape == k.shape and v.dtype == k.dtype and H == Hkv, "k, v: alike, with the pages' heads")
-    _require(k_norm_w is None or (k_norm_w.dtype == torch.float32 and k_norm_w.numel() == D
-                                  and k_norm_w.device == k.device), "k_norm_w: [256] fp32")
-    rot = _tables_check(cos, sin, table.shape[1] * ps)
-    if k.numel() == 0:
+    d = k.get_device()
+    fmt, n, H, ps = _pages_check(d, k_pages, v_pages, k_scale, v_scale, table, pos, lens, B)
+    if v.shape != k.shape or v.dtype != k.dtype or v.get_device() != d or H != Hkv:
+        raise Q35Error("q35hip: k, v: alike, with the pages' heads")
+    nb = table.shape[1]
+    rot = _rope_check(d, cos, sin, k_norm_w, nb * ps)
+    if B == 0 or T == 0:
         return
-    st = _launch(_lib.lib().q35_paged_kv_append, k, _ptr(k), *ks, _ptr(v), *vs, _DT[k.dtype], _ptr(k_norm_w), float(eps), _ptr(cos),
-                                        _ptr(sin), rot, _ptr(table), table.stride(0), table.shape[1], _ptr(pos),
-                                        _ptr(lens), _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale), fmt, n,
-                                        ps, B, T, Hkv, D, _stream(k))
+    st = _launch(_lib.lib().q35_paged_kv_append, k, k.data_ptr(), kb, kt, kh, v.data_ptr(), vb, vt, vh, _DT[k.dtype],
+                 _ptr(k_norm_w), eps, cos.data_ptr(), sin.data_ptr(), rot, table.data_ptr(), table.stride(0), nb,
+                 pos.data_ptr(), _ptr(lens), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale), fmt, n,
+                 ps, B, T, Hkv, D, _stream(k))
     check(st, "q35_paged_kv_append")
 
 
 def _paged_kv_rows_impl(k_pages, v_pages, k_scale, v_scale, table, pos, lens, T):
-    B = table.shape[0]
-    fmt, n, Hkv, ps = _pages_check(k_pages, v_pages, k_scale, v_scale, table, pos, lens, B)
+    B, nb = table.shape
+    fmt, n, Hkv, ps = _pages_check(k_pages.get_device(), k_pages, v_pages, k_scale, v_scale, table, pos, lens, B)
+    _require(T >= 0, "T: a number of tokens")
     k = torch.empty(B, Hkv, T, 256, dtype=torch.bfloat16, device=k_pages.device)
     v = torch.empty_like(k)
-    if k.numel() == 0:
+    if B == 0 or T == 0:
         return k, v
-    st = _launch(_lib.lib().q35_paged_kv_rows, k_pages, _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale), fmt, n, ps,
-                                      _ptr(table), table.stride(0), table.shape[1], _ptr(pos), _ptr(lens), _ptr(k),
-                                      _ptr(v), B, T, Hkv, 256, _stream(k_pages))
+    st = _launch(_lib.lib().q35_paged_kv_rows, k, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale),
+                 fmt, n, ps, table.data_ptr(), table.stride(0), nb, pos.data_ptr(), _ptr(lens), k.data_ptr(),
+                 v.data_ptr(), B, T, Hkv, 256, _stream(k))
     check(st, "q35_paged_kv_rows")
     return k, v
 
 
+@functools.lru_cache(maxsize=256)
+def _attn_paged_workspace(*sizes):
+    return _lib.lib().q35_gated_attn_paged_workspace_bytes(*sizes)
+
+
 def _attn_paged_impl(q, gate, k_pages, v_pages, k_scale, v_scale, table, pos, lens, cos, sin, q_norm_w, eps, scale,
                      splits, f32_out):
-    _on_gpu(cos, sin, q_norm_w)
-    _require(q.device == k_pages.device and cos.device == q.device, "q, the tables and the pages must be on one device")
-    qs = _heads_view(q, "q")
+    qb, qt, qh = _heads_view(q, "q")
     B, T, Hq, D = q.shape
-    fmt, n, Hkv, ps = _pages_check(k_pages, v_pages, k_scale, v_scale, table, pos, lens, B)
-    gs = (0, 0, 0)
+    d = q.get_device()
+    fmt, n, Hkv, ps = _pages_check(d, k_pages, v_pages, k_scale, v_scale, table, pos, lens, B)
+    gb = gt = gh = 0
     if gate is not None:
-        gs = _heads_view(gate, "gate")
-        _require(gate.shape == q.shape and gate.dtype == q.dtype and gate.device == q.device, "gate: like q")
-    _require(q_norm_w is None or (q_norm_w.dtype == torch.float32 and q_norm_w.numel() == D
-                                  and q_norm_w.device == q.device), "q_norm_w: [256] fp32")
-    rot = _tables_check(cos, sin, table.shape[1] * ps)
+        gb, gt, gh = _heads_view(gate, "gate")
+        if gate.shape != q.shape or gate.dtype != q.dtype or gate.get_device() != d:
+            raise Q35Error("q35hip: gate: like q")
+    nb = table.shape[1]
+    rot = _rope_check(d, cos, sin, q_norm_w, nb * ps)
     out = torch.empty(B, T, Hq * D, dtype=torch.float32 if f32_out else torch.bfloat16, device=q.device)
     if out.numel() == 0:
         return out
-    L = _lib.lib()
-    nbytes = L.q35_gated_attn_paged_workspace_bytes(B, T, Hq, Hkv, D, table.shape[1], ps, splits)
+    nbytes = _attn_paged_workspace(B, T, Hq, Hkv, D, nb, ps, splits)
     _require(nbytes > 0, "unsupported attention shape")
-    ws = _workspace(nbytes, q.device)
-    st = _launch(L.q35_gated_attn_paged, q, _ptr(q), *qs, _ptr(gate), *gs, _DT[q.dtype], _ptr(q_norm_w), float(eps), _ptr(cos),
-                                _ptr(sin), rot, _ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale), fmt, n, ps,
-                                _ptr(table), table.stride(0), table.shape[1], _ptr(pos), _ptr(lens), _ptr(out),
-                                _DT[out.dtype], B, T, Hq, Hkv, D, float(scale), int(splits), _ptr(ws), ws.numel(),
-                                _stream(q))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    st = _launch(_lib.lib().q35_gated_attn_paged, q, q.data_ptr(), qb, qt, qh, _ptr(gate), gb, gt, gh, _DT[q.dtype],
+                 _ptr(q_norm_w), eps, cos.data_ptr(), sin.data_ptr(), rot, k_pages.data_ptr(), v_pages.data_ptr(),
+                 _ptr(k_scale), _ptr(v_scale), fmt, n, ps, table.data_ptr(), table.stride(0), nb, pos.data_ptr(),
+                 _ptr(lens), out.data_ptr(), Q35_F32 if f32_out else Q35_BF16, B, T, Hq, Hkv, D, scale, splits,
+                 ws.data_ptr(), nbytes, _stream(q))
     check(st, "q35_gated_attn_paged")
     return out
 
 
+@functools.lru_cache(maxsize=256)
+def _verify_drafts_workspace(*sizes):
+    return _lib.lib().q35_verify_drafts_workspace_bytes(*sizes)
+
+
 def _verify_drafts_impl(logits, draft_ids, draft_probs, u, lens, temperatures, temperature):
-    _on_gpu(lens, temperatures)
-    for t in (logits, draft_ids, draft_probs, u, lens, temperatures):
-        _require(t is None or (t.is_cuda and t.device == logits.device),
-                 "inputs must be HIP device tensors on one device (there is no CPU fallback)")
-    _require(logits.dtype == torch.float32 and logits.dim() == 3 and logits.stride(2) == 1,
-             "logits: [B, K + 1, V] fp32 with dense rows")
-    B, K, V = logits.shape[0], logits.shape[1] - 1, logits.shape[2]
-    _require(K >= 0 and tuple(draft_ids.shape) == (B, K) and draft_ids.dtype == torch.int32
-             and (K <= 1 or draft_ids.stride(1) == 1), "draft_ids: [B, K] int32 with dense rows")
-    _require(tuple(u.shape) == (B, K + 1) and u.dtype == torch.float32 and (K == 0 or u.stride(1) == 1),
-             "u: [B, K + 1] fp32 with dense rows")
-    _require(draft_probs is None or (tuple(draft_probs.shape) == (B, K, V) and draft_probs.dtype == torch.float32
-                                     and draft_probs.stride(2) == 1), "draft_probs: [B, K, V] fp32 with dense rows")
-    _require(lens is None or (lens.dtype == torch.int32 and tuple(lens.shape) == (B,)), "lens: [B] int32")
-    _require(temperatures is None or (temperatures.dtype == torch.float32 and tuple(temperatures.shape) == (B,)),
-             "temperature: a number of at least 0 or [B] fp32")
-    L = _lib.lib()
-    n = torch.empty(B, dtype=torch.int32, device=logits.device)
-    tokens = torch.empty(B, K + 1, dtype=torch.int32, device=logits.device)
+    d = logits.get_device()
+    if not _dense_on(d, lens, temperatures) or d < 0 or draft_ids.get_device() != d or u.get_device() != d or \
+            (draft_probs is not None and draft_probs.get_device() != d):
+        raise Q35Error("q35hip: inputs must be HIP device tensors on one device (there is no CPU fallback), lens and "
+                       "temperature contiguous")
+    f32, i32 = torch.float32, torch.int32
+    if logits.dtype != f32 or logits.dim() != 3 or logits.stride(2) != 1 or logits.shape[1] == 0:
+        raise Q35Error("q35hip: logits: [B, K + 1, V] fp32 with dense rows")
+    B, K, V = logits.shape
+    K -= 1
+    if draft_ids.shape != (B, K) or draft_ids.dtype != i32 or (K > 1 and draft_ids.stride(1) != 1):
+        raise Q35Error("q35hip: draft_ids: [B, K] int32 with dense rows")
+    if u.shape != (B, K + 1) or u.dtype != f32 or (K and u.stride(1) != 1):
+        raise Q35Error("q35hip: u: [B, K + 1] fp32 with dense rows")
+    if draft_probs is not None and (draft_probs.shape != (B, K, V) or draft_probs.dtype != f32
+                                    or draft_probs.stride(2) != 1):
+        raise Q35Error("q35hip: draft_probs: [B, K, V] fp32 with dense rows")
+    if (lens is not None and (lens.dtype != i32 or lens.shape != (B,))) or \
+            (temperatures is not None and (temperatures.dtype != f32 or temperatures.shape != (B,))):
+        raise Q35Error("q35hip: lens: [B] int32; temperature: a number of at least 0 or [B] fp32")
+    n = torch.empty(B, dtype=i32, device=logits.device)
+    tokens = torch.empty(B, K + 1, dtype=i32, device=logits.device)
     if B == 0:
         return n, tokens
-    nbytes = L.q35_verify_drafts_workspace_bytes(B, K, V)
+    nbytes = _verify_drafts_workspace(B, K, V)
     _require(nbytes > 0, f"unsupported draft shape (B={B}, K={K}, V={V})")
-    ws = _workspace(nbytes, logits.device)
-    ps = draft_probs.stride()[:2] if draft_probs is not None else (0, 0)
-    st = _launch(L.q35_verify_drafts, logits, _ptr(logits), logits.stride(0), logits.stride(1), _ptr(draft_ids), draft_ids.stride(0),
-                             _ptr(draft_probs), *ps, _ptr(u), u.stride(0), _ptr(lens), _ptr(temperatures),
-                             float(temperature), _ptr(n), _ptr(tokens), B, K, V, _ptr(ws), ws.numel(), _stream(logits))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
+    pb, pp = draft_probs.stride()[:2] if draft_probs is not None else (0, 0)
+    st = _launch(_lib.lib().q35_verify_drafts, logits, logits.data_ptr(), logits.stride(0), logits.stride(1),
+                 draft_ids.data_ptr(), draft_ids.stride(0), _ptr(draft_probs), pb, pp, u.data_ptr(), u.stride(0),
+                 _ptr(lens), _ptr(temperatures), temperature, n.data_ptr(), tokens.data_ptr(), B, K, V, ws.data_ptr(),
+                 nbytes, _stream(logits))
     check(st, "q35_verify_drafts")
     return n, tokens
 
@@ -1281,6 +1328,13 @@ def argmax_rows(x, out=None):
     return out
 
 
+def _direct(t):
+    """Whether an op on t can be called as the function it is: a plain device tensor, nothing tracing. (The dispatcher takes
+    3 us of a call's host time, a third of what an append takes.) Anything else goes through torch.ops."""
+    return type(t) is torch.Tensor and t.is_cuda and not torch._C._len_torch_dispatch_stack() \
+        and not torch.compiler.is_compiling()
+
+
 class KVPages(NamedTuple):
     """A paged KV cache: k, v [pages, Hkv, page size, 256] bf16; or 4 bits, k, v [pages, Hkv, page size, 128] uint8 with
     k_scale, v_scale [pages, Hkv, page size, 4] bf16 (one scale per group of 64 dims, two codes a byte; include/q35hip.h
@@ -1312,14 +1366,16 @@ def paged_kv_append_(k, v, pages, table, pos, cos, sin, *, lens=None, k_norm_w=N
     table: [B, blocks] int32, row b's page of each block of page-size tokens; token t of row b goes to position
     pos[b] + t, t < lens[b] ([B] int32; None: all T). Tokens past lens, past the capacity or on a table entry that names
     no page are not written. Two rows of one call must not share a page they write to."""
-    torch.ops.q35.paged_kv_append_(k, v, *_four(pages), table, pos, lens, cos, sin, k_norm_w, float(eps))
+    op = _paged_kv_append_impl if _direct(k) else torch.ops.q35.paged_kv_append_
+    op(k, v, *_four(pages), table, pos, lens, cos, sin, k_norm_w, float(eps))
 
 
 def paged_kv_rows(pages, table, pos, T, *, lens=None):
     """Rows pos[b] .. pos[b] + T - 1 of each sequence read back from its pages: (k, v) [B, Hkv, T, 256] bf16, the layout
     of the dense caches (with pos 0 and T a multiple of 64 the caches of gated_attention_prefill_cached); zeros past
     lens, past the table and where a table entry names no page."""
-    return torch.ops.q35.paged_kv_rows(*_four(pages), table, pos, lens, int(T))
+    op = _paged_kv_rows_impl if _direct(pages[0]) else torch.ops.q35.paged_kv_rows
+    return op(*_four(pages), table, pos, lens, int(T))
 
 
 def gated_attention_paged(q, gate, pages, table, pos, cos, sin, *, lens=None, q_norm_w=None, eps=1e-6, scale=None,
@@ -1331,14 +1387,16 @@ def gated_attention_paged(q, gate, pages, table, pos, cos, sin, *, lens=None, q_
     prompt; Hq / Hkv any ratio. Returns [B, T, Hq * 256] in out_dtype (bf16 or fp32), zeros for tokens past lens or the
     table's capacity. splits: over how many blocks a row's keys are dealt (0: by the sizes)."""
     _require(out_dtype in (torch.bfloat16, torch.float32), "out_dtype: bf16 or fp32")
-    return torch.ops.q35.gated_attn_paged(q, gate, *_four(pages), table, pos, lens, cos, sin, q_norm_w, float(eps),
-                                          q.shape[-1] ** -0.5 if scale is None else float(scale), int(splits),
-                                          out_dtype == torch.float32)
+    op = _attn_paged_impl if _direct(q) else torch.ops.q35.gated_attn_paged
+    return op(q, gate, *_four(pages), table, pos, lens, cos, sin, q_norm_w, float(eps),
+              q.shape[-1] ** -0.5 if scale is None else float(scale), int(splits), out_dtype == torch.float32)
 
 
 def _four(pages):
-    _require(len(pages) in (2, 4), "pages: (k, v) or (k, v, k_scale, v_scale)")
-    return pages if len(pages) == 4 else (*pages, None, None)
+    if len(pages) == 4:
+        return pages
+    _require(len(pages) == 2, "pages: (k, v) or (k, v, k_scale, v_scale)")
+    return (*pages, None, None)
 
 
 def verify_drafts(logits, draft_ids, u, *, draft_probs=None, lens=None, temperature=1.0):
@@ -1352,7 +1410,8 @@ def verify_drafts(logits, draft_ids, u, *, draft_probs=None, lens=None, temperat
     draft: the lowest index whose running sum exceeds u[:, K] of the whole. The kept drafts and the drawn token are then
     distributed as draws from p. Returns (n_accept [B] int32, tokens [B, K + 1] int32: kept drafts, drawn token, -1)."""
     ts, t = (temperature, 0.0) if torch.is_tensor(temperature) else (None, float(temperature))
-    return torch.ops.q35.verify_drafts(logits, draft_ids, draft_probs, u, lens, ts, t)
+    op = _verify_drafts_impl if _direct(logits) else torch.ops.q35.verify_drafts
+    return op(logits, draft_ids, draft_probs, u, lens, ts, t)
 
 
 def add_rmsnorm_(x, y, w, eps=1e-6, split=False):

@@ -154,9 +154,10 @@ def test_attention_refusals():
     for kw in (dict(odt=2), dict(dt=4), dict(out=FAKE + 8), dict(q=FAKE + 8), dict(gate=FAKE + 8), dict(gst=2046),
                dict(w=FAKE + 4), dict(rot=68), dict(D=128), dict(Hq=8192), dict(T=1 << 25)):
         assert _attn(**kw) == 2, kw
-    need = q35hip.lib().q35_gated_attn_paged_workspace_bytes(2, 1, 8, 2, 256, 4, 64, 0)
-    assert need == 2 * 8 * 2 * 258 * 4  # two runs of 128 keys
-    assert _attn(wsb=need - 1) == 3 and _attn(ws=None) == 3 and _attn(ws=FAKE + 8) == 3
+    need = q35hip.lib().q35_gated_attn_paged_workspace_bytes(2, 1, 8, 2, 256, 16, 64, 0)
+    assert need == 2 * 8 * 8 * 258 * 4  # eight runs, of 128 keys each
+    assert _attn(nb=16, wsb=need - 1) == 3 and _attn(nb=16, ws=None) == 3 and _attn(nb=16, ws=FAKE + 8) == 3
+    assert _attn(splits=2, wsb=2 * 8 * 2 * 258 * 4 - 1) == 3  # 256 keys asked for in two runs
     assert q35hip.lib().q35_gated_attn_paged_workspace_bytes(2, 1, 8, 3, 256, 4, 64, 0) == 0
 
 
