@@ -103,9 +103,93 @@ __device__ __forceinline__ uint32_t cvt2(float a, float b) {
   const f32x2 v = {a, b};
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
 }
-__device__ __forceinline__ int32_t load_uniform(const int32_t* p) {
-  typedef const __attribute__((address_space(4))) int32_t* cptr;
-  return *(cptr)(uintptr_t)p;
+
+// A row of Q (this lane's four dims, scaled for base-2 exponentials) as column `col` of the scores' B operands: bf16 hi + lo,
+// or fp16 with its power of two in *fac and what the codes' offsets add to each group's product, negated, in off[][col].
+template <bool I4>
+__device__ __forceinline__ void q_store(const f32x4& x, bool there, int lane, int col, u32x4* qf, float (*off)[16],
+                                        float* fac) {
+  if constexpr (I4) {
+    // dim 64 g + 16 a + 8 u + j is step 2 g + u of lane group a; a dword's nibbles leave it in pairs (j, j + 4), those of
+    // odd j times 16
+    int ex = 0;
+    if (there)
+      ex = __builtin_amdgcn_frexp_expf(
+          wave_max(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])))));
+    _Float16* qe = reinterpret_cast<_Float16*>(qf);
+    const int base = ((2 * (lane >> 4) + ((lane >> 1) & 1)) * 64 + 16 * ((lane >> 2) & 3) + col) * 8 + (lane & 1);
+    float o = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const _Float16 hq = (_Float16)ldexpf(x[e], 5 - ex - 4 * (e & 1));
+      qe[base + 2 * e] = hq;
+      o -= (e & 1 ? 1152.f : 1032.f) * (float)hq;
+    }
+    o = add_xor4_quads(add_xor<2>(add_xor<1>(o)));
+    o = add_xor<8>(o);
+    if ((lane & 15) == 0) off[lane >> 4][col] = o;
+    if (lane == 0) *fac = ldexpf(1.f, ex - 5);
+  } else {
+    // dim 32 step + 8 a + j in order
+    __bf16* qe = reinterpret_cast<__bf16*>(qf);
+    const int o = ((lane >> 3) * 64 + 16 * ((lane >> 1) & 3) + col) * 8 + 4 * (lane & 1);
+    bf16x4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bf16_hl hl = bf16_split(x[e]);
+      hi[e] = hl.hi;
+      lo[e] = hl.lo;
+    }
+    *reinterpret_cast<bf16x4*>(qe + o) = hi;
+    *reinterpret_cast<bf16x4*>(qe + 8 * 64 * 8 + o) = lo;
+    if (lane == 0) *fac = 1.f;
+  }
+}
+// A lane's accumulators of its row into o[256], dims in order.
+template <bool I4>
+__device__ __forceinline__ void o_store(const f32x4 (&acc)[16], const float (&corr)[kPgNG], float* o, int a) {
+  if constexpr (I4) {
+#pragma unroll
+    for (int g = 0; g < kPgNG; ++g)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[4 * g + e][r] + corr[g];
+        *reinterpret_cast<f32x4*>(o + 64 * g + 16 * a + 4 * r) = v;
+      }
+  } else {
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[4 * w + e][r];
+        *reinterpret_cast<f32x4*>(o + 128 * (w >> 1) + 8 * (4 * a + r) + 4 * (w & 1)) = v;
+      }
+  }
+}
+__device__ __forceinline__ f32x4 gate_load(const PagedAttnArgs& p, int b, int t, int h, int d0) {
+  if (!p.gate) return zero4();
+  const int64_t o = b * p.gb + t * p.gt + h * p.gh + d0;
+  return p.q_f32 ? load_quad<float>((const float*)p.gate + o) : load_quad<__bf16>((const __bf16*)p.gate + o);
+}
+// out = O / L sigmoid(gate); zeros for a row that sees nothing
+__device__ __forceinline__ void out_store(const PagedAttnArgs& p, const f32x4& O, float L, bool sees, const f32x4& g,
+                                          int b, int t, int h, int d0) {
+  f32x4 v = zero4();
+  if (sees && L != 0.f) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = O[e] / L * (p.gate ? sigmoidf_(g[e]) : 1.f);
+  }
+  const int64_t oi = (((int64_t)b * p.T + t) * p.Hkv * p.G + h) * kPgD + d0;
+  if (p.out_f32) {
+    *reinterpret_cast<f32x4*>((float*)p.out + oi) = v;
+  } else {
+    const bf16x4 w = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+    *reinterpret_cast<bf16x4*>((__bf16*)p.out + oi) = w;
+  }
 }
 
 template <bool I4, int NR>
@@ -283,44 +367,10 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
           if (turns) x[e] = x[e] * cur.co[e] + sg * (cur.px[e] * rr * (1.f + wp[e])) * cur.si[e];
         }
       }
-      const int ti = i >> 4, col = i & 15;
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[e] *= p.scale * 1.4426950408889634f;
-      if constexpr (I4) {
-        // dim 64 g + 16 a + 8 u + j is step 2 g + u of lane group a; a dword's nibbles leave it in pairs (j, j + 4), those
-        // of odd j times 16
-        int ex = 0;
-        if (cur.there)
-          ex = __builtin_amdgcn_frexp_expf(
-              wave_max(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])))));
-        _Float16* qe = reinterpret_cast<_Float16*>(qf + (size_t)ti * QF);
-        const int base = ((2 * (lane >> 4) + ((lane >> 1) & 1)) * 64 + 16 * ((lane >> 2) & 3) + col) * 8 + (lane & 1);
-        float off = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const _Float16 hq = (_Float16)ldexpf(x[e], 5 - ex - 4 * (e & 1));
-          qe[base + 2 * e] = hq;
-          off -= (e & 1 ? 1152.f : 1032.f) * (float)hq;
-        }
-        off = add_xor4_quads(add_xor<2>(add_xor<1>(off)));
-        off = add_xor<8>(off);
-        if ((lane & 15) == 0) qoff[ti][lane >> 4][col] = off;
-        if (lane == 0) qfac[i] = ldexpf(1.f, ex - 5);
-      } else {
-        // dim 32 step + 8 a + j in order
-        __bf16* qe = reinterpret_cast<__bf16*>(qf + (size_t)ti * 2 * QF);
-        const int o = ((lane >> 3) * 64 + 16 * ((lane >> 1) & 3) + col) * 8 + 4 * (lane & 1);
-        bf16x4 hi, lo;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bf16_hl hl = bf16_split(x[e]);
-          hi[e] = hl.hi;
-          lo[e] = hl.lo;
-        }
-        *reinterpret_cast<bf16x4*>(qe + o) = hi;
-        *reinterpret_cast<bf16x4*>(qe + QF * 8 + o) = lo;
-        if (lane == 0) qfac[i] = 1.f;
-      }
+      const int ti = i >> 4;
+      q_store<I4>(x, cur.there, lane, i & 15, qf + (size_t)ti * QP * QF, qoff[ti], &qfac[i]);
     }
   }
 
@@ -655,28 +705,7 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
     }
     lds_barrier();  // Q, or the rows before these, have been used
     if (r0 + 16 * i + c < R) {
-      float* o = ob + ((size_t)wave * 16 + c) * kORow;
-      if constexpr (I4) {
-#pragma unroll
-        for (int g = 0; g < kPgNG; ++g)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            f32x4 v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = acc[i][4 * g + e][r] + corr[i][g];
-            *reinterpret_cast<f32x4*>(o + 64 * g + 16 * a + 4 * r) = v;
-          }
-      } else {
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            f32x4 v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = acc[i][4 * w + e][r];
-            *reinterpret_cast<f32x4*>(o + 128 * (w >> 1) + 8 * (4 * a + r) + 4 * (w & 1)) = v;
-          }
-      }
+      o_store<I4>(acc[i], corr[i], ob + ((size_t)wave * 16 + c) * kORow, a);
       if (a == 0) {
         mls[wave][c][0] = m_run[i];
         mls[wave][c][1] = l;
@@ -707,23 +736,7 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
         *reinterpret_cast<f32x4*>(p.part + slot * kPgD + d0) = O;
         if (lane < 2) p.ml[2 * slot + lane] = lane ? L : M;
       } else {
-        const int64_t oi = (((int64_t)b * p.T + t) * p.Hkv * p.G + h) * kPgD + d0;
-        f32x4 g = zero4();
-        if (p.gate) {
-          const int64_t go = b * p.gb + t * p.gt + h * p.gh + d0;
-          g = p.q_f32 ? load_quad<float>((const float*)p.gate + go) : load_quad<__bf16>((const __bf16*)p.gate + go);
-        }
-        f32x4 v = zero4();
-        if (L != 0.f && keys_seen(p, pos, len, t) > 0) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = O[e] / L * (p.gate ? sigmoidf_(g[e]) : 1.f);
-        }
-        if (p.out_f32) {
-          *reinterpret_cast<f32x4*>((float*)p.out + oi) = v;
-        } else {
-          bf16x4 w = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
-          *reinterpret_cast<bf16x4*>((__bf16*)p.out + oi) = w;
-        }
+        out_store(p, O, L, keys_seen(p, pos, len, t) > 0, gate_load(p, b, t, h, d0), b, t, h, d0);
       }
     }
   }
@@ -759,11 +772,7 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs p) 
     }
   };
   load(wave);
-  f32x4 g = zero4();
-  if (p.gate) {
-    const int64_t go = b * p.gb + t * p.gt + h * p.gh + d0;
-    g = p.q_f32 ? load_quad<float>((const float*)p.gate + go) : load_quad<__bf16>((const __bf16*)p.gate + go);
-  }
+  const f32x4 g = gate_load(p, b, t, h, d0);
   __builtin_amdgcn_sched_barrier(0);
   for (int s0 = wave; s0 < n; s0 += 32) {
     if (s0 != wave) load(s0);
@@ -800,18 +809,7 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs p) 
       for (int e = 0; e < 4; ++e) O[e] += go[w][lane][e] * f;
     }
   }
-  f32x4 v = zero4();
-  if (L != 0.f) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = O[e] / L * (p.gate ? sigmoidf_(g[e]) : 1.f);
-  }
-  const int64_t oi = (((int64_t)b * p.T + t) * p.Hkv * p.G + h) * kPgD + d0;
-  if (p.out_f32) {
-    *reinterpret_cast<f32x4*>((float*)p.out + oi) = v;
-  } else {
-    bf16x4 w = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
-    *reinterpret_cast<bf16x4*>((__bf16*)p.out + oi) = w;
-  }
+  out_store(p, O, L, true, g, b, t, h, d0);
 }
 
 // Query rows per block (in 16s) and runs per row: two blocks per CU, but one where that leaves a block no more than two

@@ -21,6 +21,12 @@ constexpr int kPgD = 256;     // head dim
 constexpr int kPgGroup = 64;  // dims per scale of the 4-bit form
 constexpr int kPgNG = kPgD / kPgGroup;
 
+// A value that a whole wave shares, as a scalar load (of memory that no kernel in flight writes).
+__device__ __forceinline__ int32_t load_uniform(const int32_t* p) {
+  typedef const __attribute__((address_space(4))) int32_t* cptr;
+  return *(cptr)(uintptr_t)p;
+}
+
 struct PagedTable {
   const int32_t* table;
   int64_t ld;
@@ -31,10 +37,9 @@ struct PagedTable {
     const int p = table[(int64_t)b * ld + blk];
     return p >= 0 && p < n_pages ? p : -1;
   }
-  // The same for arguments that a whole wave shares, as a scalar load (the table is not written while it is read).
+  // The same for arguments that a whole wave shares.
   __device__ __forceinline__ int page_uniform(int b, int blk) const {
-    typedef const __attribute__((address_space(4))) int32_t* cptr;
-    const int p = *(cptr)(uintptr_t)(table + (int64_t)b * ld + blk);
+    const int p = load_uniform(table + (int64_t)b * ld + blk);
     return p >= 0 && p < n_pages ? p : -1;
   }
   __device__ __forceinline__ int64_t capacity() const { return (int64_t)n_blocks << shift; }

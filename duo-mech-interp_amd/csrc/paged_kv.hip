@@ -5,9 +5,10 @@
 // values, four dims a lane: the row's sum of squares is one wave sum, a group of 64 dims one row of 16 lanes.
 //   bf16 pages: the arithmetic of attn_prep_kernel (fp32, then one rounding), bit for bit the rows it writes.
 //   4-bit pages: per group s = bf16(fp32(max |x| / 7)), code = 8 + clamp(rint(x / s), -7, 7). A code is a rounding decision, so
-//   norm, rotation and quotient are formed in 64 bits: which code a value gets then depends on the inputs alone and not on
-//   the order of a sum (in 32 bits about one value in 10^6 falls on the other side). fp64 multiply-adds run at the fp32
-//   rate here. A group that holds a value that is not finite gets the scale NaN: it reads back as NaN.
+//   norm, rotation and quotient are those of 64 bits: which code a value gets then depends on the inputs alone and not on
+//   the order of a sum (in 32 bits about one value in 10^6 falls on the other side). They are formed in fp32 first, and
+//   again in 64 bits only where a rounding lies closer to a tie than fp32 can tell (one row of 256 in a hundred): 6144
+//   tokens of two heads XX us against 17 in 64 bits throughout. A group that holds a value that is not finite gets the scale NaN: it reads back as NaN.
 #include "paged_kv.h"
 
 namespace q35 {
@@ -73,6 +74,37 @@ __device__ __forceinline__ uint32_t quantize_quad(const double (&x)[4], __bf16* 
   return q;
 }
 
+// The same from fp32 values, where they settle it: x[e] within 2^-20 of a[e] (at least |x[e]|) of the 64-bit value. Sets
+// *sure false in a lane that finds its scale's or a code's rounding within that error (with 2^-19 taken for it, which also
+// covers the quotient's) of a tie, or a maximum outside 1e-30 .. 1e30.
+__device__ __forceinline__ float row16_max(float v) {
+  v = fmaxf(v, lane_dpp<0xB1>(v));
+  v = fmaxf(v, lane_dpp<0x4E>(v));
+  v = fmaxf(v, lane_dpp<0x141>(v));
+  return fmaxf(v, lane_dpp<0x140>(v));
+}
+__device__ __forceinline__ uint32_t quantize_quad_f32(const f32x4& x, const f32x4& a, bool turned, __bf16* s_out,
+                                                      bool* sure) {
+  const float m = row16_max(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
+  // (what was not rotated is its own bound)
+  const float am = turned ? row16_max(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]))) : m;
+  const float s32 = m * (1.f / 7.f), off = am * (0x1p-19f / 7.f);
+  const __bf16 sb = (__bf16)s32;
+  const float s = (float)sb, inv = __builtin_amdgcn_rcpf(s), wide = inv * 0x1p-19f;
+  float far = 0.f;  // the largest distance from a code, with its error
+  uint32_t q = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float t = x[e] * inv, n = __builtin_rintf(t);
+    far = fmaxf(far, __builtin_fmaf(a[e], wide, fabsf(t - n)));
+    q |= (uint32_t)(__builtin_amdgcn_fmed3f(n, -7.f, 7.f) + 8.f) << (4 * e);
+  }
+  *s_out = sb;
+  const float sum = x[0] + x[1] + x[2] + x[3];  // (a maximum passes over a NaN, a sum does not)
+  *sure = sum == sum && m > 1e-30f && am < 1e30f && far < 0.5f && (float)(__bf16)(s32 - off) == s && (float)(__bf16)(s32 + off) == s;
+  return q;
+}
+
 struct AppendArgs {
   const void *k, *v;
   int64_t kb, kt, kh, vb, vt, vh;
@@ -84,82 +116,92 @@ struct AppendArgs {
   void *kp, *vp;
   __bf16 *ks, *vs;
   int T, Hkv;
-  int64_t jobs;
 };
 
-// Job g = ((b T + t) Hkv + h) 2 + (0: key, 1: value), one wave each.
+// Wave: one token's row of head blockIdx.y / 2, its keys (even blockIdx.y) or values, of row blockIdx.z. What bounds a long
+// prompt is the issue of about 150 vector and 100 scalar instructions a row: several rows a wave, with their loads ahead,
+// measured slower (four: 15.3 us against 13.6 for 6144 tokens of two heads), and so did 64 bits throughout (17).
 template <typename Tin, bool I4>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs p) {
-  const int lane = threadIdx.x & 63;
-  const int64_t g = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (g >= p.jobs) return;
-  const bool val = g & 1;
-  const int64_t th = g >> 1, m = th / p.Hkv;
-  const int h = (int)(th - m * p.Hkv), b = (int)(m / p.T), t = (int)(m - (int64_t)b * p.T);
+  const int lane = threadIdx.x & 63, b = blockIdx.z, h = blockIdx.y >> 1;
+  const int t = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool val = blockIdx.y & 1;
+  const int len = p.lens ? min(load_uniform(p.lens + b), p.T) : p.T;
+  const int64_t at = (int64_t)load_uniform(p.pos + b) + t;
+  if (t >= p.T) return;
   const int d0 = 4 * lane, half = p.rot >> 1;
-  const Tin* src = val ? (const Tin*)p.v + b * p.vb + t * p.vt + h * p.vh
-                       : (const Tin*)p.k + b * p.kb + t * p.kt + h * p.kh;
+  const bool turns = !val && d0 < p.rot;  // lanes past rot keep their values
+  const int pd = !turns ? d0 : d0 < half ? d0 + half : d0 - half;
+  const Tin* src = val ? (const Tin*)p.v + (b * p.vb + h * p.vh + t * p.vt) : (const Tin*)p.k + (b * p.kb + h * p.kh + t * p.kt);
   const f32x4 x = load_quad<Tin>(src + d0);
-  const int64_t at = (int64_t)p.pos[b] + t;
-  if (at < 0 || at >= p.pt.capacity() || (p.lens && t >= p.lens[b])) return;
-  const int page = p.pt.page(b, (int)(at >> p.pt.shift));
-  if (page < 0) return;
-  const int row = (int)at & ((1 << p.pt.shift) - 1);
-  const size_t slot = (((size_t)page * p.Hkv + h) << p.pt.shift) + row;
-
-  // The key's rotation partner and its table row (lanes past rot keep their values)
   f32x4 px = x, wx = zero4(), wp = zero4(), co = zero4(), si = zero4();
-  const bool turns = !val && d0 < p.rot;
-  const float sg = d0 < half ? -1.f : 1.f;
-  if (!val && p.kw) wx = load_quad<float>(p.kw + d0);
-  if (turns) {
-    const int pd = d0 < half ? d0 + half : d0 - half, j = d0 < half ? d0 : d0 - half;
+  if (!val) {
     px = load_quad<Tin>(src + pd);
-    if (p.kw) wp = load_quad<float>(p.kw + pd);
+    if (p.kw) {
+      wx = load_quad<float>(p.kw + d0);
+      wp = load_quad<float>(p.kw + pd);
+    }
+  }
+  if (t >= len || at < 0 || at >= p.pt.capacity()) return;
+  const int page = p.pt.page_uniform(b, (int)(at >> p.pt.shift));
+  if (page < 0) return;
+  if (turns) {
+    const int j = d0 < half ? d0 : d0 - half;
     co = load_quad<float>(p.cos_t + at * half + j);
     si = load_quad<float>(p.sin_t + at * half + j);
   }
-  if constexpr (!I4) {
-    f32x4 r = x;
-    if (!val) {
-      f32x4 xn = x, pn = px;
-      if (p.kw) {
-        const float ss = wave_sum(x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]);
-        const float rr = rsqrtf(ss * (1.f / kPgD) + p.eps);
+  const size_t slot = (((size_t)page * p.Hkv + h) << p.pt.shift) + ((int)at & ((1 << p.pt.shift) - 1));
+  const float sg = d0 < half ? -1.f : 1.f;
+  // in fp32 (what bf16 pages hold, rounded); big: the terms' magnitudes, which bound the error
+  f32x4 r = x, big;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          xn[e] = x[e] * rr * (1.f + wx[e]);
-          pn[e] = px[e] * rr * (1.f + wp[e]);
-        }
-      }
-      r = xn;
-      if (turns) {
+  for (int e = 0; e < 4; ++e) big[e] = fabsf(x[e]);
+  if (!val) {
+    f32x4 xn = x, pn = px;
+    if (p.kw) {
+      const float ss = wave_sum(x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]);
+      const float rr = rsqrtf(ss * (1.f / kPgD) + p.eps);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] = xn[e] * co[e] + sg * pn[e] * si[e];
+      for (int e = 0; e < 4; ++e) {
+        xn[e] = x[e] * rr * (1.f + wx[e]);
+        pn[e] = px[e] * rr * (1.f + wp[e]);
       }
     }
+    r = xn;
+    if (turns) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[e] = xn[e] * co[e] + sg * pn[e] * si[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) big[e] = turns ? fabsf(xn[e]) + fabsf(pn[e]) : fabsf(xn[e]);
+  }
+  if constexpr (!I4) {
     bf16x4 o = {(__bf16)r[0], (__bf16)r[1], (__bf16)r[2], (__bf16)r[3]};
     *reinterpret_cast<bf16x4*>((__bf16*)(val ? p.vp : p.kp) + slot * kPgD + d0) = o;
   } else {
-    double r[4] = {x[0], x[1], x[2], x[3]};
-    if (!val) {
-      double pn[4] = {px[0], px[1], px[2], px[3]};
-      if (p.kw) {
-        const double ss = wave_sum64(r[0] * r[0] + r[1] * r[1] + r[2] * r[2] + r[3] * r[3]);
-        const double rr = 1.0 / sqrt(ss * (1.0 / kPgD) + (double)p.eps);
+    __bf16 s;
+    bool sure;
+    uint32_t q = quantize_quad_f32(r, big, !val && p.rot > 0, &s, &sure);
+    if (__builtin_amdgcn_ballot_w64(!sure) != 0) {
+      double d[4] = {x[0], x[1], x[2], x[3]};
+      if (!val) {
+        double pn[4] = {px[0], px[1], px[2], px[3]};
+        if (p.kw) {
+          const double ss = wave_sum64(d[0] * d[0] + d[1] * d[1] + d[2] * d[2] + d[3] * d[3]);
+          const double rr = 1.0 / sqrt(ss * (1.0 / kPgD) + (double)p.eps);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          r[e] = r[e] * rr * (1.0 + (double)wx[e]);
-          pn[e] = pn[e] * rr * (1.0 + (double)wp[e]);
+          for (int e = 0; e < 4; ++e) {
+            d[e] = d[e] * rr * (1.0 + (double)wx[e]);
+            pn[e] = pn[e] * rr * (1.0 + (double)wp[e]);
+          }
+        }
+        if (turns) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) d[e] = d[e] * (double)co[e] + (double)sg * pn[e] * (double)si[e];
         }
       }
-      if (turns) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] = r[e] * (double)co[e] + (double)sg * pn[e] * (double)si[e];
-      }
+      q = quantize_quad(d, &s);
     }
-    __bf16 s;
-    const uint32_t q = quantize_quad(r, &s);
     char* dst = (char*)(val ? p.vp : p.kp) + slot * (kPgD / 2);
     *reinterpret_cast<uint16_t*>(dst + (val ? v_quad_byte(lane) : k_quad_byte(lane))) = (uint16_t)q;
     if ((lane & 15) == 0) (val ? p.vs : p.ks)[slot * kPgNG + (lane >> 4)] = s;
@@ -173,43 +215,62 @@ struct RowsArgs {
   const int32_t *pos, *lens;
   __bf16 *ko, *vo;
   int T, Hkv;
-  int64_t n;  // threads: B Hkv T rows of keys and of values, 32 threads each
 };
 
-// Thread i: dims 8 m .. 8 m + 7 (m = i % 32) of one row: out row (b Hkv + h) T + t, keys first, then values.
+// Block: 32 tokens of (row b, head h), keys (blockIdx.z 0) or values; thread: dims 8 m .. 8 m + 7 (m = tid % 32) of four of
+// them, all loaded before the first is stored.
 template <bool I4>
 __global__ __launch_bounds__(256) void paged_rows_kernel(RowsArgs p) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= 2 * p.n) return;
-  const bool val = i >= p.n;
-  const int64_t r = (val ? i - p.n : i) >> 5, bh = r / p.T;
-  const int m = (int)(i & 31), t = (int)(r - bh * p.T);
-  const int b = (int)(bh / p.Hkv), h = (int)(bh - (int64_t)b * p.Hkv);
-  u32x4 out = {0, 0, 0, 0};
-  const int64_t at = (int64_t)p.pos[b] + t;
-  if (at >= 0 && at < p.pt.capacity() && (!p.lens || t < p.lens[b])) {
-    const int page = p.pt.page(b, (int)(at >> p.pt.shift));
-    if (page >= 0) {
-      const size_t slot = (((size_t)page * p.Hkv + h) << p.pt.shift) + ((int)at & ((1 << p.pt.shift) - 1));
-      if constexpr (!I4) {
-        out = *reinterpret_cast<const u32x4*>((const __bf16*)(val ? p.vp : p.kp) + slot * kPgD + 8 * m);
-      } else {
-        const char* src = (const char*)(val ? p.vp : p.kp) + slot * (kPgD / 2);
-        uint32_t w;
-        if (val)
-          w = *reinterpret_cast<const uint16_t*>(src + v_quad_byte(2 * m)) |
-              (uint32_t)*reinterpret_cast<const uint16_t*>(src + v_quad_byte(2 * m + 1)) << 16;
-        else
-          w = *reinterpret_cast<const uint32_t*>(src + k_quad_byte(2 * m));
-        const float s = (float)(val ? p.vs : p.ks)[slot * kPgNG + (m >> 3)];
-        bf16x8 o;
+  const int m = threadIdx.x & 31, h = blockIdx.y % p.Hkv, b = blockIdx.y / p.Hkv;
+  const bool val = blockIdx.z;
+  const int len = p.lens ? min(load_uniform(p.lens + b), p.T) : p.T;
+  const int64_t pos = load_uniform(p.pos + b);
+  const int t0 = (int)blockIdx.x * 32 + (threadIdx.x >> 5);
+  const char* src = (const char*)(val ? p.vp : p.kp);
+  const __bf16* scale = val ? p.vs : p.ks;
+  size_t slot[4];
+  bool there[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = (__bf16)((float)((int)(w >> (4 * j) & 15) - 8) * s);
-        out = __builtin_bit_cast(u32x4, o);
-      }
+  for (int u = 0; u < 4; ++u) {
+    const int t = t0 + 8 * u;
+    const int64_t at = pos + t;
+    there[u] = t < len && at >= 0 && at < p.pt.capacity();
+    const int page = there[u] ? p.pt.page(b, (int)(at >> p.pt.shift)) : -1;
+    there[u] = page >= 0;
+    slot[u] = there[u] ? (((size_t)page * p.Hkv + h) << p.pt.shift) + ((int)at & ((1 << p.pt.shift) - 1)) : 0;
+  }
+  u32x4 out[4];
+  if constexpr (!I4) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) out[u] = *reinterpret_cast<const u32x4*>(src + slot[u] * (2 * kPgD) + 16 * m);
+  } else {
+    uint32_t w[4];
+    float s[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const char* row = src + slot[u] * (kPgD / 2);
+      if (val)
+        w[u] = *reinterpret_cast<const uint16_t*>(row + v_quad_byte(2 * m)) |
+               (uint32_t)*reinterpret_cast<const uint16_t*>(row + v_quad_byte(2 * m + 1)) << 16;
+      else
+        w[u] = *reinterpret_cast<const uint32_t*>(row + k_quad_byte(2 * m));
+      s[u] = (float)scale[slot[u] * kPgNG + (m >> 3)];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      bf16x8 o;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] = (__bf16)((float)((int)(w[u] >> (4 * j) & 15) - 8) * s[u]);
+      out[u] = __builtin_bit_cast(u32x4, o);
     }
   }
-  *reinterpret_cast<u32x4*>((val ? p.vo : p.ko) + r * kPgD + 8 * m) = out;
+  __bf16* dst = (val ? p.vo : p.ko) + ((size_t)blockIdx.y * p.T + t0) * kPgD + 8 * m;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const u32x4 zero = {0, 0, 0, 0};
+    if (t0 + 8 * u < p.T)
+      __builtin_nontemporal_store(there[u] ? out[u] : zero, reinterpret_cast<u32x4*>(dst + (size_t)8 * u * kPgD));
+  }
 }
 
 }  // namespace q35
@@ -231,12 +292,10 @@ extern "C" int q35_paged_kv_append(const void* k, int64_t k_sb, int64_t k_st, in
   if (rot < 0 || rot > D || (rot & 1) || (rot > 0 && (!cos || !sin))) return Q35_EINVAL;
   if (rot % 8 || (uintptr_t)k_norm_w & 15 || (rot > 0 && ((uintptr_t)cos | (uintptr_t)sin) & 15))
     return Q35_EUNSUPPORTED;
-  const int64_t jobs = B * T * Hkv * 2;
-  if ((jobs + 3) / 4 > 0x7fffffff) return Q35_EUNSUPPORTED;
   const AppendArgs a{k,     v,    k_sb,    k_st,    k_sh,          v_sb,          v_st,   v_sh,     k_norm_w, cos, sin, eps,
                      (int)rot, {table, ld_table, (int)n_blocks, (int)n_pages, shift}, pos, lens, k_pages, v_pages,
-                     (__bf16*)k_scale, (__bf16*)v_scale, (int)T, (int)Hkv, jobs};
-  const dim3 grid((unsigned)((jobs + 3) / 4)), block(256);
+                     (__bf16*)k_scale, (__bf16*)v_scale, (int)T, (int)Hkv};
+  const dim3 grid((unsigned)((T + 3) / 4), (unsigned)(2 * Hkv), (unsigned)B), block(256);
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (dtype == Q35_F32) {
     if (fmt == Q35_BF16) hipLaunchKernelGGL((paged_append_kernel<float, false>), grid, block, 0, st, a);
@@ -259,12 +318,11 @@ extern "C" int q35_paged_kv_rows(const void* k_pages, const void* v_pages, const
   if (chk != Q35_OK) return chk;
   if (!k_out || !v_out) return Q35_EINVAL;
   if (((uintptr_t)k_out | (uintptr_t)v_out) & 15) return Q35_EUNSUPPORTED;
-  const int64_t n = B * Hkv * T * 32;
-  if ((2 * n + 255) / 256 > 0x7fffffff) return Q35_EUNSUPPORTED;
+  if (B * Hkv > 65535) return Q35_EUNSUPPORTED;
   const RowsArgs a{k_pages, v_pages, (const __bf16*)k_scale, (const __bf16*)v_scale,
                    {table, ld_table, (int)n_blocks, (int)n_pages, shift}, pos, lens, (__bf16*)k_out, (__bf16*)v_out,
-                   (int)T, (int)Hkv, n};
-  const dim3 grid((unsigned)((2 * n + 255) / 256)), block(256);
+                   (int)T, (int)Hkv};
+  const dim3 grid((unsigned)((T + 31) / 32), (unsigned)(B * Hkv), 2), block(256);
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (fmt == Q35_BF16) hipLaunchKernelGGL(paged_rows_kernel<false>, grid, block, 0, st, a);
   else hipLaunchKernelGGL(paged_rows_kernel<true>, grid, block, 0, st, a);
