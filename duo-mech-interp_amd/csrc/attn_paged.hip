@@ -88,14 +88,6 @@ __device__ __forceinline__ float scale_of(const u32x4 (&s)[2], int r, int g) {
   return g & 1 ? bf16hi(w) : bf16lo(w);
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-  v = fmaxf(v, lane_dpp<0xB1>(v));
-  v = fmaxf(v, lane_dpp<0x4E>(v));
-  v = fmaxf(v, lane_dpp<0x141>(v));
-  v = fmaxf(v, lane_dpp<0x140>(v));
-  const lane_pair q = lane_swap<16>(v);
-  return max_xor32(fmaxf(q.a, q.b));
-}
 __device__ __forceinline__ f32x4 mfma16h(const u32x4& a, const f16x8& b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), b, c, 0, 0, 0);
 }
@@ -115,7 +107,7 @@ __device__ __forceinline__ void q_store(const f32x4& x, bool there, int lane, in
     int ex = 0;
     if (there)
       ex = __builtin_amdgcn_frexp_expf(
-          wave_max(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])))));
+          wave_max_f32(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])))));
     _Float16* qe = reinterpret_cast<_Float16*>(qf);
     const int base = ((2 * (lane >> 4) + ((lane >> 1) & 1)) * 64 + 16 * ((lane >> 2) & 3) + col) * 8 + (lane & 1);
     float o = 0.f;

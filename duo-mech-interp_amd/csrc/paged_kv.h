@@ -21,12 +21,6 @@ constexpr int kPgD = 256;     // head dim
 constexpr int kPgGroup = 64;  // dims per scale of the 4-bit form
 constexpr int kPgNG = kPgD / kPgGroup;
 
-// A value that a whole wave shares, as a scalar load (of memory that no kernel in flight writes).
-__device__ __forceinline__ int32_t load_uniform(const int32_t* p) {
-  typedef const __attribute__((address_space(4))) int32_t* cptr;
-  return *(cptr)(uintptr_t)p;
-}
-
 struct PagedTable {
   const int32_t* table;
   int64_t ld;

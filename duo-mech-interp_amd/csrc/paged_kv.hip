@@ -13,34 +13,6 @@
 
 namespace q35 {
 
-// The value of the lane that DPP control CTRL names, for 64-bit values.
-template <int CTRL> __device__ __forceinline__ double dpp64(double v) {
-  const u32x2 w = __builtin_bit_cast(u32x2, v);
-  u32x2 r;
-  r.x = __builtin_amdgcn_mov_dpp(w.x, CTRL, 0xF, 0xF, false);
-  r.y = __builtin_amdgcn_mov_dpp(w.y, CTRL, 0xF, 0xF, false);
-  return __builtin_bit_cast(double, r);
-}
-template <int OFF> __device__ __forceinline__ double swap_add64(double v) {
-  const u32x2 w = __builtin_bit_cast(u32x2, v);
-  const auto lo = OFF == 32 ? __builtin_amdgcn_permlane32_swap(w.x, w.x, false, false)
-                            : __builtin_amdgcn_permlane16_swap(w.x, w.x, false, false);
-  const auto hi = OFF == 32 ? __builtin_amdgcn_permlane32_swap(w.y, w.y, false, false)
-                            : __builtin_amdgcn_permlane16_swap(w.y, w.y, false, false);
-  u32x2 a, b;
-  a.x = lo[0];
-  a.y = hi[0];
-  b.x = lo[1];
-  b.y = hi[1];
-  return __builtin_bit_cast(double, a) + __builtin_bit_cast(double, b);
-}
-__device__ __forceinline__ double wave_sum64(double v) {
-  v += dpp64<0xB1>(v);
-  v += dpp64<0x4E>(v);
-  v += dpp64<0x141>(v);
-  v += dpp64<0x140>(v);
-  return swap_add64<32>(swap_add64<16>(v));
-}
 __device__ __forceinline__ double row16_max64(double v) {
   v = fmax(v, dpp64<0xB1>(v));
   v = fmax(v, dpp64<0x4E>(v));
@@ -77,17 +49,11 @@ __device__ __forceinline__ uint32_t quantize_quad(const double (&x)[4], __bf16* 
 // The same from fp32 values, where they settle it: x[e] within 2^-20 of a[e] (at least |x[e]|) of the 64-bit value. Sets
 // *sure false in a lane that finds its scale's or a code's rounding within that error (with 2^-19 taken for it, which also
 // covers the quotient's) of a tie, or a maximum outside 1e-30 .. 1e30.
-__device__ __forceinline__ float row16_max(float v) {
-  v = fmaxf(v, lane_dpp<0xB1>(v));
-  v = fmaxf(v, lane_dpp<0x4E>(v));
-  v = fmaxf(v, lane_dpp<0x141>(v));
-  return fmaxf(v, lane_dpp<0x140>(v));
-}
 __device__ __forceinline__ uint32_t quantize_quad_f32(const f32x4& x, const f32x4& a, bool turned, __bf16* s_out,
                                                       bool* sure) {
-  const float m = row16_max(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
+  const float m = row16_max_f32(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
   // (what was not rotated is its own bound)
-  const float am = turned ? row16_max(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]))) : m;
+  const float am = turned ? row16_max_f32(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]))) : m;
   const float s32 = m * (1.f / 7.f), off = am * (0x1p-19f / 7.f);
   const __bf16 sb = (__bf16)s32;
   const float s = (float)sb, inv = __builtin_amdgcn_rcpf(s), wide = inv * 0x1p-19f;

@@ -137,6 +137,12 @@ __device__ __forceinline__ float softplus_f(float x) { return x > 20.f ? x : log
 // The "memory" clobber keeps the compiler from moving memory accesses across it.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// A value that a whole wave shares, as a scalar load (of memory that no kernel in flight writes).
+__device__ __forceinline__ int32_t load_uniform(const int32_t* p) {
+  typedef const __attribute__((address_space(4))) int32_t* cptr;
+  return *(cptr)(uintptr_t)p;
+}
+
 // Lane exchanges on the vector ALU: DPP within rows of 16 lanes, the row swaps of gfx950 across rows. __shfl_xor goes
 // through LDS (ds_bpermute), one round trip of the LDS pipe per step of a reduction. The sums are bitwise those of the
 // xor butterflies they replace. Measured: gate/up GEMV at 3 rows 6.2 -> 6.1 us, attention prefill at 4096 tokens (two
@@ -181,6 +187,45 @@ __device__ __forceinline__ float wave_sum(float v) {
   v += lane_dpp<0x124>(v);
   v = add_xor<2>(v);
   return add_xor<1>(v);
+}
+
+// The same exchanges for 64-bit values: their halves move separately.
+template <int CTRL> __device__ __forceinline__ double dpp64(double v) {
+  const u32x2 w = __builtin_bit_cast(u32x2, v);
+  u32x2 r;
+  r.x = __builtin_amdgcn_mov_dpp(w.x, CTRL, 0xF, 0xF, false);
+  r.y = __builtin_amdgcn_mov_dpp(w.y, CTRL, 0xF, 0xF, false);
+  return __builtin_bit_cast(double, r);
+}
+template <int OFF> __device__ __forceinline__ double swap_add64(double v) {
+  static_assert(OFF == 16 || OFF == 32, "row swaps");
+  const u32x2 w = __builtin_bit_cast(u32x2, v);
+  const auto lo = OFF == 32 ? __builtin_amdgcn_permlane32_swap(w.x, w.x, false, false)
+                            : __builtin_amdgcn_permlane16_swap(w.x, w.x, false, false);
+  const auto hi = OFF == 32 ? __builtin_amdgcn_permlane32_swap(w.y, w.y, false, false)
+                            : __builtin_amdgcn_permlane16_swap(w.y, w.y, false, false);
+  const u32x2 a = {lo[0], hi[0]}, b = {lo[1], hi[1]};
+  return __builtin_bit_cast(double, a) + __builtin_bit_cast(double, b);
+}
+// Sum over the wave: quads, halves of a row, rows, then the rows.
+__device__ __forceinline__ double wave_sum64(double v) {
+  v += dpp64<0xB1>(v);
+  v += dpp64<0x4E>(v);
+  v += dpp64<0x141>(v);
+  v += dpp64<0x140>(v);
+  return swap_add64<32>(swap_add64<16>(v));
+}
+// Maximum over the 16 lanes of a row, and over the wave.
+__device__ __forceinline__ float row16_max_f32(float v) {
+  v = fmaxf(v, lane_dpp<0xB1>(v));
+  v = fmaxf(v, lane_dpp<0x4E>(v));
+  v = fmaxf(v, lane_dpp<0x141>(v));
+  return fmaxf(v, lane_dpp<0x140>(v));
+}
+__device__ __forceinline__ float wave_max_f32(float v) {
+  v = row16_max_f32(v);
+  const lane_pair q = lane_swap<16>(v);
+  return max_xor32(fmaxf(q.a, q.b));
 }
 
 }  // namespace q35

@@ -47,12 +47,12 @@ struct VerifyArgs {
 };
 
 __device__ __forceinline__ int v_len(const VerifyArgs& p, int b) {
-  return p.lens ? min(max(p.lens[b], 0), p.K) : p.K;
+  return p.lens ? min(max(load_uniform(p.lens + b), 0), p.K) : p.K;
 }
-// 1 / temperature, 0 for the argmax
+// log2(e) / temperature, 0 for the argmax
 __device__ __forceinline__ double v_inv_temp(const VerifyArgs& p, int b) {
-  const float t = p.temps ? p.temps[b] : p.temp;
-  return t > 0.f ? 1.0 / (double)t : 0.0;
+  const float t = p.temps ? __int_as_float(load_uniform(reinterpret_cast<const int32_t*>(p.temps) + b)) : p.temp;
+  return t > 0.f ? 1.4426950408889634074 / (double)t : 0.0;
 }
 // The position's draft when it is a token, else -1
 __device__ __forceinline__ int v_draft(const VerifyArgs& p, int b, int i, int len) {
@@ -61,44 +61,32 @@ __device__ __forceinline__ int v_draft(const VerifyArgs& p, int b, int i, int le
   return id >= 0 && id < p.V ? id : -1;
 }
 
-// e^t for t <= 0 to 2e-14 relative: t = n ln 2 + r with |r| <= ln 2 / 2 (ln 2 in two parts, the first with trailing zeros,
-// so that n times it is exact), the Taylor series of e^r to r^11 (the rest is below r^12 / 12! = 6e-15). 17 operations of
-// 64 bits against about 45 of the library's full-range exp: the chunk sums of 160 positions of 151,936 tokens 40.6 -> 34.9 us.
-__device__ __forceinline__ double exp_neg(double t) {
-  t = fmax(t, -800.0);  // 0 from there on, also for -inf
-  const double n = __builtin_rint(t * 1.4426950408889634);
-  double r = __builtin_fma(-n, 0x1.62e42fefa0000p-1, t);
-  r = __builtin_fma(-n, 0x1.cf79abc9e3b3ap-40, r);
-  double e = 1.0 / 39916800.0;
-  e = __builtin_fma(e, r, 1.0 / 3628800.0);
-  e = __builtin_fma(e, r, 1.0 / 362880.0);
-  e = __builtin_fma(e, r, 1.0 / 40320.0);
-  e = __builtin_fma(e, r, 1.0 / 5040.0);
-  e = __builtin_fma(e, r, 1.0 / 720.0);
-  e = __builtin_fma(e, r, 1.0 / 120.0);
-  e = __builtin_fma(e, r, 1.0 / 24.0);
-  e = __builtin_fma(e, r, 1.0 / 6.0);
-  e = __builtin_fma(e, r, 0.5);
-  e = __builtin_fma(e, r, 1.0);
-  e = __builtin_fma(e, r, 1.0);
+// 2^y for y <= 0 to 1e-11 relative: y = n + f with |f| <= 1/2, the Taylor series of 2^f = e^(f ln 2) to f^9 (the rest is
+// below (ln 2 / 2)^10 / 10! = 7e-12; y's own rounding adds 2^-53 |y|). 14 operations of 64 bits; the library's full-range exp
+// takes 45.
+__device__ __forceinline__ double exp2_neg(double y) {
+  constexpr double L = 0.69314718055994530942, L2 = L * L, L4 = L2 * L2, L8 = L4 * L4;
+  y = fmax(y, -1100.0);  // 0 from there on, also for -inf
+  const double n = __builtin_rint(y), f = y - n;
+  double e = L8 * L / 362880.0;
+  e = __builtin_fma(e, f, L8 / 40320.0);
+  e = __builtin_fma(e, f, L4 * L2 * L / 5040.0);
+  e = __builtin_fma(e, f, L4 * L2 / 720.0);
+  e = __builtin_fma(e, f, L4 * L / 120.0);
+  e = __builtin_fma(e, f, L4 / 24.0);
+  e = __builtin_fma(e, f, L2 * L / 6.0);
+  e = __builtin_fma(e, f, L2 / 2.0);
+  e = __builtin_fma(e, f, L);
+  e = __builtin_fma(e, f, 1.0);
   return __builtin_ldexp(e, (int)n);
 }
-// exp((x - m) / T): 1 at the maximum (also an infinite one), 0 for NaN
+// exp((x - m) / T) for x <= m (no NaN), inv_t = log2(e) / T: 1 at the maximum, also an infinite one.
 __device__ __forceinline__ double v_weight(float x, float m, double inv_t) {
-  const double e = exp_neg(((double)x - (double)m) * inv_t);
-  return x == m ? 1.0 : x < m ? e : 0.0;
+  return x == m ? 1.0 : exp2_neg(((double)x - (double)m) * inv_t);
 }
+// A NaN counts as -inf.
+__device__ __forceinline__ float v_clean(float x) { return fmaxf(x, -INFINITY); }
 
-__device__ __forceinline__ double wave_sum_f64(double v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  return v;
-}
-__device__ __forceinline__ float wave_max_f32(float v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-  return v;
-}
 __device__ __forceinline__ int wave_min_i32(int v) {
 #pragma unroll
   for (int o = 32; o; o >>= 1) v = min(v, __shfl_xor(v, o));
@@ -141,7 +129,10 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs p) {
   __shared__ double ss[4];
   float m = -INFINITY;
 #pragma unroll
-  for (int k = 0; k < kVPer; ++k) m = fmaxf(m, x[k]);
+  for (int k = 0; k < kVPer; ++k) {
+    x[k] = v_clean(x[k]);
+    m = fmaxf(m, x[k]);
+  }
   m = wave_max_f32(m);
   if (lane == 0) sm[wave] = m;
   __syncthreads();
@@ -149,12 +140,19 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs p) {
   int idx = 0x7fffffff;
   double s = 0.0;
   if (inv_t > 0.0) {
+    if (draft >= base && draft < base + kVChunk) {  // the draft's weight is no part of its chunk's sum
 #pragma unroll
-    for (int k = 0; k < kVPer; ++k) {
-      const double w = v_weight(x[k], m, inv_t);
-      s += v_index(base, tid, k) == draft ? 0.0 : w;
+      for (int k = 0; k < kVPer; ++k)
+        if (v_index(base, tid, k) == draft) x[k] = -INFINITY;
     }
-    s = wave_sum_f64(s);
+    if (fabsf(m) < INFINITY) {
+#pragma unroll
+      for (int k = 0; k < kVPer; ++k) s += exp2_neg(((double)x[k] - (double)m) * inv_t);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kVPer; ++k) s += x[k] == m ? 1.0 : 0.0;
+    }
+    s = wave_sum64(s);
   } else {
 #pragma unroll
     for (int k = kVPer - 1; k >= 0; --k)
@@ -172,44 +170,59 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs p) {
   }
 }
 
-// The chunks of each position of row b folded, one wave per position in turn: the maximum, its index, 1 / sum, and
-// whether the draft is kept. Returns n once every thread has them.
+// The chunks of each position of row b folded: the maximum, its index, 1 / sum, and whether the draft is kept. The chunks
+// of as many positions as fit are fetched together with the positions' drafts and what is asked of those, then one wave
+// folds a position. Returns n once every thread has them.
+constexpr int kVFold = 1024;  // chunks held at a time, and the most that a position may have
 struct VFold {
+  VStat st[kVFold];
   double inv_z[kVMaxK + 1];
-  float max[kVMaxK + 1];
-  int idx[kVMaxK + 1], keep[kVMaxK + 1];
+  float max[kVMaxK + 1], x[kVMaxK + 1], q[kVMaxK + 1], u[kVMaxK + 1];
+  int idx[kVMaxK + 1], keep[kVMaxK + 1], draft[kVMaxK + 1];
 };
-__device__ __forceinline__ int v_fold(const VerifyArgs& p, int b, int len, double inv_t, int lane, int wave, int waves,
-                                      VFold& f) {
-  for (int i = wave; i <= len; i += waves) {
-    const VStat* st = p.st + ((size_t)b * (p.K + 1) + i) * p.C;
-    const int draft = v_draft(p, b, i, len);
-    const float xd = draft >= 0 ? p.x[b * p.xb + i * p.xp + draft] : -INFINITY;
-    const double q = draft >= 0 && p.q ? (double)p.q[b * p.qb + i * p.qp + draft] : 1.0;
-    const float u = i < len ? p.u[b * p.ub + i] : 0.f;
-    float M = -INFINITY;
-    for (int k = lane; k < p.C; k += 64) M = fmaxf(M, st[k].max);
-    M = wave_max_f32(M);
-    double z = 0.0;
-    int idx = 0x7fffffff;
-    for (int k = lane; k < p.C; k += 64) {
-      const VStat s = st[k];
-      if (s.max > -INFINITY) z += s.sum * v_weight(s.max, M, inv_t);
-      if (s.max == M) idx = min(idx, s.idx);
-    }
-    z = wave_sum_f64(z);
-    idx = wave_min_i32(idx);
-    const double wd = draft >= 0 && M > -INFINITY ? v_weight(xd, M, inv_t) : 0.0;
-    z += wd;
-    if (lane == 0) {
-      const double pr = inv_t > 0.0 ? wd / z : draft == idx ? 1.0 : 0.0;
-      f.inv_z[i] = 1.0 / z;
-      f.max[i] = M;
-      f.idx[i] = idx;
-      f.keep[i] = draft >= 0 && M > -INFINITY && (double)u * q < pr;
-    }
+template <int THREADS>
+__device__ __forceinline__ int v_fold(const VerifyArgs& p, int b, int len, double inv_t, int tid, VFold& f) {
+  const int lane = tid & 63, wave = tid >> 6, per = max(kVFold / p.C, 1);
+  if (tid < p.K) {  // (whether the row has this position is known later than its draft)
+    const int id = p.ids[b * p.idb + tid];
+    const bool token = id >= 0 && id < p.V;
+    f.x[tid] = token ? v_clean(p.x[b * p.xb + tid * p.xp + id]) : -INFINITY;
+    f.q[tid] = token && p.q ? p.q[b * p.qb + tid * p.qp + id] : 1.f;
+    f.u[tid] = p.u[b * p.ub + tid];
+    f.draft[tid] = token ? id : -1;
   }
-  __syncthreads();
+  for (int i0 = 0; i0 <= len; i0 += per) {
+    const int n = min(per, len + 1 - i0);
+    const VStat* src = p.st + ((size_t)b * (p.K + 1) + i0) * p.C;
+    for (int k = tid; k < n * p.C; k += THREADS) f.st[k] = src[k];
+    __syncthreads();
+    for (int j = wave; j < n; j += THREADS / 64) {
+      const int i = i0 + j, draft = i < len ? f.draft[i] : -1;
+      const VStat* st = f.st + j * p.C;
+      float M = -INFINITY;
+      for (int k = lane; k < p.C; k += 64) M = fmaxf(M, st[k].max);
+      M = wave_max_f32(M);
+      double z = 0.0;
+      int idx = 0x7fffffff;
+      for (int k = lane; k < p.C; k += 64) {
+        const VStat s = st[k];
+        if (s.max > -INFINITY) z += s.sum * v_weight(s.max, M, inv_t);
+        if (s.max == M) idx = min(idx, s.idx);
+      }
+      z = wave_sum64(z);
+      if (!(inv_t > 0.0)) idx = wave_min_i32(idx);
+      const double wd = draft >= 0 && M > -INFINITY ? v_weight(f.x[i], M, inv_t) : 0.0;
+      z += wd;
+      if (lane == 0) {
+        const double pr = inv_t > 0.0 ? wd / z : draft == idx ? 1.0 : 0.0;
+        f.inv_z[i] = 1.0 / z;
+        f.max[i] = M;
+        f.idx[i] = idx;
+        f.keep[i] = draft >= 0 && M > -INFINITY && (double)f.u[i] * (double)f.q[i] < pr;
+      }
+    }
+    __syncthreads();
+  }
   int n = 0;
   while (n < len && f.keep[n]) ++n;
   return n;
@@ -221,7 +234,7 @@ __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs p) {
   const double inv_t = v_inv_temp(p, b);
   if (!(inv_t > 0.0) || len == 0) return;
   __shared__ VFold f;
-  const int n = v_fold(p, b, len, inv_t, lane, wave, 4, f);
+  const int n = v_fold<256>(p, b, len, inv_t, tid, f);
   const float M = f.max[n];
   if (n == len || !(M > -INFINITY)) return;  // nothing was refused: the draw takes the chunks' own sums
   const double inv_z = f.inv_z[n];
@@ -230,8 +243,8 @@ __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs p) {
   v_load_chunk(p.q + b * p.qb + n * p.qp, base, p.V, tid, q, 0.f);
   double s = 0.0;
 #pragma unroll
-  for (int k = 0; k < kVPer; ++k) s += fmax(v_weight(x[k], M, inv_t) * inv_z - (double)q[k], 0.0);
-  s = wave_sum_f64(s);
+  for (int k = 0; k < kVPer; ++k) s += fmax(v_weight(v_clean(x[k]), M, inv_t) * inv_z - (double)q[k], 0.0);
+  s = wave_sum64(s);
   __shared__ double ss[4];
   if (lane == 0) ss[wave] = s;
   __syncthreads();
@@ -243,66 +256,74 @@ __global__ __launch_bounds__(1024) void verify_draw_kernel(VerifyArgs p) {
   const int len = v_len(p, b);
   const double inv_t = v_inv_temp(p, b);
   __shared__ VFold f;
-  __shared__ double pre[16], s_target;
-  __shared__ int s_chunk, s_kind, s_token, s_last;
+  __shared__ double pre[16], chunk_w[kVFold];
+  __shared__ int s_token, s_last;
   const float us = p.u[b * p.ub + p.K];
-  const int n = v_fold(p, b, len, inv_t, lane, wave, 16, f);
+  const int n = v_fold<1024>(p, b, len, inv_t, tid, f);
   const float M = f.max[n];
   const bool refused = n < len;
-  const int draft = v_draft(p, b, n, len);
+  const int draft = refused ? f.draft[n] : -1;
   int token = M > -INFINITY ? f.idx[n] : 0;
   if (inv_t > 0.0 && M > -INFINITY) {
     const double inv_z = f.inv_z[n];
     const VStat* st = p.st + ((size_t)b * (p.K + 1) + n) * p.C;
-    // Weight of chunk k: kind 0 max(p - q, 0), kind 1 p without the draft, kind 2 p
-    auto weight = [&](int k, int kind) -> double {
-      if (kind == 0) return p.mass[(size_t)b * p.C + k];
-      const VStat s = st[k];
-      double w = s.max > -INFINITY ? s.sum * v_weight(s.max, M, inv_t) : 0.0;
-      if (kind == 2 && draft >= 0 && k == draft / kVChunk) w += v_weight(p.x[b * p.xb + n * p.xp + draft], M, inv_t);
-      return w * inv_z;
+    // Weight of each chunk into LDS: kind 0 of max(p - q, 0), kind 1 of p without the draft, kind 2 of p
+    const bool here = (len + 1) * p.C <= kVFold;  // the position's chunks are still in LDS
+    auto weights = [&](int kind) {
+      for (int k = tid; k < p.C; k += 1024) {
+        double w;
+        if (kind == 0) {
+          w = p.mass[(size_t)b * p.C + k];
+        } else {
+          const VStat s = here ? f.st[n * p.C + k] : st[k];
+          w = s.max > -INFINITY ? s.sum * v_weight(s.max, M, inv_t) : 0.0;
+          if (kind == 2 && draft >= 0 && k == draft / kVChunk) w += v_weight(f.x[n], M, inv_t);
+          w *= inv_z;
+        }
+        chunk_w[k] = w;
+      }
+      __syncthreads();
     };
-    if (wave == 0) {
-      int kind = !refused ? 2 : p.q ? 0 : 1;
-      double tot = 0.0;
-      for (int k0 = 0; k0 < p.C; k0 += 64) tot += wave_sum_f64(k0 + lane < p.C ? weight(k0 + lane, kind) : 0.0);
-      if (!(tot > 0.0)) {  // nothing is left behind the refusal (q = p to the last bit): p itself
-        kind = 2;
-        tot = 0.0;
-        for (int k0 = 0; k0 < p.C; k0 += 64) tot += wave_sum_f64(k0 + lane < p.C ? weight(k0 + lane, kind) : 0.0);
-      }
-      const double target = (double)us * tot;
-      double run = 0.0, before = 0.0;
-      int chunk = -1, last = 0;
-      for (int k0 = 0; k0 < p.C && chunk < 0; k0 += 64) {
-        const double w = k0 + lane < p.C ? weight(k0 + lane, kind) : 0.0;
-        double inc = w;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-          const double v = __shfl_up(inc, o);
-          if (lane >= o) inc += v;
-        }
-        const unsigned long long over = __builtin_amdgcn_ballot_w64(w > 0.0 && run + inc > target);
-        const unsigned long long some = __builtin_amdgcn_ballot_w64(w > 0.0);
-        if (some) last = k0 + 63 - __builtin_clzll(some);
-        if (over) {
-          const int l = __builtin_ctzll(over);
-          chunk = k0 + l;
-          before = run + __shfl(inc - w, l);
-        }
-        run += __shfl(inc, 63);
-      }
-      if (lane == 0) {
-        s_chunk = chunk >= 0 ? chunk : last;
-        s_target = chunk >= 0 ? target - before : INFINITY;  // in no chunk: the last token with weight
-        s_kind = kind;
-        s_token = 0x7fffffff;
-        s_last = 0;
-      }
+    int kind = !refused ? 2 : p.q ? 0 : 1;
+    weights(kind);
+    double tot = 0.0;
+    for (int k0 = 0; k0 < p.C; k0 += 64) tot += wave_sum64(k0 + lane < p.C ? chunk_w[k0 + lane] : 0.0);
+    if (!(tot > 0.0)) {  // (the same for all waves) nothing is left behind the refusal, q = p to the last bit: p itself
+      kind = 2;
+      __syncthreads();
+      weights(kind);
+      tot = 0.0;
+      for (int k0 = 0; k0 < p.C; k0 += 64) tot += wave_sum64(k0 + lane < p.C ? chunk_w[k0 + lane] : 0.0);
     }
-    __syncthreads();
+    // every wave finds the chunk
+    const double all = (double)us * tot;
+    double run = 0.0, before = 0.0;
+    int chunk = -1, last_chunk = 0;
+    for (int k0 = 0; k0 < p.C && chunk < 0; k0 += 64) {
+      const double w = k0 + lane < p.C ? chunk_w[k0 + lane] : 0.0;
+      double inc = w;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const double v = __shfl_up(inc, o);
+        if (lane >= o) inc += v;
+      }
+      const unsigned long long over = __builtin_amdgcn_ballot_w64(w > 0.0 && run + inc > all);
+      const unsigned long long some = __builtin_amdgcn_ballot_w64(w > 0.0);
+      if (some) last_chunk = k0 + 63 - __builtin_clzll(some);
+      if (over) {
+        const int l = __builtin_ctzll(over);
+        chunk = k0 + l;
+        before = run + __shfl(inc - w, l);
+      }
+      run += __shfl(inc, 63);
+    }
+    const double target = chunk >= 0 ? all - before : INFINITY;  // in no chunk: the last token with weight
+    if (tid == 0) {
+      s_token = 0x7fffffff;
+      s_last = 0;
+    }
     constexpr int PER = kVChunk / 1024;
-    const int base = s_chunk * kVChunk + tid * PER, kind = s_kind;
+    const int base = (chunk >= 0 ? chunk : last_chunk) * kVChunk + tid * PER;
     const float* xr = p.x + b * p.xb + n * p.xp;
     const float* qr = kind == 0 ? p.q + b * p.qb + n * p.qp : nullptr;
     double w[PER], sum = 0.0;
@@ -310,7 +331,7 @@ __global__ __launch_bounds__(1024) void verify_draw_kernel(VerifyArgs p) {
     float xv[PER], qv[PER];
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      xv[k] = base + k < p.V ? xr[base + k] : -INFINITY;
+      xv[k] = base + k < p.V ? v_clean(xr[base + k]) : -INFINITY;
       qv[k] = kind == 0 && base + k < p.V ? qr[base + k] : 0.f;
     }
 #pragma unroll
@@ -331,9 +352,8 @@ __global__ __launch_bounds__(1024) void verify_draw_kernel(VerifyArgs p) {
     }
     if (lane == 63) pre[wave] = inc;
     __syncthreads();
-    double run = inc - sum;
+    run = inc - sum;
     for (int k = 0; k < wave; ++k) run += pre[k];
-    const double target = s_target;
     int hit = 0x7fffffff;
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
@@ -356,7 +376,7 @@ static int64_t v_chunks(int64_t V) { return (V + kVChunk - 1) / kVChunk; }
 
 extern "C" size_t q35_verify_drafts_workspace_bytes(int64_t B, int64_t K, int64_t V) {
   using namespace q35;
-  if (B <= 0 || K < 0 || V <= 0 || B > 65535 || K > kVMaxK || V > 0x7fff0000 || B * (K + 1) > 65535) return 0;
+  if (B <= 0 || K < 0 || V <= 0 || B > 65535 || K > kVMaxK || V > (int64_t)kVFold * kVChunk || B * (K + 1) > 65535) return 0;
   const size_t C = v_chunks(V);
   return (size_t)B * (K + 1) * C * sizeof(VStat) + (size_t)B * C * sizeof(double);
 }
