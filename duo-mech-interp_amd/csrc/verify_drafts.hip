@@ -228,6 +228,8 @@ __device__ __forceinline__ int v_fold(const VerifyArgs& p, int b, int len, doubl
   return n;
 }
 
+// (One chunk a block, each with a fold of its own: four chunks to a block of 1024 threads that share one measured 19.4 us
+// against 13.5 for 32 rows of up to eight drafts.)
 __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int c = blockIdx.x, b = blockIdx.y, len = v_len(p, b), base = c * kVChunk;
@@ -328,12 +330,22 @@ __global__ __launch_bounds__(1024) void verify_draw_kernel(VerifyArgs p) {
     const float* qr = kind == 0 ? p.q + b * p.qb + n * p.qp : nullptr;
     double w[PER], sum = 0.0;
     int last = -1;
-    float xv[PER], qv[PER];
+    float xv[PER], qv[PER] = {0.f, 0.f, 0.f, 0.f};
+    static_assert(PER == 4, "one vector a thread");
+    auto quad = [&](const float* row, float fill, float (&v)[PER]) {
+      if (base + PER <= p.V && ((uintptr_t)row & 15) == 0) {
+        const f32x4 w = *reinterpret_cast<const f32x4*>(row + base);
 #pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      xv[k] = base + k < p.V ? v_clean(xr[base + k]) : -INFINITY;
-      qv[k] = kind == 0 && base + k < p.V ? qr[base + k] : 0.f;
-    }
+        for (int k = 0; k < PER; ++k) v[k] = w[k];
+      } else {
+#pragma unroll
+        for (int k = 0; k < PER; ++k) v[k] = base + k < p.V ? row[base + k] : fill;
+      }
+    };
+    quad(xr, -INFINITY, xv);
+    if (kind == 0) quad(qr, 0.f, qv);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) xv[k] = v_clean(xv[k]);
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
       double v = v_weight(xv[k], M, inv_t) * inv_z;
@@ -360,8 +372,11 @@ __global__ __launch_bounds__(1024) void verify_draw_kernel(VerifyArgs p) {
       run += w[k];
       if (run > target && w[k] > 0.0) hit = min(hit, base + k);
     }
-    if (hit != 0x7fffffff) atomicMin(&s_token, hit);
-    if (last >= 0) atomicMax(&s_last, last);
+    // the wave's first hit and last weight are those of its first and last such lane (1024 atomics on one word took 8 us)
+    const unsigned long long hits = __builtin_amdgcn_ballot_w64(hit != 0x7fffffff);
+    const unsigned long long some = __builtin_amdgcn_ballot_w64(last >= 0);
+    if (hits && lane == __builtin_ctzll(hits)) atomicMin(&s_token, hit);
+    if (some && lane == 63 - __builtin_clzll(some)) atomicMax(&s_last, last);
     __syncthreads();
     token = s_token != 0x7fffffff ? s_token : s_last;
   }

@@ -594,8 +594,7 @@ int q35_gated_attn_paged(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh
  * p_n: the lowest index whose running sum exceeds u[b, K] times the whole. Formed in 64 bits. n_accept: [B] int32;
  * tokens: [B, K + 1] int32, the kept drafts, the drawn token, then -1. A NaN logit counts as -inf; a row with no logit
  * above -inf keeps no draft and gives token 0; a draft outside 0 .. V - 1 is refused. K <= 255, B (K + 1) <= 65535,
- * V <= 4,194,304.
- * Needs q35_verify_drafts_workspace_bytes(B, K, V) bytes of workspace, 16-byte aligned.
+ * V <= 4,194,304. Needs q35_verify_drafts_workspace_bytes(B, K, V) bytes of workspace, 16-byte aligned.
  */
 size_t q35_verify_drafts_workspace_bytes(int64_t B, int64_t K, int64_t V);
 int q35_verify_drafts(const float* logits, int64_t l_sb, int64_t l_sp, const int32_t* draft_ids, int64_t d_sb,
