@@ -230,45 +230,47 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
   // With 32 rows the values are loaded behind the round's scores and the keys' scales behind its values: at two waves per
   // SIMD there are 256 registers, 136 of them accumulators.
   constexpr bool kLate = I4 && NR == 2;
-  // (the empty asm keeps a base in scalar registers: folded with a lane's offset it would take two vector ones)
+  // (the empty asm keeps a base in scalar registers: folded with a lane's offset it would take two vector ones; the pointer
+  // is made a global one again behind it, a generic one would make flat loads, which LDS waits count too)
+  typedef const __attribute__((address_space(1))) char* gptr;
   auto base_of = [](const void* pages, size_t bytes) {
-    const char* src = (const char*)pages + bytes;
+    uintptr_t src = (uintptr_t)pages + bytes;
     asm("" : "+s"(src));
-    return src;
+    return (gptr)src;
   };
   auto ks_load = [&](const Tile& t, KTile<I4>& k) {
     if constexpr (I4) {
-      const char* sc = base_of(p.ks, t.slot * 8);
-      k.s[0] = *reinterpret_cast<const u32x4*>(sc + s_off);
-      k.s[1] = *reinterpret_cast<const u32x4*>(sc + (s_off + 16));
+      const gptr sc = base_of(p.ks, t.slot * 8);
+      k.s[0] = *(const __attribute__((address_space(1))) u32x4*)(sc + s_off);
+      k.s[1] = *(const __attribute__((address_space(1))) u32x4*)(sc + (s_off + 16));
     }
   };
   auto k_load = [&](const Tile& t, KTile<I4>& k) {
-    const char* src = base_of(p.kp, t.slot * (I4 ? 128 : 512));
+    const gptr src = base_of(p.kp, t.slot * (I4 ? 128 : 512));
     if constexpr (I4) {
-      k.c[0] = *reinterpret_cast<const u32x4*>(src + k_off);
-      k.c[1] = *reinterpret_cast<const u32x4*>(src + (k_off + 16));
+      k.c[0] = *(const __attribute__((address_space(1))) u32x4*)(src + k_off);
+      k.c[1] = *(const __attribute__((address_space(1))) u32x4*)(src + (k_off + 16));
       if constexpr (!kLate) ks_load(t, k);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) k.c[i] = *reinterpret_cast<const bf16x8*>(src + (k_off + 64 * i));
+      for (int i = 0; i < 8; ++i) k.c[i] = *(const __attribute__((address_space(1))) bf16x8*)(src + (k_off + 64 * i));
     }
   };
   auto v_load = [&](const Tile& t, VTile<I4>& v, int key0) {
-    const char* src = base_of(p.vp, t.slot * (I4 ? 128 : 512));
+    const gptr src = base_of(p.vp, t.slot * (I4 ? 128 : 512));
     if constexpr (I4) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v.c[r] = *reinterpret_cast<const u32x2*>(src + (v_off + 128 * r));
-      const char* sc = base_of(p.vs, t.slot * 8);
-      v.s[0] = *reinterpret_cast<const u32x4*>(sc + s_off);
-      v.s[1] = *reinterpret_cast<const u32x4*>(sc + (s_off + 16));
+      for (int r = 0; r < 4; ++r) v.c[r] = *(const __attribute__((address_space(1))) u32x2*)(src + (v_off + 128 * r));
+      const gptr sc = base_of(p.vs, t.slot * 8);
+      v.s[0] = *(const __attribute__((address_space(1))) u32x4*)(sc + s_off);
+      v.s[1] = *(const __attribute__((address_space(1))) u32x4*)(sc + (s_off + 16));
     } else {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         // rows past the last key may hold anything, and 0 times infinity is NaN: read the last key's row instead
         const uint32_t row = max(min(4 * a + r, n_last - key0), 0);
-        v.c[r][0] = *reinterpret_cast<const u32x4*>(src + (v_off + 512 * row));
-        v.c[r][1] = *reinterpret_cast<const u32x4*>(src + (v_off + 512 * row + 256));
+        v.c[r][0] = *(const __attribute__((address_space(1))) u32x4*)(src + (v_off + 512 * row));
+        v.c[r][1] = *(const __attribute__((address_space(1))) u32x4*)(src + (v_off + 512 * row + 256));
       }
     }
   };
