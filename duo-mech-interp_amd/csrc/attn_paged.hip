@@ -96,45 +96,56 @@ __device__ __forceinline__ uint32_t cvt2(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
 }
 
-// A row of Q (this lane's four dims, scaled for base-2 exponentials) as column `col` of the scores' B operands: bf16 hi + lo,
-// or fp16 with its power of two in *fac and what the codes' offsets add to each group's product, negated, in off[][col].
+__device__ __forceinline__ float row16_sum(float v) {
+  v += lane_dpp<0xB1>(v);
+  v += lane_dpp<0x4E>(v);
+  v += lane_dpp<0x141>(v);
+  return v + lane_dpp<0x140>(v);
+}
+// A row of Q, 16 lanes of 16 dims (x[q][e] of lane j: dim 64 q + 4 j + e, scaled for base-2 exponentials), as column `col` of
+// the scores' B operands: bf16 hi + lo, or fp16 with its power of two in *fac and what the codes' offsets add to each
+// group's product, negated, in off[][col].
 template <bool I4>
-__device__ __forceinline__ void q_store(const f32x4& x, bool there, int lane, int col, u32x4* qf, float (*off)[16],
-                                        float* fac) {
+__device__ __forceinline__ void q_store(const f32x4 (&x)[4], int j, int col, u32x4* qf, float (*off)[16], float* fac) {
   if constexpr (I4) {
-    // dim 64 g + 16 a + 8 u + j is step 2 g + u of lane group a; a dword's nibbles leave it in pairs (j, j + 4), those of
-    // odd j times 16
-    int ex = 0;
-    if (there)
-      ex = __builtin_amdgcn_frexp_expf(
-          wave_max_f32(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])))));
-    _Float16* qe = reinterpret_cast<_Float16*>(qf);
-    const int base = ((2 * (lane >> 4) + ((lane >> 1) & 1)) * 64 + 16 * ((lane >> 2) & 3) + col) * 8 + (lane & 1);
-    float o = 0.f;
+    // dim 64 g + 16 a + 8 u + k is step 2 g + u of lane group a; a dword's nibbles leave it in pairs (k, k + 4), those of
+    // odd k times 16
+    float m = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const _Float16 hq = (_Float16)ldexpf(x[e], 5 - ex - 4 * (e & 1));
-      qe[base + 2 * e] = hq;
-      o -= (e & 1 ? 1152.f : 1032.f) * (float)hq;
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(x[q][e]));
+    const int ex = __builtin_amdgcn_frexp_expf(row16_max_f32(m));  // (0 for 0 and for what is not finite)
+    _Float16* qe = reinterpret_cast<_Float16*>(qf) + (((j >> 1) & 1) * 64 + 16 * (j >> 2) + col) * 8 + (j & 1);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float o = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const _Float16 hq = (_Float16)ldexpf(x[q][e], 5 - ex - 4 * (e & 1));
+        qe[q * 1024 + 2 * e] = hq;
+        o -= (e & 1 ? 1152.f : 1032.f) * (float)hq;
+      }
+      o = row16_sum(o);
+      if (j == 0) off[q][col] = o;
     }
-    o = add_xor4_quads(add_xor<2>(add_xor<1>(o)));
-    o = add_xor<8>(o);
-    if ((lane & 15) == 0) off[lane >> 4][col] = o;
-    if (lane == 0) *fac = ldexpf(1.f, ex - 5);
+    if (j == 0) *fac = ldexpf(1.f, ex - 5);
   } else {
-    // dim 32 step + 8 a + j in order
-    __bf16* qe = reinterpret_cast<__bf16*>(qf);
-    const int o = ((lane >> 3) * 64 + 16 * ((lane >> 1) & 3) + col) * 8 + 4 * (lane & 1);
-    bf16x4 hi, lo;
+    // dim 32 step + 8 a + k in order
+    __bf16* qe = reinterpret_cast<__bf16*>(qf) + ((j >> 3) * 64 + 16 * ((j >> 1) & 3) + col) * 8 + 4 * (j & 1);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const bf16_hl hl = bf16_split(x[e]);
-      hi[e] = hl.hi;
-      lo[e] = hl.lo;
+    for (int q = 0; q < 4; ++q) {
+      bf16x4 hi, lo;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bf16_hl hl = bf16_split(x[q][e]);
+        hi[e] = hl.hi;
+        lo[e] = hl.lo;
+      }
+      *reinterpret_cast<bf16x4*>(qe + q * 1024) = hi;
+      *reinterpret_cast<bf16x4*>(qe + 8 * 64 * 8 + q * 1024) = lo;
     }
-    *reinterpret_cast<bf16x4*>(qe + o) = hi;
-    *reinterpret_cast<bf16x4*>(qe + 8 * 64 * 8 + o) = lo;
-    if (lane == 0) *fac = 1.f;
+    if (j == 0) *fac = 1.f;
   }
 }
 // A lane's accumulators of its row into o[256], dims in order.
@@ -275,41 +286,32 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
     }
   };
 
-  // ---- Q's rows, one wave each: row i of the block (i = wave, wave + 4, ...) is token r / G, head r % G of the group. The
-  // first row's loads go out ahead of the tiles': loads return in order.
+  // ---- Q's rows, 16 lanes each: tile i's row 4 wave + lane / 16, token r / G, head r % G of the group. The first tile's
+  // loads go out ahead of the keys': loads return in order.
   struct QRow {
-    f32x4 x, px, co, si;
-    bool there;
+    f32x4 x[4], px[4], co[4], si[4];
   };
-  const int half = p.rot >> 1, d0 = 4 * lane;
-  const bool turns = d0 < p.rot;
-  const int pd = !turns ? d0 : d0 < half ? d0 + half : d0 - half, pj = d0 < half ? d0 : d0 - half;
-  auto q_load = [&](int i) -> QRow {
-    QRow w = {zero4(), zero4(), zero4(), zero4(), false};
-    const int r = r0 + i, t = r / p.G, h = kvh * p.G + r - t * p.G;
-    w.there = i < ROWS && r < R && keys_seen(p, pos, len, t) > 0;
-    if (w.there) {
-      const int64_t o = b * p.qb + t * p.qt + h * p.qh;
-      if (p.q_f32) {
-        w.x = load_quad<float>((const float*)p.q + o + d0);
-        w.px = load_quad<float>((const float*)p.q + o + pd);
-      } else {
-        w.x = load_quad<__bf16>((const __bf16*)p.q + o + d0);
-        w.px = load_quad<__bf16>((const __bf16*)p.q + o + pd);
-      }
-      if (turns) {
-        w.co = load_quad<float>(p.cos_t + (pos + t) * half + pj);
-        w.si = load_quad<float>(p.sin_t + (pos + t) * half + pj);
+  const int half = p.rot >> 1, d0 = 4 * lane, qj = lane & 15, qcol = 4 * wave + (lane >> 4);
+  auto q_load = [&](int i, QRow& w) {
+    const int r = r0 + 16 * i + qcol, t = r / p.G, h = kvh * p.G + r - t * p.G;
+    const bool there = r < R && keys_seen(p, pos, len, t) > 0;
+    const int64_t o = b * p.qb + t * p.qt + h * p.qh;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int d = 64 * q + 4 * qj, pd = d >= p.rot ? d : d < half ? d + half : d - half, pj = d < half ? d : d - half;
+      w.x[q] = w.px[q] = w.co[q] = w.si[q] = zero4();
+      if (there) {
+        w.x[q] = p.q_f32 ? load_quad<float>((const float*)p.q + o + d) : load_quad<__bf16>((const __bf16*)p.q + o + d);
+        if (d < p.rot) {
+          w.px[q] = p.q_f32 ? load_quad<float>((const float*)p.q + o + pd) : load_quad<__bf16>((const __bf16*)p.q + o + pd);
+          w.co[q] = load_quad<float>(p.cos_t + (pos + t) * half + pj);
+          w.si[q] = load_quad<float>(p.sin_t + (pos + t) * half + pj);
+        }
       }
     }
-    return w;
   };
-  f32x4 wx = zero4(), wp = zero4();
-  if (p.qw) {
-    wx = load_quad<float>(p.qw + d0);
-    wp = load_quad<float>(p.qw + pd);
-  }
-  QRow row = q_load(wave);
+  QRow row;
+  q_load(0, row);
   __builtin_amdgcn_sched_barrier(0);
 
   // ---- the first round's tiles, in flight while Q is prepared. The next round's tiles are loaded while this one's are
@@ -341,30 +343,43 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
   }
   __builtin_amdgcn_sched_barrier(0);
 
-  // ---- Q: norm, rotation, scale log2(e), the split into hi + lo or the power of two, into LDS as B operands
+  // ---- Q: norm, rotation, scale log2(e), the split into hi + lo or the power of two, into LDS as B operands (rows that are
+  // not there: zeros)
   if (work) {
-#pragma unroll 1
-    for (int i = wave; i < ROWS; i += 4) {
-      const QRow cur = row;
-      row = q_load(i + 4);
-      f32x4 x = cur.x;
-      if (cur.there) {
-        float rr = 1.f;
-        if (p.qw) {
-          const float ss = wave_sum(x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]);
-          rr = rsqrtf(ss * (1.f / kPgD) + p.eps);
-        }
-        const float sg = d0 < half ? -1.f : 1.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[e] = x[e] * rr * (1.f + wx[e]);
-          if (turns) x[e] = x[e] * cur.co[e] + sg * (cur.px[e] * rr * (1.f + wp[e])) * cur.si[e];
+    for (int i = 0; i < NR; ++i) {
+      if (i) q_load(i, row);
+      float rr = 1.f;
+      f32x4 wx[4], wp[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int d = 64 * q + 4 * qj, pd = d >= p.rot ? d : d < half ? d + half : d - half;
+        wx[q] = wp[q] = zero4();
+        if (p.qw) {
+          wx[q] = load_quad<float>(p.qw + d);
+          wp[q] = load_quad<float>(p.qw + pd);
         }
       }
+      if (p.qw) {
+        float ss = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] *= p.scale * 1.4426950408889634f;
-      const int ti = i >> 4;
-      q_store<I4>(x, cur.there, lane, i & 15, qf + (size_t)ti * QP * QF, qoff[ti], &qfac[i]);
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ss += row.x[q][e] * row.x[q][e];
+        rr = rsqrtf(row16_sum(ss) * (1.f / kPgD) + p.eps);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int d = 64 * q + 4 * qj;
+        const float sg = d < half ? -1.f : 1.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x = row.x[q][e] * rr * (1.f + wx[q][e]);
+          if (d < p.rot) x = x * row.co[q][e] + sg * (row.px[q][e] * rr * (1.f + wp[q][e])) * row.si[q][e];
+          row.x[q][e] = x * (p.scale * 1.4426950408889634f);
+        }
+      }
+      q_store<I4>(row.x, qj, qcol, qf + (size_t)i * QP * QF, qoff[i], &qfac[16 * i + qcol]);
     }
   }
 
