@@ -721,8 +721,10 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
       }
     }
     lds_barrier();
-#pragma unroll 1
-    for (int j = wave; j < 16 && r0 + 16 * i + j < R; j += 4) {
+#pragma unroll
+    for (int jj = 0; jj < 4; ++jj) {
+      const int j = 4 * jj + wave;
+      if (r0 + 16 * i + j >= R) break;
       const int r = r0 + 16 * i + j, t = r / p.G, h = kvh * p.G + r - t * p.G;
       float M = -INFINITY;
 #pragma unroll
