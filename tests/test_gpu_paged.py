@@ -323,6 +323,28 @@ def test_attention_infinite_values_that_are_attended_to(fmt):
 
 
 @pytest.mark.parametrize("fmt", ["bf16", "int4"])
+@pytest.mark.parametrize("T,splits", [(1, 1), (1, 3), (5, 1), (5, 3)])
+def test_attention_scores_that_are_nan(fmt, T, splits):
+    """A query that is NaN, and a key that is NaN and alone in its wave's last round: NaN for the heads they reach, and for
+    no other."""
+    n = 257 if T == 1 else 261  # key 256 is the only one of its 32 that the first token sees
+    d = make(fmt, 3, T, 4, 2, 16, [n, n, n])
+    d["y"][0, 0, 512 * 1 + 7] = math.nan  # row 0, token 0, head 1
+    page, row = int(d["table"][1, 256 // 16]), 256 % 16  # row 1, key 256 of key head 1
+    if fmt == "bf16":
+        d["pages"][0][page, 1, row, 3] = math.nan
+    else:
+        d["pages"][2][page, 1, row, 0] = math.nan
+    announce(f"paged attention {fmt} NaN scores T {T} splits {splits}")
+    nan = attend(to(d, device()), splits=splits).view(3, T, 4, 256).isnan().cpu()
+    assert bool((nan.any(-1) == nan.all(-1)).all())
+    want = torch.zeros(3, T, 4, dtype=torch.bool)
+    want[0, 0, 1] = True
+    want[1, :, 2:] = True
+    assert torch.equal(nan.any(-1), want)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int4"])
 @pytest.mark.parametrize("T", [1, 4])
 def test_attention_rows_that_see_nothing(fmt, T):
     """Positions below 0 and past the table, no tokens, and rows all of whose pages are missing give zeros."""
