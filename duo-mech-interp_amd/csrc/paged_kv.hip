@@ -8,7 +8,8 @@
 //   norm, rotation and quotient are those of 64 bits: which code a value gets then depends on the inputs alone and not on
 //   the order of a sum (in 32 bits about one value in 10^6 falls on the other side). They are formed in fp32 first, and
 //   again in 64 bits only where a rounding lies closer to a tie than fp32 can tell (one row of 256 in a hundred): 6144
-//   tokens of two heads XX us against 17 in 64 bits throughout. A group that holds a value that is not finite gets the scale NaN: it reads back as NaN.
+//   tokens of two heads 11.3 us against 17 in 64 bits throughout. A group that holds a
+//   value that is not finite gets the scale NaN: it reads back as NaN.
 #include "paged_kv.h"
 
 namespace q35 {
@@ -67,7 +68,8 @@ __device__ __forceinline__ uint32_t quantize_quad_f32(const f32x4& x, const f32x
   }
   *s_out = sb;
   const float sum = x[0] + x[1] + x[2] + x[3];  // (a maximum passes over a NaN, a sum does not)
-  *sure = sum == sum && m > 1e-30f && am < 1e30f && far < 0.5f && (float)(__bf16)(s32 - off) == s && (float)(__bf16)(s32 + off) == s;
+  *sure = sum == sum && m > 1e-30f && am < 1e30f && far < 0.5f && (float)(__bf16)(s32 - off) == s &&
+          (float)(__bf16)(s32 + off) == s;
   return q;
 }
 
@@ -120,13 +122,15 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs p) {
   const float sg = d0 < half ? -1.f : 1.f;
   // in fp32 (what bf16 pages hold, rounded); big: the terms' magnitudes, which bound the error
   f32x4 r = x, big;
+  bool norm_ok = true;
 #pragma unroll
   for (int e = 0; e < 4; ++e) big[e] = fabsf(x[e]);
   if (!val) {
     f32x4 xn = x, pn = px;
     if (p.kw) {
       const float ss = wave_sum(x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]);
-      const float rr = rsqrtf(ss * (1.f / kPgD) + p.eps);
+      const float ms = ss * (1.f / kPgD) + p.eps, rr = rsqrtf(ms);
+      norm_ok = ms > 1e-30f;  // (smaller squares lose bits)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         xn[e] = x[e] * rr * (1.f + wx[e]);
@@ -148,7 +152,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs p) {
     __bf16 s;
     bool sure;
     uint32_t q = quantize_quad_f32(r, big, !val && p.rot > 0, &s, &sure);
-    if (__builtin_amdgcn_ballot_w64(!sure) != 0) {
+    if (__builtin_amdgcn_ballot_w64(!(sure && norm_ok)) != 0) {
       double d[4] = {x[0], x[1], x[2], x[3]};
       if (!val) {
         double pn[4] = {px[0], px[1], px[2], px[3]};

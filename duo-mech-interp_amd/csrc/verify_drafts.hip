@@ -49,10 +49,10 @@ struct VerifyArgs {
 __device__ __forceinline__ int v_len(const VerifyArgs& p, int b) {
   return p.lens ? min(max(load_uniform(p.lens + b), 0), p.K) : p.K;
 }
-// log2(e) / temperature, 0 for the argmax
+// log2(e) / temperature, 0 for the argmax (an infinite temperature leaves the tokens above -inf alike)
 __device__ __forceinline__ double v_inv_temp(const VerifyArgs& p, int b) {
   const float t = p.temps ? __int_as_float(load_uniform(reinterpret_cast<const int32_t*>(p.temps) + b)) : p.temp;
-  return t > 0.f ? 1.4426950408889634074 / (double)t : 0.0;
+  return t > 0.f ? fmax(1.4426950408889634074 / (double)t, 1e-300) : 0.0;
 }
 // The position's draft when it is a token, else -1
 __device__ __forceinline__ int v_draft(const VerifyArgs& p, int b, int i, int len) {

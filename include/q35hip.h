@@ -569,7 +569,8 @@ int q35_paged_kv_rows(const void* k_pages, const void* v_pages, const void* k_sc
  *   out: [B, T, Hq * D] in out_dtype (16-byte aligned), zeros for tokens that are not there or see no key.
  *   Hq a multiple of Hkv (any ratio). splits <= 0 lets the library choose over how many blocks a row's keys are dealt
  *   (at most one per 128 keys of capacity). Needs q35_gated_attn_paged_workspace_bytes(...) bytes of workspace, 16-byte
- *   aligned; calls that share one workspace must not overlap.
+ *   aligned; calls that share one workspace must not overlap. T Hq / Hkv up to 2^24, in at most 65535 / Hkv blocks of 32
+ *   rows (16 where all fit in one).
  */
 size_t q35_gated_attn_paged_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t n_blocks,
                                             int64_t page_size, int64_t splits);
@@ -588,12 +589,14 @@ int q35_gated_attn_paged(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh
  *   draft was drawn from, or NULL for drafts held for certain (q = 1 at the draft)
  *   u: [B, K + 1] fp32 in [0, 1) (row stride u_sb): u[b, i] for draft i, u[b, K] for the drawn token
  *   lens: [B] int32, the drafts of each row (clamped to 0 .. K), or NULL for K
- *   temperatures: [B] fp32 on the device, or NULL for `temperature` on every row; 0 is the argmax (lowest index)
+ *   temperatures: [B] fp32 on the device, or NULL for `temperature` on every row; 0 (on the device also less) is the
+ *   argmax (lowest index)
  * With p_i = softmax(logits[b, i] / temperature): draft i is kept while u[b, i] q_i(x_i) < p_i(x_i); behind the first
  * refusal n the token is drawn from max(p_n - q_n, 0) (from p_n should that be nothing), behind the last draft from
  * p_n: the lowest index whose running sum exceeds u[b, K] times the whole. Formed in 64 bits. n_accept: [B] int32;
  * tokens: [B, K + 1] int32, the kept drafts, the drawn token, then -1. A NaN logit counts as -inf; a row with no logit
- * above -inf keeps no draft and gives token 0; a draft outside 0 .. V - 1 is refused. K <= 255, B (K + 1) <= 65535,
+ * above -inf keeps no draft and gives token 0; a draft outside 0 .. V - 1 is refused; a NaN draft
+ * probability refuses its draft, and its token is not drawn. K <= 255, B (K + 1) <= 65535,
  * V <= 4,194,304. Needs q35_verify_drafts_workspace_bytes(B, K, V) bytes of workspace, 16-byte aligned.
  */
 size_t q35_verify_drafts_workspace_bytes(int64_t B, int64_t K, int64_t V);

@@ -168,7 +168,7 @@ def verify_drafts(logits, draft_ids, u, draft_probs=None, lens=None, temperature
             w = torch.zeros(V, dtype=torch.float64)
             w[int((x == m).nonzero()[0])] = 1
             return w
-        w = torch.where(x == m, 1.0, torch.exp((x - m) / T))
+        w = torch.where(x == m, 1.0, torch.where(x == -math.inf, 0.0, torch.exp((x - m) / T)))
         return w / w.sum()
     for b in range(B):
         T = float(temperature[b]) if torch.is_tensor(temperature) else float(temperature)
@@ -192,7 +192,7 @@ def verify_drafts(logits, draft_ids, u, draft_probs=None, lens=None, temperature
                     less = draft_probs[b, i].double()
                 elif 0 <= int(draft_ids[b, i]) < V:
                     less[int(draft_ids[b, i])] = 1
-                left = (p - less).clamp_min(0)
+                left = torch.nan_to_num(p - less, nan=0.0).clamp_min(0)
                 r = left if left.sum() > 0 else p
             run = r.cumsum(0)
             over = (run > float(u[b, K]) * run[-1]).nonzero()

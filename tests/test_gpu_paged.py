@@ -460,6 +460,121 @@ def test_another_stream_and_calls_side_by_side():
         assert all(torch.equal(x, want[i]) for x in got[i])
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "int4"])
+def test_pages_past_32_bits(fmt):
+    """Pages more than 2^32 bytes into the pool (and, in bf16, 2^31 elements)."""
+    dev = device()
+    d = make(fmt, 2, 3, 4, 2, 64, [150, 70], lens=[3, 2])
+    nb = d["table"].shape[1]
+    row = 512 if fmt == "bf16" else 128
+    n = (1 << 32) // (2 * 64 * row) + 2 * nb + 2
+    announce(f"paged {fmt} pages past 32 bits")
+    want_pages = oracle_append(d)
+    g = to(d, dev)
+    small = g["pages"]
+    m = small[0].shape[0]
+    big = tuple(None if p is None else torch.empty(n, *p.shape[1:], dtype=p.dtype, device=dev) for p in small)
+    for p, q in zip(big, small):
+        if p is not None:
+            p[n - m:] = q
+    far = dict(g, pages=big, table=g["table"] + (n - m))
+    append(far)
+    same_pages(fmt, [None if p is None else p[n - m:] for p in big], want_pages)
+    after = dict(d, pages=tuple(None if p is None else p[n - m:].cpu() for p in big))
+    check_attention(after, attend(far))
+    k, v = ops.paged_kv_rows(big, far["table"], torch.zeros_like(far["pos"]), 70)
+    wk, wv = paged.paged_rows(after["pages"], d["table"], torch.zeros_like(d["pos"]), 70)
+    assert torch.equal(k.cpu().double(), wk.bfloat16().double()) and torch.equal(v.cpu().double(), wv.bfloat16().double())
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int4"])
+def test_attention_over_a_prompt(fmt):
+    """A prompt's own tokens from position 0 on, ragged, six heads over two."""
+    d = make(fmt, 2, 700, 6, 2, 64, [700, 333], lens=[700, 333])
+    announce(f"paged attention {fmt} prompt of 700")
+    check_attention(d, attend(to(d, device())))
+
+
+@pytest.mark.parametrize("T", [1, 6])
+def test_attention_more_splits_than_rounds(T):
+    d = make("int4", 2, T, 8, 2, 32, [3000, 130])
+    announce(f"paged attention T {T}, 5000 splits")
+    check_attention(d, attend(to(d, device()), splits=5000))
+
+
+def test_append_of_tiny_values_without_eps():
+    """Squares below the smallest normal number, and an eps of 0: the codes of 64 bits all the same."""
+    d = make("int4", 1, 40, 2, 2, 16, [40])
+    scale = 10.0 ** -torch.arange(40).float()[:, None]
+    d["y"] = d["y"] * scale
+    _, _, k, v = columns(d["y"], 2, 2)
+    pages = tuple(p.clone() for p in d["pages"])
+    paged.paged_append(k, v, pages, d["table"], d["pos"], d["cos"], d["sin"], d["lens"], d["kw"], eps=0.0)
+    g = to(d, device())
+    _, _, k, v = columns(g["y"], 2, 2)
+    announce("paged append of tiny values")
+    ops.paged_kv_append_(k, v, g["pages"], g["table"], g["pos"], g["cos"], g["sin"], k_norm_w=g["kw"], eps=0.0)
+    same_pages("int4", g["pages"], pages)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int4"])
+def test_calls_through_the_dispatcher(fmt):
+    """torch.ops, a dispatch mode and inference mode give what the plain calls give; meta tensors the shapes."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    dev = device()
+    g = to(make(fmt, 2, 3, 8, 2, 16, [70, 33], lens=[3, 2]), dev)
+    announce(f"paged calls through the dispatcher {fmt}")
+    other = dict(g, pages=tuple(None if p is None else p.clone() for p in g["pages"]))
+    append(g)
+    want = attend(g)
+    rows = ops.paged_kv_rows(g["pages"], g["table"], g["pos"], 3, lens=g["lens"])
+    seen = []
+
+    class Record(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+    with Record():
+        append(other)
+        got = attend(other)
+        got_rows = ops.paged_kv_rows(other["pages"], g["table"], g["pos"], 3, lens=g["lens"])
+    assert {"q35.paged_kv_append_.default", "q35.gated_attn_paged.default", "q35.paged_kv_rows.default"} <= set(seen)
+    assert torch.equal(got, want) and all(torch.equal(a, b) for a, b in zip(got_rows, rows))
+    for a, b in zip(g["pages"], other["pages"]):
+        assert a is None or torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    with torch.inference_mode():
+        assert torch.equal(attend(g), want)
+    meta = {k: v.to("meta") if torch.is_tensor(v) else v for k, v in g.items()}
+    meta["pages"] = tuple(None if p is None else p.to("meta") for p in g["pages"])
+    out = attend(meta)
+    assert out.shape == want.shape and out.dtype == want.dtype and out.device.type == "meta"
+
+
+def test_graphs_on_two_streams_share_nothing():
+    """Two captured steps replayed at once on two streams, several times."""
+    dev = device()
+    gs, outs, want = [], [], []
+    announce("paged graphs on two streams")
+    for s in range(2):
+        g = to(make("int4", 2, 2, 8, 2, 64, [3000, 2500], seed=s), dev)
+        want.append(attend(g))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = attend(g)
+        gs.append((graph, g))
+        outs.append(out)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for (graph, _), s in zip(gs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
 def test_refusals_on_the_device():
     dev = device()
     d = to(make("int4", 1, 1, 8, 2, 16, [5]), dev)

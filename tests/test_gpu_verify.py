@@ -152,3 +152,46 @@ def test_verify_refusals_on_the_device():
                  lambda: ops.verify_drafts(x, ids, u, temperature=torch.ones(3, device=dev))):
         with pytest.raises(Q35Error):
             call()
+
+
+def test_verify_infinite_temperature_and_nan_draft_probabilities():
+    """The tokens above -inf alike; a NaN among the draft's probabilities refuses its draft and leaves its token undrawn."""
+    x, ids, u, q, lens = make(4, 2, 5000, seed=3, probs=True)
+    x[:, :, 1000:3000] = -math.inf
+    announce("verify infinite temperature, NaN probabilities")
+    both(x, ids, u, q, lens, math.inf)
+    both(x, ids, u, q, lens, torch.tensor([math.inf, 1.0, 0.0, -2.0]))
+    q[:, :, 77] = math.nan
+    ids[0, 0] = ids[1, 1] = 77
+    n, _ = both(x, ids, u, q)
+    assert int(n[0]) == 0 and int(n[1]) <= 1
+
+
+def test_verify_most_drafts_and_largest_vocabulary():
+    x, ids, u, q, _ = make(2, 255, 300, seed=8, probs=True, spread=0.1)
+    q = x[:, :-1].softmax(-1)  # nearly every draft is kept
+    announce("verify K 255, V 4194304")
+    n, _ = both(x, ids, u, q)
+    x, ids, u, q, _ = make(1, 1, 4194304, seed=8, spread=0.5)
+    both(x, ids, u, q)
+    dev = device()
+    with pytest.raises(Q35Error):
+        ops.verify_drafts(torch.zeros(1, 1, 4194305, device=dev), torch.zeros(1, 0, dtype=torch.int32, device=dev),
+                          torch.zeros(1, 1, device=dev))
+    with pytest.raises(Q35Error):
+        ops.verify_drafts(torch.zeros(1, 257, 8, device=dev), torch.zeros(1, 256, dtype=torch.int32, device=dev),
+                          torch.zeros(1, 257, device=dev))
+
+
+def test_verify_rows_past_32_bits():
+    """Rows of logits more than 2^32 bytes apart."""
+    dev = device()
+    x, ids, u, q, lens = make(2, 1, 3001, seed=12)
+    announce("verify rows past 32 bits")
+    far = (1 << 31) + 64  # elements
+    pool = torch.empty(far + 2 * 3001, device=dev)
+    wide = pool.as_strided((2, 2, 3001), (far, 3001, 1))
+    wide.copy_(x.to(dev))
+    got = ops.verify_drafts(wide, ids.to(dev), u.to(dev))
+    want = paged.verify_drafts(x, ids, u)
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
