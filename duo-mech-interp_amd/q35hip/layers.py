@@ -2,6 +2,7 @@
 
     gated_deltanet_layer(x, p, conv_state, rec_state, head_scale=None) -> y
     gated_attention_layer(x, p, k_cache, v_cache, pos) -> y
+    gated_attention_layer_paged(x, p, pages, table, pos) -> y
     residual_steer_add(x, vecs, rows) -> x
 
 `p` holds one layer's weights under HF's parameter names (transformers 5.15.0 models/qwen3_5/modeling_qwen3_5.py,
@@ -12,7 +13,8 @@ HF:426-429 and HF:641-654; the engine's names at engine/model.js:89-112 map one 
                    o_proj [H, Hq*D], q_norm [D], k_norm [D]
 States are caller-owned device tensors mutated in place, as the engine's buffers are (engine/model.js:308-342):
 conv_state [B, K-1, C] fp32 (the last K-1 conv inputs, oldest first, engine/model.js:333), rec_state [B, Hv, dk, dv]
-fp32, k_cache / v_cache [B, Hkv, max_len, D] bf16 holding rotated keys and values by position.
+fp32, k_cache / v_cache [B, Hkv, max_len, D] bf16 holding rotated keys and values by position; or, of a pool that many
+sequences share, pages in bf16 or 4 bits (ops.kv_pages) and a block table.
 
 Any weight may also come as int8 with fp32 scales ("<name>.q" / "<name>.s", one scale per group of 128 inputs as the
 engine stores every linear, engine/model.js:3-5 and engine/kernels.js:15-47, or one per row; "<name>" then holds the
@@ -278,6 +280,33 @@ def gated_attention_layer(x, p, k_cache, v_cache, pos, *, rope_theta=1e7, partia
     # bf16 o straight into the int8 GEMM (the product of o.float(), bitwise); fp32 for the other forms
     xo = o if (T > 1 and wq_o is not None and o.shape[-1] % 64 == 0) else o.float()
     return linear(xo, p["o_proj"], wq_o, ws_o, residual=residual, fixed_order=fixed_order)
+
+
+def gated_attention_layer_paged(x, p, pages, table, pos, *, lens=None, rope_theta=1e7, partial_rotary_factor=0.25,
+                                eps=1e-6, prenorm=None, residual=None, fixed_order=False):
+    """gated_attention_layer over a paged KV cache in bf16 or 4 bits (ops.kv_pages; head dim 256): a decode step (T = 1),
+    the check of drafted tokens (a few), a chunk of a prompt (many). x: [B, T, H] fp32; token t < lens[b] of row b (lens
+    [B] int32 on the device, None: all T) sits at position pos[b] + t ([B] int32 on the device); its key and value go into
+    the pages that table ([B, blocks] int32) names, and it attends to positions 0 .. pos[b] + t. Tokens past lens, or past
+    the table, leave the pages alone and give 0 (residual: itself). The call synchronises with nothing, and a HIP graph
+    that holds it follows table, pos and lens. prenorm, residual, fixed_order: see gated_attention_layer."""
+    B, T, _ = x.shape
+    D = p["q_norm"].numel()
+    Hq = p["q_proj"].shape[0] // (2 * D)
+    Hkv = p["k_proj"].shape[0] // D
+    cos, sin = rope_tables(table.shape[1] * pages[0].shape[2], int(D * partial_rotary_factor), rope_theta, x.device)
+    y = linear(x, attn_in_weight(p), *_q8(p, "_in_fused"), prenorm=prenorm)
+    q, k, v = y.split([2 * Hq * D, Hkv * D, Hkv * D], -1)
+    q = q.unflatten(-1, (Hq, 2 * D))
+    ops.paged_kv_append_(k.unflatten(-1, (Hkv, D)), v.unflatten(-1, (Hkv, D)), pages, table, pos, cos, sin, lens=lens,
+                         k_norm_w=p["k_norm"].float().contiguous(), eps=eps)
+    # as the dense layer: fp32 for the GEMV of a few rows, bf16 for the int8 GEMM
+    wq_o, ws_o = _q8(p, "o_proj")
+    half = B * T > 8 and wq_o is not None
+    o = ops.gated_attention_paged(q[..., :D], q[..., D:], pages, table, pos, cos, sin, lens=lens,
+                                  q_norm_w=p["q_norm"].float().contiguous(), eps=eps, scale=1.0 / math.sqrt(D),
+                                  out_dtype=torch.bfloat16 if half else torch.float32)
+    return linear(o, p["o_proj"], wq_o, ws_o, residual=residual, fixed_order=fixed_order)
 
 
 def residual_steer_add(x, vecs, rows=None):

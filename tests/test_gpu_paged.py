@@ -17,7 +17,7 @@ import torch
 
 from gpu_util import announce, device
 from oracle import paged
-from q35hip import ops, workloads
+from q35hip import layers, ops, workloads
 
 pytestmark = pytest.mark.gpu
 
@@ -573,6 +573,66 @@ def test_graphs_on_two_streams_share_nothing():
                 graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int4"])
+@pytest.mark.parametrize("T,lens", [(1, None), (3, [3, 0]), (40, [40, 17])])
+def test_layer(fmt, T, lens):
+    """The attention layer over pages, with an o_proj of 1 so that its output is the attention's: its projection's columns
+    through the oracle. Then with a residual, added in place."""
+    dev = device()
+    d = make(fmt, 2, T, 2, 1, 32, [T + 30, (lens or [T] * 2)[1] + 5], lens=lens)
+    g = torch.Generator().manual_seed(T)
+    p = {n: (torch.randn(w, 512, generator=g) * 0.05).to(dev) for n, w in (("q_proj", 1024), ("k_proj", 256), ("v_proj", 256))}
+    p["o_proj"] = torch.eye(512, device=dev)
+    p["q_norm"], p["k_norm"] = d["qw"].to(dev), d["kw"].to(dev)
+    x = torch.randn(2, T, 512, generator=g).to(dev)
+    gpu = to(d, dev)
+    announce(f"paged attention layer {fmt} T {T} lens {lens}")
+    out = layers.gated_attention_layer_paged(x, p, gpu["pages"], gpu["table"], gpu["pos"], lens=gpu["lens"])
+    d["y"] = layers.linear(x, layers.attn_in_weight(p)).cpu()
+    d["cos"], d["sin"] = (t.cpu() for t in layers.rope_tables(d["table"].shape[1] * 32, 64, 1e7, dev))
+    want = oracle_append(d)
+    same_pages(fmt, gpu["pages"], want)
+    d["pages"] = tuple(None if t is None else t.cpu() for t in gpu["pages"])
+    check_attention(d, out)
+    res = torch.randn(2, T, 512, generator=g).to(dev)
+    got = layers.gated_attention_layer_paged(x, p, gpu["pages"], gpu["table"], gpu["pos"], lens=gpu["lens"],
+                                             residual=res.clone(), fixed_order=True)
+    assert torch.equal(got, res + out)
+
+
+def test_layer_in_int8_against_the_dense_layer():
+    """int8 weights, a prompt and then steps of one token: the dense layer's outputs but for the two attentions' roundings
+    (2^-8 a weight and 2^-8 an output of each, over sum w |v|, carried through |o_proj|)."""
+    dev = device()
+    g = torch.Generator().manual_seed(5)
+    H, Hq, Hkv = 512, 4, 2
+    p = {}
+    for n, (r, c) in dict(q_proj=(Hq * 512, H), k_proj=(Hkv * 256, H), v_proj=(Hkv * 256, H), o_proj=(H, Hq * 256)).items():
+        q = torch.randint(-127, 128, (r, c), generator=g, dtype=torch.int8)
+        s = torch.full((r, c // 128), 0.001)
+        p[n + ".q"], p[n + ".s"] = q.to(dev), s.to(dev)
+        p[n] = (q.float() * 0.001).to(dev)
+    p["q_norm"], p["k_norm"] = (0.1 * torch.randn(256, generator=g).to(dev) for _ in range(2))
+    announce("paged attention layer in int8 against the dense one")
+    B, n, blocks = 2, 64, 2
+    kc, vc = (torch.zeros(B, Hkv, 128, 256, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    pages = ops.kv_pages(B * blocks, Hkv, 64, dev)
+    table = torch.tensor([[2, 0], [1, 3]], dtype=torch.int32, device=dev)
+    at = 0
+    for T in (n, 1, 1, 5):
+        x = torch.randn(B, T, H, generator=g).to(dev)
+        pos = torch.full((B,), at, dtype=torch.int32, device=dev)
+        got = layers.gated_attention_layer_paged(x, p, pages, table, pos)
+        want = layers.gated_attention_layer(x, p, kc, vc, at if T == n else pos)
+        k, v = ops.paged_kv_rows(pages, table, torch.zeros_like(pos), 128)
+        # (bitwise where both read the projection in fp32, and one rounding apart otherwise)
+        assert bool(((k.float() - kc.float()).abs() <= kc.float().abs() * 2.0 ** -7 + 1e-6).all())
+        vmax = vc[:, :, :at + T].abs().amax((2, 3)).float().amax(1)  # >= sum w |v|
+        bound = (2 * (2.0 ** -8 + 2.0 ** -8) + 2.0 ** -12) * vmax[:, None, None] * p["o_proj"].abs().sum(-1)
+        assert bool(((got - want).abs() <= bound).all())
+        at += T
 
 
 def test_refusals_on_the_device():
