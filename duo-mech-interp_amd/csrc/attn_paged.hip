@@ -65,7 +65,6 @@ __device__ __forceinline__ int run_keys(int n, int S) {
 template <bool I4> struct KTile;
 template <> struct KTile<true> {
   u32x4 c[2];  // codes: dword 2 g + u
-  u32x4 s[2];  // scales of keys 4 a + r: four bf16 each
 };
 template <> struct KTile<false> {
   bf16x8 c[8];
@@ -73,7 +72,6 @@ template <> struct KTile<false> {
 template <bool I4> struct VTile;
 template <> struct VTile<true> {
   u32x2 c[4];  // key 4 a + r: 16 bits per group
-  u32x4 s[2];
 };
 template <> struct VTile<false> {
   u32x4 c[4][2];  // key 4 a + r: dims 8 c .. and 128 + 8 c ..
@@ -83,8 +81,12 @@ __device__ __forceinline__ bf16x8 as_bf16x8(uint32_t a, uint32_t b, uint32_t c, 
   const u32x4 r = {a, b, c, d};
   return __builtin_bit_cast(bf16x8, r);
 }
-__device__ __forceinline__ float scale_of(const u32x4 (&s)[2], int r, int g) {
-  const uint32_t w = s[r >> 1][2 * (r & 1) + (g >> 1)];
+// The scale of key 4 a + r and group g, of a tile's (four bf16 a key).
+struct Scales {
+  u32x4 s[2];
+};
+__device__ __forceinline__ float scale_of(const Scales& t, int r, int g) {
+  const uint32_t w = t.s[r >> 1][2 * (r & 1) + (g >> 1)];
   return g & 1 ? bf16hi(w) : bf16lo(w);
 }
 
@@ -208,6 +210,7 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
   __shared__ float qoff[NR][kPgNG][16];  // what the codes' offsets add to a group's product, negated
   __shared__ float qfac[ROWS];           // the power of two taken out of a row of Q
   __shared__ float mls[4][16][2];
+  __shared__ __attribute__((aligned(16))) uint32_t sbuf[I4 ? 4 : 1][2][64];  // scales of a wave's keys and values
   u32x4* qf = reinterpret_cast<u32x4*>(lds);  // [NR][hi, lo][8 steps][64 lanes]
   float* ob = reinterpret_cast<float*>(lds);  // [4 waves][16][kORow], once Q has been used
 
@@ -236,11 +239,8 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
     const int page = p.pt.page_uniform(b, min(key0, n_last) >> p.pt.shift);
     return {(((size_t)max(page, 0) * p.Hkv + kvh) << p.pt.shift) + (key0 & pmask), page >= 0};
   };
-  const uint32_t k_off = I4 ? 128 * c + 32 * a : 512 * c + 16 * a, s_off = 32 * a;
+  const uint32_t k_off = I4 ? 128 * c + 32 * a : 512 * c + 16 * a;
   const uint32_t v_off = I4 ? 128 * 4 * a + 8 * c : 16 * c;
-  // With 32 rows the values are loaded behind the round's scores and the keys' scales behind its values: at two waves per
-  // SIMD there are 256 registers, 136 of them accumulators.
-  constexpr bool kLate = I4 && NR == 2;
   // (the empty asm keeps a base in scalar registers: folded with a lane's offset it would take two vector ones; the pointer
   // is made a global one again behind it, a generic one would make flat loads, which LDS waits count too)
   typedef const __attribute__((address_space(1))) char* gptr;
@@ -249,11 +249,23 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
     asm("" : "+s"(src));
     return (gptr)src;
   };
-  auto ks_load = [&](const Tile& t, KTile<I4>& k) {
+  // The scales of a wave's 32 keys are 256 bytes, a dword a lane; they pass through LDS to the lanes that need them, four
+  // keys' of a tile each, when these need them (held by the lanes from their load on they took 32 registers).
+  auto s_load = [&](const __bf16* pages, const Tile (&t)[2]) -> uint32_t {
+    if constexpr (!I4) return 0;
+    const gptr s0 = base_of(pages, t[0].slot * 8), s1 = base_of(pages, t[1].slot * 8);
+    return *(const __attribute__((address_space(1))) uint32_t*)((lane < 32 ? s0 : s1) + 4 * (lane & 31));
+  };
+  auto s_share = [&](uint32_t mine, uint32_t* buf, Scales (&s)[2]) {
     if constexpr (I4) {
-      const gptr sc = base_of(p.ks, t.slot * 8);
-      k.s[0] = *(const __attribute__((address_space(1))) u32x4*)(sc + s_off);
-      k.s[1] = *(const __attribute__((address_space(1))) u32x4*)(sc + (s_off + 16));
+      buf[lane] = mine;
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) s[u].s[h] = *reinterpret_cast<const u32x4*>(buf + 32 * u + 8 * a + 4 * h);
     }
   };
   auto k_load = [&](const Tile& t, KTile<I4>& k) {
@@ -261,7 +273,6 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
     if constexpr (I4) {
       k.c[0] = *(const __attribute__((address_space(1))) u32x4*)(src + k_off);
       k.c[1] = *(const __attribute__((address_space(1))) u32x4*)(src + (k_off + 16));
-      if constexpr (!kLate) ks_load(t, k);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) k.c[i] = *(const __attribute__((address_space(1))) bf16x8*)(src + (k_off + 64 * i));
@@ -272,9 +283,6 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
     if constexpr (I4) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) v.c[r] = *(const __attribute__((address_space(1))) u32x2*)(src + (v_off + 128 * r));
-      const gptr sc = base_of(p.vs, t.slot * 8);
-      v.s[0] = *(const __attribute__((address_space(1))) u32x4*)(sc + s_off);
-      v.s[1] = *(const __attribute__((address_space(1))) u32x4*)(sc + (s_off + 16));
     } else {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -319,10 +327,10 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
   // than nothing: with no branch around the loads every wait counts how many of them may stay in flight.
   KTile<I4> kt[2];
   VTile<I4> vt[2];
-  Tile vtile[2] = {{0, true}, {0, true}};
   bool okv[2] = {true, true};
   int key = k0 + 32 * wave, next = key;
   Tile nt[2] = {{0, true}, {0, true}};
+  uint32_t ks_mine = 0, vs_mine = 0;
   if (key < k1) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) nt[u] = tile_at(key + 16 * u);
@@ -330,13 +338,11 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
     for (int u = 0; u < 2; ++u) {
       okv[u] = nt[u].ok;
       k_load(nt[u], kt[u]);
-      if constexpr (kLate) ks_load(nt[u], kt[u]);
     }
+    ks_mine = s_load(p.ks, nt);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if constexpr (kLate) vtile[u] = nt[u];
-      else v_load(nt[u], vt[u], key + 16 * u);
-    }
+    for (int u = 0; u < 2; ++u) v_load(nt[u], vt[u], key + 16 * u);
+    vs_mine = s_load(p.vs, nt);
     if (key + kRound < k1) next = key + kRound;
 #pragma unroll
     for (int u = 0; u < 2; ++u) nt[u] = tile_at(next + 16 * u);
@@ -430,6 +436,8 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
 #pragma unroll
       for (int i = 0; i < NR; ++i) sc[u][i] = zero4();
     if constexpr (I4) {
+      Scales ks[2];
+      s_share(ks_mine, sbuf[wave][0], ks);
 #pragma unroll
       for (int g = 0; g < kPgNG; ++g) {
         u32x4 ka[2][2];  // [tile][u]
@@ -460,7 +468,7 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
             f32x4 d = mfma16h(ka[u][0], h0, z);
             d = mfma16h(ka[u][1], h1, d);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sc[u][i][r] += scale_of(kt[u].s, r, g) * d[r];
+            for (int r = 0; r < 4; ++r) sc[u][i][r] += scale_of(ks[u], r, g) * d[r];
           }
         }
         if constexpr (NR > 1) __builtin_amdgcn_sched_barrier(0);
@@ -480,12 +488,9 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
           if (st & 1) __builtin_amdgcn_sched_barrier(0);
         }
     }
-    if constexpr (kLate) {
-      v_load(vtile[0], vt[0], key);
-      v_load(vtile[1], vt[1], key + 16);
-    }
     k_load(nt[0], kt[0]);
     k_load(nt[1], kt[1]);
+    ks_mine = s_load(p.ks, nt);
     const int after = next + kRound < k1 ? next + kRound : next;
     const Tile nn[2] = {tile_at(after), tile_at(after + 16)};
     __builtin_amdgcn_sched_barrier(0);
@@ -549,6 +554,8 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
     __builtin_amdgcn_sched_barrier(0);
     // ---- P V
     if constexpr (I4) {
+      Scales vs[2];
+      s_share(vs_mine, sbuf[wave][1], vs);
       bool odd = false;  // a scale that is not finite, next to a weight of 0
       if (masked) {
         uint32_t any = 0;
@@ -557,7 +564,7 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
 #pragma unroll
           for (int w = 0; w < 2; ++w)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) any |= ((vt[u].s[w][k] & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
+            for (int k = 0; k < 4; ++k) any |= ((vs[u].s[w][k] & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
         odd = __builtin_amdgcn_ballot_w64(any != 0) != 0;
       }
       const bf16x2 m24 = {(__bf16)-24.f, (__bf16)-24.f};
@@ -566,7 +573,7 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
         float w[NR][8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const float sv = scale_of(vt[k >> 2].s, k & 3, g);
+          const float sv = scale_of(vs[k >> 2], k & 3, g);
 #pragma unroll
           for (int i = 0; i < NR; ++i) w[i][k] = pr[i][k] * sv;
         }
@@ -685,15 +692,12 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      if constexpr (kLate) {
-        vtile[u] = nt[u];
-        ks_load(nt[u], kt[u]);
-      } else {
-        v_load(nt[u], vt[u], next + 16 * u);
-      }
+      v_load(nt[u], vt[u], next + 16 * u);
       okv[u] = nt[u].ok;
-      nt[u] = nn[u];
     }
+    vs_mine = s_load(p.vs, nt);
+    nt[0] = nn[0];
+    nt[1] = nn[1];
     key += kRound;
     next = after;
   }
