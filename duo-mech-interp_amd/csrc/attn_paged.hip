@@ -18,9 +18,16 @@
 // mantissa of a power of two: keys 1024 + n and, from the nibble above, 1024 + 16 n in fp16 (Q / 16 against it), 5
 // operations for 8 values; values 16 + n in bf16 (fp16 would not hold weight times scale). The offsets leave again: the
 // keys' products start from minus the offsets' part of the sum, formed from the same rounded Q; the values' by the sum of
-// the rounded weights times -24. Scales apply outside the codes: a key's to its group's partial score (fp32), a value's
-// to the exponential before its rounding. What bounds the 4-bit form is the vector ALU's issue (every round unpacks 64 K
-// values' nibbles), so masks and constants are kept where one v_and_or_b32 takes both.
+// the rounded weights times -24, which a product of its own collects for all four groups (row r of its A operand is -24
+// where r % 4 is the group). Scales apply outside the codes: a key's to its group's partial score (fp32), a value's to the
+// exponential before its rounding. What bounds the 4-bit form is the vector ALU's issue: about 570 operations beside 72
+// matrix products for 32 rows x 32 keys, half of them unpacking, so masks and constants are kept where one v_and_or_b32
+// takes both, scales and offsets come from LDS in the form in which they are used, and what only masked rounds or scales
+// that are not finite need stays behind branches.
+//
+// Measured (8 query and 2 key heads; a 1 GiB copy runs at 5.2 TB/s, a large bf16 product at 1190 TFLOP/s): one token for 32
+// rows of up to 8192 bf16 keys 93 to 95 us (5.1 TB/s); five tokens a row against 4-bit keys 49 us (2.7 TB/s, 119 TFLOP/s);
+// 512 tokens of one row behind 16 K 4-bit keys 122 us (497 TFLOP/s); one token of three rows of 8192 4-bit keys 14 us.
 //
 // A row's keys are dealt over S blocks in runs of whole 128-key rounds by the row's own length, read on the device: the
 // grid is sized by the table's capacity, the work by what is cached. With S > 1 the blocks leave (max, sum, acc) and a
@@ -81,15 +88,6 @@ __device__ __forceinline__ bf16x8 as_bf16x8(uint32_t a, uint32_t b, uint32_t c, 
   const u32x4 r = {a, b, c, d};
   return __builtin_bit_cast(bf16x8, r);
 }
-// The scale of key 4 a + r and group g, of a tile's (four bf16 a key).
-struct Scales {
-  u32x4 s[2];
-};
-__device__ __forceinline__ float scale_of(const Scales& t, int r, int g) {
-  const uint32_t w = t.s[r >> 1][2 * (r & 1) + (g >> 1)];
-  return g & 1 ? bf16hi(w) : bf16lo(w);
-}
-
 __device__ __forceinline__ f32x4 mfma16h(const u32x4& a, const f16x8& b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), b, c, 0, 0, 0);
 }
@@ -108,7 +106,7 @@ __device__ __forceinline__ float row16_sum(float v) {
 // the scores' B operands: bf16 hi + lo, or fp16 with its power of two in *fac and what the codes' offsets add to each
 // group's product, negated, in off[][col].
 template <bool I4>
-__device__ __forceinline__ void q_store(const f32x4 (&x)[4], int j, int col, u32x4* qf, float (*off)[16], float* fac) {
+__device__ __forceinline__ void q_store(const f32x4 (&x)[4], int j, int col, u32x4* qf, f32x4 (*off)[16], float* fac) {
   if constexpr (I4) {
     // dim 64 g + 16 a + 8 u + k is step 2 g + u of lane group a; a dword's nibbles leave it in pairs (k, k + 4), those of
     // odd k times 16
@@ -129,7 +127,7 @@ __device__ __forceinline__ void q_store(const f32x4 (&x)[4], int j, int col, u32
         o -= (e & 1 ? 1152.f : 1032.f) * (float)hq;
       }
       o = row16_sum(o);
-      if (j == 0) off[q][col] = o;
+      if (j == 0) off[q][col] = f32x4{o, o, o, o};
     }
     if (j == 0) *fac = ldexpf(1.f, ex - 5);
   } else {
@@ -152,7 +150,7 @@ __device__ __forceinline__ void q_store(const f32x4 (&x)[4], int j, int col, u32
 }
 // A lane's accumulators of its row into o[256], dims in order.
 template <bool I4>
-__device__ __forceinline__ void o_store(const f32x4 (&acc)[16], const float (&corr)[kPgNG], float* o, int a) {
+__device__ __forceinline__ void o_store(const f32x4 (&acc)[16], const f32x4& corr, float* o, int a) {
   if constexpr (I4) {
 #pragma unroll
     for (int g = 0; g < kPgNG; ++g)
@@ -207,10 +205,11 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
 
   constexpr int kQBytes = NR * QP * QF * 16, kOBytes = 4 * 16 * kORow * 4;
   __shared__ __attribute__((aligned(16))) char lds[kQBytes > kOBytes ? kQBytes : kOBytes];
-  __shared__ float qoff[NR][kPgNG][16];  // what the codes' offsets add to a group's product, negated
+  __shared__ f32x4 qoff[NR][kPgNG][16];  // what the codes' offsets add to a group's product, negated (four times: a C operand)
   __shared__ float qfac[ROWS];           // the power of two taken out of a row of Q
   __shared__ float mls[4][16][2];
-  __shared__ __attribute__((aligned(16))) uint32_t sbuf[I4 ? 4 : 1][2][64];  // scales of a wave's keys and values
+  __shared__ __attribute__((aligned(16))) float sbuf[I4 ? 4 : 1][2][kPgNG][32];  // scales of a wave's keys and values
+  __shared__ u32x4 m24[7];  // -24 eight times between zeros
   u32x4* qf = reinterpret_cast<u32x4*>(lds);  // [NR][hi, lo][8 steps][64 lanes]
   float* ob = reinterpret_cast<float*>(lds);  // [4 waves][16][kORow], once Q has been used
 
@@ -249,24 +248,25 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
     asm("" : "+s"(src));
     return (gptr)src;
   };
-  // The scales of a wave's 32 keys are 256 bytes, a dword a lane; they pass through LDS to the lanes that need them, four
-  // keys' of a tile each, when these need them (held by the lanes from their load on they took 32 registers).
+  // The scales of a wave's 32 keys are 256 bytes, a dword a lane: they pass through LDS, as fp32, to the lanes that need
+  // them, four keys' of a tile at a time (loaded by these lanes they took 32 registers and 64 operations a round more).
   auto s_load = [&](const __bf16* pages, const Tile (&t)[2]) -> uint32_t {
     if constexpr (!I4) return 0;
     const gptr s0 = base_of(pages, t[0].slot * 8), s1 = base_of(pages, t[1].slot * 8);
     return *(const __attribute__((address_space(1))) uint32_t*)((lane < 32 ? s0 : s1) + 4 * (lane & 31));
   };
-  auto s_share = [&](uint32_t mine, uint32_t* buf, Scales (&s)[2]) {
-    if constexpr (I4) {
-      buf[lane] = mine;
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) s[u].s[h] = *reinterpret_cast<const u32x4*>(buf + 32 * u + 8 * a + 4 * h);
-    }
+  auto s_share = [&](uint32_t mine, float (*buf)[32]) {
+    buf[2 * (lane & 1)][lane >> 1] = bf16lo(mine);
+    buf[2 * (lane & 1) + 1][lane >> 1] = bf16hi(mine);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  };
+  struct Scales {  // of keys 4 a + r of two tiles, one group
+    f32x4 s[2];
+  };
+  auto s_read = [&](const float (*buf)[32], int g) -> Scales {
+    return {{*reinterpret_cast<const f32x4*>(&buf[g][4 * a]), *reinterpret_cast<const f32x4*>(&buf[g][16 + 4 * a])}};
   };
   auto k_load = [&](const Tile& t, KTile<I4>& k) {
     const gptr src = base_of(p.kp, t.slot * (I4 ? 128 : 512));
@@ -397,20 +397,20 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
     seen[i] = r < R ? keys_seen(p, pos, len, r / p.G) : n_max;
   }
   f32x4 acc[NR][16];
-  float corr[NR][kPgNG];  // 4 bits: -24 times the sum of a group's weights, over this lane's keys
+  f32x4 corr[NR];  // 4 bits: -24 times the sum of the weights, of groups 0 .. 3
   float m_run[NR], l_run[NR], fac[NR];
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[i][e] = zero4();
-#pragma unroll
-    for (int g = 0; g < kPgNG; ++g) corr[i][g] = 0.f;
+    corr[i] = zero4();
     m_run[i] = -INFINITY;
     l_run[i] = 0.f;
   }
   // constants of the unpacking: the masks in scalar, the or-ed values in vector registers (one v_and_or_b32 takes both)
   uint32_t mk0 = 0x000F000Fu, mk1 = 0x00F000F0u, mv = 0x00780078u, ck = 0x64006400u, cv = 0x41804180u;
   asm("" : "+s"(mk0), "+s"(mk1), "+s"(mv), "+v"(ck), "+v"(cv));
+  if (I4 && tid < 7) m24[tid] = tid == 3 ? u32x4{0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u} : u32x4{0, 0, 0, 0};
   lds_barrier();
 #pragma unroll
   for (int i = 0; i < NR; ++i) fac[i] = qfac[16 * i + c];
@@ -422,10 +422,7 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
 #pragma unroll
     for (int k = 0; k < 8; ++k) qreg[k] = qf[64 * k + lane];
 #pragma unroll
-    for (int g = 0; g < kPgNG; ++g) {
-      const float z = qoff[0][g][c];
-      zreg[g] = f32x4{z, z, z, z};
-    }
+    for (int g = 0; g < kPgNG; ++g) zreg[g] = qoff[0][g][c];
   }
 
   while (key < k1) {
@@ -436,10 +433,10 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
 #pragma unroll
       for (int i = 0; i < NR; ++i) sc[u][i] = zero4();
     if constexpr (I4) {
-      Scales ks[2];
-      s_share(ks_mine, sbuf[wave][0], ks);
+      s_share(ks_mine, sbuf[wave][0]);
 #pragma unroll
       for (int g = 0; g < kPgNG; ++g) {
+        const Scales ks = s_read(sbuf[wave][0], g);
         u32x4 ka[2][2];  // [tile][u]
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -460,15 +457,14 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
             const u32x4* qi = qf + (size_t)i * QF + 2 * g * 64 + lane;
             h0 = __builtin_bit_cast(f16x8, qi[0]);
             h1 = __builtin_bit_cast(f16x8, qi[64]);
-            const float z1 = qoff[i][g][c];
-            z = f32x4{z1, z1, z1, z1};
+            z = qoff[i][g][c];
           }
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             f32x4 d = mfma16h(ka[u][0], h0, z);
             d = mfma16h(ka[u][1], h1, d);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sc[u][i][r] += scale_of(ks[u], r, g) * d[r];
+            for (int r = 0; r < 4; ++r) sc[u][i][r] += ks.s[u][r] * d[r];
           }
         }
         if constexpr (NR > 1) __builtin_amdgcn_sched_barrier(0);
@@ -554,46 +550,33 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
     __builtin_amdgcn_sched_barrier(0);
     // ---- P V
     if constexpr (I4) {
-      Scales vs[2];
-      s_share(vs_mine, sbuf[wave][1], vs);
-      bool odd = false;  // a scale that is not finite, next to a weight of 0
-      if (masked) {
-        uint32_t any = 0;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int w = 0; w < 2; ++w)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) any |= ((vs[u].s[w][k] & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
-        odd = __builtin_amdgcn_ballot_w64(any != 0) != 0;
-      }
-      const bf16x2 m24 = {(__bf16)-24.f, (__bf16)-24.f};
+      s_share(vs_mine, sbuf[wave][1]);
+      // a scale that is not finite or may make a weight so (2^118 and more)
+      const bool wild = __builtin_amdgcn_ballot_w64((((vs_mine & 0x7F807F80u) + 0x05800580u) & 0x80008000u) != 0) != 0;
 #pragma unroll
       for (int g = 0; g < kPgNG; ++g) {
+        const Scales vs = s_read(sbuf[wave][1], g);
         float w[NR][8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float sv = scale_of(vs[k >> 2], k & 3, g);
+        for (int k = 0; k < 8; ++k)
 #pragma unroll
-          for (int i = 0; i < NR; ++i) w[i][k] = pr[i][k] * sv;
-        }
-        if (odd) {
+          for (int i = 0; i < NR; ++i) w[i][k] = pr[i][k] * vs.s[k >> 2][k & 3];
+        if (wild && masked) {
           // a key that a row does not see weighs nothing there, whatever its scale is
 #pragma unroll
           for (int i = 0; i < NR; ++i)
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
+            for (int k = 0; k < 8; ++k) {
+              asm volatile("" : "+v"(pr[i][k]));  // (keeps the comparisons inside the branch)
               if (pr[i][k] == 0.f) w[i][k] = 0.f;
+            }
         }
         bf16x8 pg[NR];
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
           u32x4 pw;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            pw[k] = cvt2(w[i][2 * k], w[i][2 * k + 1]);
-            corr[i][g] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, (uint32_t)pw[k]), m24, corr[i][g], false);
-          }
+          for (int k = 0; k < 4; ++k) pw[k] = cvt2(w[i][2 * k], w[i][2 * k + 1]);
           pg[i] = __builtin_bit_cast(bf16x8, pw);
         }
         uint32_t x[4];
@@ -610,6 +593,22 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
 #pragma unroll
           for (int i = 0; i < NR; ++i) acc[i][4 * g + e] = mfma16(va, pg[i], acc[i][4 * g + e]);
         }
+        if (wild) {
+          // (not finite: has reached its own group's sums, and must not the other groups')
+#pragma unroll
+          for (int i = 0; i < NR; ++i) {
+            u32x4 pw = __builtin_bit_cast(u32x4, pg[i]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if ((pw[k] & 0x7F80u) == 0x7F80u) pw[k] &= 0xFFFF0000u;
+              if ((pw[k] & 0x7F800000u) == 0x7F800000u) pw[k] &= 0xFFFFu;
+            }
+            pg[i] = __builtin_bit_cast(bf16x8, pw);
+          }
+        }
+        const bf16x8 off = __builtin_bit_cast(bf16x8, m24[(c & 3) + 3 - g]);  // -24 in the rows of group g
+#pragma unroll
+        for (int i = 0; i < NR; ++i) corr[i] = mfma16(off, pg[i], corr[i]);
         if constexpr (NR > 1) __builtin_amdgcn_sched_barrier(0);
       }
     } else {
@@ -709,13 +708,6 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
     float l = l_run[i];
     lane_pair q = lane_swap<16>(l);
     l = add_xor<32>(q.a + q.b);
-    if constexpr (I4) {
-#pragma unroll
-      for (int g = 0; g < kPgNG; ++g) {
-        q = lane_swap<16>(corr[i][g]);
-        corr[i][g] = add_xor<32>(q.a + q.b);
-      }
-    }
     lds_barrier();  // Q, or the rows before these, have been used
     if (r0 + 16 * i + c < R) {
       o_store<I4>(acc[i], corr[i], ob + ((size_t)wave * 16 + c) * kORow, a);
