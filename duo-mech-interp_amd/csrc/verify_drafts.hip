@@ -49,10 +49,10 @@ struct VerifyArgs {
 __device__ __forceinline__ int v_len(const VerifyArgs& p, int b) {
   return p.lens ? min(max(load_uniform(p.lens + b), 0), p.K) : p.K;
 }
-// log2(e) / temperature, 0 for the argmax (an infinite temperature leaves the tokens above -inf alike)
+// 32 log2(e) / temperature, 0 for the argmax (an infinite temperature leaves the tokens above -inf alike)
 __device__ __forceinline__ double v_inv_temp(const VerifyArgs& p, int b) {
   const float t = p.temps ? __int_as_float(load_uniform(reinterpret_cast<const int32_t*>(p.temps) + b)) : p.temp;
-  return t > 0.f ? fmax(1.4426950408889634074 / (double)t, 1e-300) : 0.0;
+  return t > 0.f ? fmax(32.0 * 1.4426950408889634074 / (double)t, 1e-300) : 0.0;
 }
 // The position's draft when it is a token, else -1
 __device__ __forceinline__ int v_draft(const VerifyArgs& p, int b, int i, int len) {
@@ -61,28 +61,34 @@ __device__ __forceinline__ int v_draft(const VerifyArgs& p, int b, int i, int le
   return id >= 0 && id < p.V ? id : -1;
 }
 
-// 2^y for y <= 0 to 1e-11 relative: y = n + f with |f| <= 1/2, the Taylor series of 2^f = e^(f ln 2) to f^9 (the rest is
-// below (ln 2 / 2)^10 / 10! = 7e-12; y's own rounding adds 2^-53 |y|). 14 operations of 64 bits; the library's full-range exp
-// takes 45.
-__device__ __forceinline__ double exp2_neg(double y) {
-  constexpr double L = 0.69314718055994530942, L2 = L * L, L4 = L2 * L2, L8 = L4 * L4;
-  y = fmax(y, -1100.0);  // 0 from there on, also for -inf
-  const double n = __builtin_rint(y), f = y - n;
-  double e = L8 * L / 362880.0;
-  e = __builtin_fma(e, f, L8 / 40320.0);
-  e = __builtin_fma(e, f, L4 * L2 * L / 5040.0);
-  e = __builtin_fma(e, f, L4 * L2 / 720.0);
-  e = __builtin_fma(e, f, L4 * L / 120.0);
-  e = __builtin_fma(e, f, L4 / 24.0);
-  e = __builtin_fma(e, f, L2 * L / 6.0);
-  e = __builtin_fma(e, f, L2 / 2.0);
-  e = __builtin_fma(e, f, L);
-  e = __builtin_fma(e, f, 1.0);
-  return __builtin_ldexp(e, (int)n);
+// 2^(z / 32) for z <= 0 to 2e-12 relative: z = 32 n + j + r with |r| <= 1/2, as 2^n 2^(j / 32) 2^(r / 32): a table in LDS (32
+// entries of 8 bytes, one pair of banks each: no conflicts) and the Taylor series of e^(r ln 2 / 32) to r^4 (the rest is
+// below (ln 2 / 64)^5 / 5! = 1.3e-12; z's own rounding adds 2^-53 |z| / 32). 11 operations of 64 bits; a series over |f| <= 1/2
+// to f^9 takes 14, and these operations are what bounds the passes over the vocabulary (32 rows of up to 8 drafts: 28.7 us
+// with 14, 19.3 without any).
+constexpr int kVTab = 32;
+__device__ __forceinline__ double exp2_neg(double z, const double* tab) {
+  constexpr double c1 = 0.69314718055994530942 / kVTab, c2 = c1 * c1 / 2.0, c3 = c1 * c2 / 3.0, c4 = c1 * c3 / 4.0;
+  z = fmax(z, -1100.0 * kVTab);  // 0 from there on, also for -inf
+  const double n = __builtin_rint(z), r = z - n;
+  const int k = (int)n;
+  const double e = __builtin_fma(__builtin_fma(__builtin_fma(__builtin_fma(c4, r, c3), r, c2), r, c1), r, 1.0);
+  return __builtin_ldexp(e * tab[k & (kVTab - 1)], k >> 5);
 }
-// exp((x - m) / T) for x <= m (no NaN), inv_t = log2(e) / T: 1 at the maximum, also an infinite one.
-__device__ __forceinline__ double v_weight(float x, float m, double inv_t) {
-  return x == m ? 1.0 : exp2_neg(((double)x - (double)m) * inv_t);
+// Threads 0 .. 31 fill the table (a barrier before its use is the caller's): the series of 2^f to f^13, |f| <= 1/2.
+__device__ __forceinline__ void exp2_table(double* tab, int tid) {
+  if (tid >= kVTab) return;
+  constexpr double L = 0.69314718055994530942;
+  const bool up = 2 * tid > kVTab;
+  const double f = (double)(up ? tid - kVTab : tid) * (L / kVTab);
+  double e = 1.0;
+#pragma unroll
+  for (int k = 13; k > 0; --k) e = __builtin_fma(e * (1.0 / k), f, 1.0);
+  tab[tid] = up ? 2.0 * e : e;
+}
+// exp((x - m) / T) for x <= m (no NaN), inv_t = 32 log2(e) / T: 1 at the maximum, also an infinite one.
+__device__ __forceinline__ double v_weight(float x, float m, double inv_t, const double* tab) {
+  return x == m ? 1.0 : exp2_neg(((double)x - (double)m) * inv_t, tab);
 }
 // A NaN counts as -inf.
 __device__ __forceinline__ float v_clean(float x) { return fmaxf(x, -INFINITY); }
@@ -126,7 +132,8 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs p) {
   v_load_chunk(p.x + b * p.xb + i * p.xp, base, p.V, tid, x, -INFINITY);
   __shared__ float sm[4];
   __shared__ int si[4];
-  __shared__ double ss[4];
+  __shared__ double ss[4], tab[kVTab];
+  exp2_table(tab, tid);
   float m = -INFINITY;
 #pragma unroll
   for (int k = 0; k < kVPer; ++k) {
@@ -147,7 +154,7 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs p) {
     }
     if (fabsf(m) < INFINITY) {
 #pragma unroll
-      for (int k = 0; k < kVPer; ++k) s += exp2_neg(((double)x[k] - (double)m) * inv_t);
+      for (int k = 0; k < kVPer; ++k) s += exp2_neg(((double)x[k] - (double)m) * inv_t, tab);
     } else {
 #pragma unroll
       for (int k = 0; k < kVPer; ++k) s += x[k] == m ? 1.0 : 0.0;
@@ -179,10 +186,12 @@ struct VFold {
   double inv_z[kVMaxK + 1];
   float max[kVMaxK + 1], x[kVMaxK + 1], q[kVMaxK + 1], u[kVMaxK + 1];
   int idx[kVMaxK + 1], keep[kVMaxK + 1], draft[kVMaxK + 1];
+  double tab[kVTab];
 };
 template <int THREADS>
 __device__ __forceinline__ int v_fold(const VerifyArgs& p, int b, int len, double inv_t, int tid, VFold& f) {
   const int lane = tid & 63, wave = tid >> 6, per = max(kVFold / p.C, 1);
+  exp2_table(f.tab, tid);
   if (tid < p.K) {  // (whether the row has this position is known later than its draft)
     const int id = p.ids[b * p.idb + tid];
     const bool token = id >= 0 && id < p.V;
@@ -206,12 +215,12 @@ __device__ __forceinline__ int v_fold(const VerifyArgs& p, int b, int len, doubl
       int idx = 0x7fffffff;
       for (int k = lane; k < p.C; k += 64) {
         const VStat s = st[k];
-        if (s.max > -INFINITY) z += s.sum * v_weight(s.max, M, inv_t);
+        if (s.max > -INFINITY) z += s.sum * v_weight(s.max, M, inv_t, f.tab);
         if (s.max == M) idx = min(idx, s.idx);
       }
       z = wave_sum64(z);
       if (!(inv_t > 0.0)) idx = wave_min_i32(idx);
-      const double wd = draft >= 0 && M > -INFINITY ? v_weight(f.x[i], M, inv_t) : 0.0;
+      const double wd = draft >= 0 && M > -INFINITY ? v_weight(f.x[i], M, inv_t, f.tab) : 0.0;
       z += wd;
       if (lane == 0) {
         const double pr = inv_t > 0.0 ? wd / z : draft == idx ? 1.0 : 0.0;
@@ -245,7 +254,7 @@ __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs p) {
   v_load_chunk(p.q + b * p.qb + n * p.qp, base, p.V, tid, q, 0.f);
   double s = 0.0;
 #pragma unroll
-  for (int k = 0; k < kVPer; ++k) s += fmax(v_weight(v_clean(x[k]), M, inv_t) * inv_z - (double)q[k], 0.0);
+  for (int k = 0; k < kVPer; ++k) s += fmax(v_weight(v_clean(x[k]), M, inv_t, f.tab) * inv_z - (double)q[k], 0.0);
   s = wave_sum64(s);
   __shared__ double ss[4];
   if (lane == 0) ss[wave] = s;
@@ -278,8 +287,8 @@ __global__ __launch_bounds__(1024) void verify_draw_kernel(VerifyArgs p) {
           w = p.mass[(size_t)b * p.C + k];
         } else {
           const VStat s = here ? f.st[n * p.C + k] : st[k];
-          w = s.max > -INFINITY ? s.sum * v_weight(s.max, M, inv_t) : 0.0;
-          if (kind == 2 && draft >= 0 && k == draft / kVChunk) w += v_weight(f.x[n], M, inv_t);
+          w = s.max > -INFINITY ? s.sum * v_weight(s.max, M, inv_t, f.tab) : 0.0;
+          if (kind == 2 && draft >= 0 && k == draft / kVChunk) w += v_weight(f.x[n], M, inv_t, f.tab);
           w *= inv_z;
         }
         chunk_w[k] = w;
@@ -348,7 +357,7 @@ __global__ __launch_bounds__(1024) void verify_draw_kernel(VerifyArgs p) {
     for (int k = 0; k < PER; ++k) xv[k] = v_clean(xv[k]);
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      double v = v_weight(xv[k], M, inv_t) * inv_z;
+      double v = v_weight(xv[k], M, inv_t, f.tab) * inv_z;
       if (kind == 0) v = fmax(v - (double)qv[k], 0.0);
       if (kind == 1 && base + k == draft) v = 0.0;
       w[k] = v;
