@@ -32,6 +32,8 @@
 // A row's keys are dealt over S blocks in runs of whole 128-key rounds by the row's own length, read on the device: the
 // grid is sized by the table's capacity, the work by what is cached. With S > 1 the blocks leave (max, sum, acc) and a
 // second kernel merges them; blocks whose run is empty leave nothing and are not read.
+#include <algorithm>
+
 #include "paged_kv.h"
 
 namespace q35 {
@@ -820,16 +822,20 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs p) 
   out_store(p, O, L, true, g, b, t, h, d0);
 }
 
-// Query rows per block (in 16s) and runs per row: two blocks per CU, but one where that leaves a block no more than two
-// rounds (three rows of 8192 4-bit keys: 64 runs 17.2 us, 32 runs 15.3, 16 runs 18.8). A table of two rounds is not split
+// Query rows per block, in 16s: two, which halves the unpacking and the LDS reads per row, but one where all rows fit in it
+// (32 rows of up to 8192 keys, one token of four heads: bf16 95.9 us against 102.6, 4 bits 37.7 against 43.3) and for three
+// 16s against codes, a quarter of whose work would be for rows that are not there (nine tokens of four heads: 64.6 against
+// 70.7; 512 tokens, where none are: 150 against 123, bf16 303 against 185; five tokens, two 16s: 52.8 against 49.3).
+// Runs per row: two blocks per CU, but one where that leaves a block no more than two
+// rounds (three rows of 8192 4-bit keys: 64 runs 16.1 us, 32 runs 14.1, 16 runs 16.7). A table of two rounds is not split
 // (256 keys, one row: 11.9 us against 12.5 for two runs and their merge, 4 bits 9.9 against 11.2; four rounds 16.4 against
 // 12.7, 4 bits 12.6 against 11.3).
 struct PagedPlan {
   int NR, RB, S;
 };
-static PagedPlan paged_plan(int64_t B, int64_t T, int64_t Hkv, int64_t G, int64_t capacity, int64_t splits) {
-  const int64_t R = T * G;
-  const int NR = R <= 16 ? 1 : 2;
+static PagedPlan paged_plan(int64_t B, int64_t T, int64_t Hkv, int64_t G, int64_t capacity, int64_t splits, int fmt) {
+  const int64_t R = T * G, tiles = (R + 15) / 16;
+  const int NR = tiles == 1 || (tiles == 3 && fmt == Q35_I4_G64) ? 1 : 2;
   const int64_t RB = (R + 16 * NR - 1) / (16 * NR), base = B * Hkv * RB;
   const int64_t most = (capacity + kRound - 1) / kRound;
   int64_t S = splits;
@@ -852,9 +858,11 @@ extern "C" size_t q35_gated_attn_paged_workspace_bytes(int64_t B, int64_t T, int
   if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || D != kPgD || Hq % Hkv || n_blocks <= 0 || page_size <= 0 ||
       B > 65535 || T > (1 << 24) || Hq > 4096 || n_blocks > (1 << 26) || page_size > 1024)
     return 0;
-  const PagedPlan pl = paged_plan(B, T, Hkv, Hq / Hkv, n_blocks * page_size, splits);
-  if (pl.S == 1) return 256;
-  return (size_t)B * T * Hq * pl.S * (kPgD + 2) * sizeof(float);
+  int S = 0;  // the larger of the two formats'
+  for (const int fmt : {(int)Q35_BF16, (int)Q35_I4_G64})
+    S = std::max(S, paged_plan(B, T, Hkv, Hq / Hkv, n_blocks * page_size, splits, fmt).S);
+  if (S == 1) return 256;
+  return (size_t)B * T * Hq * S * (kPgD + 2) * sizeof(float);
 }
 
 extern "C" int q35_gated_attn_paged(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* gate,
@@ -880,7 +888,7 @@ extern "C" int q35_gated_attn_paged(const void* q, int64_t q_sb, int64_t q_st, i
     return Q35_EUNSUPPORTED;
   const int64_t G = Hq / Hkv;
   if (Hq > 4096 || T * G > (1 << 24)) return Q35_EUNSUPPORTED;
-  const PagedPlan pl = paged_plan(B, T, Hkv, G, n_blocks * page_size, splits);
+  const PagedPlan pl = paged_plan(B, T, Hkv, G, n_blocks * page_size, splits, fmt);
   if (Hkv * pl.RB > 65535 || T * Hq > 0x7fffffff) return Q35_EUNSUPPORTED;
   const size_t rows = (size_t)B * T * Hq * pl.S;
   if (pl.S > 1 && (!workspace || workspace_bytes < rows * (kPgD + 2) * sizeof(float) || (uintptr_t)workspace & 15))

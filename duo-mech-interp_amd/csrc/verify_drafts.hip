@@ -15,6 +15,11 @@
 // random number falls and the token in it. A refusal with draft probabilities needs the sums of max(p - q, 0), which
 // depend on n: verify_mass_kernel between the two forms them (every block of a row finds the same n, from the same numbers
 // in the same order). Nothing depends on the order in which blocks run.
+//
+// Measured, V = 151,936: three rows of 4 certain drafts 12 us (statistics 5.3, draw 8: a launch and a chain of dependent loads
+// each); 32 rows of 0 .. 8 drafts with probabilities 47 us (statistics 26 for 97 MB, 3.7 TB/s; mass 12; draw 9), 43 with the
+// launches overlapped in a stream of calls. Chunks of 8192, or several positions a block, measured slower: the statistics
+// kernel hides its loads by many short blocks.
 #include "q35_common.h"
 #include "q35hip.h"
 
@@ -63,9 +68,9 @@ __device__ __forceinline__ int v_draft(const VerifyArgs& p, int b, int i, int le
 
 // 2^(z / 32) for z <= 0 to 2e-12 relative: z = 32 n + j + r with |r| <= 1/2, as 2^n 2^(j / 32) 2^(r / 32): a table in LDS (32
 // entries of 8 bytes, one pair of banks each: no conflicts) and the Taylor series of e^(r ln 2 / 32) to r^4 (the rest is
-// below (ln 2 / 64)^5 / 5! = 1.3e-12; z's own rounding adds 2^-53 |z| / 32). 11 operations of 64 bits; a series over |f| <= 1/2
-// to f^9 takes 14, and these operations are what bounds the passes over the vocabulary (32 rows of up to 8 drafts: 28.7 us
-// with 14, 19.3 without any).
+// below (ln 2 / 64)^5 / 5! = 1.3e-12; z's own rounding adds 2^-53 |z| / 32). 11 operations of 64 bits where a series over
+// |f| <= 1/2 to f^9 takes 14: they come on top of the loads in the passes over the vocabulary (statistics of 32 rows of up to
+// 8 drafts: 28.7 us with 14, 26.3 with 11, 19.3 with one).
 constexpr int kVTab = 32;
 __device__ __forceinline__ double exp2_neg(double z, const double* tab) {
   constexpr double c1 = 0.69314718055994530942 / kVTab, c2 = c1 * c1 / 2.0, c3 = c1 * c2 / 3.0, c4 = c1 * c3 / 4.0;

@@ -495,6 +495,17 @@ def test_attention_over_a_prompt(fmt):
     check_attention(d, attend(to(d, device())))
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "int4"])
+@pytest.mark.parametrize("T,Hq,lens", [(9, 4, [9, 4]), (12, 4, [12, 1]), (17, 3, [0, 17]), (13, 5, [13, 13])])
+def test_attention_rows_over_three_to_five_tiles(fmt, T, Hq, lens):
+    """36, 48, 51 and 65 query rows of one key head, over keys in one run and in several."""
+    d = make(fmt, 2, T, Hq, 1, 16, [600, 40], lens=lens)
+    announce(f"paged attention {fmt} T {T} heads {Hq} lens {lens}")
+    g = to(d, device())
+    for splits in (0, 1, 4):
+        check_attention(d, attend(g, splits=splits))
+
+
 @pytest.mark.parametrize("T", [1, 6])
 def test_attention_more_splits_than_rounds(T):
     d = make("int4", 2, T, 8, 2, 32, [3000, 130])
