@@ -26,8 +26,9 @@
 // that are not finite need stays behind branches.
 //
 // Measured (8 query and 2 key heads; a 1 GiB copy runs at 5.2 TB/s, a large bf16 product at 1190 TFLOP/s): one token for 32
-// rows of up to 8192 bf16 keys 93 to 95 us (5.1 TB/s); five tokens a row against 4-bit keys 49 us (2.7 TB/s, 119 TFLOP/s);
-// 512 tokens of one row behind 16 K 4-bit keys 122 us (497 TFLOP/s); one token of three rows of 8192 4-bit keys 14 us.
+// rows of up to 8192 bf16 keys 93 to 95 us (5.1 TB/s); five tokens a row against 4-bit keys 47 us (2.8 TB/s, 124 TFLOP/s);
+// 512 tokens of one row behind 16 K 4-bit keys 116 us (524 TFLOP/s), bf16 185; one token of three rows of 8192 4-bit keys
+// 14 us.
 //
 // A row's keys are dealt over S blocks in runs of whole 128-key rounds by the row's own length, read on the device: the
 // grid is sized by the table's capacity, the work by what is cached. With S > 1 the blocks leave (max, sum, acc) and a
@@ -752,12 +753,17 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
   }
 }
 
-// The runs of one query row joined: block = (row, kv head) x batch row, wave w folds runs w, w + 4, ..., eight runs'
-// loads in flight.
+// The runs of a query row (of batch row blockIdx.y) joined, U runs' loads in flight: by one wave, four rows a block, while
+// that takes one go, else by the block's four waves, wave w folding runs w, w + 4, ... (512 tokens of 8 heads in 4 runs 5.4 us
+// by one wave a row, 12.4 by four; 32 rows of five tokens in 8 runs 4.2 and 6.0).
+template <int W, int U>
 __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs p) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d0 = 4 * lane;
-  const int kvh = blockIdx.x % p.Hkv, r = blockIdx.x / p.Hkv, b = blockIdx.y;
+  const int lane = threadIdx.x & 63, d0 = 4 * lane;
+  const int wave = W == 1 ? 0 : threadIdx.x >> 6;
+  const int row = W == 1 ? 4 * (int)blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : (int)blockIdx.x;
+  const int kvh = row % p.Hkv, r = row / p.Hkv, b = blockIdx.y;
   const int R = p.T * p.G, t = r / p.G, h = kvh * p.G + r - t * p.G;
+  if (W == 1 && r >= R) return;
   const int64_t pos = load_uniform(p.pos + b);
   const int len = p.lens ? min(max(load_uniform(p.lens + b), 0), p.T) : p.T;
   const int seen = keys_seen(p, pos, len, t);
@@ -769,13 +775,13 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs p) 
   const size_t base = (((size_t)b * p.Hkv + kvh) * R + r) * p.S;
   float M = -INFINITY, L = 0.f;
   f32x4 O = zero4();
-  // the first eight runs are loaded without knowing n (slots of the workspace, whatever they hold), the gate with them
-  f32x4 pv[8];
-  float m[8], l[8];
+  // the first runs are loaded without knowing n (slots of the workspace, whatever they hold), the gate with them
+  f32x4 pv[U];
+  float m[U], l[U];
   auto load = [&](int s0) {
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const size_t s = base + min(s0 + 4 * u, p.S - 1);
+    for (int u = 0; u < U; ++u) {
+      const size_t s = base + min(s0 + W * u, p.S - 1);
       pv[u] = *reinterpret_cast<const f32x4*>(p.part + s * kPgD + d0);
       m[u] = p.ml[2 * s];
       l[u] = p.ml[2 * s + 1];
@@ -784,18 +790,32 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs p) 
   load(wave);
   const f32x4 g = gate_load(p, b, t, h, d0);
   __builtin_amdgcn_sched_barrier(0);
-  for (int s0 = wave; s0 < n; s0 += 32) {
+  for (int s0 = wave; s0 < n; s0 += W * U) {
     if (s0 != wave) load(s0);
+    // (selects, not branches, so that all loads are in flight together; a slot past n may hold anything)
+    float mn = M;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      if (s0 + 4 * u >= n || m[u] == -INFINITY) continue;
-      const float mn = fmaxf(M, m[u]);
-      const float c0 = __builtin_amdgcn_exp2f(M - mn), c1 = __builtin_amdgcn_exp2f(m[u] - mn);
-      L = L * c0 + l[u] * c1;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) O[e] = O[e] * c0 + pv[u][e] * c1;
-      M = mn;
+    for (int u = 0; u < U; ++u) {
+      m[u] = s0 + W * u < n ? m[u] : -INFINITY;
+      mn = fmaxf(mn, m[u]);
     }
+    const float c0 = M > -INFINITY ? __builtin_amdgcn_exp2f(M - mn) : 0.f;
+    L *= c0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) O[e] *= c0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = m[u] > -INFINITY;
+      const float c1 = in ? __builtin_amdgcn_exp2f(m[u] - mn) : 0.f;
+      L += in ? l[u] * c1 : 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) O[e] += in ? pv[u][e] * c1 : 0.f;
+    }
+    M = mn;
+  }
+  if constexpr (W == 1) {
+    out_store(p, O, L, true, g, b, t, h, d0);
+    return;
   }
   __shared__ float gm[4], gl[4];
   __shared__ f32x4 go[4][64];
@@ -916,7 +936,9 @@ extern "C" int q35_gated_attn_paged(const void* q, int64_t q_sb, int64_t q_st, i
     if (pl.NR == 1) Q35_PAGED(true, 1); else Q35_PAGED(true, 2);
   }
 #undef Q35_PAGED
-  if (pl.S > 1)
-    hipLaunchKernelGGL(paged_attn_merge_kernel, dim3((unsigned)(T * Hq), (unsigned)B), block, 0, st, a);
+  const unsigned n = (unsigned)(T * Hq);
+  if (pl.S > 8) hipLaunchKernelGGL((paged_attn_merge_kernel<4, 8>), dim3(n, (unsigned)B), block, 0, st, a);
+  else if (pl.S > 4) hipLaunchKernelGGL((paged_attn_merge_kernel<1, 8>), dim3((n + 3) / 4, (unsigned)B), block, 0, st, a);
+  else if (pl.S > 1) hipLaunchKernelGGL((paged_attn_merge_kernel<1, 4>), dim3((n + 3) / 4, (unsigned)B), block, 0, st, a);
   return hipGetLastError() == hipSuccess ? Q35_OK : Q35_ELAUNCH;
 }
