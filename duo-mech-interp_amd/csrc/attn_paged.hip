@@ -27,7 +27,7 @@
 //
 // Measured (8 query and 2 key heads; a 1 GiB copy runs at 5.2 TB/s, a large bf16 product at 1190 TFLOP/s): one token for 32
 // rows of up to 8192 bf16 keys 93 to 95 us (5.1 TB/s); five tokens a row against 4-bit keys 47 us (2.8 TB/s, 124 TFLOP/s);
-// 512 tokens of one row behind 16 K 4-bit keys 116 us (524 TFLOP/s), bf16 185; one token of three rows of 8192 4-bit keys
+// 512 tokens of one row behind 16 K 4-bit keys 116 us (524 TFLOP/s), bf16 167; one token of three rows of 8192 4-bit keys
 // 14 us.
 //
 // A row's keys are dealt over S blocks in runs of whole 128-key rounds by the row's own length, read on the device: the
@@ -148,7 +148,6 @@ __device__ __forceinline__ void q_store(const f32x4 (&x)[4], int j, int col, u32
       *reinterpret_cast<bf16x4*>(qe + q * 1024) = hi;
       *reinterpret_cast<bf16x4*>(qe + 8 * 64 * 8 + q * 1024) = lo;
     }
-    if (j == 0) *fac = 1.f;
   }
 }
 // A lane's accumulators of its row into o[256], dims in order.
@@ -199,7 +198,7 @@ __device__ __forceinline__ void out_store(const PagedAttnArgs& p, const f32x4& O
 }
 
 template <bool I4, int NR>
-__global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(PagedAttnArgs p) {
+__global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttnArgs p) {
   constexpr int ROWS = 16 * NR, QP = I4 ? 1 : 2, QF = 8 * 64;  // parts of Q, 16-byte operands of one
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, a = lane >> 4;
@@ -281,6 +280,10 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
       for (int i = 0; i < 8; ++i) k.c[i] = *(const __attribute__((address_space(1))) bf16x8*)(src + (k_off + 64 * i));
     }
   };
+  // 32 rows against bf16: K's and V's operands share 64 registers (at two waves per SIMD there are 256, 136 of them
+  // accumulators). As the scores release K's, V's are loaded, and the next K's as the sums release V's (512 tokens behind 16 K
+  // keys 167 us; with registers for both, at one wave per SIMD, 185).
+  constexpr bool kTurns = !I4 && NR == 2;
   auto v_load = [&](const Tile& t, VTile<I4>& v, int key0) {
     const gptr src = base_of(p.vp, t.slot * (I4 ? 128 : 512));
     if constexpr (I4) {
@@ -294,6 +297,16 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
         v.c[r][0] = *(const __attribute__((address_space(1))) u32x4*)(src + (v_off + 512 * row));
         v.c[r][1] = *(const __attribute__((address_space(1))) u32x4*)(src + (v_off + 512 * row + 256));
       }
+    }
+  };
+  auto k_part = [&](const Tile& t, KTile<I4>& k, int st) {
+    if constexpr (kTurns)
+      k.c[st] = *(const __attribute__((address_space(1))) bf16x8*)(base_of(p.kp, t.slot * 512) + (k_off + 64 * st));
+  };
+  auto v_part = [&](const Tile& t, VTile<I4>& v, int key0, int a4, int w, int r) {
+    if constexpr (kTurns) {
+      const uint32_t row = max(min(a4 + r, n_last - key0), 0);
+      v.c[r][w] = *(const __attribute__((address_space(1))) u32x4*)(base_of(p.vp, t.slot * 512) + (v_off + 512 * row + 256 * w));
     }
   };
 
@@ -332,7 +345,7 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
   VTile<I4> vt[2];
   bool okv[2] = {true, true};
   int key = k0 + 32 * wave, next = key;
-  Tile nt[2] = {{0, true}, {0, true}};
+  Tile nt[2] = {{0, true}, {0, true}}, vt_at[2] = {{0, true}, {0, true}};
   uint32_t ks_mine = 0, vs_mine = 0;
   if (key < k1) {
 #pragma unroll
@@ -343,8 +356,12 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
       k_load(nt[u], kt[u]);
     }
     ks_mine = s_load(p.ks, nt);
+    if constexpr (!kTurns) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) v_load(nt[u], vt[u], key + 16 * u);
+      for (int u = 0; u < 2; ++u) v_load(nt[u], vt[u], key + 16 * u);
+    }
+    vt_at[0] = nt[0];
+    vt_at[1] = nt[1];
     vs_mine = s_load(p.vs, nt);
     if (key + kRound < k1) next = key + kRound;
 #pragma unroll
@@ -416,7 +433,7 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
   if (I4 && tid < 7) m24[tid] = tid == 3 ? u32x4{0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u, 0xC1C0C1C0u} : u32x4{0, 0, 0, 0};
   lds_barrier();
 #pragma unroll
-  for (int i = 0; i < NR; ++i) fac[i] = qfac[16 * i + c];
+  for (int i = 0; i < NR; ++i) fac[i] = I4 ? qfac[16 * i + c] : 1.f;
   // 16 rows against codes: Q's operands and the offsets stay in registers
   constexpr bool kQReg = I4 && NR == 1;
   u32x4 qreg[kQReg ? 8 : 1];
@@ -429,6 +446,8 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
   }
 
   while (key < k1) {
+    int a4 = 4 * a;
+    if constexpr (kTurns) asm volatile("" : "+v"(a4));  // (else 4 a + r are four more registers through the loop)
     // ---- scores, two tiles of 16 keys against each 16 rows
     f32x4 sc[2][NR];
 #pragma unroll
@@ -484,11 +503,19 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
             sc[u][i] = mfma16(kt[u].c[st], hi, sc[u][i]);
             sc[u][i] = mfma16(kt[u].c[st], lo, sc[u][i]);
           }
-          if (st & 1) __builtin_amdgcn_sched_barrier(0);
+          if (!kTurns && (st & 1)) __builtin_amdgcn_sched_barrier(0);
+          if (kTurns && i == NR - 1) {
+            __builtin_amdgcn_sched_barrier(0);
+            v_part(vt_at[0], vt[0], key, a4, st >> 2, st & 3);
+            v_part(vt_at[1], vt[1], key + 16, a4, st >> 2, st & 3);
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
     }
-    k_load(nt[0], kt[0]);
-    k_load(nt[1], kt[1]);
+    if constexpr (!kTurns) {
+      k_load(nt[0], kt[0]);
+      k_load(nt[1], kt[1]);
+    }
     ks_mine = s_load(p.ks, nt);
     const int after = next + kRound < k1 ? next + kRound : next;
     const Tile nn[2] = {tile_at(after), tile_at(after + 16)};
@@ -502,7 +529,7 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (key + 16 * u + 4 * a + r >= seen[i] || !okv[u]) sc[u][i][r] = -INFINITY;
+            if (key + 16 * u + a4 + r >= seen[i] || !okv[u]) sc[u][i][r] = -INFINITY;
     }
     // ---- running maximum (with a slack of 2^8 before the accumulators are rescaled) and the exponentials
     float pr[NR][8], mx[NR];
@@ -615,14 +642,6 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
         if constexpr (NR > 1) __builtin_amdgcn_sched_barrier(0);
       }
     } else {
-      bf16x8 pg[NR];
-#pragma unroll
-      for (int i = 0; i < NR; ++i) {
-        u32x4 pw;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) pw[k] = cvt2(pr[i][2 * k], pr[i][2 * k + 1]);
-        pg[i] = __builtin_bit_cast(bf16x8, pw);
-      }
       bool odd = false;  // a value that is not finite, next to a weight of 0
       if (masked) {
         uint32_t any = 0;
@@ -649,11 +668,13 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
                 const uint32_t word = vt[j >> 2].c[j & 3][w][k];
-                const uint32_t v = (word >> (16 * hl)) & 0xFFFFu, one = 0x3F80u << (16 * (j & 1));
+                const uint32_t v = (word >> (16 * hl)) & 0xFFFFu;
+                uint32_t one = 0x3F80u << (16 * (j & 1)), rest = word & ~(0xFFFFu << (16 * hl));
+                asm volatile("" : "+v"(one), "+v"(rest));  // (no register of theirs outside this branch)
                 const bool bad = (v & 0x7F80u) == 0x7F80u;
                 up4[j >> 1] |= bad && v != 0xFF80u ? one : 0u;
                 dn4[j >> 1] |= bad && v != 0x7F80u ? one : 0u;
-                vt[j >> 2].c[j & 3][w][k] = bad ? word & ~(0xFFFFu << (16 * hl)) : word;
+                vt[j >> 2].c[j & 3][w][k] = bad ? rest : word;
               }
 #pragma unroll
               for (int i = 0; i < NR; ++i) {
@@ -673,6 +694,14 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
               __builtin_amdgcn_sched_barrier(0);
             }
       }
+      bf16x8 pg[NR];
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        u32x4 pw;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) pw[k] = cvt2(pr[i][2 * k], pr[i][2 * k + 1]);
+        pg[i] = __builtin_bit_cast(bf16x8, pw);
+      }
 #pragma unroll
       for (int w = 0; w < 2; ++w)
 #pragma unroll
@@ -690,11 +719,20 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
             for (int i = 0; i < NR; ++i) acc[i][e] = mfma16(va, pg[i], acc[i][e]);
           }
           __builtin_amdgcn_sched_barrier(0);
+          if (kTurns && k == 3) {
+#pragma unroll
+            for (int st = 4 * w; st < 4 * w + 4; ++st) {
+              k_part(nt[0], kt[0], st);
+              k_part(nt[1], kt[1], st);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      v_load(nt[u], vt[u], next + 16 * u);
+      if constexpr (!kTurns) v_load(nt[u], vt[u], next + 16 * u);
+      vt_at[u] = nt[u];
       okv[u] = nt[u].ok;
     }
     vs_mine = s_load(p.vs, nt);
@@ -706,18 +744,19 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
 
   // ---- 16 rows at a time: each wave's rows (those that are there) into LDS, dims in order, then the four waves joined, one
   // wave per row: the result, or the run's partial
+  const int le = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)), ce = le & 15, ae = le >> 4, de = 4 * le;
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
     float l = l_run[i];
     lane_pair q = lane_swap<16>(l);
     l = add_xor<32>(q.a + q.b);
     lds_barrier();  // Q, or the rows before these, have been used
-    if (r0 + 16 * i + c < R) {
-      o_store<I4>(acc[i], corr[i], ob + ((size_t)wave * 16 + c) * kORow, a);
-      if (a == 0) {
+    if (r0 + 16 * i + ce < R) {
+      o_store<I4>(acc[i], corr[i], ob + ((size_t)wave * 16 + ce) * kORow, ae);
+      if (ae == 0) {
         // (scores that are all NaN leave no maximum: their sum is joined all the same)
-        mls[wave][c][0] = m_run[i] == -INFINITY && l != l ? 0.f : m_run[i];
-        mls[wave][c][1] = l;
+        mls[wave][ce][0] = m_run[i] == -INFINITY && l != l ? 0.f : m_run[i];
+        mls[wave][ce][1] = l;
       }
     }
     lds_barrier();
@@ -737,17 +776,17 @@ __global__ __launch_bounds__(256, I4 || NR == 1 ? 2 : 1) void paged_attn_kernel(
           if (mls[w][j][0] == -INFINITY) continue;  // nothing seen
           const float f = __builtin_amdgcn_exp2f(mls[w][j][0] - M);
           L += mls[w][j][1] * f;
-          const f32x4 v = *reinterpret_cast<const f32x4*>(ob + ((size_t)w * 16 + j) * kORow + d0);
+          const f32x4 v = *reinterpret_cast<const f32x4*>(ob + ((size_t)w * 16 + j) * kORow + de);
 #pragma unroll
           for (int e = 0; e < 4; ++e) O[e] += v[e] * f;
         }
       }
       if (p.S > 1) {
         const size_t slot = (((size_t)b * p.Hkv + kvh) * R + r) * p.S + s;
-        *reinterpret_cast<f32x4*>(p.part + slot * kPgD + d0) = O;
-        if (lane < 2) p.ml[2 * slot + lane] = lane ? L : M;
+        *reinterpret_cast<f32x4*>(p.part + slot * kPgD + de) = O;
+        if (le < 2) p.ml[2 * slot + le] = le ? L : M;
       } else {
-        out_store(p, O, L, keys_seen(p, pos, len, t) > 0, gate_load(p, b, t, h, d0), b, t, h, d0);
+        out_store(p, O, L, keys_seen(p, pos, len, t) > 0, gate_load(p, b, t, h, de), b, t, h, de);
       }
     }
   }
@@ -845,7 +884,7 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs p) 
 // Query rows per block, in 16s: two, which halves the unpacking and the LDS reads per row, but one where all rows fit in it
 // (32 rows of up to 8192 keys, one token of four heads: bf16 95.9 us against 102.6, 4 bits 37.7 against 43.3) and for three
 // 16s against codes, a quarter of whose work would be for rows that are not there (nine tokens of four heads: 64.6 against
-// 70.7; 512 tokens, where none are: 150 against 123, bf16 303 against 185; five tokens, two 16s: 52.8 against 49.3).
+// 70.7; 512 tokens, where none are: 150 against 123, bf16 303 against 167; five tokens, two 16s: 52.8 against 49.3).
 // Runs per row: two blocks per CU, but one where that leaves a block no more than two
 // rounds (three rows of 8192 4-bit keys: 64 runs 16.1 us, 32 runs 14.1, 16 runs 16.7). A table of two rounds is not split
 // (256 keys, one row: 11.9 us against 12.5 for two runs and their merge, 4 bits 9.9 against 11.2; four rounds 16.4 against
