@@ -294,7 +294,9 @@ def gated_attention_layer_paged(x, p, pages, table, pos, *, lens=None, rope_thet
     D = p["q_norm"].numel()
     Hq = p["q_proj"].shape[0] // (2 * D)
     Hkv = p["k_proj"].shape[0] // D
-    cos, sin = rope_tables(table.shape[1] * pages[0].shape[2], int(D * partial_rotary_factor), rope_theta, x.device)
+    # (tables of a power of two of positions: a table of pages that grows from call to call keeps the cache of these small)
+    n_pos = 1 << max(table.shape[1] * pages[0].shape[2] - 1, 0).bit_length()
+    cos, sin = rope_tables(n_pos, int(D * partial_rotary_factor), rope_theta, x.device)
     y = linear(x, attn_in_weight(p), *_q8(p, "_in_fused"), prenorm=prenorm)
     q, k, v = y.split([2 * Hq * D, Hkv * D, Hkv * D], -1)
     q = q.unflatten(-1, (Hq, 2 * D))
