@@ -513,6 +513,38 @@ def test_attention_more_splits_than_rounds(T):
     check_attention(d, attend(to(d, device()), splits=5000))
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "int4"])
+@pytest.mark.parametrize("T", [1, 6])
+def test_attention_over_four_million_keys(fmt, T):
+    """A table that names one page 4096 times: the page's keys, each as often as a token sees it. The splits make a block's
+    run 8192 keys (the n of the bound's sums)."""
+    ps, blocks = 1024, 4096
+    d = make(fmt, 1, T, 4, 2, ps, [T], norm=False, rot=0, nb=1)
+    cap = ps * blocks
+    d["pos"] = torch.tensor([cap - T], dtype=torch.int32)
+    q, gate, _, _ = columns(d["y"], 4, 2)
+    page = int(d["table"][0, 0])
+    g = to(d, device())
+    g["table"] = g["table"].expand(1, blocks).contiguous()
+    announce(f"paged attention {fmt} T {T} over 4194304 keys")
+    out = attend(g, splits=512).cpu().double().view(T, 4, 256)
+    k, v = (paged.row_values(d["pages"][i][page], None if d["pages"][2 + i] is None else d["pages"][2 + i][page], w)
+            for i, w in ((0, "k"), (1, "v")))  # [Hkv, page, 256]
+    sv = torch.zeros_like(v) if d["pages"][3] is None else d["pages"][3][page].double().repeat_interleave(64, -1)
+    for t in range(T):
+        often = blocks - (torch.arange(ps) > ps - T + t).double()
+        for h in range(4):
+            w = often * torch.exp(k[h // 2] @ q[0, t, h].double() / 16)
+            w = w / w.sum()
+            sg = torch.sigmoid(gate[0, t, h].double())
+            ref, amp, step = (w @ v[h // 2]) * sg, (w @ v[h // 2].abs()) * sg, (w @ sv[h // 2]) * sg
+            prod = float((k[h // 2].abs() @ q[0, t, h].double().abs()).max()) / 16
+            q_off = 2.0 ** -15 + (2.0 ** -12 if fmt == "int4" else 0)
+            bound = (2.0 ** -8 + 2 * q_off * prod + 2.0 ** -16) * amp + (8192 / 32 + 16) * 2.0 ** -19 * step \
+                + (2.0 ** -8 + 2.0 ** -20) * ref.abs() * (1 + 2.0 ** -7)
+            assert float(((out[t, h] - ref).abs() / bound).max()) <= 1
+
+
 def test_append_of_tiny_values_without_eps():
     """Squares below the smallest normal number, and an eps of 0: the codes of 64 bits all the same."""
     d = make("int4", 1, 40, 2, 2, 16, [40])

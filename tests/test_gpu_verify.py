@@ -195,3 +195,16 @@ def test_verify_rows_past_32_bits():
     got = ops.verify_drafts(wide, ids.to(dev), u.to(dev))
     want = paged.verify_drafts(x, ids, u)
     assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
+
+
+def test_verify_broadcast_logits():
+    """One row's logits for every sequence, as an expanded view, each with its own random numbers."""
+    dev = device()
+    x, ids, u, q, _ = make(5, 3, 4099, seed=21, probs=True)
+    announce("verify broadcast logits")
+    one, qone = x[:1].to(dev), q[:1].to(dev)
+    ids = ids[:1].expand(5, 3)
+    got = ops.verify_drafts(one.expand(5, 4, 4099), ids.to(dev).contiguous(), u.to(dev),
+                            draft_probs=qone.expand(5, 3, 4099))
+    want = paged.verify_drafts(x[:1].expand(5, 4, 4099), ids, u, q[:1].expand(5, 3, 4099))
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
