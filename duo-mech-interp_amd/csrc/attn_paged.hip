@@ -87,10 +87,6 @@ template <> struct VTile<false> {
   u32x4 c[4][2];  // key 4 a + r: dims 8 c .. and 128 + 8 c ..
 };
 
-__device__ __forceinline__ bf16x8 as_bf16x8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  const u32x4 r = {a, b, c, d};
-  return __builtin_bit_cast(bf16x8, r);
-}
 __device__ __forceinline__ f32x4 mfma16h(const u32x4& a, const f16x8& b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), b, c, 0, 0, 0);
 }
