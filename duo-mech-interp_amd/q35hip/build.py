@@ -1,6 +1,7 @@
 """Build recipe of libq35hip.so: every csrc/*.hip compiled for gfx950 with hipcc, linked into one shared library that
-exports the C ABI declared in include/q35hip.h. The library lands next to this file (in-tree) so that it travels with
-the source tree and is what the Python package loads.
+exports the C ABI declared in include/q35hip.h; and of the Python extension _paged_host.so (csrc/paged_host.cpp, host code over
+torch's C++ interface). Both land next to this file (in-tree) so that they travel with the source tree and are what the
+Python package loads.
 
     python -m q35hip.build          (from duo-mech-interp_amd/)
 """
@@ -9,6 +10,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)                      # duo-mech-interp_amd/
@@ -18,6 +20,7 @@ INCLUDE = os.path.join(REPO, "include")
 BUILD_DIR = os.path.join(ROOT, "_build")
 LIB_NAME = "libq35hip.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
+HOST_PATH = os.path.join(PKG_DIR, "_paged_host.so")
 
 ARCH = "gfx950"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -44,15 +47,33 @@ def _compile(src):
     return obj
 
 
+def _build_host():
+    """HOST_PATH: no device code, torch's libraries (loaded before it) by name."""
+    import torch
+    t = os.path.dirname(torch.__file__)
+    tmp = HOST_PATH + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I" + INCLUDE,
+           "-I" + os.path.join(t, "include"), "-I" + os.path.join(t, "include", "torch", "csrc", "api", "include"),
+           "-I" + sysconfig.get_paths()["include"], os.path.join(CSRC, "paged_host.cpp"), "-o", tmp,
+           "-L" + os.path.join(t, "lib"), "-lc10", "-ltorch_cpu", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"paged_host.cpp failed:\n{r.stderr}")
+    os.replace(tmp, HOST_PATH)
+
+
 def build(verbose=False, jobs=None):
-    """Compile every kernel source and link LIB_PATH. Always rebuilds."""
+    """Compile every kernel source and link LIB_PATH, and HOST_PATH beside it. Always rebuilds."""
     if not os.path.exists(HIPCC):
         raise RuntimeError(f"hipcc not found at {HIPCC}")
     os.makedirs(BUILD_DIR, exist_ok=True)
     srcs = sources()
     jobs = jobs or min(len(srcs), max(1, (os.cpu_count() or 4)))
     with concurrent.futures.ThreadPoolExecutor(max_workers=jobs) as ex:
+        host = ex.submit(_build_host)
         objs = list(ex.map(_compile, srcs))
+        host.result()
     tmp = LIB_PATH + ".tmp"
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp] + objs
     r = subprocess.run(cmd, capture_output=True, text=True)
@@ -60,7 +81,7 @@ def build(verbose=False, jobs=None):
         raise RuntimeError(f"link failed:\n{r.stderr}")
     os.replace(tmp, LIB_PATH)
     if verbose:
-        print(f"built {LIB_PATH} from {len(srcs)} sources")
+        print(f"built {LIB_PATH} from {len(srcs)} sources, and {HOST_PATH}")
     return LIB_PATH
 
 

@@ -13,7 +13,7 @@ tests/engine_ref.py):
 Every op runs on the current HIP stream of its inputs' device; inputs are validated here (device, dtype, layout,
 shape) and a bad call raises RuntimeError. CPU tensors raise: there is no CPU path in the product.
 """
-import functools
+import ctypes
 import math
 from typing import NamedTuple, Optional
 
@@ -32,15 +32,6 @@ def _ptr(t):
 def _stream(t):
     # the handle of t's device's current stream, without a Stream object around it (0.1 us against 2.0 a call)
     return torch._C._cuda_getCurrentRawStream(t.get_device())
-
-
-def _launch(fn, t, *args):
-    """fn(*args) with t's device current (a kernel is launched on the current device)."""
-    d = t.get_device()
-    if d == torch._C._cuda_getDevice():
-        return fn(*args)
-    with torch.cuda.device(d):
-        return fn(*args)
 
 
 def _require(cond, msg):
@@ -357,174 +348,42 @@ def _attn_prefill_cached_proj_impl(y, q_norm_w, k_norm_w, eps, k_cache, v_cache,
 
 
 # ---------------------------------------------------------------- paged KV cache
-# A decode step makes these calls eagerly for every layer, so their checks are plain comparisons in one pass each.
-def _heads_view(x, what):
-    """A [B, T, H, 256] fp32 or bf16 view (rows of 256 dense, anything else strided): its strides of B, T and H."""
-    if not x.is_cuda:
-        raise Q35Error("q35hip: inputs must be HIP device tensors (there is no CPU fallback)")
-    s = x.stride()
-    if len(s) != 4 or s[3] != 1 or x.shape[3] != 256 or x.dtype not in _DT:
-        raise Q35Error(f"q35hip: {what}: [B, T, heads, 256] fp32 or bf16 with dense rows")
-    return s[0], s[1], s[2]
+_HOST = None
 
 
-def _dense_on(d, *ts):
-    """Whether every tensor is dense and on device d."""
-    for t in ts:
-        if t is not None and not (t.get_device() == d and t.is_contiguous()):
-            if not t.is_cuda:
-                raise Q35Error("q35hip: inputs must be HIP device tensors (there is no CPU fallback)")
-            return False
-    return True
+def _paged_host():
+    """The extension that checks the arguments of the paged-cache ops, makes their outputs and calls the C ABI
+    (csrc/paged_host.cpp): a decode step makes these calls eagerly for every layer."""
+    global _HOST
+    if _HOST is None:
+        lib = _lib.lib()
+        try:
+            from . import _paged_host as host
+        except ImportError as e:
+            raise Q35Error(f"q35hip: the extension _paged_host is missing or does not load ({e}); build it with "
+                           "__graft_entry__.build() (python -m q35hip.build)") from None
+        host.bind(Q35Error, check, torch._C._cuda_getCurrentRawStream,
+                  *(ctypes.cast(getattr(lib, f), ctypes.c_void_p).value for f in (
+                      "q35_paged_kv_append", "q35_paged_kv_rows", "q35_gated_attn_paged_workspace_bytes",
+                      "q35_gated_attn_paged", "q35_verify_drafts_workspace_bytes", "q35_verify_drafts")))
+        _HOST = host
+    return _HOST
 
 
-def _pages_check(d, k_pages, v_pages, k_scale, v_scale, table, pos, lens, B):
-    """The format, n_pages, Hkv and page size of a paged cache on device d; its table, positions and lengths checked for
-    B rows."""
-    if not _dense_on(d, k_pages, v_pages, k_scale, v_scale, pos, lens):
-        raise Q35Error("q35hip: pages, pos and lens must be contiguous and on one device with the other inputs")
-    i32 = torch.int32
-    if table.get_device() != d or table.dtype != i32 or table.dim() != 2 or table.shape[0] != B or table.stride(1) != 1:
-        raise Q35Error("q35hip: table: [B, blocks] int32 with dense rows, on the pages' device")
-    if pos.dtype != i32 or pos.shape != (B,) or (lens is not None and (lens.dtype != i32 or lens.shape != (B,))):
-        raise Q35Error("q35hip: pos, lens: [B] int32")
-    shape, dt = k_pages.shape, k_pages.dtype
-    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype != dt:
-        raise Q35Error("q35hip: pages: k and v alike, [pages, Hkv, page size, ...]")
-    n, Hkv, ps, w = shape
-    if dt == torch.bfloat16:
-        if w != 256:
-            raise Q35Error("q35hip: bf16 pages: [pages, Hkv, page size, 256]")
-        return Q35_BF16, n, Hkv, ps
-    if dt != torch.uint8 or w != 128:
-        raise Q35Error("q35hip: 4-bit pages: [pages, Hkv, page size, 128] uint8")
-    for s in (k_scale, v_scale):
-        if s is None or s.dtype != torch.bfloat16 or s.shape != (n, Hkv, ps, 4):
-            raise Q35Error("q35hip: 4-bit pages: k_scale, v_scale [pages, Hkv, page size, 4] bf16")
-    return Q35_I4_G64, n, Hkv, ps
+def _paged_kv_append_impl(*args):
+    _paged_host().paged_kv_append(*args)
 
 
-def _rope_check(d, cos, sin, norm_w, rows):
-    """rot of cos / sin tables of at least `rows` rows; norm_w None or [256] fp32."""
-    f32 = torch.float32
-    if not _dense_on(d, cos, sin, norm_w):
-        raise Q35Error("q35hip: cos, sin and the norm weight must be contiguous and on one device with the other inputs")
-    shape = cos.shape
-    if cos.dtype != f32 or sin.dtype != f32 or len(shape) != 2 or sin.shape != shape or \
-            (norm_w is not None and (norm_w.dtype != f32 or norm_w.shape != (256,))):
-        raise Q35Error("q35hip: cos, sin: [P, rot / 2] fp32; norm weight: [256] fp32")
-    if shape[0] < rows and shape[1]:
-        raise Q35Error(f"q35hip: cos/sin tables need {rows} rows")
-    return 2 * shape[1]
+def _paged_kv_rows_impl(*args):
+    return _paged_host().paged_kv_rows(*args)
 
 
-def _paged_kv_append_impl(k, v, k_pages, v_pages, k_scale, v_scale, table, pos, lens, cos, sin, k_norm_w, eps):
-    kb, kt, kh = _heads_view(k, "k")
-    vb, vt, vh = _heads_view(v, "v")
-    B, T, Hkv, D = k.shape
-    d = k.get_device()
-    fmt, n, H, ps = _pages_check(d, k_pages, v_pages, k_scale, v_scale, table, pos, lens, B)
-    if v.shape != k.shape or v.dtype != k.dtype or v.get_device() != d or H != Hkv:
-        raise Q35Error("q35hip: k, v: alike, with the pages' heads")
-    nb = table.shape[1]
-    rot = _rope_check(d, cos, sin, k_norm_w, nb * ps)
-    if B == 0 or T == 0:
-        return
-    st = _launch(_lib.lib().q35_paged_kv_append, k, k.data_ptr(), kb, kt, kh, v.data_ptr(), vb, vt, vh, _DT[k.dtype],
-                 _ptr(k_norm_w), eps, cos.data_ptr(), sin.data_ptr(), rot, table.data_ptr(), table.stride(0), nb,
-                 pos.data_ptr(), _ptr(lens), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale), fmt, n,
-                 ps, B, T, Hkv, D, _stream(k))
-    check(st, "q35_paged_kv_append")
+def _attn_paged_impl(*args):
+    return _paged_host().gated_attn_paged(*args)
 
 
-def _paged_kv_rows_impl(k_pages, v_pages, k_scale, v_scale, table, pos, lens, T):
-    B, nb = table.shape
-    fmt, n, Hkv, ps = _pages_check(k_pages.get_device(), k_pages, v_pages, k_scale, v_scale, table, pos, lens, B)
-    _require(T >= 0, "T: a number of tokens")
-    k = torch.empty(B, Hkv, T, 256, dtype=torch.bfloat16, device=k_pages.device)
-    v = torch.empty_like(k)
-    if B == 0 or T == 0:
-        return k, v
-    st = _launch(_lib.lib().q35_paged_kv_rows, k, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale),
-                 fmt, n, ps, table.data_ptr(), table.stride(0), nb, pos.data_ptr(), _ptr(lens), k.data_ptr(),
-                 v.data_ptr(), B, T, Hkv, 256, _stream(k))
-    check(st, "q35_paged_kv_rows")
-    return k, v
-
-
-@functools.lru_cache(maxsize=256)
-def _attn_paged_workspace(*sizes):
-    return _lib.lib().q35_gated_attn_paged_workspace_bytes(*sizes)
-
-
-def _attn_paged_impl(q, gate, k_pages, v_pages, k_scale, v_scale, table, pos, lens, cos, sin, q_norm_w, eps, scale,
-                     splits, f32_out):
-    qb, qt, qh = _heads_view(q, "q")
-    B, T, Hq, D = q.shape
-    d = q.get_device()
-    fmt, n, Hkv, ps = _pages_check(d, k_pages, v_pages, k_scale, v_scale, table, pos, lens, B)
-    gb = gt = gh = 0
-    if gate is not None:
-        gb, gt, gh = _heads_view(gate, "gate")
-        if gate.shape != q.shape or gate.dtype != q.dtype or gate.get_device() != d:
-            raise Q35Error("q35hip: gate: like q")
-    nb = table.shape[1]
-    rot = _rope_check(d, cos, sin, q_norm_w, nb * ps)
-    out = torch.empty(B, T, Hq * D, dtype=torch.float32 if f32_out else torch.bfloat16, device=q.device)
-    if out.numel() == 0:
-        return out
-    nbytes = _attn_paged_workspace(B, T, Hq, Hkv, D, nb, ps, splits)
-    _require(nbytes > 0, "unsupported attention shape")
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    st = _launch(_lib.lib().q35_gated_attn_paged, q, q.data_ptr(), qb, qt, qh, _ptr(gate), gb, gt, gh, _DT[q.dtype],
-                 _ptr(q_norm_w), eps, cos.data_ptr(), sin.data_ptr(), rot, k_pages.data_ptr(), v_pages.data_ptr(),
-                 _ptr(k_scale), _ptr(v_scale), fmt, n, ps, table.data_ptr(), table.stride(0), nb, pos.data_ptr(),
-                 _ptr(lens), out.data_ptr(), Q35_F32 if f32_out else Q35_BF16, B, T, Hq, Hkv, D, scale, splits,
-                 ws.data_ptr(), nbytes, _stream(q))
-    check(st, "q35_gated_attn_paged")
-    return out
-
-
-@functools.lru_cache(maxsize=256)
-def _verify_drafts_workspace(*sizes):
-    return _lib.lib().q35_verify_drafts_workspace_bytes(*sizes)
-
-
-def _verify_drafts_impl(logits, draft_ids, draft_probs, u, lens, temperatures, temperature):
-    d = logits.get_device()
-    if not _dense_on(d, lens, temperatures) or d < 0 or draft_ids.get_device() != d or u.get_device() != d or \
-            (draft_probs is not None and draft_probs.get_device() != d):
-        raise Q35Error("q35hip: inputs must be HIP device tensors on one device (there is no CPU fallback), lens and "
-                       "temperature contiguous")
-    f32, i32 = torch.float32, torch.int32
-    if logits.dtype != f32 or logits.dim() != 3 or logits.stride(2) != 1 or logits.shape[1] == 0:
-        raise Q35Error("q35hip: logits: [B, K + 1, V] fp32 with dense rows")
-    B, K, V = logits.shape
-    K -= 1
-    if draft_ids.shape != (B, K) or draft_ids.dtype != i32 or (K > 1 and draft_ids.stride(1) != 1):
-        raise Q35Error("q35hip: draft_ids: [B, K] int32 with dense rows")
-    if u.shape != (B, K + 1) or u.dtype != f32 or (K and u.stride(1) != 1):
-        raise Q35Error("q35hip: u: [B, K + 1] fp32 with dense rows")
-    if draft_probs is not None and (draft_probs.shape != (B, K, V) or draft_probs.dtype != f32
-                                    or draft_probs.stride(2) != 1):
-        raise Q35Error("q35hip: draft_probs: [B, K, V] fp32 with dense rows")
-    if (lens is not None and (lens.dtype != i32 or lens.shape != (B,))) or \
-            (temperatures is not None and (temperatures.dtype != f32 or temperatures.shape != (B,))):
-        raise Q35Error("q35hip: lens: [B] int32; temperature: a number of at least 0 or [B] fp32")
-    n = torch.empty(B, dtype=i32, device=logits.device)
-    tokens = torch.empty(B, K + 1, dtype=i32, device=logits.device)
-    if B == 0:
-        return n, tokens
-    nbytes = _verify_drafts_workspace(B, K, V)
-    _require(nbytes > 0, f"unsupported draft shape (B={B}, K={K}, V={V})")
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
-    pb, pp = draft_probs.stride()[:2] if draft_probs is not None else (0, 0)
-    st = _launch(_lib.lib().q35_verify_drafts, logits, logits.data_ptr(), logits.stride(0), logits.stride(1),
-                 draft_ids.data_ptr(), draft_ids.stride(0), _ptr(draft_probs), pb, pp, u.data_ptr(), u.stride(0),
-                 _ptr(lens), _ptr(temperatures), temperature, n.data_ptr(), tokens.data_ptr(), B, K, V, ws.data_ptr(),
-                 nbytes, _stream(logits))
-    check(st, "q35_verify_drafts")
-    return n, tokens
+def _verify_drafts_impl(*args):
+    return _paged_host().verify_drafts(*args)
 
 
 def _resid_add_impl(x, vecs, vec_of_row):
@@ -1366,7 +1225,7 @@ def paged_kv_append_(k, v, pages, table, pos, cos, sin, *, lens=None, k_norm_w=N
     table: [B, blocks] int32, row b's page of each block of page-size tokens; token t of row b goes to position
     pos[b] + t, t < lens[b] ([B] int32; None: all T). Tokens past lens, past the capacity or on a table entry that names
     no page are not written. Two rows of one call must not share a page they write to."""
-    op = _paged_kv_append_impl if _direct(k) else torch.ops.q35.paged_kv_append_
+    op = _paged_host().paged_kv_append if _direct(k) else torch.ops.q35.paged_kv_append_
     op(k, v, *_four(pages), table, pos, lens, cos, sin, k_norm_w, float(eps))
 
 
@@ -1374,7 +1233,7 @@ def paged_kv_rows(pages, table, pos, T, *, lens=None):
     """Rows pos[b] .. pos[b] + T - 1 of each sequence read back from its pages: (k, v) [B, Hkv, T, 256] bf16, the layout
     of the dense caches (with pos 0 and T a multiple of 64 the caches of gated_attention_prefill_cached); zeros past
     lens, past the table and where a table entry names no page."""
-    op = _paged_kv_rows_impl if _direct(pages[0]) else torch.ops.q35.paged_kv_rows
+    op = _paged_host().paged_kv_rows if _direct(pages[0]) else torch.ops.q35.paged_kv_rows
     return op(*_four(pages), table, pos, lens, int(T))
 
 
@@ -1387,7 +1246,7 @@ def gated_attention_paged(q, gate, pages, table, pos, cos, sin, *, lens=None, q_
     prompt; Hq / Hkv any ratio. Returns [B, T, Hq * 256] in out_dtype (bf16 or fp32), zeros for tokens past lens or the
     table's capacity. splits: over how many blocks a row's keys are dealt (0: by the sizes)."""
     _require(out_dtype in (torch.bfloat16, torch.float32), "out_dtype: bf16 or fp32")
-    op = _attn_paged_impl if _direct(q) else torch.ops.q35.gated_attn_paged
+    op = _paged_host().gated_attn_paged if _direct(q) else torch.ops.q35.gated_attn_paged
     return op(q, gate, *_four(pages), table, pos, lens, cos, sin, q_norm_w, float(eps),
               q.shape[-1] ** -0.5 if scale is None else float(scale), int(splits), out_dtype == torch.float32)
 
@@ -1410,7 +1269,7 @@ def verify_drafts(logits, draft_ids, u, *, draft_probs=None, lens=None, temperat
     draft: the lowest index whose running sum exceeds u[:, K] of the whole. The kept drafts and the drawn token are then
     distributed as draws from p. Returns (n_accept [B] int32, tokens [B, K + 1] int32: kept drafts, drawn token, -1)."""
     ts, t = (temperature, 0.0) if torch.is_tensor(temperature) else (None, float(temperature))
-    op = _verify_drafts_impl if _direct(logits) else torch.ops.q35.verify_drafts
+    op = _paged_host().verify_drafts if _direct(logits) else torch.ops.q35.verify_drafts
     return op(logits, draft_ids, draft_probs, u, lens, ts, t)
 
 
