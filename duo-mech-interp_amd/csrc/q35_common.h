@@ -215,6 +215,23 @@ __device__ __forceinline__ double wave_sum64(double v) {
   v += dpp64<0x140>(v);
   return swap_add64<32>(swap_add64<16>(v));
 }
+// Running sum over the wave: within rows of 16 lanes by shifts, then the rows' last lanes on to the rows behind them.
+template <int CTRL, int ROWS> __device__ __forceinline__ double dpp64_or_0(double v) {
+  const u32x2 w = __builtin_bit_cast(u32x2, v);
+  u32x2 r;
+  r.x = __builtin_amdgcn_update_dpp(0, w.x, CTRL, ROWS, 0xF, true);
+  r.y = __builtin_amdgcn_update_dpp(0, w.y, CTRL, ROWS, 0xF, true);
+  return __builtin_bit_cast(double, r);
+}
+__device__ __forceinline__ double wave_scan64(double v) {
+  v += dpp64_or_0<0x111, 0xF>(v);  // row_shr:1
+  v += dpp64_or_0<0x112, 0xF>(v);
+  v += dpp64_or_0<0x114, 0xF>(v);
+  v += dpp64_or_0<0x118, 0xF>(v);
+  v += dpp64_or_0<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+  v += dpp64_or_0<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
 // Maximum over the 16 lanes of a row, and over the wave.
 __device__ __forceinline__ float row16_max_f32(float v) {
   v = fmaxf(v, lane_dpp<0xB1>(v));

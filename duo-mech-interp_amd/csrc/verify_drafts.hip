@@ -47,6 +47,7 @@ struct VerifyArgs {
   float temp;
   int K, V, C;
   VStat* st;
+  float2* dv;    // [B][K + 1]: the draft's logit (NaN as -inf) and probability, where the draft is a token
   double* mass;  // [B][C], with draft probabilities: sums of max(p_n - q_n, 0) behind a refusal
   int32_t *n_out, *tokens;
 };
@@ -133,6 +134,9 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs p) {
   if (i > len) return;
   const double inv_t = v_inv_temp(p, b);
   const int draft = v_draft(p, b, i, len);
+  const bool mine = draft >= base && draft < base + kVChunk;
+  if (mine && tid == 0)
+    p.dv[blockIdx.y] = {v_clean(p.x[b * p.xb + i * p.xp + draft]), p.q ? p.q[b * p.qb + i * p.qp + draft] : 1.f};
   float x[kVPer];
   v_load_chunk(p.x + b * p.xb + i * p.xp, base, p.V, tid, x, -INFINITY);
   __shared__ float sm[4];
@@ -152,7 +156,7 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs p) {
   int idx = 0x7fffffff;
   double s = 0.0;
   if (inv_t > 0.0) {
-    if (draft >= base && draft < base + kVChunk) {  // the draft's weight is no part of its chunk's sum
+    if (mine) {  // the draft's weight is no part of its chunk's sum
 #pragma unroll
       for (int k = 0; k < kVPer; ++k)
         if (v_index(base, tid, k) == draft) x[k] = -INFINITY;
@@ -183,8 +187,9 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs p) {
 }
 
 // The chunks of each position of row b folded: the maximum, its index, 1 / sum, and whether the draft is kept. The chunks
-// of as many positions as fit are fetched together with the positions' drafts and what is asked of those, then one wave
-// folds a position. Returns n once every thread has them.
+// of as many positions as fit are fetched together with the positions' drafts and what is asked of those, whatever the row's
+// length (which arrives with them: no load waits for another), then one wave folds a position. Returns n once every thread
+// has them.
 constexpr int kVFold = 1024;  // chunks held at a time, and the most that a position may have
 struct VFold {
   VStat st[kVFold];
@@ -197,18 +202,20 @@ template <int THREADS>
 __device__ __forceinline__ int v_fold(const VerifyArgs& p, int b, int len, double inv_t, int tid, VFold& f) {
   const int lane = tid & 63, wave = tid >> 6, per = max(kVFold / p.C, 1);
   exp2_table(f.tab, tid);
-  if (tid < p.K) {  // (whether the row has this position is known later than its draft)
+  if (tid < p.K) {
     const int id = p.ids[b * p.idb + tid];
-    const bool token = id >= 0 && id < p.V;
-    f.x[tid] = token ? v_clean(p.x[b * p.xb + tid * p.xp + id]) : -INFINITY;
-    f.q[tid] = token && p.q ? p.q[b * p.qb + tid * p.qp + id] : 1.f;
+    const float2 d = p.dv[(size_t)b * (p.K + 1) + tid];
+    f.x[tid] = d.x;
+    f.q[tid] = d.y;
     f.u[tid] = p.u[b * p.ub + tid];
-    f.draft[tid] = token ? id : -1;
+    f.draft[tid] = id >= 0 && id < p.V ? id : -1;
   }
-  for (int i0 = 0; i0 <= len; i0 += per) {
-    const int n = min(per, len + 1 - i0);
+  int i0 = 0;
+  do {
+    const int there = min(per, p.K + 1 - i0) * p.C;
     const VStat* src = p.st + ((size_t)b * (p.K + 1) + i0) * p.C;
-    for (int k = tid; k < n * p.C; k += THREADS) f.st[k] = src[k];
+    for (int k = tid; k < there; k += THREADS) f.st[k] = src[k];
+    const int n = min(per, len + 1 - i0);
     __syncthreads();
     for (int j = wave; j < n; j += THREADS / 64) {
       const int i = i0 + j, draft = i < len ? f.draft[i] : -1;
@@ -236,7 +243,8 @@ __device__ __forceinline__ int v_fold(const VerifyArgs& p, int b, int len, doubl
       }
     }
     __syncthreads();
-  }
+    i0 += per;
+  } while (i0 <= len);
   int n = 0;
   while (n < len && f.keep[n]) ++n;
   return n;
@@ -316,13 +324,7 @@ __global__ __launch_bounds__(1024) void verify_draw_kernel(VerifyArgs p) {
     double run = 0.0, before = 0.0;
     int chunk = -1, last_chunk = 0;
     for (int k0 = 0; k0 < p.C && chunk < 0; k0 += 64) {
-      const double w = k0 + lane < p.C ? chunk_w[k0 + lane] : 0.0;
-      double inc = w;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const double v = __shfl_up(inc, o);
-        if (lane >= o) inc += v;
-      }
+      const double w = k0 + lane < p.C ? chunk_w[k0 + lane] : 0.0, inc = wave_scan64(w);
       const unsigned long long over = __builtin_amdgcn_ballot_w64(w > 0.0 && run + inc > all);
       const unsigned long long some = __builtin_amdgcn_ballot_w64(w > 0.0);
       if (some) last_chunk = k0 + 63 - __builtin_clzll(some);
@@ -370,12 +372,7 @@ __global__ __launch_bounds__(1024) void verify_draw_kernel(VerifyArgs p) {
       if (v > 0.0) last = base + k;
     }
     // sums before this thread's values: a scan within the wave, then over the waves
-    double inc = sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const double v = __shfl_up(inc, o);
-      if (lane >= o) inc += v;
-    }
+    const double inc = wave_scan64(sum);
     if (lane == 63) pre[wave] = inc;
     __syncthreads();
     run = inc - sum;
@@ -407,7 +404,7 @@ extern "C" size_t q35_verify_drafts_workspace_bytes(int64_t B, int64_t K, int64_
   using namespace q35;
   if (B <= 0 || K < 0 || V <= 0 || B > 65535 || K > kVMaxK || V > (int64_t)kVFold * kVChunk || B * (K + 1) > 65535) return 0;
   const size_t C = v_chunks(V);
-  return (size_t)B * (K + 1) * C * sizeof(VStat) + (size_t)B * C * sizeof(double);
+  return (size_t)B * (K + 1) * C * sizeof(VStat) + (size_t)B * C * sizeof(double) + (size_t)B * (K + 1) * sizeof(float2);
 }
 
 extern "C" int q35_verify_drafts(const float* logits, int64_t l_sb, int64_t l_sp, const int32_t* draft_ids, int64_t d_sb,
@@ -427,8 +424,9 @@ extern "C" int q35_verify_drafts(const float* logits, int64_t l_sb, int64_t l_sp
   const int C = (int)v_chunks(V);
   VStat* st = (VStat*)workspace;
   double* mass = (double*)(st + (size_t)B * (K + 1) * C);
+  float2* dv = (float2*)(mass + (size_t)B * C);
   const VerifyArgs a{logits, l_sb, l_sp, draft_ids, d_sb, K > 0 ? draft_probs : nullptr, p_sb, p_sp, u, u_sb, lens,
-                     temperatures, temperature, (int)K, (int)V, C, st, mass, n_accept, tokens};
+                     temperatures, temperature, (int)K, (int)V, C, st, dv, mass, n_accept, tokens};
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(verify_stats_kernel, dim3(C, (unsigned)(B * (K + 1))), dim3(256), 0, s, a);
   if (a.q) hipLaunchKernelGGL(verify_mass_kernel, dim3(C, (unsigned)B), dim3(256), 0, s, a);
