@@ -1224,7 +1224,7 @@ def paged_kv_append_(k, v, pages, table, pos, cos, sin, *, lens=None, k_norm_w=N
     when it is given and rotated at their positions (cos, sin: [P, rot / 2] fp32, P at least the table's capacity).
     table: [B, blocks] int32, row b's page of each block of page-size tokens; token t of row b goes to position
     pos[b] + t, t < lens[b] ([B] int32; None: all T). Tokens past lens, past the capacity or on a table entry that names
-    no page are not written. Two rows of one call must not share a page they write to."""
+    no page are not written. The table entries that a call writes to must all name different pages."""
     op = _paged_host().paged_kv_append if _direct(k) else torch.ops.q35.paged_kv_append_
     op(k, v, *_four(pages), table, pos, lens, cos, sin, k_norm_w, float(eps))
 
