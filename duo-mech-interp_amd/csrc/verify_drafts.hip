@@ -16,9 +16,9 @@
 // depend on n: verify_mass_kernel between the two forms them (every block of a row finds the same n, from the same numbers
 // in the same order). Nothing depends on the order in which blocks run.
 //
-// Measured, V = 151,936: three rows of 4 certain drafts 11 us (statistics 5.3, draw 6.9: a launch and a chain of dependent loads
-// each); 32 rows of 0 .. 8 drafts with probabilities 45.6 us (statistics 26.5 for 97 MB, 3.7 TB/s; mass 12; draw 7.6). Chunks of 8192, or several positions a block, measured slower: the statistics
-// kernel hides its loads by many short blocks.
+// Measured, V = 151,936: three rows of 4 certain drafts 11 us (statistics 5.3, draw 6.9: a launch and a chain of dependent
+// loads each); 32 rows of 0 .. 8 drafts with probabilities 45 us (statistics 27 for 97 MB, 3.6 TB/s; mass 12; draw 8). Chunks
+// of 8192, or several positions a block, measured slower: the statistics kernel hides its loads by many short blocks.
 #include "q35_common.h"
 #include "q35hip.h"
 
