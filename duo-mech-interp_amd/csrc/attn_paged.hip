@@ -21,13 +21,13 @@
 // the rounded weights times -24, which a product of its own collects for all four groups (row r of its A operand is -24
 // where r % 4 is the group). Scales apply outside the codes: a key's to its group's partial score (fp32), a value's to the
 // exponential before its rounding. What bounds the 4-bit form is the vector ALU's issue: about 570 operations beside 72
-// matrix products for 32 rows x 32 keys, half of them unpacking, so masks and constants are kept where one v_and_or_b32
+// matrix products for 32 rows x 32 keys, two fifths of them unpacking, so masks and constants are kept where one v_and_or_b32
 // takes both, scales and offsets come from LDS in the form in which they are used, and what only masked rounds or scales
 // that are not finite need stays behind branches.
 //
 // Measured (8 query and 2 key heads; a 1 GiB copy runs at 5.2 TB/s, a large bf16 product at 1190 TFLOP/s): one token for 32
 // rows of up to 8192 bf16 keys 93 to 95 us (5.1 TB/s); five tokens a row against 4-bit keys 47 us (2.8 TB/s, 124 TFLOP/s);
-// 512 tokens of one row behind 16 K 4-bit keys 116 us (524 TFLOP/s), bf16 167; one token of three rows of 8192 4-bit keys
+// 512 tokens of one row behind 16 K 4-bit keys 115 us (528 TFLOP/s), bf16 165; one token of three rows of 8192 4-bit keys
 // 14 us.
 //
 // A row's keys are dealt over S blocks in runs of whole 128-key rounds by the row's own length, read on the device: the
@@ -319,7 +319,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttnArgs p) {
   };
   // 32 rows against bf16: K's and V's operands share 64 registers (at two waves per SIMD there are 256, 136 of them
   // accumulators). As the scores release K's, V's are loaded, and the next K's as the sums release V's (512 tokens behind 16 K
-  // keys 167 us; with registers for both, at one wave per SIMD, 185).
+  // keys 165 us; with registers for both, at one wave per SIMD, 185).
   constexpr bool kTurns = !I4 && NR == 2;
   auto v_load = [&](const Tile& t, VTile<I4>& v, int key0) {
     const gptr src = base_of(p.vp, t.slot * (I4 ? 128 : 512));
@@ -912,7 +912,7 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs p) 
 // Query rows per block, in 16s: two, which halves the unpacking and the LDS reads per row, but one where all rows fit in it
 // (32 rows of up to 8192 keys, one token of four heads: bf16 95.9 us against 102.6, 4 bits 37.7 against 43.3) and for three
 // 16s against codes, a quarter of whose work would be for rows that are not there (nine tokens of four heads: 64.6 against
-// 70.7; 512 tokens, where none are: 150 against 123, bf16 303 against 167; five tokens, two 16s: 52.8 against 49.3).
+// 70.7; 512 tokens, where none are: 150 against 123, bf16 303 against 165; five tokens, two 16s: 52.8 against 49.3).
 // Runs per row: two blocks per CU, but one where that leaves a block no more than two
 // rounds (three rows of 8192 4-bit keys: 64 runs 16.1 us, 32 runs 14.1, 16 runs 16.7). A table of two rounds is not split
 // (256 keys, one row: 11.9 us against 12.5 for two runs and their merge, 4 bits 9.9 against 11.2; four rounds 16.4 against
