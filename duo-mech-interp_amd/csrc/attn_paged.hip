@@ -5,7 +5,7 @@
 //   attention, engine/kernels_qwen35.js:73-123). The new tokens' keys are in the pages already.
 //
 // A block takes 16 NR query rows (row r = t G + head of the group, G = Hq / Hkv) of one kv head against one run of the
-// row's keys; its four waves take 32 keys each in turn. Both products run with the keys on the matrix core's row side:
+// row's keys; its four waves (or eight) take 32 keys each in turn. Both products run with the keys on the matrix core's row side:
 //   S^T [keys x rows]  = K Q^T   A: 16 keys of K as they lie in the page, B: Q from LDS
 //   O^T [dims x rows] += V^T P^T A: V^T formed in registers, B: the exponentials, which S^T's layout hands over as they
 //                                are (lane: row l % 16, keys 4 (l / 16) + r of two 16-key tiles)
@@ -203,39 +203,41 @@ __device__ __forceinline__ void out_store(const PagedAttnArgs& p, const f32x4& O
   }
 }
 
-template <bool I4, int NR>
-__global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttnArgs p) {
-  constexpr int ROWS = 16 * NR, QP = I4 ? 1 : 2, QF = 8 * 64;  // parts of Q, 16-byte operands of one
+template <bool I4, int NR, int W>
+__global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(PagedAttnArgs p) {
+  constexpr int ROWS = 16 * NR, KEYS = 32 * W, QP = I4 ? 1 : 2, QF = 8 * 64;  // parts of Q, 16-byte operands of one
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, a = lane >> 4;
   const int s = blockIdx.x, kvh = blockIdx.y % p.Hkv, rb = blockIdx.y / p.Hkv, b = blockIdx.z;
   const int R = p.T * p.G, r0 = rb * ROWS;
 
-  constexpr int kQBytes = NR * QP * QF * 16, kOBytes = 4 * 16 * kORow * 4;
+  constexpr int kQBytes = NR * QP * QF * 16, kOBytes = W * 16 * kORow * 4;
   __shared__ __attribute__((aligned(16))) char lds[kQBytes > kOBytes ? kQBytes : kOBytes];
   __shared__ f32x4 qoff[NR][kPgNG][16];  // what the codes' offsets add to a group's product, negated (four times: a C operand)
   __shared__ float qfac[ROWS];           // the power of two taken out of a row of Q
-  __shared__ float mls[4][16][2];
-  __shared__ __attribute__((aligned(16))) float sbuf[I4 ? 4 : 1][2][kPgNG][32];  // scales of a wave's keys and values
+  __shared__ float mls[W][16][2];
+  __shared__ __attribute__((aligned(16))) float sbuf[I4 ? W : 1][2][kPgNG][32];  // scales of a wave's keys and values
   __shared__ u32x4 m24[7];  // -24 eight times between zeros
   u32x4* qf = reinterpret_cast<u32x4*>(lds);  // [NR][hi, lo][8 steps][64 lanes]
-  float* ob = reinterpret_cast<float*>(lds);  // [4 waves][16][kORow], once Q has been used
+  float* ob = reinterpret_cast<float*>(lds);  // [W waves][16][kORow], once Q has been used
 
-  // ---- Q's rows, 16 lanes each: tile i's row 4 wave + lane / 16, token r / G, head r % G of the group. Their loads and the norm
+  // ---- Q's rows, 16 lanes each, four waves a tile: row 4 (wave % 4) + lane / 16 of it, token r / G, head r % G of the group. Their loads and the norm
   // weight's go out before anything is known of the row's position, raw, so that nothing waits for them yet (16 rows of 16 bf16
   // tokens 25.4 -> 23.4 us, 512 tokens behind 16 K keys 117.4 -> 115.3).
-  const int half = p.rot >> 1, qj = lane & 15, qcol = 4 * wave + (lane >> 4);
-  u32x4 qx[NR][4], qp[NR][4];
+  const int half = p.rot >> 1, qj = lane & 15, qcol = 4 * (wave & 3) + (lane >> 4);
+  constexpr int QT = W == 4 ? NR : 1;  // tiles that a wave prepares: all, or tile wave / 4 where there is one
+  const int q0 = W == 4 ? 0 : wave >> 2;
+  u32x4 qx[QT][4], qp[QT][4];
   f32x4 wx[4], wp[4];
   auto pair_of = [&](int d) { return d >= p.rot ? d : d < half ? d + half : d - half; };
 #pragma unroll
-  for (int i = 0; i < NR; ++i) {
-    const int r = r0 + 16 * i + qcol, t = r / p.G, h = kvh * p.G + r - t * p.G;
+  for (int i = 0; i < QT; ++i) {
+    const int r = r0 + 16 * (q0 + i) + qcol, t = r / p.G, h = kvh * p.G + r - t * p.G;
     const int64_t o = b * p.qb + t * p.qt + h * p.qh;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       qx[i][q] = qp[i][q] = u32x4{0, 0, 0, 0};
-      if (r < R) {
+      if (r < R && q0 + i < NR) {
         const int d = 64 * q + 4 * qj;
         qx[i][q] = quad_raw(p.q, p.q_f32, o + d);
         if (d < p.rot) qp[i][q] = quad_raw(p.q, p.q_f32, o + pair_of(d));
@@ -349,11 +351,11 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttnArgs p) {
 
   // the rows' angles, ahead of the keys: loads return in order (the second tile's against bf16 when the first is done: there
   // are no registers for both beside the keys)
-  constexpr int kAngles = kTurns ? 1 : NR;
+  constexpr int kAngles = kTurns ? 1 : QT;
   f32x4 co[kAngles][4], si[kAngles][4];
   auto angles = [&](int i, f32x4 (&co)[4], f32x4 (&si)[4]) {
-    const int tk = (r0 + 16 * i + qcol) / p.G;
-    const bool there = r0 + 16 * i + qcol < R && keys_seen(p, pos, len, tk) > 0;
+    const int tk = (r0 + 16 * (q0 + i) + qcol) / p.G;
+    const bool there = r0 + 16 * (q0 + i) + qcol < R && q0 + i < NR && keys_seen(p, pos, len, tk) > 0;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int d = 64 * q + 4 * qj, pj = d < half ? d : d - half;
@@ -393,7 +395,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttnArgs p) {
     vt_at[0] = nt[0];
     vt_at[1] = nt[1];
     vs_mine = s_load(p.vs, nt);
-    if (key + kRound < k1) next = key + kRound;
+    if (key + KEYS < k1) next = key + KEYS;
 #pragma unroll
     for (int u = 0; u < 2; ++u) nt[u] = tile_at(next + 16 * u);
   }
@@ -401,11 +403,11 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttnArgs p) {
 
   // ---- Q: norm, rotation, scale log2(e), the split into hi + lo or the power of two, into LDS as B operands (rows that are
   // not there: zeros)
-  if (work) {
+  if (work && q0 < NR) {
 #pragma unroll
-    for (int i = 0; i < NR; ++i) {
-      const int tk = (r0 + 16 * i + qcol) / p.G, ia = i < kAngles ? i : 0;
-      const bool there = r0 + 16 * i + qcol < R && keys_seen(p, pos, len, tk) > 0;
+    for (int i = 0; i < QT; ++i) {
+      const int tk = (r0 + 16 * (q0 + i) + qcol) / p.G, ia = i < kAngles ? i : 0;
+      const bool there = r0 + 16 * (q0 + i) + qcol < R && keys_seen(p, pos, len, tk) > 0;
       if (i >= kAngles) angles(i, co[0], si[0]);
       f32x4 x[4], px[4];
 #pragma unroll
@@ -433,7 +435,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttnArgs p) {
           x[q][e] = v * (p.scale * 1.4426950408889634f);
         }
       }
-      q_store<I4>(x, qj, qcol, qf + (size_t)i * QP * QF, qoff[i], &qfac[16 * i + qcol]);
+      q_store<I4>(x, qj, qcol, qf + (size_t)(q0 + i) * QP * QF, qoff[q0 + i], &qfac[16 * (q0 + i) + qcol]);
     }
   }
 
@@ -545,7 +547,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttnArgs p) {
       k_load(nt[1], kt[1]);
     }
     ks_mine = s_load(p.ks, nt);
-    const int after = next + kRound < k1 ? next + kRound : next;
+    const int after = next + KEYS < k1 ? next + KEYS : next;
     const Tile nn[2] = {tile_at(after), tile_at(after + 16)};
     __builtin_amdgcn_sched_barrier(0);
     // ---- masks, only where some row does not see every key of the two tiles
@@ -766,11 +768,11 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttnArgs p) {
     vs_mine = s_load(p.vs, nt);
     nt[0] = nn[0];
     nt[1] = nn[1];
-    key += kRound;
+    key += KEYS;
     next = after;
   }
 
-  // ---- 16 rows at a time: each wave's rows (those that are there) into LDS, dims in order, then the four waves joined, one
+  // ---- 16 rows at a time: each wave's rows (those that are there) into LDS, dims in order, then the waves joined, one
   // wave per row: the result, or the run's partial
   const int le = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)), ce = le & 15, ae = le >> 4, de = 4 * le;
 #pragma unroll
@@ -789,18 +791,18 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttnArgs p) {
     }
     lds_barrier();
 #pragma unroll
-    for (int jj = 0; jj < 4; ++jj) {
-      const int j = 4 * jj + wave;
+    for (int jj = 0; jj < 16 / W; ++jj) {
+      const int j = W * jj + wave;
       if (r0 + 16 * i + j >= R) break;
       const int r = r0 + 16 * i + j, t = r / p.G, h = kvh * p.G + r - t * p.G;
       float M = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) M = fmaxf(M, mls[w][j][0]);
+      for (int w = 0; w < W; ++w) M = fmaxf(M, mls[w][j][0]);
       float L = 0.f;
       f32x4 O = zero4();
       if (M > -INFINITY) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < W; ++w) {
           if (mls[w][j][0] == -INFINITY) continue;  // nothing seen
           const float f = __builtin_amdgcn_exp2f(mls[w][j][0] - M);
           L += mls[w][j][1] * f;
@@ -917,24 +919,32 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs p) 
 // rounds (three rows of 8192 4-bit keys: 64 runs 16.1 us, 32 runs 14.1, 16 runs 16.7). A table of two rounds is not split
 // (256 keys, one row: 11.9 us against 12.5 for two runs and their merge, 4 bits 9.9 against 11.2; four rounds 16.4 against
 // 12.7, 4 bits 12.6 against 11.3).
+// Eight waves to a block, at one block per CU, for tables of two to four rounds that then need no merge either: up to three
+// rounds of codes (one row of 384 keys 10.1 us against 10.6 for three runs, 32 rows 10.7 against 11.4; four rounds, 32 rows:
+// 12.3 against 11.8) and two of bf16 for 32 query rows (18.4 against 19.5; one token's 16: 15.2 against 13.4: one CU then
+// loads what two share); and all of them, but one token's two of bf16, where 65 to 256 blocks would be dealt to the CUs
+// unevenly (80 rows of 384 keys: 19.2 us against 23.8, 4 bits 11.8 against 16.2).
 struct PagedPlan {
-  int NR, RB, S;
+  int NR, RB, S, W;
 };
 static PagedPlan paged_plan(int64_t B, int64_t T, int64_t Hkv, int64_t G, int64_t capacity, int64_t splits, int fmt) {
   const int64_t R = T * G, tiles = (R + 15) / 16;
   const int NR = tiles == 1 || (tiles == 3 && fmt == Q35_I4_G64) ? 1 : 2;
   const int64_t RB = (R + 16 * NR - 1) / (16 * NR), base = B * Hkv * RB;
   const int64_t most = (capacity + kRound - 1) / kRound;
+  const bool i4 = fmt == Q35_I4_G64;
+  const bool eight = base <= 256 && most > 1 && most <= 4 &&
+                     (base > 64 ? i4 || NR == 2 || most > 2 : i4 ? most <= 3 : NR == 2 && most == 2);
   int64_t S = splits;
   if (S <= 0) {
     S = (512 + base - 1) / base;
     if (most <= 2 * S) S = (256 + base - 1) / base;
-    if (most <= 2) S = 1;
+    if (most <= 2 || eight) S = 1;
   }
   if (S > most) S = most;
   if (S > 1024) S = 1024;
   if (S < 1) S = 1;
-  return {NR, (int)RB, (int)S};
+  return {NR, (int)RB, (int)S, S == 1 && eight ? 8 : 4};
 }
 
 }  // namespace q35
@@ -996,7 +1006,11 @@ extern "C" int q35_gated_attn_paged(const void* q, int64_t q_sb, int64_t q_st, i
   a.T = (int)T, a.Hkv = (int)Hkv, a.G = (int)G, a.S = pl.S, a.RB = pl.RB;
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid(pl.S, (unsigned)(Hkv * pl.RB), (unsigned)B), block(256);
-#define Q35_PAGED(I4, NR) hipLaunchKernelGGL((paged_attn_kernel<I4, NR>), grid, block, 0, st, a)
+#define Q35_PAGED(I4, NR)                                                                            \
+  do {                                                                                               \
+    if (pl.W == 8) hipLaunchKernelGGL((paged_attn_kernel<I4, NR, 8>), grid, dim3(512), 0, st, a);    \
+    else hipLaunchKernelGGL((paged_attn_kernel<I4, NR, 4>), grid, block, 0, st, a);                  \
+  } while (0)
   if (fmt == Q35_BF16) {
     if (pl.NR == 1) Q35_PAGED(false, 1); else Q35_PAGED(false, 2);
   } else {

@@ -506,6 +506,21 @@ def test_attention_rows_over_three_to_five_tiles(fmt, T, Hq, lens):
         check_attention(d, attend(g, splits=splits))
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "int4"])
+@pytest.mark.parametrize("B,T,nb", [(2, 1, 2), (2, 1, 3), (2, 1, 4), (2, 6, 2), (2, 6, 3), (40, 1, 3), (40, 6, 4), (70, 1, 2),
+                                    (130, 2, 3)])
+def test_attention_over_tables_of_two_to_four_rounds(fmt, B, T, nb):
+    """Tables of 256 to 512 keys for few rows and many: one block of eight waves, of four, or several and their merge."""
+    ctx = [128 * nb - (37 * b) % (128 * nb - T) for b in range(B)]
+    d = make(fmt, B, T, 4, 2, 128, ctx, nb=nb)
+    announce(f"paged attention {fmt} B {B} T {T} table of {128 * nb}")
+    g = to(d, device())
+    out = attend(g)
+    check_attention(d, out)
+    if B == 2:
+        check_attention(d, attend(g, splits=1))
+
+
 @pytest.mark.parametrize("T", [1, 6])
 def test_attention_more_splits_than_rounds(T):
     d = make("int4", 2, T, 8, 2, 32, [3000, 130])
