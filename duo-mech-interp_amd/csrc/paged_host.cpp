@@ -127,6 +127,15 @@ Pages pages_of(PyObject* const* a, int64_t d, int64_t B) {
   return p;
 }
 
+// Their addresses.
+struct PagesAt {
+  void *k, *v, *ks, *vs;
+  int32_t *table, *pos, *lens;
+  explicit PagesAt(const Pages& p)
+      : k(data(p.k)), v(data(p.v)), ks(data(p.ks)), vs(data(p.vs)), table(data<int32_t>(p.table)), pos(data<int32_t>(p.pos)),
+        lens(data<int32_t>(p.lens)) {}
+};
+
 struct Rope {
   const Tensor &cos, &sin;
   const Tensor* norm_w;
@@ -145,11 +154,26 @@ Rope rope_of(PyObject* const* a, int64_t d, int64_t rows) {
   return r;
 }
 
+struct RopeAt {
+  float *cos, *sin, *norm_w;
+  explicit RopeAt(const Rope& r) : cos(data<float>(r.cos)), sin(data<float>(r.sin)), norm_w(data<float>(r.norm_w)) {}
+};
+
 Tensor make(at::IntArrayRef size, at::ScalarType s, const Tensor& like) {
   return at::empty(size, at::TensorOptions().dtype(s).device(like.device()));
 }
 
-// call(stream) with t's device current and the interpreter free, its status checked.
+// Gives the interpreter lock up for as long as it lives, however its scope is left.
+struct Unlocked {
+  PyThreadState* state = PyEval_SaveThread();
+  Unlocked() = default;
+  Unlocked(const Unlocked&) = delete;
+  Unlocked& operator=(const Unlocked&) = delete;
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
+
+// call(stream) with t's device current and the interpreter free, its status checked. `call` holds its pointers already (init
+// captures of the lambda): a tensor without storage refuses to give one, by an exception, and before anything runs.
 template <typename F> void launch(const Tensor& t, const char* name, F&& call) {
   PyObject* d = PyLong_FromLongLong(t.get_device());
   PyObject* h = d ? PyObject_CallOneArg(g_stream, d) : nullptr;
@@ -161,9 +185,8 @@ template <typename F> void launch(const Tensor& t, const char* name, F&& call) {
   int status;
   {
     const c10::DeviceGuard guard(t.device());
-    PyThreadState* state = PyEval_SaveThread();
+    const Unlocked unlocked;
     status = call(static_cast<q35_stream_t>(stream));
-    PyEval_RestoreThread(state);
   }
   if (status != Q35_OK) {
     Py_XDECREF(PyObject_CallFunction(g_check, "is", status, name));
@@ -204,11 +227,10 @@ PyObject* paged_kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Rope r = rope_of(a + 9, d, p.blocks * p.size);
     const double eps = number(a[12]);
     if (B && T)
-      launch(k, "q35_paged_kv_append", [&](q35_stream_t st) {
-        return g_append(data(k), kv.b, kv.t, kv.h, data(v), vv.b, vv.t, vv.h, kv.dtype, data<float>(r.norm_w), (float)eps,
-                        data<float>(r.cos), data<float>(r.sin), r.rot, data<int32_t>(p.table), p.ld, p.blocks,
-                        data<int32_t>(p.pos), data<int32_t>(p.lens), data(p.k), data(p.v), data(p.ks), data(p.vs), p.fmt,
-                        p.n, p.size, B, T, p.heads, 256, st);
+      launch(k, "q35_paged_kv_append", [&, at = PagesAt(p), ro = RopeAt(r), xk = data(k), xv = data(v)](q35_stream_t st) {
+        return g_append(xk, kv.b, kv.t, kv.h, xv, vv.b, vv.t, vv.h, kv.dtype, ro.norm_w, (float)eps, ro.cos, ro.sin, r.rot,
+                        at.table, p.ld, p.blocks, at.pos, at.lens, at.k, at.v, at.ks, at.vs, p.fmt, p.n, p.size, B, T,
+                        p.heads, 256, st);
       });
     Py_RETURN_NONE;
   });
@@ -222,9 +244,9 @@ PyObject* paged_kv_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (T < 0) refuse("T: a number of tokens");
     const Tensor k = make({B, p.heads, T, 256}, at::kBFloat16, p.k), v = make({B, p.heads, T, 256}, at::kBFloat16, p.k);
     if (B && T)
-      launch(p.k, "q35_paged_kv_rows", [&](q35_stream_t st) {
-        return g_rows(data(p.k), data(p.v), data(p.ks), data(p.vs), p.fmt, p.n, p.size, data<int32_t>(p.table), p.ld,
-                      p.blocks, data<int32_t>(p.pos), data<int32_t>(p.lens), data(k), data(v), B, T, p.heads, 256, st);
+      launch(p.k, "q35_paged_kv_rows", [&, at = PagesAt(p), ko = data(k), vo = data(v)](q35_stream_t st) {
+        return g_rows(at.k, at.v, at.ks, at.vs, p.fmt, p.n, p.size, at.table, p.ld, p.blocks, at.pos, at.lens, ko, vo, B, T,
+                      p.heads, 256, st);
       });
     return Py_BuildValue("(NN)", THPVariable_Wrap(k), THPVariable_Wrap(v));
   });
@@ -253,12 +275,11 @@ PyObject* gated_attn_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
       const size_t bytes = g_attn_bytes(B, T, Hq, p.heads, 256, p.blocks, p.size, splits);
       if (!bytes) refuse("unsupported attention shape");
       const Tensor ws = make({(int64_t)bytes}, at::kByte, q);
-      launch(q, "q35_gated_attn_paged", [&](q35_stream_t st) {
-        return g_attn(data(q), qv.b, qv.t, qv.h, data(gate), gv.b, gv.t, gv.h, qv.dtype, data<float>(r.norm_w), (float)eps,
-                      data<float>(r.cos), data<float>(r.sin), r.rot, data(p.k), data(p.v), data(p.ks), data(p.vs), p.fmt,
-                      p.n, p.size, data<int32_t>(p.table), p.ld, p.blocks, data<int32_t>(p.pos), data<int32_t>(p.lens),
-                      data(out), f32 ? Q35_F32 : Q35_BF16, B, T, Hq, p.heads, 256, (float)scale, splits, data(ws), bytes,
-                      st);
+      launch(q, "q35_gated_attn_paged", [&, at = PagesAt(p), ro = RopeAt(r), xq = data(q), xg = data(gate), o = data(out),
+                                         w = data(ws)](q35_stream_t st) {
+        return g_attn(xq, qv.b, qv.t, qv.h, xg, gv.b, gv.t, gv.h, qv.dtype, ro.norm_w, (float)eps, ro.cos, ro.sin, r.rot,
+                      at.k, at.v, at.ks, at.vs, p.fmt, p.n, p.size, at.table, p.ld, p.blocks, at.pos, at.lens, o,
+                      f32 ? Q35_F32 : Q35_BF16, B, T, Hq, p.heads, 256, (float)scale, splits, w, bytes, st);
       });
     }
     return THPVariable_Wrap(out);
@@ -294,11 +315,13 @@ PyObject* verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t n) {
         refuse("unsupported draft shape (B=" + std::to_string(B) + ", K=" + std::to_string(K) + ", V=" + std::to_string(V) +
                ")");
       const Tensor ws = make({(int64_t)bytes}, at::kByte, x);
-      launch(x, "q35_verify_drafts", [&](q35_stream_t st) {
-        return g_verify(data<float>(x), x.stride(0), x.stride(1), data<int32_t>(ids), ids.stride(0), data<float>(probs),
-                        probs ? probs->stride(0) : 0, probs ? probs->stride(1) : 0, data<float>(u), u.stride(0),
-                        data<int32_t>(lens), data<float>(temps), (float)temperature, data<int32_t>(accepted),
-                        data<int32_t>(tokens), B, K, V, data(ws), bytes, st);
+      const int64_t xs[2] = {x.stride(0), x.stride(1)}, qs[2] = {probs ? probs->stride(0) : 0, probs ? probs->stride(1) : 0};
+      const int64_t is = ids.stride(0), us = u.stride(0);
+      launch(x, "q35_verify_drafts", [&, xa = data<float>(x), ia = data<int32_t>(ids), qa = data<float>(probs),
+                                      ua = data<float>(u), la = data<int32_t>(lens), ta = data<float>(temps),
+                                      na = data<int32_t>(accepted), ka = data<int32_t>(tokens), w = data(ws)](q35_stream_t st) {
+        return g_verify(xa, xs[0], xs[1], ia, is, qa, qs[0], qs[1], ua, us, la, ta, (float)temperature, na, ka, B, K, V, w,
+                        bytes, st);
       });
     }
     return Py_BuildValue("(NN)", THPVariable_Wrap(accepted), THPVariable_Wrap(tokens));

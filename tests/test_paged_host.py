@@ -42,3 +42,62 @@ def test_arguments_are_counted_and_typed():
 def test_bind_takes_nine_arguments():
     with pytest.raises(TypeError):
         ops._paged_host().bind(Q35Error)
+
+
+# The extension bound to entry points that do nothing, for tensors on a device that is not there. In a process of its own: a
+# fault in it ends that process, and the binding is for good.
+STUBS = """
+import ctypes
+import sys
+sys.path.insert(0, {root!r})
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+from q35hip import Q35Error, _lib, ops
+
+h = ops._paged_host()
+done = []
+call = ctypes.CFUNCTYPE(ctypes.c_int)(lambda: done.append(1) or 0)
+size = ctypes.CFUNCTYPE(ctypes.c_size_t)(lambda: 256)
+h.bind(Q35Error, _lib.check, lambda d: 0, *(ctypes.cast(f, ctypes.c_void_p).value for f in (call, call, size, call, size, call)))
+
+
+def fake(*size, dtype=torch.float32):
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        return torch.zeros(*size, dtype=dtype, device="cuda:0")
+
+
+kv, x, u = fake(3, 1, 1, 2, 256), fake(3, 1, 2, 5), fake(3, 1, 2)  # three of each, to be mapped over
+pages = (*(fake(3, 2, 16, 256, dtype=torch.bfloat16) for _ in range(2)), None, None)
+at = (fake(1, 2, dtype=torch.int32), fake(1, dtype=torch.int32))
+rope = (fake(32, 32), fake(32, 32))
+ids = fake(1, 1, dtype=torch.int32)
+"""
+
+
+def run_with_stubs(body):
+    import os
+    import subprocess
+    import sys
+    import textwrap
+    from q35hip import build
+    r = subprocess.run([sys.executable, "-c", STUBS.format(root=build.ROOT) + textwrap.dedent(body)], capture_output=True,
+                       text=True, timeout=300, env=dict(os.environ, PYTHONFAULTHANDLER="1"))
+    assert r.returncode == 0, r.stdout + r.stderr[-3000:]
+    return r.stdout
+
+
+def test_a_tensor_without_storage_raises():
+    """A wrapper of functorch's has no address to give: an exception out of the extension, with the interpreter lock held."""
+    out = run_with_stubs("""
+        calls = [(lambda k: h.paged_kv_append(k, k, *pages, *at, None, *rope, None, 1e-6), kv),
+                 (lambda p: h.paged_kv_rows(p, p, None, None, *at, None, 4), torch.stack([pages[0]] * 3)),
+                 (lambda q: h.gated_attn_paged(q, None, *pages, *at, None, *rope, None, 1e-6, 0.1, 0, False), kv),
+                 (lambda u: h.verify_drafts(x[0], ids, None, u, None, None, 1.0), u)]
+        for f, arg in calls:
+            try:
+                torch.vmap(lambda t: (f(t), t)[1])(arg)
+            except RuntimeError as e:
+                print("raised", type(e).__name__, "storage" in str(e))
+        print("called", len(done))
+        """)
+    assert out.count("raised") == 4 and "called 0" in out, out
