@@ -6,6 +6,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -59,6 +60,17 @@ int64_t integer(PyObject* o) {
   if (v == -1 && PyErr_Occurred()) throw PyFailed{};
   return v;
 }
+// A device tensor whose memory holds its values, as nobody else's business: not a functorch or functionalization wrapper, a
+// subclass, a view that is negated or conjugated when read, and nothing that autograd follows.
+bool plain(PyObject* o) {
+  if (!THPVariable_Check(o)) return true;  // (a number or None)
+  if (!THPVariable_CheckExact(o)) return false;
+  constexpr c10::DispatchKeySet own({c10::DispatchKey::CUDA, c10::DispatchKey::ADInplaceOrView, c10::DispatchKey::AutogradCUDA,
+                                     c10::DispatchKey::AutocastCUDA});
+  const Tensor& t = THPVariable_Unpack(o);
+  return (t.key_set().raw_repr() & ~own.raw_repr()) == 0 && !(at::GradMode::is_enabled() && t.requires_grad());
+}
+
 template <typename T = void> T* data(const Tensor& t) { return static_cast<T*>(t.data_ptr()); }
 template <typename T = void> T* data(const Tensor* t) { return t ? static_cast<T*>(t->data_ptr()) : nullptr; }
 
@@ -328,6 +340,11 @@ PyObject* verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// Any arguments: whether an op on them is the functions above and nothing more.
+PyObject* direct(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(0, 0, [&]() -> PyObject* { return PyBool_FromLong(std::all_of(a, a + n, plain)); });
+}
+
 // error, check, stream, then the addresses of the six functions of the C ABI
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 9) {
@@ -355,8 +372,9 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 #define Q35_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef g_methods[] = {Q35_METHOD(bind),          Q35_METHOD(paged_kv_append), Q35_METHOD(paged_kv_rows),
-                           Q35_METHOD(gated_attn_paged), Q35_METHOD(verify_drafts), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef g_methods[] = {Q35_METHOD(bind),          Q35_METHOD(direct),           Q35_METHOD(paged_kv_append),
+                           Q35_METHOD(paged_kv_rows), Q35_METHOD(gated_attn_paged), Q35_METHOD(verify_drafts),
+                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_paged_host", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -1187,11 +1187,16 @@ def argmax_rows(x, out=None):
     return out
 
 
-def _direct(t):
-    """Whether an op on t can be called as the function it is: a plain device tensor, nothing tracing. (The dispatcher takes
-    3 us of a call's host time, a third of what an append takes.) Anything else goes through torch.ops."""
-    return type(t) is torch.Tensor and t.is_cuda and not torch._C._len_torch_dispatch_stack() \
-        and not torch.compiler.is_compiling()
+def _call(name, op, *args):
+    """The op on these arguments: as the extension's function `name` where they are plain device tensors and nothing follows
+    the call (the dispatcher takes 3 us of a call's host time, a third of what an append takes), else through torch.ops."""
+    x = args[0]
+    if torch.is_tensor(x) and x.is_cuda and not torch._C._len_torch_dispatch_stack() \
+            and torch._C._functorch.maybe_current_level() is None and not torch.compiler.is_compiling():
+        host = _paged_host()
+        if host.direct(*args):
+            return getattr(host, name)(*args)
+    return op(*args)
 
 
 class KVPages(NamedTuple):
@@ -1225,16 +1230,15 @@ def paged_kv_append_(k, v, pages, table, pos, cos, sin, *, lens=None, k_norm_w=N
     table: [B, blocks] int32, row b's page of each block of page-size tokens; token t of row b goes to position
     pos[b] + t, t < lens[b] ([B] int32; None: all T). Tokens past lens, past the capacity or on a table entry that names
     no page are not written. The table entries that a call writes to must all name different pages."""
-    op = _paged_host().paged_kv_append if _direct(k) else torch.ops.q35.paged_kv_append_
-    op(k, v, *_four(pages), table, pos, lens, cos, sin, k_norm_w, float(eps))
+    _call("paged_kv_append", torch.ops.q35.paged_kv_append_, k, v, *_four(pages), table, pos, lens, cos, sin, k_norm_w,
+          float(eps))
 
 
 def paged_kv_rows(pages, table, pos, T, *, lens=None):
     """Rows pos[b] .. pos[b] + T - 1 of each sequence read back from its pages: (k, v) [B, Hkv, T, 256] bf16, the layout
     of the dense caches (with pos 0 and T a multiple of 64 the caches of gated_attention_prefill_cached); zeros past
     lens, past the table and where a table entry names no page."""
-    op = _paged_host().paged_kv_rows if _direct(pages[0]) else torch.ops.q35.paged_kv_rows
-    return op(*_four(pages), table, pos, lens, int(T))
+    return _call("paged_kv_rows", torch.ops.q35.paged_kv_rows, *_four(pages), table, pos, lens, int(T))
 
 
 def gated_attention_paged(q, gate, pages, table, pos, cos, sin, *, lens=None, q_norm_w=None, eps=1e-6, scale=None,
@@ -1246,9 +1250,9 @@ def gated_attention_paged(q, gate, pages, table, pos, cos, sin, *, lens=None, q_
     prompt; Hq / Hkv any ratio. Returns [B, T, Hq * 256] in out_dtype (bf16 or fp32), zeros for tokens past lens or the
     table's capacity. splits: over how many blocks a row's keys are dealt (0: by the sizes)."""
     _require(out_dtype in (torch.bfloat16, torch.float32), "out_dtype: bf16 or fp32")
-    op = _paged_host().gated_attn_paged if _direct(q) else torch.ops.q35.gated_attn_paged
-    return op(q, gate, *_four(pages), table, pos, lens, cos, sin, q_norm_w, float(eps),
-              q.shape[-1] ** -0.5 if scale is None else float(scale), int(splits), out_dtype == torch.float32)
+    return _call("gated_attn_paged", torch.ops.q35.gated_attn_paged, q, gate, *_four(pages), table, pos, lens, cos, sin,
+                 q_norm_w, float(eps), q.shape[-1] ** -0.5 if scale is None else float(scale), int(splits),
+                 out_dtype == torch.float32)
 
 
 def _four(pages):
@@ -1269,8 +1273,7 @@ def verify_drafts(logits, draft_ids, u, *, draft_probs=None, lens=None, temperat
     draft: the lowest index whose running sum exceeds u[:, K] of the whole. The kept drafts and the drawn token are then
     distributed as draws from p. Returns (n_accept [B] int32, tokens [B, K + 1] int32: kept drafts, drawn token, -1)."""
     ts, t = (temperature, 0.0) if torch.is_tensor(temperature) else (None, float(temperature))
-    op = _paged_host().verify_drafts if _direct(logits) else torch.ops.q35.verify_drafts
-    return op(logits, draft_ids, draft_probs, u, lens, ts, t)
+    return _call("verify_drafts", torch.ops.q35.verify_drafts, logits, draft_ids, draft_probs, u, lens, ts, t)
 
 
 def add_rmsnorm_(x, y, w, eps=1e-6, split=False):

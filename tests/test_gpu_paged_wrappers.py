@@ -1,0 +1,63 @@
+"""The paged-cache ops on tensors that stand for others (vmap, functionalization, negated views), under autograd, in traces and
+compiled functions: what the plain calls give."""
+import pytest
+import torch
+
+from gpu_util import announce, device
+from q35hip import ops
+from test_gpu_paged import append, attend, columns, make, to
+
+pytestmark = pytest.mark.gpu
+
+
+def drafts(B, K, V, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    dev = device()
+    return (torch.randn(B, K + 1, V, generator=g).to(dev), torch.randint(0, V, (B, K), generator=g).int().to(dev),
+            torch.rand(5, B, K + 1, generator=g).to(dev))
+
+
+def test_vmap():
+    """Mapped over any argument, the first or another."""
+    x, ids, us = drafts(3, 2, 1000)
+    announce("paged ops under vmap")
+    want = [ops.verify_drafts(x, ids, u) for u in us]
+    n, tok = torch.vmap(lambda u: ops.verify_drafts(x, ids, u))(us)
+    assert all(torch.equal(n[i], w[0]) and torch.equal(tok[i], w[1]) for i, w in enumerate(want))
+    g = to(make("int4", 2, 3, 4, 2, 16, [70, 33], lens=[3, 2]), device())
+    q, gate, _, _ = columns(g["y"], 4, 2)
+    qs = torch.stack([q, 2 * q, -q])
+    rest = (g["pages"], g["table"], g["pos"], g["cos"], g["sin"])
+    out = torch.vmap(lambda q: ops.gated_attention_paged(q, gate, *rest))(qs)
+    assert all(torch.equal(out[i], ops.gated_attention_paged(qs[i], gate, *rest)) for i in range(3))
+    pos = torch.tensor([[0, 3], [5, 1]], dtype=torch.int32, device=q.device)
+    k, v = torch.vmap(lambda p: ops.paged_kv_rows(g["pages"], g["table"], p, 9))(pos)
+    for i in range(2):
+        wk, wv = ops.paged_kv_rows(g["pages"], g["table"], pos[i], 9)
+        assert torch.equal(k[i], wk) and torch.equal(v[i], wv)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int4"])
+def test_negated_views_and_functional_tensors(fmt):
+    g = to(make(fmt, 2, 3, 4, 2, 16, [70, 33], lens=[3, 2]), device())
+    q, gate, _, _ = columns(g["y"], 4, 2)
+    rest = (g["pages"], g["table"], g["pos"], g["cos"], g["sin"])
+    announce(f"paged attention {fmt}, negated views and functional tensors")
+    want = ops.gated_attention_paged(-q, -gate, *rest)
+    for a, b in ((-q, torch._neg_view(gate)), (torch._neg_view(q), -gate)):
+        assert torch.equal(ops.gated_attention_paged(a, b, *rest), want)
+    assert torch.equal(torch.func.functionalize(lambda q: ops.gated_attention_paged(q, -gate, *rest))(-q), want)
+
+
+def test_parameters_and_inputs_that_ask_for_a_gradient():
+    """Parameters are tensors like others; autograd is told that there is no gradient, as by every op of the package."""
+    g = to(make("bf16", 2, 3, 4, 2, 16, [70, 33], lens=[3, 2]), device())
+    q, gate, _, _ = columns(g["y"], 4, 2)
+    rest = (g["pages"], g["table"], g["pos"], g["cos"], g["sin"])
+    announce("paged attention, parameters")
+    want = ops.gated_attention_paged(q, gate, *rest, q_norm_w=g["qw"])
+    w = torch.nn.Parameter(g["qw"])
+    with torch.no_grad():
+        assert torch.equal(ops.gated_attention_paged(q, gate, *rest, q_norm_w=w), want)
+    out = ops.gated_attention_paged(q, gate, *rest, q_norm_w=w)
+    assert torch.equal(out, want) and out.requires_grad

@@ -101,3 +101,27 @@ def test_a_tensor_without_storage_raises():
         print("called", len(done))
         """)
     assert out.count("raised") == 4 and "called 0" in out, out
+
+
+def test_wrapped_tensors_go_through_the_dispatcher():
+    """vmap, functionalization and a tensor that is negated when read, in any argument: none reaches the extension."""
+    out = run_with_stubs("""
+        logits = torch.stack([x[0]] * 3)
+        n, tok = torch.vmap(lambda l: ops.verify_drafts(l, ids, u[0]))(logits)
+        print("mapped", tuple(n.shape), tuple(tok.shape))
+        n, tok = torch.vmap(lambda w: ops.verify_drafts(x[0], ids, w))(u)  # (the first argument is not wrapped)
+        print("mapped", tuple(n.shape), tuple(tok.shape))
+        o = torch.vmap(lambda q: ops.gated_attention_paged(q, None, pages, *at, *rope))(kv)
+        print("mapped", tuple(o.shape))
+        o, _ = torch.vmap(lambda p: ops.paged_kv_rows((p, p), *at, 4))(torch.stack([pages[0]] * 3))
+        print("mapped", tuple(o.shape))
+        o = ops.gated_attention_paged(torch._to_functional_tensor(kv[0]), None, pages, *at, *rope)
+        print("functional", tuple(o.shape))
+        with torch.enable_grad():
+            print("direct", h.direct(kv[0]), h.direct(torch._to_functional_tensor(kv[0])), h.direct(1.0, None),
+                  h.direct(torch.zeros(2)))
+        print("called", len(done))
+        """)
+    for line in ("mapped (3, 1) (3, 1, 2)\nmapped (3, 1) (3, 1, 2)\nmapped (3, 1, 1, 512)\nmapped (3, 1, 2, 4, 256)",
+                 "functional (1, 1, 512)", "direct False False True False", "called 0"):
+        assert line in out, out
