@@ -1191,8 +1191,9 @@ def _call(name, op, *args):
     """The op on these arguments: as the extension's function `name` where they are plain device tensors and nothing follows
     the call (the dispatcher takes 3 us of a call's host time, a third of what an append takes), else through torch.ops."""
     x = args[0]
-    if torch.is_tensor(x) and x.is_cuda and not torch._C._len_torch_dispatch_stack() \
-            and torch._C._functorch.maybe_current_level() is None and not torch.compiler.is_compiling():
+    # (is_compiling ahead of all else: a compiler folds the branch there, and could not follow what is asked behind it)
+    if not torch.compiler.is_compiling() and torch.is_tensor(x) and x.is_cuda \
+            and not torch._C._len_torch_dispatch_stack() and torch._C._functorch.maybe_current_level() is None:
         host = _paged_host()
         if host.direct(*args):
             return getattr(host, name)(*args)

@@ -61,3 +61,23 @@ def test_parameters_and_inputs_that_ask_for_a_gradient():
         assert torch.equal(ops.gated_attention_paged(q, gate, *rest, q_norm_w=w), want)
     out = ops.gated_attention_paged(q, gate, *rest, q_norm_w=w)
     assert torch.equal(out, want) and out.requires_grad
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int4"])
+def test_compiled_whole(fmt):
+    g = to(make(fmt, 2, 3, 4, 2, 16, [70, 33], lens=[3, 2]), device())
+    x, ids, us = drafts(2, 2, 500)
+    other = dict(g, pages=tuple(None if p is None else p.clone() for p in g["pages"]))
+
+    def step(y, pages, u):
+        q, gate, k, v = columns(y, 4, 2)
+        rope = (g["cos"], g["sin"])
+        ops.paged_kv_append_(k, v, pages, g["table"], g["pos"], *rope, lens=g["lens"], k_norm_w=g["kw"])
+        o = ops.gated_attention_paged(q, gate, pages, g["table"], g["pos"], *rope, lens=g["lens"])
+        return o, *ops.paged_kv_rows(pages, g["table"], g["pos"], 3), *ops.verify_drafts(x, ids, u)
+    announce(f"paged ops compiled {fmt}")
+    got = torch.compile(step, fullgraph=True, backend="eager")(g["y"], other["pages"], us[0])
+    want = step(g["y"], g["pages"], us[0])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for a, b in zip(g["pages"], other["pages"]):
+        assert a is None or torch.equal(a.view(torch.uint8), b.view(torch.uint8))

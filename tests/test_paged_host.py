@@ -125,3 +125,26 @@ def test_wrapped_tensors_go_through_the_dispatcher():
     for line in ("mapped (3, 1) (3, 1, 2)\nmapped (3, 1) (3, 1, 2)\nmapped (3, 1, 1, 512)\nmapped (3, 1, 2, 4, 256)",
                  "functional (1, 1, 512)", "direct False False True False", "called 0"):
         assert line in out, out
+
+
+def test_a_compiled_function_holds_the_ops_whole():
+    """torch.compile without a break in the graph, for all four."""
+    out = run_with_stubs("""
+        seen = []
+
+        def backend(gm, inputs):
+            seen.extend(str(n.target) for n in gm.graph.nodes if "q35" in str(n.target))
+            return gm.forward
+
+        def step(k, q, u):
+            ops.paged_kv_append_(k, k, pages, *at, *rope)
+            a, _ = ops.paged_kv_rows(pages, *at, 4)
+            o = ops.gated_attention_paged(q, None, pages, *at, *rope)
+            return a, o, *ops.verify_drafts(x[0], ids, u, temperature=0.5)
+
+        r = torch.compile(step, fullgraph=True, backend=backend)(kv[0], kv[0], u[0])
+        print([tuple(t.shape) for t in r], len(seen), *seen)
+        """)
+    assert "[(1, 2, 4, 256), (1, 1, 512), (1,), (1, 2)] 4" in out, out
+    for name in ("paged_kv_append_", "paged_kv_rows", "gated_attn_paged", "verify_drafts"):
+        assert f"q35.{name}" in out, out
