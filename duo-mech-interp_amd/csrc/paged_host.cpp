@@ -9,6 +9,7 @@
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -340,9 +341,15 @@ PyObject* verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// Any arguments: whether an op on them is the functions above and nothing more.
+// Any arguments: whether an op on them is the functions above and nothing more. Whatever follows a thread's calls (a trace, a
+// dispatch mode, a transform) has its key among those that the thread includes in every dispatch.
 PyObject* direct(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return guarded(0, 0, [&]() -> PyObject* { return PyBool_FromLong(std::all_of(a, a + n, plain)); });
+  return guarded(0, 0, [&]() -> PyObject* {
+    constexpr c10::DispatchKeySet always({c10::DispatchKey::BackendSelect, c10::DispatchKey::ADInplaceOrView});
+    const auto local = c10::impl::tls_local_dispatch_key_set();
+    const bool followed = (local.included_.raw_repr() & ~local.excluded_.raw_repr() & ~always.raw_repr()) != 0;
+    return PyBool_FromLong(!followed && std::all_of(a, a + n, plain));
+  });
 }
 
 // error, check, stream, then the addresses of the six functions of the C ABI

@@ -1192,8 +1192,7 @@ def _call(name, op, *args):
     the call (the dispatcher takes 3 us of a call's host time, a third of what an append takes), else through torch.ops."""
     x = args[0]
     # (is_compiling ahead of all else: a compiler folds the branch there, and could not follow what is asked behind it)
-    if not torch.compiler.is_compiling() and torch.is_tensor(x) and x.is_cuda \
-            and not torch._C._len_torch_dispatch_stack() and torch._C._functorch.maybe_current_level() is None:
+    if not torch.compiler.is_compiling() and torch.is_tensor(x) and x.is_cuda:
         host = _paged_host()
         if host.direct(*args):
             return getattr(host, name)(*args)

@@ -81,3 +81,26 @@ def test_compiled_whole(fmt):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     for a, b in zip(g["pages"], other["pages"]):
         assert a is None or torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int4"])
+def test_a_trace_run_on_other_inputs(fmt):
+    """torch.jit.trace records the ops: what it gives for other queries, keys and random numbers is what the calls give."""
+    g = to(make(fmt, 2, 3, 4, 2, 16, [70, 33], lens=[3, 2]), device())
+    x, ids, us = drafts(2, 2, 500)
+    other = tuple(None if p is None else p.clone() for p in g["pages"])
+
+    def step(y, u, *pages):
+        q, gate, k, v = columns(y, 4, 2)
+        rope = (g["cos"], g["sin"])
+        ops.paged_kv_append_(k, v, pages, g["table"], g["pos"], *rope, lens=g["lens"], k_norm_w=g["kw"])
+        o = ops.gated_attention_paged(q, gate, pages, g["table"], g["pos"], *rope, lens=g["lens"])
+        return o, *ops.paged_kv_rows(pages, g["table"], g["pos"], 3), *ops.verify_drafts(x, ids, u)
+    announce(f"paged ops traced {fmt}")
+    traced = torch.jit.trace(step, (g["y"], us[0], *(p.clone() for p in g["pages"] if p is not None)), check_trace=False)
+    y = 0.5 * g["y"].flip(0)
+    got = traced(y, us[1], *(p for p in other if p is not None))
+    want = step(y, us[1], *g["pages"])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for a, b in zip(g["pages"], other):
+        assert a is None or torch.equal(a.view(torch.uint8), b.view(torch.uint8))

@@ -148,3 +148,42 @@ def test_a_compiled_function_holds_the_ops_whole():
     assert "[(1, 2, 4, 256), (1, 1, 512), (1,), (1, 2)] 4" in out, out
     for name in ("paged_kv_append_", "paged_kv_rows", "gated_attn_paged", "verify_drafts"):
         assert f"q35.{name}" in out, out
+
+
+def test_a_trace_records_the_ops(monkeypatch):
+    """torch.jit.trace and a dispatch mode, over tensors that pass for device ones: nothing but torch.ops is called."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    host, called = ops._paged_host(), []
+
+    class Host:
+        direct = staticmethod(lambda *args: host.direct())  # (what is asked of the thread, not of the tensors)
+
+        def __getattr__(self, name):
+            return lambda *args: (called.append(name), (args[0], args[1]))[1]
+    monkeypatch.setattr(ops, "_HOST", Host())
+
+    def meta(*size, dtype=torch.float32):
+        return torch.zeros(*size, dtype=dtype, device="meta")
+    args = (meta(1, 1, 2, 256), meta(3, 2, 16, 256, dtype=torch.bfloat16), meta(1, 2, dtype=torch.int32),
+            meta(1, dtype=torch.int32), meta(32, 32), meta(1, 2, 5), meta(1, 1, dtype=torch.int32), meta(1, 2))
+
+    def step(kv, page, table, pos, rope, x, ids, u):
+        ops.paged_kv_append_(kv, kv, (page, page), table, pos, rope, rope)
+        o = ops.gated_attention_paged(kv, None, (page, page), table, pos, rope, rope)
+        return o, *ops.paged_kv_rows((page, page), table, pos, 4), *ops.verify_drafts(x, ids, u)
+    with monkeypatch.context() as m:
+        m.setattr(torch.Tensor, "is_cuda", property(lambda t: True))
+        assert ops._HOST.direct()
+        graph = torch.jit.trace(step, args, check_trace=False).inlined_graph
+        recorded = [n.kind() for n in graph.nodes()]
+        seen = []
+
+        class Record(TorchDispatchMode):
+            def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+                seen.append(str(func))
+                return func(*args, **(kwargs or {}))
+        with Record():
+            step(*args)
+    assert not called
+    for name in ("paged_kv_append_", "paged_kv_rows", "gated_attn_paged", "verify_drafts"):
+        assert f"q35::{name}" in recorded and f"q35.{name}.default" in seen, (name, recorded, seen)
