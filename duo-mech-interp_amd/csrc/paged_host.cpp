@@ -341,15 +341,21 @@ PyObject* verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// Any arguments: whether an op on them is the functions above and nothing more. Whatever follows a thread's calls (a trace, a
+// Whether an op on these arguments is the functions above and nothing more. Whatever follows a thread's calls (a trace, a
 // dispatch mode, a transform) has its key among those that the thread includes in every dispatch.
-PyObject* direct(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return guarded(0, 0, [&]() -> PyObject* {
-    constexpr c10::DispatchKeySet always({c10::DispatchKey::BackendSelect, c10::DispatchKey::ADInplaceOrView});
-    const auto local = c10::impl::tls_local_dispatch_key_set();
-    const bool followed = (local.included_.raw_repr() & ~local.excluded_.raw_repr() & ~always.raw_repr()) != 0;
-    return PyBool_FromLong(!followed && std::all_of(a, a + n, plain));
-  });
+bool direct_on(PyObject* const* a, Py_ssize_t n) {
+  constexpr c10::DispatchKeySet always({c10::DispatchKey::BackendSelect, c10::DispatchKey::ADInplaceOrView});
+  const auto local = c10::impl::tls_local_dispatch_key_set();
+  const bool followed = (local.included_.raw_repr() & ~local.excluded_.raw_repr() & ~always.raw_repr()) != 0;
+  return !followed && std::all_of(a, a + n, plain);
+}
+// Any arguments -> that as a bool.
+PyObject* direct(PyObject*, PyObject* const* a, Py_ssize_t n) { return PyBool_FromLong(direct_on(a, n)); }
+// The op where it is so, else NotImplemented.
+template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
+PyObject* try_direct(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  if (direct_on(a, n)) return F(self, a, n);
+  Py_RETURN_NOTIMPLEMENTED;
 }
 
 // error, check, stream, then the addresses of the six functions of the C ABI
@@ -378,9 +384,10 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
-#define Q35_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef g_methods[] = {Q35_METHOD(bind),          Q35_METHOD(direct),           Q35_METHOD(paged_kv_append),
-                           Q35_METHOD(paged_kv_rows), Q35_METHOD(gated_attn_paged), Q35_METHOD(verify_drafts),
+#define Q35_FAST(name, f) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
+#define Q35_METHOD(f) Q35_FAST(#f, f), Q35_FAST("try_" #f, try_direct<f>)
+PyMethodDef g_methods[] = {Q35_FAST("bind", bind),       Q35_FAST("direct", direct),   Q35_METHOD(paged_kv_append),
+                           Q35_METHOD(paged_kv_rows),    Q35_METHOD(gated_attn_paged), Q35_METHOD(verify_drafts),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_paged_host", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

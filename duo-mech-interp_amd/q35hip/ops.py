@@ -1188,14 +1188,13 @@ def argmax_rows(x, out=None):
 
 
 def _call(name, op, *args):
-    """The op on these arguments: as the extension's function `name` where they are plain device tensors and nothing follows
-    the call (the dispatcher takes 3 us of a call's host time, a third of what an append takes), else through torch.ops."""
-    x = args[0]
+    """The op on these arguments: as the extension's function where they are plain device tensors and nothing follows the call
+    (the dispatcher takes 3 us of a call's host time, a third of what an append takes), else through torch.ops."""
     # (is_compiling ahead of all else: a compiler folds the branch there, and could not follow what is asked behind it)
-    if not torch.compiler.is_compiling() and torch.is_tensor(x) and x.is_cuda:
-        host = _paged_host()
-        if host.direct(*args):
-            return getattr(host, name)(*args)
+    if not torch.compiler.is_compiling() and isinstance(args[0], torch.Tensor) and args[0].is_cuda:
+        out = getattr(_HOST or _paged_host(), name)(*args)
+        if out is not NotImplemented:
+            return out
     return op(*args)
 
 
@@ -1230,7 +1229,7 @@ def paged_kv_append_(k, v, pages, table, pos, cos, sin, *, lens=None, k_norm_w=N
     table: [B, blocks] int32, row b's page of each block of page-size tokens; token t of row b goes to position
     pos[b] + t, t < lens[b] ([B] int32; None: all T). Tokens past lens, past the capacity or on a table entry that names
     no page are not written. The table entries that a call writes to must all name different pages."""
-    _call("paged_kv_append", torch.ops.q35.paged_kv_append_, k, v, *_four(pages), table, pos, lens, cos, sin, k_norm_w,
+    _call("try_paged_kv_append", torch.ops.q35.paged_kv_append_, k, v, *_four(pages), table, pos, lens, cos, sin, k_norm_w,
           float(eps))
 
 
@@ -1238,7 +1237,7 @@ def paged_kv_rows(pages, table, pos, T, *, lens=None):
     """Rows pos[b] .. pos[b] + T - 1 of each sequence read back from its pages: (k, v) [B, Hkv, T, 256] bf16, the layout
     of the dense caches (with pos 0 and T a multiple of 64 the caches of gated_attention_prefill_cached); zeros past
     lens, past the table and where a table entry names no page."""
-    return _call("paged_kv_rows", torch.ops.q35.paged_kv_rows, *_four(pages), table, pos, lens, int(T))
+    return _call("try_paged_kv_rows", torch.ops.q35.paged_kv_rows, *_four(pages), table, pos, lens, int(T))
 
 
 def gated_attention_paged(q, gate, pages, table, pos, cos, sin, *, lens=None, q_norm_w=None, eps=1e-6, scale=None,
@@ -1250,7 +1249,7 @@ def gated_attention_paged(q, gate, pages, table, pos, cos, sin, *, lens=None, q_
     prompt; Hq / Hkv any ratio. Returns [B, T, Hq * 256] in out_dtype (bf16 or fp32), zeros for tokens past lens or the
     table's capacity. splits: over how many blocks a row's keys are dealt (0: by the sizes)."""
     _require(out_dtype in (torch.bfloat16, torch.float32), "out_dtype: bf16 or fp32")
-    return _call("gated_attn_paged", torch.ops.q35.gated_attn_paged, q, gate, *_four(pages), table, pos, lens, cos, sin,
+    return _call("try_gated_attn_paged", torch.ops.q35.gated_attn_paged, q, gate, *_four(pages), table, pos, lens, cos, sin,
                  q_norm_w, float(eps), q.shape[-1] ** -0.5 if scale is None else float(scale), int(splits),
                  out_dtype == torch.float32)
 
@@ -1273,7 +1272,7 @@ def verify_drafts(logits, draft_ids, u, *, draft_probs=None, lens=None, temperat
     draft: the lowest index whose running sum exceeds u[:, K] of the whole. The kept drafts and the drawn token are then
     distributed as draws from p. Returns (n_accept [B] int32, tokens [B, K + 1] int32: kept drafts, drawn token, -1)."""
     ts, t = (temperature, 0.0) if torch.is_tensor(temperature) else (None, float(temperature))
-    return _call("verify_drafts", torch.ops.q35.verify_drafts, logits, draft_ids, draft_probs, u, lens, ts, t)
+    return _call("try_verify_drafts", torch.ops.q35.verify_drafts, logits, draft_ids, draft_probs, u, lens, ts, t)
 
 
 def add_rmsnorm_(x, y, w, eps=1e-6, split=False):
