@@ -192,12 +192,12 @@ struct RowsArgs {
   int T, Hkv;
 };
 
-// Block: 32 tokens of (row b, head h), keys (blockIdx.z 0) or values; thread: dims 8 m .. 8 m + 7 (m = tid % 32) of four of
+// Block: 32 tokens of row blockIdx.z, head blockIdx.y / 2, its keys (even blockIdx.y) or values; thread: dims 8 m .. 8 m + 7 (m = tid % 32) of four of
 // them, all loaded before the first is stored.
 template <bool I4>
 __global__ __launch_bounds__(256) void paged_rows_kernel(RowsArgs p) {
-  const int m = threadIdx.x & 31, h = blockIdx.y % p.Hkv, b = blockIdx.y / p.Hkv;
-  const bool val = blockIdx.z;
+  const int m = threadIdx.x & 31, h = blockIdx.y >> 1, b = blockIdx.z;
+  const bool val = blockIdx.y & 1;
   const int len = p.lens ? min(load_uniform(p.lens + b), p.T) : p.T;
   const int64_t pos = load_uniform(p.pos + b);
   const int t0 = (int)blockIdx.x * 32 + (threadIdx.x >> 5);
@@ -239,7 +239,7 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(RowsArgs p) {
       out[u] = __builtin_bit_cast(u32x4, o);
     }
   }
-  __bf16* dst = (val ? p.vo : p.ko) + ((size_t)blockIdx.y * p.T + t0) * kPgD + 8 * m;
+  __bf16* dst = (val ? p.vo : p.ko) + (((size_t)b * p.Hkv + h) * p.T + t0) * kPgD + 8 * m;
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
     const u32x4 zero = {0, 0, 0, 0};
@@ -293,11 +293,10 @@ extern "C" int q35_paged_kv_rows(const void* k_pages, const void* v_pages, const
   if (chk != Q35_OK) return chk;
   if (!k_out || !v_out) return Q35_EINVAL;
   if (((uintptr_t)k_out | (uintptr_t)v_out) & 15) return Q35_EUNSUPPORTED;
-  if (B * Hkv > 65535) return Q35_EUNSUPPORTED;
   const RowsArgs a{k_pages, v_pages, (const __bf16*)k_scale, (const __bf16*)v_scale,
                    {table, ld_table, (int)n_blocks, (int)n_pages, shift}, pos, lens, (__bf16*)k_out, (__bf16*)v_out,
                    (int)T, (int)Hkv};
-  const dim3 grid((unsigned)((T + 31) / 32), (unsigned)(B * Hkv), 2), block(256);
+  const dim3 grid((unsigned)((T + 31) / 32), (unsigned)(2 * Hkv), (unsigned)B), block(256);
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (fmt == Q35_BF16) hipLaunchKernelGGL(paged_rows_kernel<false>, grid, block, 0, st, a);
   else hipLaunchKernelGGL(paged_rows_kernel<true>, grid, block, 0, st, a);
