@@ -11,6 +11,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import warnings
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)                      # duo-mech-interp_amd/
@@ -64,7 +65,8 @@ def _build_host():
 
 
 def build(verbose=False, jobs=None):
-    """Compile every kernel source and link LIB_PATH, and HOST_PATH beside it. Always rebuilds."""
+    """Compile every kernel source and link LIB_PATH, and HOST_PATH beside it. Always rebuilds. The C library needs hipcc
+    alone: where the extension cannot be built (no g++, no Python headers) a warning says why, and the ops that need it raise."""
     if not os.path.exists(HIPCC):
         raise RuntimeError(f"hipcc not found at {HIPCC}")
     os.makedirs(BUILD_DIR, exist_ok=True)
@@ -73,15 +75,19 @@ def build(verbose=False, jobs=None):
     with concurrent.futures.ThreadPoolExecutor(max_workers=jobs) as ex:
         host = ex.submit(_build_host)
         objs = list(ex.map(_compile, srcs))
-        host.result()
     tmp = LIB_PATH + ".tmp"
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp] + objs
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stderr}")
     os.replace(tmp, LIB_PATH)
+    failed = host.exception()
+    if failed is not None:
+        if os.path.exists(HOST_PATH):
+            os.remove(HOST_PATH)  # (an earlier one's calls need not fit this library)
+        warnings.warn(f"q35hip: {HOST_PATH} could not be built, the paged-cache ops will raise: {failed}")
     if verbose:
-        print(f"built {LIB_PATH} from {len(srcs)} sources, and {HOST_PATH}")
+        print(f"built {LIB_PATH} from {len(srcs)} sources" + ("" if failed is not None else f", and {HOST_PATH}"))
     return LIB_PATH
 
 
