@@ -30,21 +30,35 @@ import math
 import torch
 
 from . import ops
+from ._lib import Q35Error
 
 _ROPE_CACHE = {}
 
 
 def rope_tables(n_pos, rot, theta, device):
     """cos / sin [n_pos, rot/2] fp32 of angle pos * theta^(-2j/rot) (HF:105-125 inv_freq in fp32, then the fp32
-    product by position), cached per (n_pos, rot, theta, device)."""
+    product by position), cached per (n_pos, rot, theta, device). New tables are formed on the host and copied, which the
+    call waits for: inside a stream capture that raises, so build them (or call the layer) once ahead of it."""
     key = (int(n_pos), int(rot), float(theta), str(device))
     t = _ROPE_CACHE.get(key)
     if t is None:
+        if torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise Q35Error(f"q35hip: the rotation tables of {n_pos} positions are not built yet, and a stream capture cannot: "
+                           "call layers.rope_tables or the layer once ahead of it")
         inv_freq = 1.0 / (theta ** (torch.arange(0, rot, 2, dtype=torch.int64).to(torch.float) / rot))
         ang = torch.arange(n_pos, dtype=torch.float32)[:, None] * inv_freq[None, :]
         t = (ang.cos().contiguous().to(device), ang.sin().contiguous().to(device))
         _ROPE_CACHE[key] = t
     return t
+
+
+def _rope_tables_over(capacity, rot, theta, device):
+    """Tables of at least `capacity` positions: the shortest that are there, else new ones of a power of two of positions (a
+    table of pages that grows from call to call makes few of them, and one that shrinks none). None is ever dropped: a captured
+    graph may read it."""
+    at = (int(rot), float(theta), str(device))
+    fit = [k[0] for k in list(_ROPE_CACHE) if k[1:] == at and k[0] >= capacity]
+    return rope_tables(min(fit) if fit else 1 << max(capacity - 1, 0).bit_length(), rot, theta, device)
 
 
 def rmsnorm_1p(x, w, eps=1e-6):
@@ -288,15 +302,14 @@ def gated_attention_layer_paged(x, p, pages, table, pos, *, lens=None, rope_thet
     the check of drafted tokens (a few), a chunk of a prompt (many). x: [B, T, H] fp32; token t < lens[b] of row b (lens
     [B] int32 on the device, None: all T) sits at position pos[b] + t ([B] int32 on the device); its key and value go into
     the pages that table ([B, blocks] int32) names, and it attends to positions 0 .. pos[b] + t. Tokens past lens, or past
-    the table, leave the pages alone and give 0 (residual: itself). The call synchronises with nothing, and a HIP graph
-    that holds it follows table, pos and lens. prenorm, residual, fixed_order: see gated_attention_layer."""
+    the table, leave the pages alone and give 0 (residual: itself). A HIP graph that holds the call follows table, pos and
+    lens. The first call stacks the weights, and the first over a table of more positions than any before waits for the
+    rotation tables (rope_tables), so make one of each ahead of a capture; other calls synchronise with nothing. prenorm, residual, fixed_order: see gated_attention_layer."""
     B, T, _ = x.shape
     D = p["q_norm"].numel()
     Hq = p["q_proj"].shape[0] // (2 * D)
     Hkv = p["k_proj"].shape[0] // D
-    # (tables of a power of two of positions: a table of pages that grows from call to call keeps the cache of these small)
-    n_pos = 1 << max(table.shape[1] * pages[0].shape[2] - 1, 0).bit_length()
-    cos, sin = rope_tables(n_pos, int(D * partial_rotary_factor), rope_theta, x.device)
+    cos, sin = _rope_tables_over(table.shape[1] * pages[0].shape[2], int(D * partial_rotary_factor), rope_theta, x.device)
     y = linear(x, attn_in_weight(p), *_q8(p, "_in_fused"), prenorm=prenorm)
     q, k, v = y.split([2 * Hq * D, Hkv * D, Hkv * D], -1)
     q = q.unflatten(-1, (Hq, 2 * D))

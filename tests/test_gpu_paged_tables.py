@@ -4,7 +4,7 @@ import torch
 
 from gpu_util import announce, device
 from oracle import paged
-from q35hip import Q35Error, ops
+from q35hip import Q35Error, layers, ops
 from test_gpu_paged import append, make, oracle_append, same_pages, to
 
 pytestmark = pytest.mark.gpu
@@ -41,3 +41,36 @@ def test_rows_of_65535_sequences(fmt):
         assert torch.equal(x.cpu(), want.transpose(1, 2))
     with pytest.raises(Q35Error):
         ops.paged_kv_rows(g["pages"], table[:1].expand(B + 1, 2).contiguous().to(dev), torch.zeros(B + 1, dtype=torch.int32, device=dev), 1)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int4"])
+def test_a_captured_layer(fmt):
+    """The attention layer in a HIP graph: refused while its rotation tables are not there, and once they are each replay at
+    new positions gives what the eager call gives."""
+    dev = device()
+    g = torch.Generator().manual_seed(7)
+    B, nb = 3, 6
+    p = {n: (torch.randn(*s, generator=g) * 0.05).to(dev)
+         for n, s in (("q_proj", (1024, 256)), ("k_proj", (256, 256)), ("v_proj", (256, 256)), ("o_proj", (256, 512)))}
+    p["q_norm"], p["k_norm"] = (0.1 * torch.randn(256, generator=g).to(dev) for _ in range(2))
+    table = torch.randperm(B * nb, generator=g).view(B, nb).int().to(dev)
+    mine, eager = (ops.kv_pages(B * nb, 1, 32, dev, fmt) for _ in range(2))
+    x, pos = torch.randn(B, 1, 256, generator=g).to(dev), torch.zeros(B, dtype=torch.int32, device=dev)
+    theta = 1e7 + (fmt == "int4")  # (tables of this test's own)
+    announce(f"paged layer captured {fmt}")
+    with pytest.raises(Q35Error, match="capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            layers.gated_attention_layer_paged(x, p, mine, table, pos, rope_theta=theta + 2)
+    layers.gated_attention_layer_paged(x, p, mine, table, pos, rope_theta=theta)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layers.gated_attention_layer_paged(x, p, mine, table, pos, rope_theta=theta)
+    for step in range(5):
+        x.copy_(torch.randn(B, 1, 256, generator=g).to(dev))
+        graph.replay()
+        want = layers.gated_attention_layer_paged(x, p, eager, table, pos, rope_theta=theta)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        for a, b in zip(mine, eager):
+            assert a is None or torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+        pos += torch.tensor([1, 0, 1], dtype=torch.int32, device=dev)
