@@ -49,7 +49,7 @@ inline int paged_check(const void* k_pages, const void* v_pages, const void* k_s
                        const int32_t* pos, int64_t B, int64_t T, int64_t Hkv, int64_t D, int* shift) {
   if (!k_pages || !v_pages || !table || !pos) return Q35_EINVAL;
   if (B <= 0 || T <= 0 || Hkv <= 0 || D <= 0 || n_blocks <= 0 || n_pages <= 0 || page_size <= 0) return Q35_EINVAL;
-  if (B > 1 && ld_table < n_blocks) return Q35_EINVAL;
+  if (B > 1 && ld_table < n_blocks && ld_table != 0) return Q35_EINVAL;  // (0: one table for all rows)
   if (fmt != Q35_BF16 && fmt != Q35_I4_G64) return Q35_EUNSUPPORTED;
   if (fmt == Q35_I4_G64 && (!k_scale || !v_scale)) return Q35_EINVAL;
   if (D != kPgD || page_size < 16 || page_size > 1024 || (page_size & (page_size - 1))) return Q35_EUNSUPPORTED;

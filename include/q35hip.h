@@ -525,8 +525,8 @@ int q35_argmax_rows(const float* x, int64_t ldx, int64_t rows, int64_t n, int32_
 
 /*
  * Paged KV caches. k_pages, v_pages: [n_pages, Hkv, page_size, ...], page_size a power of two of 16 .. 1024, D = 256,
- * 16-byte aligned. table: [B, ld_table] int32 on the device, entry j < n_blocks of row b the page of its tokens
- * j page_size .. (j + 1) page_size - 1; the entries that one call appends to must all name different pages. pos: [B] int32 on
+ * 16-byte aligned. table: [B, ld_table] int32 on the device (ld_table 0: one table that all rows read), entry j < n_blocks of
+ * row b the page of its tokens j page_size .. (j + 1) page_size - 1; the entries that one call appends to must all name different pages. pos: [B] int32 on
  * the device, the position of each row's first token of the call; lens: [B] int32 on the device, how many of the call's T
  * tokens row b has (clamped to 0 .. T), or NULL for T. Token t of row b sits at pos[b] + t. A token that is not there
  * (t >= lens[b], or a position outside 0 .. n_blocks page_size - 1) is not written and attends to nothing. A table entry

@@ -5,7 +5,7 @@ import torch
 from gpu_util import announce, device
 from oracle import paged
 from q35hip import Q35Error, layers, ops
-from test_gpu_paged import append, make, oracle_append, same_pages, to
+from test_gpu_paged import append, attend, check_attention, make, oracle_append, same_pages, to
 
 pytestmark = pytest.mark.gpu
 
@@ -74,3 +74,19 @@ def test_a_captured_layer(fmt):
         for a, b in zip(mine, eager):
             assert a is None or torch.equal(a.view(torch.uint8), b.view(torch.uint8))
         pos += torch.tensor([1, 0, 1], dtype=torch.int32, device=dev)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int4"])
+@pytest.mark.parametrize("T", [1, 5])
+def test_one_table_for_all_rows(fmt, T):
+    """Several rows of queries over one sequence's pages, its table expanded: as with the table repeated."""
+    d = make(fmt, 3, T, 8, 2, 16, [300, 290, 17], seed=9)
+    d["table"] = d["table"][:1].repeat(3, 1)
+    g = to(d, device())
+    announce(f"paged {fmt} T{T}, an expanded table")
+    one = dict(g, table=g["table"][:1].expand(3, -1))
+    out = attend(one)
+    check_attention(d, out)
+    assert torch.equal(out, attend(g))
+    for a, b in zip(*(ops.paged_kv_rows(x["pages"], x["table"], x["pos"], T) for x in (one, g))):
+        assert torch.equal(a, b)
