@@ -104,3 +104,25 @@ def test_a_trace_run_on_other_inputs(fmt):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     for a, b in zip(g["pages"], other):
         assert a is None or torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_a_token_drawn_from_the_stack_s_logits():
+    """K = 0 on what the hybrid stack gives: the oracle's tokens for the same logits, and what the next step takes."""
+    import os
+    import sys
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), "golden"))
+    from oracle import paged
+    from q35hip import model
+    from tiny_weights import tiny_config, tiny_inputs, tiny_weights
+    dev, cfg = device(), tiny_config()
+    ids, _ = tiny_inputs(cfg)
+    m = model.HybridModel(cfg, tiny_weights(cfg), dev, max_len=256, rows=2)
+    announce("tokens drawn from the stack's logits")
+    logits, _ = m.forward(ids)
+    g = torch.Generator().manual_seed(1)
+    for _ in range(4):
+        u = torch.rand(2, 1, generator=g)
+        n, tok = ops.verify_drafts(logits[:, None], logits.new_empty(2, 0, dtype=torch.int32), u.to(dev), temperature=0.7)
+        want = paged.verify_drafts(logits[:, None].cpu(), torch.empty(2, 0, dtype=torch.int32), u, temperature=0.7)
+        assert torch.equal(n.cpu(), want[0]) and torch.equal(tok.cpu(), want[1])
+        logits, _ = m.forward(tok)
