@@ -10,9 +10,13 @@
 //   O^T [dims x rows] += V^T P^T A: V^T formed in registers, B: the exponentials, which S^T's layout hands over as they
 //                                are (lane: row l % 16, keys 4 (l / 16) + r of two 16-key tiles)
 // so that no score or probability crosses lanes except for a row's maximum (two exchanges) and, at the end, its sum.
-// The exponentials are rounded to bf16 (one rounding of 2^-9 per weight, with the value's scale already in it); sums, maxima
-// and accumulators are fp32. Against bf16 keys Q is held as bf16 hi + lo parts (two products, 2^-17 of q); against 4-bit
-// codes as fp16, each row scaled by a power of two to a largest value of 16 to 32 (2^-12 of q).
+// Sums, maxima and accumulators are fp32. What is rounded to fewer bits, because the matrix core takes no fp32 operands and
+// parts of them (hi + lo) double a product: the exponentials to bf16 (at most 2^-8 of each weight, with the value's scale
+// already in it), in both formats and for either output; Q, against bf16 keys as bf16 hi + lo (two products, 2^-16 of q),
+// against 4-bit codes, whose vector work leaves no room for a second one, as fp16, each row scaled by a power of two to a
+// largest value of 16 to 32 (2^-11 of q). In the norm of the output this is 1.1e-3 to 1.7e-3 of 64 bits (fp32 output, 100 to
+// 4000 keys), against 1.6e-3 of the dense decode kernel, which rounds q to bf16, and 2.8e-3 of the dense prefill over the
+// cache; a bf16 output's own rounding is 1.65e-3 and makes it 2.0e-3 to 2.4e-3.
 //
 // 4 bits: a code n enters the products as a small whole number that the operand type holds exactly, its bits or-ed into the
 // mantissa of a power of two: keys 1024 + n and, from the nibble above, 1024 + 16 n in fp16 (Q / 16 against it), 5
@@ -25,10 +29,10 @@
 // takes both, scales and offsets come from LDS in the form in which they are used, and what only masked rounds or scales
 // that are not finite need stays behind branches.
 //
-// Measured (8 query and 2 key heads; a 1 GiB copy runs at 5.2 TB/s, a large bf16 product at 1190 TFLOP/s): one token for 32
-// rows of up to 8192 bf16 keys 93 to 95 us (5.1 TB/s); five tokens a row against 4-bit keys 47 us (2.8 TB/s, 124 TFLOP/s);
-// 512 tokens of one row behind 16 K 4-bit keys 115 us (528 TFLOP/s), bf16 165; one token of three rows of 8192 4-bit keys
-// 14 us.
+// Measured (8 query and 2 key heads; a 1 GiB copy runs at 5.2 TB/s, a large bf16 product at 1380 TFLOP/s): one token for 32
+// rows of up to 8192 bf16 keys 93 to 96 us (5.1 TB/s), 4-bit keys 37 (3.5 TB/s); up to five tokens a row against 4-bit keys 45 to
+// 49 us (2.8 TB/s), bf16 104 (4.7 TB/s); 512 tokens of one row behind 16 K 4-bit keys 115 us (528 TFLOP/s), bf16 165; one token
+// of three rows of 8192 4-bit keys 14 us.
 //
 // A row's keys are dealt over S blocks in runs of whole 128-key rounds by the row's own length, read on the device: the
 // grid is sized by the table's capacity, the work by what is cached. With S > 1 the blocks leave (max, sum, acc) and a

@@ -8,12 +8,13 @@
 //   norm, rotation and quotient are those of 64 bits: which code a value gets then depends on the inputs alone and not on
 //   the order of a sum (in 32 bits about one value in 10^6 falls on the other side). They are formed in fp32 first, and
 //   again in 64 bits only where a rounding lies closer to a tie than fp32 can tell (one row of 256 in a hundred): 6144
-//   tokens of two heads, columns of an fp32 projection, 11.7 us (28 MB, 2.4 TB/s) against 17 in 64 bits throughout. A group
+//   tokens of two heads, columns of an fp32 projection, 11.0 us (29 MB, 2.6 TB/s) against 17 in 64 bits throughout. A group
 //   that holds a value that is not finite gets the scale NaN: it reads back as NaN.
-//   Few tokens are a launch and one chain of loads: three of two heads 2.3 us, 32 rows of up to five 3.4.
+//   Few tokens are a launch and one chain of loads: three of two heads 2.3 us, 32 rows of up to five 3.2; 6144
+//   tokens into bf16 pages 9.6 us (38 MB, 3.9 TB/s).
 //
 // paged_rows_kernel: (code - 8) s, or the bf16 row, per 8 dims a thread. Bounded by memory: 8 rows of up to 8192 4-bit tokens
-// of two heads 26 us (153 MB, most of it the bf16 rows written; a 1 GiB copy runs at 5.2 TB/s).
+// of two heads 26.5 us (153 MB, most of it the bf16 rows written; a 1 GiB copy runs at 5.2 TB/s), bf16 rows 49 (5.0 TB/s).
 #include "paged_kv.h"
 
 namespace q35 {
@@ -92,8 +93,9 @@ struct AppendArgs {
 };
 
 // Wave: one token's row of head blockIdx.y / 2, its keys (even blockIdx.y) or values, of row blockIdx.z. What bounds a long
-// prompt is the issue of about 150 vector and 100 scalar instructions a row: several rows a wave, with their loads ahead,
-// measured an eighth slower (four a wave, 6144 tokens of two heads), and so did 64 bits throughout (17 us).
+// prompt is latency: a wave has one row in flight, and its position, page, angles, reductions and store follow each other (the
+// vector ALU is 37 % busy with about 150 operations a row). Several rows a wave, with their loads ahead, measured an eighth
+// slower all the same (four a wave, 6144 tokens of two heads).
 template <typename Tin, bool I4>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs p) {
   const int lane = threadIdx.x & 63, b = blockIdx.z, h = blockIdx.y >> 1;

@@ -126,3 +126,27 @@ def test_a_token_drawn_from_the_stack_s_logits():
         want = paged.verify_drafts(logits[:, None].cpu(), torch.empty(2, 0, dtype=torch.int32), u, temperature=0.7)
         assert torch.equal(n.cpu(), want[0]) and torch.equal(tok.cpu(), want[1])
         logits, _ = m.forward(tok)
+
+
+@pytest.mark.parametrize("T", [1, 3])
+def test_layer_with_parameters_outside_no_grad(T):
+    """Weights as nn.Parameter with grad mode on: the layer's values, with and without a residual, as under no_grad."""
+    from q35hip import layers
+    dev = device()
+    g = torch.Generator().manual_seed(3)
+    p = {n: torch.nn.Parameter((torch.randn(*s, generator=g) * 0.05).to(dev))
+         for n, s in (("q_proj", (1024, 256)), ("k_proj", (256, 256)), ("v_proj", (256, 256)), ("o_proj", (256, 512)),
+                      ("q_norm", (256,)), ("k_norm", (256,)))}
+    x, res = (torch.randn(2, T, 256, generator=g).to(dev) for _ in range(2))
+    table = torch.tensor([[0, 3], [2, 1]], dtype=torch.int32, device=dev)
+    pos = torch.tensor([0, 20], dtype=torch.int32, device=dev)
+    announce(f"paged layer with parameters, T {T}")
+    out = []
+    for grad in (False, True):
+        pages = ops.kv_pages(4, 1, 16, dev, "int4")
+        with torch.set_grad_enabled(grad):
+            a = layers.gated_attention_layer_paged(x, dict(p), pages, table, pos)
+            b = layers.gated_attention_layer_paged(x, dict(p), pages, table, pos, residual=res.clone(), fixed_order=True)
+        out.append((a.detach(), b.detach(), *pages))
+    for a, b in zip(*out):
+        assert torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
