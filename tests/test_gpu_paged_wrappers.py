@@ -150,3 +150,33 @@ def test_layer_with_parameters_outside_no_grad(T):
         out.append((a.detach(), b.detach(), *pages))
     for a, b in zip(*out):
         assert torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
+
+
+def test_calls_from_two_threads():
+    """Each thread on a stream of its own (the extension gives the interpreter lock up in a call): the results of one."""
+    import threading
+    dev = device()
+    gs = [to(make(fmt, 2, 3, 8, 2, 64, [900, 130], lens=[3, 2], seed=i), dev) for i, fmt in enumerate(("bf16", "int4"))]
+    want = [attend(g) for g in gs]
+    x, ids, us = drafts(3, 2, 20000)
+    drawn = ops.verify_drafts(x, ids, us[0])
+    torch.cuda.synchronize()
+    bad = []
+
+    def run(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(60):
+                    out, n = attend(gs[i]), ops.verify_drafts(x, ids, us[0])
+                    torch.cuda.current_stream().synchronize()
+                    if not (torch.equal(out, want[i]) and all(torch.equal(a, b) for a, b in zip(n, drawn))):
+                        bad.append(i)
+        except Exception as e:  # (to the thread that asserts)
+            bad.append(e)
+    announce("paged calls from two threads")
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not bad and not any(t.is_alive() for t in threads), bad
