@@ -246,7 +246,8 @@ def _attn(s):
 
 
 def _kept(x, cuts):
-    """x [rows, V] -> weights [rows, V] in 64 bits (the most likely token's is 1), and which tokens are kept."""
+    """x [rows, V] -> the tokens from the most likely one down, their weights in 64 bits (the first one's is 1), and which of
+    them are kept (the first ones)."""
     def col(v):
         return v[:, None] if torch.is_tensor(v) else torch.full((x.shape[0], 1), v, device=DEV)
     t, k, p, m = (col(cuts[n]) for n in ("temperature", "top_k", "top_p", "min_p"))
@@ -258,25 +259,24 @@ def _kept(x, cuts):
     w0 = w * keep
     ahead = w0.cumsum(-1) - w0
     keep = keep & ((p >= 1) | (ahead < p.double() * w0.sum(-1, keepdim=True))) & (w >= m.double())
-    keep = torch.where(t > 0, keep | (rank == 0), rank == 0)
-    return torch.zeros_like(w).scatter(1, order, w), torch.zeros_like(keep).scatter(1, order, keep)
+    return order, w, torch.where(t > 0, keep | (rank == 0), rank == 0)
 
 
 def _sample(s):
     c = s["case"]
-    w, keep = _kept(s["x"], s["cuts"])
+    order, w, keep = _kept(s["x"], s["cuts"])
     w = w * keep
     run = w.cumsum(-1)
     over = run > s["u"].double()[:, None] * run[:, -1:]
-    last = c["V"] - 1 - keep.flip(-1).int().argmax(-1)
-    token = torch.where(over.any(-1), over.int().argmax(-1), last).int()
-    return (token, (w / run[:, -1:]).float()) if c["probs"] else token
+    at = torch.where(over.any(-1), over.int().argmax(-1), keep.sum(-1) - 1)
+    token = order.gather(1, at[:, None])[:, 0].int()
+    return (token, torch.zeros_like(w).scatter(1, order, w / run[:, -1:]).float()) if c["probs"] else token
 
 
 def _filter(s):
     x = s["x"]
-    _, keep = _kept(x.flatten(0, 1), s["cuts"])
-    return torch.where(keep.view_as(x), x, torch.full_like(x, -INF))
+    order, _, keep = _kept(x.flatten(0, 1), s["cuts"])
+    return torch.where(torch.zeros_like(keep).scatter(1, order, keep).view_as(x), x, torch.full_like(x, -INF))
 
 
 def _codes(x):
