@@ -56,7 +56,14 @@ struct PagedAttnArgs {
   void* out;
   float *part, *ml;  // S > 1: O [B][Hkv][T G][S][256], (max, sum) [B][Hkv][T G][S][2]
   int T, Hkv, G, S, RB;
+  // sequences whose tables begin with the same n_sh keys: the runs of these (Sp) and of a sequence's own keys (S) leave their
+  // parts in part and ml [B T Hq][Sp + S]
+  int B, n_sh, Sp;
 };
+
+// What a block's keys are: a row's; or, of sequences that share their first keys, these, for the rows of all of them, or a
+// row's own.
+enum PagedKeys : int { kAllKeys = 0, kSharedKeys = 1, kOwnKeys = 2 };
 
 typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
 typedef __attribute__((__vector_size__(8 * sizeof(_Float16)))) _Float16 f16x8;
@@ -207,13 +214,14 @@ __device__ __forceinline__ void out_store(const PagedAttnArgs& p, const f32x4& O
   }
 }
 
-template <bool I4, int NR, int W>
+template <bool I4, int NR, int W, int KEYS_OF = kAllKeys>
 __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(PagedAttnArgs p) {
+  constexpr bool kPre = KEYS_OF == kSharedKeys, kOwn = KEYS_OF == kOwnKeys;
   constexpr int ROWS = 16 * NR, KEYS = 32 * W, QP = I4 ? 1 : 2, QF = 8 * 64;  // parts of Q, 16-byte operands of one
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, a = lane >> 4;
   const int s = blockIdx.x, kvh = blockIdx.y % p.Hkv, rb = blockIdx.y / p.Hkv, b = blockIdx.z;
-  const int R = p.T * p.G, r0 = rb * ROWS;
+  const int R = (kPre ? p.B : 1) * p.T * p.G, r0 = rb * ROWS;
 
   constexpr int kQBytes = NR * QP * QF * 16, kOBytes = W * 16 * kORow * 4;
   __shared__ __attribute__((aligned(16))) char lds[kQBytes > kOBytes ? kQBytes : kOBytes];
@@ -237,7 +245,8 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(PagedAttnArgs p) 
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
     const int r = r0 + 16 * (q0 + i) + qcol, t = r / p.G, h = kvh * p.G + r - t * p.G;
-    const int64_t o = b * p.qb + t * p.qt + h * p.qh;
+    int64_t o = b * p.qb + t * p.qt + h * p.qh;
+    if constexpr (kPre) o = (t / p.T) * p.qb + (t % p.T) * p.qt + h * p.qh;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       qx[i][q] = qp[i][q] = u32x4{0, 0, 0, 0};
@@ -258,8 +267,18 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(PagedAttnArgs p) 
   }
   __builtin_amdgcn_sched_barrier(0);
 
-  const int64_t pos = load_uniform(p.pos + b);
-  const int len = p.lens ? min(max(load_uniform(p.lens + b), 0), p.T) : p.T;
+  const int64_t pos = kPre ? 0 : load_uniform(p.pos + b);
+  const int len = kPre ? 0 : p.lens ? min(max(load_uniform(p.lens + b), 0), p.T) : p.T;
+  // of the rows of all sequences: the position of row r's token, and how many of the shared keys it sees
+  struct Place {
+    int64_t at;
+    int seen;
+  };
+  auto place = [&](int r) -> Place {
+    const int tt = r / p.G, br = tt / p.T, t = tt - br * p.T;
+    const int64_t at = p.pos[br];
+    return {at + t, min(keys_seen(p, at, p.lens ? min(max(p.lens[br], 0), p.T) : p.T, t), p.n_sh)};
+  };
   // the row's keys: those of its last token that is there (a later one sees more)
   int n_row = 0;
   if (len > 0) n_row = (int)min(max(pos + len, (int64_t)0), p.pt.capacity());
@@ -267,12 +286,16 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(PagedAttnArgs p) 
   // what this block's rows see at most and at least
   int n_max = 0;
   if (t0 < len) n_max = (int)min(max(pos + min(t1, len - 1) + 1, (int64_t)0), p.pt.capacity());
-  const int run = run_keys(n_row, p.S);
-  const int k0 = s * run, k1 = min(k0 + run, n_max);
+  if constexpr (kPre) n_max = p.n_sh;
+  const int kb = kOwn ? p.n_sh : 0;
+  const int run = kPre ? __builtin_amdgcn_readfirstlane(run_keys(p.n_sh, p.Sp)) : run_keys(kOwn ? max(n_row - kb, 0) : n_row, p.S);
+  const int k0 = kb + s * run, k1 = min(k0 + run, n_max);
   const bool work = k0 < k1;
-  if (!work && p.S > 1) return;  // the merge does not read empty runs' slots
+  if (!work && (KEYS_OF != kAllKeys || p.S > 1)) return;  // the merge does not read empty runs' slots
 
-  const int n_min = keys_seen(p, pos, len, t0), n_last = n_max - 1, pmask = (1 << p.pt.shift) - 1;
+  int n_min = keys_seen(p, pos, len, t0);
+  if constexpr (kPre) n_min = p.n_sh;  // (less where a row is inside the shared part: below)
+  const int n_last = n_max - 1, pmask = (1 << p.pt.shift) - 1;
   // 16 keys from key0 on: the page (that of the last key for a tile past it, whose keys are masked) and the row in it.
   // Bases are scalar, a lane's part of the address 32 bits.
   struct Tile {
@@ -359,14 +382,21 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(PagedAttnArgs p) 
   f32x4 co[kAngles][4], si[kAngles][4];
   auto angles = [&](int i, f32x4 (&co)[4], f32x4 (&si)[4]) {
     const int tk = (r0 + 16 * (q0 + i) + qcol) / p.G;
-    const bool there = r0 + 16 * (q0 + i) + qcol < R && q0 + i < NR && keys_seen(p, pos, len, tk) > 0;
+    bool there = r0 + 16 * (q0 + i) + qcol < R && q0 + i < NR && keys_seen(p, pos, len, tk) > 0;
+    int64_t at = pos + tk;
+    if constexpr (kPre) {
+      const int r = r0 + 16 * (q0 + i) + qcol;
+      const Place pl = place(min(r, R - 1));
+      there = r < R && q0 + i < NR && pl.seen > 0;
+      at = pl.at;
+    }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int d = 64 * q + 4 * qj, pj = d < half ? d : d - half;
       co[q] = si[q] = zero4();
       if (there && d < p.rot) {
-        co[q] = load_quad<float>(p.cos_t + (pos + tk) * half + pj);
-        si[q] = load_quad<float>(p.sin_t + (pos + tk) * half + pj);
+        co[q] = load_quad<float>(p.cos_t + at * half + pj);
+        si[q] = load_quad<float>(p.sin_t + at * half + pj);
       }
     }
   };
@@ -411,7 +441,8 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(PagedAttnArgs p) 
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
       const int tk = (r0 + 16 * (q0 + i) + qcol) / p.G, ia = i < kAngles ? i : 0;
-      const bool there = r0 + 16 * (q0 + i) + qcol < R && keys_seen(p, pos, len, tk) > 0;
+      bool there = r0 + 16 * (q0 + i) + qcol < R && keys_seen(p, pos, len, tk) > 0;
+      if constexpr (kPre) there = r0 + 16 * (q0 + i) + qcol < R && place(min(r0 + 16 * (q0 + i) + qcol, R - 1)).seen > 0;
       if (i >= kAngles) angles(i, co[0], si[0]);
       f32x4 x[4], px[4];
 #pragma unroll
@@ -449,6 +480,13 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(PagedAttnArgs p) 
     // rows that are not there are not stored: let them see what the others do, so that they ask for no mask
     const int r = r0 + 16 * i + c;
     seen[i] = r < R ? keys_seen(p, pos, len, r / p.G) : n_max;
+    if constexpr (kPre) seen[i] = r < R ? place(min(r, R - 1)).seen : n_max;
+  }
+  if constexpr (kPre) {
+    bool less = false;
+#pragma unroll
+    for (int i = 0; i < NR; ++i) less |= seen[i] < n_max;
+    if (__builtin_amdgcn_ballot_w64(less) != 0) n_min = 0;
   }
   f32x4 acc[NR][16];
   f32x4 corr[NR];  // 4 bits: -24 times the sum of the weights, of groups 0 .. 3
@@ -815,8 +853,10 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(PagedAttnArgs p) 
           for (int e = 0; e < 4; ++e) O[e] += v[e] * f;
         }
       }
-      if (p.S > 1) {
-        const size_t slot = (((size_t)b * p.Hkv + kvh) * R + r) * p.S + s;
+      if (KEYS_OF != kAllKeys || p.S > 1) {
+        size_t slot = (((size_t)b * p.Hkv + kvh) * R + r) * p.S + s;
+        if constexpr (KEYS_OF != kAllKeys)
+          slot = (((size_t)(kPre ? 0 : b) * p.T + t) * p.Hkv * p.G + h) * (p.Sp + p.S) + (kPre ? s : p.Sp + s);
         *reinterpret_cast<f32x4*>(p.part + slot * kPgD + de) = O;
         if (le < 2) p.ml[2 * slot + le] = le ? L : M;
       } else {
@@ -915,6 +955,61 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs p) 
   out_store(p, O, L, true, g, b, t, h, d0);
 }
 
+// A query row's runs over the shared and over its own keys joined, one wave a row.
+__global__ __launch_bounds__(256) void paged_attn_shared_merge_kernel(PagedAttnArgs p) {
+  constexpr int U = 8;
+  const int lane = threadIdx.x & 63, d0 = 4 * lane;
+  const int64_t row = 4 * (int64_t)blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int Hq = p.Hkv * p.G;
+  if (row >= (int64_t)p.B * p.T * Hq) return;
+  const int h = (int)(row % Hq), tt = (int)(row / Hq), b = tt / p.T, t = tt - b * p.T;
+  const int64_t pos = load_uniform(p.pos + b);
+  const int len = p.lens ? min(max(load_uniform(p.lens + b), 0), p.T) : p.T;
+  const int seen = keys_seen(p, pos, len, t);
+  int n_row = 0;
+  if (len > 0) n_row = (int)min(max(pos + len, (int64_t)0), p.pt.capacity());
+  const int run0 = run_keys(p.n_sh, p.Sp), run1 = run_keys(max(n_row - p.n_sh, 0), p.S);
+  // runs that hold keys this row sees
+  const int n0 = (min(seen, p.n_sh) + run0 - 1) / run0, n1 = seen > p.n_sh ? (seen - p.n_sh + run1 - 1) / run1 : 0;
+  const int n = n0 + n1;
+  const size_t base = (size_t)row * (p.Sp + p.S);
+  float M = -INFINITY, L = 0.f;
+  f32x4 O = zero4();
+  const f32x4 g = gate_load(p, b, t, h, d0);
+  for (int s0 = 0; s0 < n; s0 += U) {
+    f32x4 pv[U];
+    float m[U], l[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = min(s0 + u, n - 1);
+      const size_t s = base + (i < n0 ? i : p.Sp + i - n0);
+      pv[u] = *reinterpret_cast<const f32x4*>(p.part + s * kPgD + d0);
+      m[u] = p.ml[2 * s];
+      l[u] = p.ml[2 * s + 1];
+    }
+    float mn = M;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      m[u] = s0 + u < n ? m[u] : -INFINITY;
+      mn = fmaxf(mn, m[u]);
+    }
+    const float c0 = M > -INFINITY ? __builtin_amdgcn_exp2f(M - mn) : 0.f;
+    L *= c0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) O[e] *= c0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = m[u] > -INFINITY;
+      const float c1 = in ? __builtin_amdgcn_exp2f(m[u] - mn) : 0.f;
+      L += in ? l[u] * c1 : 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) O[e] += in ? pv[u][e] * c1 : 0.f;
+    }
+    M = mn;
+  }
+  out_store(p, O, L, true, g, b, t, h, d0);
+}
+
 // Query rows per block, in 16s: two, which halves the unpacking and the LDS reads per row, but one where all rows fit in it
 // (32 rows of up to 8192 keys, one token of four heads: bf16 95.9 us against 102.6, 4 bits 37.7 against 43.3) and for three
 // 16s against codes, a quarter of whose work would be for rows that are not there (nine tokens of four heads: 64.6 against
@@ -951,6 +1046,56 @@ static PagedPlan paged_plan(int64_t B, int64_t T, int64_t Hkv, int64_t G, int64_
   return {NR, (int)RB, (int)S, S == 1 && eight ? 8 : 4};
 }
 
+// The checks and arguments that both entry points share.
+static int paged_attn_args(PagedAttnArgs& a, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* gate,
+                           int64_t g_sb, int64_t g_st, int64_t g_sh, int dtype, const float* q_norm_w, float eps,
+                           const float* cos, const float* sin, int64_t rot, const void* k_pages, const void* v_pages,
+                           const void* k_scale, const void* v_scale, int fmt, int64_t n_pages, int64_t page_size,
+                           const int32_t* table, int64_t ld_table, int64_t n_blocks, const int32_t* pos, const int32_t* lens,
+                           void* out, int out_dtype, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, float scale) {
+  int shift = 0;
+  int chk = paged_check(k_pages, v_pages, k_scale, v_scale, fmt, table, ld_table, n_blocks, n_pages, page_size, pos, B,
+                        T, Hkv, D, &shift);
+  if (chk == Q35_OK) chk = view_check(q, dtype, q_sb, q_st, q_sh);
+  if (chk == Q35_OK && gate) chk = view_check(gate, dtype, g_sb, g_st, g_sh);
+  if (chk != Q35_OK) return chk;
+  if (!out || Hq <= 0 || Hq % Hkv || rot < 0 || rot > D || (rot & 1) || (rot > 0 && (!cos || !sin))) return Q35_EINVAL;
+  if (out_dtype != Q35_BF16 && out_dtype != Q35_F32) return Q35_EUNSUPPORTED;
+  if (rot % 8 || (uintptr_t)q_norm_w & 15 || (rot > 0 && ((uintptr_t)cos | (uintptr_t)sin) & 15) ||
+      (uintptr_t)out & 15)
+    return Q35_EUNSUPPORTED;
+  if (Hq > 4096 || T * (Hq / Hkv) > (1 << 24)) return Q35_EUNSUPPORTED;
+  a.q = q;
+  a.gate = gate;
+  a.qb = q_sb, a.qt = q_st, a.qh = q_sh, a.gb = g_sb, a.gt = g_st, a.gh = g_sh;
+  a.qw = q_norm_w, a.cos_t = cos, a.sin_t = sin;
+  a.eps = eps, a.scale = scale;
+  a.rot = (int)rot, a.q_f32 = dtype == Q35_F32, a.out_f32 = out_dtype == Q35_F32;
+  a.pt = {table, ld_table, (int)n_blocks, (int)n_pages, shift};
+  a.pos = pos, a.lens = lens;
+  a.kp = k_pages, a.vp = v_pages, a.ks = (const __bf16*)k_scale, a.vs = (const __bf16*)v_scale;
+  a.out = out;
+  a.T = (int)T, a.Hkv = (int)Hkv, a.G = (int)(Hq / Hkv);
+  return Q35_OK;
+}
+
+// Of sequences that share their first n_sh keys: tiles and runs of these for the rows of all, and of each one's own keys.
+struct SharedPlan {
+  int NP, RBP, SP;  // 16s of rows, tiles and runs over the shared keys
+  PagedPlan own;
+};
+static int shared_runs(int64_t base, int64_t keys) {
+  const int64_t most = (keys + kRound - 1) / kRound;
+  int64_t S = (512 + base - 1) / base;
+  if (most <= 2 * S) S = (256 + base - 1) / base;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({S, most, 1024}));
+}
+static SharedPlan shared_plan(int64_t B, int64_t T, int64_t Hkv, int64_t G, int64_t n_sh, int64_t n_own) {
+  const int64_t R = B * T * G, NP = R <= 16 ? 1 : 2, RBP = (R + 16 * NP - 1) / (16 * NP);
+  const int64_t own = T * G, NR = own <= 16 ? 1 : 2, RB = (own + 16 * NR - 1) / (16 * NR);
+  return {(int)NP, (int)RBP, shared_runs(Hkv * RBP, n_sh), {(int)NR, (int)RB, shared_runs(B * Hkv * RB, n_own), 4}};
+}
+
 }  // namespace q35
 
 extern "C" size_t q35_gated_attn_paged_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
@@ -976,38 +1121,20 @@ extern "C" int q35_gated_attn_paged(const void* q, int64_t q_sb, int64_t q_st, i
                                     float scale, int64_t splits, void* workspace, size_t workspace_bytes,
                                     q35_stream_t stream) {
   using namespace q35;
-  int shift = 0;
-  int chk = paged_check(k_pages, v_pages, k_scale, v_scale, fmt, table, ld_table, n_blocks, n_pages, page_size, pos, B,
-                        T, Hkv, D, &shift);
-  if (chk == Q35_OK) chk = view_check(q, dtype, q_sb, q_st, q_sh);
-  if (chk == Q35_OK && gate) chk = view_check(gate, dtype, g_sb, g_st, g_sh);
+  PagedAttnArgs a{};
+  const int chk = paged_attn_args(a, q, q_sb, q_st, q_sh, gate, g_sb, g_st, g_sh, dtype, q_norm_w, eps, cos, sin, rot, k_pages,
+                                  v_pages, k_scale, v_scale, fmt, n_pages, page_size, table, ld_table, n_blocks, pos, lens, out,
+                                  out_dtype, B, T, Hq, Hkv, D, scale);
   if (chk != Q35_OK) return chk;
-  if (!out || Hq <= 0 || Hq % Hkv || rot < 0 || rot > D || (rot & 1) || (rot > 0 && (!cos || !sin))) return Q35_EINVAL;
-  if (out_dtype != Q35_BF16 && out_dtype != Q35_F32) return Q35_EUNSUPPORTED;
-  if (rot % 8 || (uintptr_t)q_norm_w & 15 || (rot > 0 && ((uintptr_t)cos | (uintptr_t)sin) & 15) ||
-      (uintptr_t)out & 15)
-    return Q35_EUNSUPPORTED;
   const int64_t G = Hq / Hkv;
-  if (Hq > 4096 || T * G > (1 << 24)) return Q35_EUNSUPPORTED;
   const PagedPlan pl = paged_plan(B, T, Hkv, G, n_blocks * page_size, splits, fmt);
   if (Hkv * pl.RB > 65535 || T * Hq > 0x7fffffff) return Q35_EUNSUPPORTED;
   const size_t rows = (size_t)B * T * Hq * pl.S;
   if (pl.S > 1 && (!workspace || workspace_bytes < rows * (kPgD + 2) * sizeof(float) || (uintptr_t)workspace & 15))
     return Q35_EWORKSPACE;
-  PagedAttnArgs a{};
-  a.q = q;
-  a.gate = gate;
-  a.qb = q_sb, a.qt = q_st, a.qh = q_sh, a.gb = g_sb, a.gt = g_st, a.gh = g_sh;
-  a.qw = q_norm_w, a.cos_t = cos, a.sin_t = sin;
-  a.eps = eps, a.scale = scale;
-  a.rot = (int)rot, a.q_f32 = dtype == Q35_F32, a.out_f32 = out_dtype == Q35_F32;
-  a.pt = {table, ld_table, (int)n_blocks, (int)n_pages, shift};
-  a.pos = pos, a.lens = lens;
-  a.kp = k_pages, a.vp = v_pages, a.ks = (const __bf16*)k_scale, a.vs = (const __bf16*)v_scale;
-  a.out = out;
   a.part = (float*)workspace;
   a.ml = a.part ? a.part + rows * kPgD : nullptr;
-  a.T = (int)T, a.Hkv = (int)Hkv, a.G = (int)G, a.S = pl.S, a.RB = pl.RB;
+  a.S = pl.S, a.RB = pl.RB;
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid(pl.S, (unsigned)(Hkv * pl.RB), (unsigned)B), block(256);
 #define Q35_PAGED(I4, NR)                                                                            \
@@ -1025,5 +1152,59 @@ extern "C" int q35_gated_attn_paged(const void* q, int64_t q_sb, int64_t q_st, i
   if (pl.S > 8) hipLaunchKernelGGL((paged_attn_merge_kernel<4, 8>), dim3(n, (unsigned)B), block, 0, st, a);
   else if (pl.S > 4) hipLaunchKernelGGL((paged_attn_merge_kernel<1, 8>), dim3((n + 3) / 4, (unsigned)B), block, 0, st, a);
   else if (pl.S > 1) hipLaunchKernelGGL((paged_attn_merge_kernel<1, 4>), dim3((n + 3) / 4, (unsigned)B), block, 0, st, a);
+  return hipGetLastError() == hipSuccess ? Q35_OK : Q35_ELAUNCH;
+}
+
+extern "C" size_t q35_gated_attn_paged_shared_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                                                              int64_t n_blocks, int64_t page_size, int64_t shared_blocks) {
+  using namespace q35;
+  if (shared_blocks < 0 || shared_blocks > n_blocks) return 0;
+  const size_t all = q35_gated_attn_paged_workspace_bytes(B, T, Hq, Hkv, D, n_blocks, page_size, 0);
+  if (all == 0 || shared_blocks == 0) return all;
+  const SharedPlan pl = shared_plan(B, T, Hkv, Hq / Hkv, shared_blocks * page_size, (n_blocks - shared_blocks) * page_size);
+  return (size_t)B * T * Hq * (pl.SP + pl.own.S) * (kPgD + 2) * sizeof(float);
+}
+
+extern "C" int q35_gated_attn_paged_shared(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* gate, int64_t g_sb,
+                                           int64_t g_st, int64_t g_sh, int dtype, const float* q_norm_w, float eps,
+                                           const float* cos, const float* sin, int64_t rot, const void* k_pages,
+                                           const void* v_pages, const void* k_scale, const void* v_scale, int fmt,
+                                           int64_t n_pages, int64_t page_size, const int32_t* table, int64_t ld_table,
+                                           int64_t n_blocks, int64_t shared_blocks, const int32_t* pos, const int32_t* lens,
+                                           void* out, int out_dtype, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                                           float scale, void* workspace, size_t workspace_bytes, q35_stream_t stream) {
+  using namespace q35;
+  if (shared_blocks < 0 || shared_blocks > n_blocks) return Q35_EINVAL;
+  if (shared_blocks == 0)
+    return q35_gated_attn_paged(q, q_sb, q_st, q_sh, gate, g_sb, g_st, g_sh, dtype, q_norm_w, eps, cos, sin, rot, k_pages,
+                                v_pages, k_scale, v_scale, fmt, n_pages, page_size, table, ld_table, n_blocks, pos, lens, out,
+                                out_dtype, B, T, Hq, Hkv, D, scale, 0, workspace, workspace_bytes, stream);
+  PagedAttnArgs a{};
+  const int chk = paged_attn_args(a, q, q_sb, q_st, q_sh, gate, g_sb, g_st, g_sh, dtype, q_norm_w, eps, cos, sin, rot, k_pages,
+                                  v_pages, k_scale, v_scale, fmt, n_pages, page_size, table, ld_table, n_blocks, pos, lens, out,
+                                  out_dtype, B, T, Hq, Hkv, D, scale);
+  if (chk != Q35_OK) return chk;
+  const SharedPlan pl = shared_plan(B, T, Hkv, Hq / Hkv, shared_blocks * page_size, (n_blocks - shared_blocks) * page_size);
+  const int64_t rows = B * T * Hq;
+  if (B * T * (Hq / Hkv) > (1 << 24) || Hkv * pl.RBP > 65535 || Hkv * pl.own.RB > 65535 || rows > 0x7fffffff)
+    return Q35_EUNSUPPORTED;
+  const size_t slots = (size_t)rows * (pl.SP + pl.own.S);
+  if (!workspace || workspace_bytes < slots * (kPgD + 2) * sizeof(float) || (uintptr_t)workspace & 15) return Q35_EWORKSPACE;
+  a.part = (float*)workspace;
+  a.ml = a.part + slots * kPgD;
+  a.S = pl.own.S, a.RB = pl.own.RB;
+  a.B = (int)B, a.n_sh = (int)(shared_blocks * page_size), a.Sp = pl.SP;
+  const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const bool i4 = fmt == Q35_I4_G64;
+#define Q35_SHARED(I4, NR, KEYS, GRID) hipLaunchKernelGGL((paged_attn_kernel<I4, NR, 4, KEYS>), GRID, dim3(256), 0, st, a)
+  const dim3 gp(pl.SP, (unsigned)(Hkv * pl.RBP)), go(pl.own.S, (unsigned)(Hkv * pl.own.RB), (unsigned)B);
+  if (pl.NP == 1) { if (i4) Q35_SHARED(true, 1, kSharedKeys, gp); else Q35_SHARED(false, 1, kSharedKeys, gp); }
+  else { if (i4) Q35_SHARED(true, 2, kSharedKeys, gp); else Q35_SHARED(false, 2, kSharedKeys, gp); }
+  if (n_blocks > shared_blocks) {
+    if (pl.own.NR == 1) { if (i4) Q35_SHARED(true, 1, kOwnKeys, go); else Q35_SHARED(false, 1, kOwnKeys, go); }
+    else { if (i4) Q35_SHARED(true, 2, kOwnKeys, go); else Q35_SHARED(false, 2, kOwnKeys, go); }
+  }
+#undef Q35_SHARED
+  hipLaunchKernelGGL(paged_attn_shared_merge_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
   return hipGetLastError() == hipSuccess ? Q35_OK : Q35_ELAUNCH;
 }

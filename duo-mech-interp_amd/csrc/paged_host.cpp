@@ -37,6 +37,13 @@ decltype(&q35_gated_attn_paged_workspace_bytes) g_attn_bytes = nullptr;
 decltype(&q35_gated_attn_paged) g_attn = nullptr;
 decltype(&q35_verify_drafts_workspace_bytes) g_verify_bytes = nullptr;
 decltype(&q35_verify_drafts) g_verify = nullptr;
+decltype(&q35_gated_attn_paged_shared_workspace_bytes) g_shared_bytes = nullptr;
+decltype(&q35_gated_attn_paged_shared) g_shared = nullptr;
+decltype(&q35_sample_tokens_workspace_bytes) g_sample_bytes = nullptr;
+decltype(&q35_sample_tokens) g_sample = nullptr;
+decltype(&q35_quantize_rows_i8) g_quantize = nullptr;
+decltype(&q35_add_rmsnorm_i8) g_norm_i8 = nullptr;
+decltype(&q35_gemm_i8) g_gemm_i8 = nullptr;
 
 // A Python error is set already.
 struct PyFailed {};
@@ -341,6 +348,228 @@ PyObject* verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// As gated_attn_paged up to scale, then f32_out, shared_blocks -> out
+PyObject* gated_attn_paged_shared(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 16, [&]() -> PyObject* {
+    const Tensor& q = tensor(a[0]);
+    const Tensor* gate = optional(a[1]);
+    const View qv = heads_view(q, "q");
+    const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), d = q.get_device();
+    const Pages p = pages_of(a + 2, d, B);
+    View gv{0, 0, 0, qv.dtype};
+    if (gate) {
+      gv = heads_view(*gate, "gate");
+      if (gate->sizes() != q.sizes() || gv.dtype != qv.dtype || gate->get_device() != d) refuse("gate: like q");
+    }
+    const Rope r = rope_of(a + 9, d, p.blocks * p.size);
+    const double eps = number(a[12]), scale = number(a[13]);
+    const int f32 = PyObject_IsTrue(a[14]);
+    if (f32 < 0) throw PyFailed{};
+    const int64_t shared = integer(a[15]);
+    if (shared < 0 || shared > p.blocks) refuse("shared_blocks: 0 up to the table's blocks");
+    const Tensor out = make({B, T, Hq * 256}, f32 ? at::kFloat : at::kBFloat16, q);
+    if (out.numel()) {
+      const size_t bytes = g_shared_bytes(B, T, Hq, p.heads, 256, p.blocks, p.size, shared);
+      if (!bytes) refuse("unsupported attention shape");
+      const Tensor ws = make({(int64_t)bytes}, at::kByte, q);
+      launch(q, "q35_gated_attn_paged_shared", [&, at = PagesAt(p), ro = RopeAt(r), xq = data(q), xg = data(gate), o = data(out),
+                                                w = data(ws)](q35_stream_t st) {
+        return g_shared(xq, qv.b, qv.t, qv.h, xg, gv.b, gv.t, gv.h, qv.dtype, ro.norm_w, (float)eps, ro.cos, ro.sin, r.rot,
+                        at.k, at.v, at.ks, at.vs, p.fmt, p.n, p.size, at.table, p.ld, p.blocks, shared, at.pos, at.lens, o,
+                        f32 ? Q35_F32 : Q35_BF16, B, T, Hq, p.heads, 256, (float)scale, w, bytes, st);
+      });
+    }
+    return THPVariable_Wrap(out);
+  });
+}
+
+// temperatures, temperature, top_ks, top_k, top_ps, top_p, min_ps, min_p: a row's settings
+struct Cuts {
+  const Tensor *t, *k, *p, *m;
+  double temperature, top_p, min_p;
+  int64_t top_k;
+};
+Cuts cuts_of(PyObject* const* a, int64_t d, int64_t B) {
+  const Cuts c{optional(a[0]), optional(a[2]), optional(a[4]), optional(a[6]),
+               number(a[1]),   number(a[5]),   number(a[7]),   integer(a[3])};
+  if (!dense_on(d, {c.t, c.k, c.p, c.m})) refuse("per-row settings must be contiguous and on the logits' device");
+  for (const Tensor* s : {c.t, c.p, c.m})
+    if (s && (!is(*s, at::kFloat) || s->dim() != 1 || s->size(0) != B))
+      refuse("temperature, top_p, min_p: numbers or [B] fp32");
+  if (!ints_per_row(c.k, B)) refuse("top_k: a number or [B] int32");
+  if (!(c.temperature >= 0) || c.top_p != c.top_p || c.min_p != c.min_p)
+    refuse("temperature: at least 0; top_p, min_p: numbers");
+  return c;
+}
+// Logits [B, V] or [B, P, V] with dense rows.
+struct Logits {
+  int64_t B, P, V, sb, sp;
+};
+Logits logits_of(const Tensor& x, bool positions) {
+  if (!x.is_cuda()) refuse(kNotOnGpu);
+  const bool three = x.dim() == 3;
+  if (!(x.dim() == 2 || (positions && three)) || !is(x, at::kFloat) || x.stride(-1) != 1 || x.size(-1) == 0)
+    refuse(positions ? "logits: [B, V] or [B, P, V] fp32 with dense rows" : "logits: [B, V] fp32 with dense rows");
+  return {x.size(0), three ? x.size(1) : 1, x.size(-1), x.stride(0), three ? x.stride(1) : x.size(-1)};
+}
+void sample(const Tensor& x, const Logits& l, const Tensor* u, const Cuts& c, const Tensor* tokens, int kind, const Tensor* out) {
+  const size_t bytes = g_sample_bytes(l.B, l.P, l.V);
+  if (!bytes) refuse("unsupported number of rows or tokens");
+  const Tensor ws = make({(int64_t)bytes}, at::kByte, x);
+  const int64_t us = u ? u->stride(0) : 0;
+  launch(x, "q35_sample_tokens", [&, xa = data<float>(x), ua = data<float>(u), ta = data<float>(c.t), ka = data<int32_t>(c.k),
+                                  pa = data<float>(c.p), ma = data<float>(c.m), to = data<int32_t>(tokens), o = data<float>(out),
+                                  w = data(ws)](q35_stream_t st) {
+    return g_sample(xa, l.sb, l.sp, ua, us, ta, (float)c.temperature, ka, c.top_k, pa, (float)c.top_p, ma, (float)c.min_p, to,
+                    kind, o, l.B, l.P, l.V, w, bytes, st);
+  });
+}
+
+// logits, u, temperatures, temperature, top_ks, top_k, top_ps, top_p, min_ps, min_p, want_probs -> (tokens, probs or empty)
+PyObject* sample_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 11, [&]() -> PyObject* {
+    const Tensor &x = tensor(a[0]), &u = tensor(a[1]);
+    const Logits l = logits_of(x, false);
+    const int64_t d = x.get_device();
+    if (!u.is_cuda()) refuse(kNotOnGpu);
+    if (u.get_device() != d || !is(u, at::kFloat) || u.dim() != 1 || u.size(0) != l.B)
+      refuse("u: [B] fp32 on the logits' device");
+    const Cuts c = cuts_of(a + 2, d, l.B);
+    const int want = PyObject_IsTrue(a[10]);
+    if (want < 0) throw PyFailed{};
+    const Tensor tokens = make({l.B}, at::kInt, x), probs = want ? make({l.B, l.V}, at::kFloat, x) : make({0}, at::kFloat, x);
+    if (l.B) sample(x, l, &u, c, &tokens, want, want ? &probs : nullptr);
+    return Py_BuildValue("(NN)", THPVariable_Wrap(tokens), THPVariable_Wrap(probs));
+  });
+}
+
+// logits, temperatures, temperature, top_ks, top_k, top_ps, top_p, min_ps, min_p -> logits
+PyObject* filter_logits(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 9, [&]() -> PyObject* {
+    const Tensor& x = tensor(a[0]);
+    const Logits l = logits_of(x, true);
+    const Cuts c = cuts_of(a + 1, x.get_device(), l.B);
+    const Tensor out = make(x.sizes(), at::kFloat, x);
+    if (l.B && l.P) sample(x, l, nullptr, c, nullptr, 2, &out);
+    return THPVariable_Wrap(out);
+  });
+}
+
+// Rows [..., K] whose last dim is dense and that are evenly strided: how many, and how far apart.
+struct Rows {
+  int64_t M, K, ld;
+};
+Rows rows_of(const Tensor& x, const char* what) {
+  if (x.dim() < 1 || x.size(-1) == 0 || x.stride(-1) != 1) refuse(std::string(what) + ": [..., K] with dense rows");
+  const int64_t K = x.size(-1), M = x.numel() / K;
+  int64_t ld = K;
+  if (x.dim() > 1 && M > 1) {
+    int64_t at = x.dim() - 2;
+    while (at > 0 && x.size(at) == 1) --at;
+    ld = x.stride(at);
+    int64_t want = ld * x.size(at);
+    for (int64_t i = at - 1; i >= 0; --i) {
+      if (x.size(i) != 1 && x.stride(i) != want) refuse(std::string(what) + ": rows must be evenly strided");
+      want *= x.size(i);
+    }
+    if (ld < K) refuse(std::string(what) + ": rows must not overlap");
+  }
+  return {M, K, ld};
+}
+Tensor scales_for(const Tensor& x) {
+  return make(x.sizes().slice(0, x.dim() - 1), at::kFloat, x);
+}
+
+// x -> (q, s)
+PyObject* quantize_rows_i8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 1, [&]() -> PyObject* {
+    const Tensor& x = tensor(a[0]);
+    if (!x.is_cuda()) refuse(kNotOnGpu);
+    if (!(is(x, at::kFloat) || is(x, at::kBFloat16))) refuse("x: fp32 or bf16");
+    const Rows r = rows_of(x, "x");
+    const Tensor q = make(x.sizes(), at::kChar, x), s = scales_for(x);
+    if (r.M)
+      launch(x, "q35_quantize_rows_i8", [&, xa = data(x), qa = data<int8_t>(q), sa = data<float>(s)](q35_stream_t st) {
+        return g_quantize(xa, r.ld, is(x, at::kFloat) ? Q35_F32 : Q35_BF16, qa, sa, r.M, r.K, st);
+      });
+    return Py_BuildValue("(NN)", THPVariable_Wrap(q), THPVariable_Wrap(s));
+  });
+}
+
+// x, y, w, eps -> (q, s); x += y in place
+PyObject* add_rmsnorm_i8_(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 4, [&]() -> PyObject* {
+    const Tensor &x = tensor(a[0]), &w = tensor(a[2]);
+    const Tensor* y = optional(a[1]);
+    const double eps = number(a[3]);
+    if (!x.is_cuda() || !w.is_cuda() || (y && !y->is_cuda())) refuse(kNotOnGpu);
+    const int64_t d = x.get_device();
+    if (!is(x, at::kFloat) || (y && (!is(*y, at::kFloat) || y->sizes() != x.sizes() || y->get_device() != d)))
+      refuse("x: fp32; y like x");
+    const Rows r = rows_of(x, "x"), ry = y ? rows_of(*y, "y") : Rows{0, 0, 0};
+    if (!dense_on(d, {&w}) || !is(w, at::kFloat) || w.numel() != r.K) refuse("w: [K] fp32 on x's device");
+    const Tensor q = make(x.sizes(), at::kChar, x), s = scales_for(x);
+    if (r.M)
+      launch(x, "q35_add_rmsnorm_i8", [&, xa = data<float>(x), ya = data<float>(y), wa = data<float>(w), qa = data<int8_t>(q),
+                                       sa = data<float>(s)](q35_stream_t st) {
+        return g_norm_i8(xa, r.ld, ya, ry.ld, wa, qa, sa, r.M, r.K, (float)eps, st);
+      });
+    return Py_BuildValue("(NN)", THPVariable_Wrap(q), THPVariable_Wrap(s));
+  });
+}
+
+// q, q_scale, W, w_scale, y or None, epilogue, pushes, T, cap -> y
+PyObject* gemm_i8_(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 9, [&]() -> PyObject* {
+    const Tensor &q = tensor(a[0]), &qs = tensor(a[1]), &W = tensor(a[2]), &ws = tensor(a[3]);
+    const Tensor *given = optional(a[4]), *pushes = optional(a[6]), *cap = optional(a[8]);
+    const int64_t epilogue = integer(a[5]), T = integer(a[7]);
+    if (!q.is_cuda() || !W.is_cuda() || (given && !given->is_cuda())) refuse(kNotOnGpu);
+    const int64_t d = q.get_device();
+    if (!dense_on(d, {&qs, &W, &ws, pushes})) refuse("scales, W and pushes must be contiguous and on q's device");
+    if (!is(q, at::kChar) || !is(W, at::kChar) || W.dim() != 2 || !is(qs, at::kFloat) || !is(ws, at::kFloat))
+      refuse("q: [..., K] int8, W: [N, K] int8, scales fp32");
+    const Rows r = rows_of(q, "q");
+    const int64_t N = W.size(0), M = r.M;
+    if (W.size(1) != r.K || qs.numel() != M || ws.dim() != 1 || ws.size(0) != N)
+      refuse("q, W and their scales disagree (q_scale: one a row of q, w_scale: [N])");
+    const bool swiglu = epilogue == 2;
+    const int64_t No = swiglu ? N / 2 : N;
+    if (swiglu && N % 2) refuse("SwiGLU: W holds (gate, up) pairs of rows");
+    Tensor y;
+    if (given) {
+      y = *given;
+    } else {
+      auto sz = q.sizes().vec();
+      sz.back() = No;
+      y = make(sz, at::kFloat, q);
+    }
+    if (!is(y, at::kFloat) || y.get_device() != d || y.dim() < 1 || y.size(-1) != No || y.numel() != M * No)
+      refuse("y: one row of N (SwiGLU: N / 2) fp32 for each of q's, on its device");
+    if (pushes && (!is(*pushes, at::kInt) || pushes->dim() != 2 || pushes->size(1) != 6))
+      refuse("pushes: [n, 6] int32 records (see pack_pushes)");
+    int64_t ldc = 0, ldcr = 0;
+    if (cap) {
+      if (!swiglu || !cap->is_cuda() || cap->get_device() != d || !is(*cap, at::kFloat) || cap->dim() < 2 ||
+          cap->dim() > 3 || cap->stride(-1) != 1 || cap->size(-1) != No || cap->numel() != M * No || T < 1 ||
+          (cap->dim() == 3 && cap->size(1) != T))
+        refuse("capture (SwiGLU only): [rows, T, N / 2] or [M, N / 2] fp32 on q's device with unit neuron stride");
+      ldc = cap->stride(-2);
+      ldcr = cap->dim() == 3 ? cap->stride(0) : ldc * T;
+    }
+    if (M && No) {
+      const Rows ry = rows_of(y, "y");
+      launch(q, "q35_gemm_i8", [&, qa = data<int8_t>(q), sa = data<float>(qs), wa = data<int8_t>(W), wsa = data<float>(ws),
+                                ya = data<float>(y), pa = static_cast<const q35_push*>(data(pushes)),
+                                ca = data<float>(cap)](q35_stream_t st) {
+        return g_gemm_i8(qa, M > 1 ? r.ld : r.K, sa, wa, wsa, ya, ry.ld, M, N, r.K, (int)epilogue, pa,
+                         pushes ? pushes->size(0) : 0, T, ca, ldc, ldcr, st);
+      });
+    }
+    return THPVariable_Wrap(y);
+  });
+}
+
 // Whether an op on these arguments is the functions above and nothing more. Whatever follows a thread's calls (a trace, a
 // dispatch mode, a transform) has its key among those that the thread includes in every dispatch.
 bool direct_on(PyObject* const* a, Py_ssize_t n) {
@@ -384,10 +613,34 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
+// the addresses of the seven functions of the C ABI that came later
+PyObject* bind_sampling(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 7) {
+    PyErr_SetString(PyExc_TypeError, "bind_sampling: seven addresses");
+    return nullptr;
+  }
+  void* f[7];
+  for (int i = 0; i < 7; ++i) {
+    f[i] = PyLong_AsVoidPtr(a[i]);
+    if (PyErr_Occurred()) return nullptr;
+  }
+  g_shared_bytes = reinterpret_cast<decltype(g_shared_bytes)>(f[0]);
+  g_shared = reinterpret_cast<decltype(g_shared)>(f[1]);
+  g_sample_bytes = reinterpret_cast<decltype(g_sample_bytes)>(f[2]);
+  g_sample = reinterpret_cast<decltype(g_sample)>(f[3]);
+  g_quantize = reinterpret_cast<decltype(g_quantize)>(f[4]);
+  g_norm_i8 = reinterpret_cast<decltype(g_norm_i8)>(f[5]);
+  g_gemm_i8 = reinterpret_cast<decltype(g_gemm_i8)>(f[6]);
+  Py_RETURN_NONE;
+}
+
 #define Q35_FAST(name, f) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 #define Q35_METHOD(f) Q35_FAST(#f, f), Q35_FAST("try_" #f, try_direct<f>)
 PyMethodDef g_methods[] = {Q35_FAST("bind", bind),       Q35_FAST("direct", direct),   Q35_METHOD(paged_kv_append),
                            Q35_METHOD(paged_kv_rows),    Q35_METHOD(gated_attn_paged), Q35_METHOD(verify_drafts),
+                           Q35_FAST("bind_sampling", bind_sampling), Q35_METHOD(gated_attn_paged_shared),
+                           Q35_METHOD(sample_tokens), Q35_METHOD(filter_logits), Q35_METHOD(quantize_rows_i8),
+                           Q35_METHOD(add_rmsnorm_i8_), Q35_METHOD(gemm_i8_),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_paged_host", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

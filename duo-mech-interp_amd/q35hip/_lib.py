@@ -27,6 +27,9 @@ EXPORTS = [
     "q35_gdn_decode_sliced", "q35_gemv_norm_conv", "q35_gemv_gated_norm", "q35_gdn_chunk_prefill_conv",
     "q35_paged_kv_append", "q35_paged_kv_rows", "q35_gated_attn_paged_workspace_bytes", "q35_gated_attn_paged",
     "q35_verify_drafts_workspace_bytes", "q35_verify_drafts",
+    "q35_gated_attn_paged_shared_workspace_bytes", "q35_gated_attn_paged_shared",
+    "q35_sample_tokens_workspace_bytes", "q35_sample_tokens",
+    "q35_quantize_rows_i8", "q35_add_rmsnorm_i8", "q35_gemm_i8",
 ]
 
 Q35_F32, Q35_BF16, Q35_I8, Q35_I8_G128, Q35_I4_G64 = 0, 1, 2, 3, 4
@@ -96,6 +99,14 @@ _SIGS = {
                               I64, I64, P, P, P, I32, I64, I64, I64, I64, I64, F32, I64, P, SZ, P], I32),
     "q35_verify_drafts_workspace_bytes": ([I64, I64, I64], SZ),
     "q35_verify_drafts": ([P, I64, I64, P, I64, P, I64, I64, P, I64, P, P, F32, P, P, I64, I64, I64, P, SZ, P], I32),
+    "q35_gated_attn_paged_shared_workspace_bytes": ([I64, I64, I64, I64, I64, I64, I64, I64], SZ),
+    "q35_gated_attn_paged_shared": ([P, I64, I64, I64, P, I64, I64, I64, I32, P, F32, P, P, I64, P, P, P, P, I32, I64, I64, P,
+                                     I64, I64, I64, P, P, P, I32, I64, I64, I64, I64, I64, F32, P, SZ, P], I32),
+    "q35_sample_tokens_workspace_bytes": ([I64, I64, I64], SZ),
+    "q35_sample_tokens": ([P, I64, I64, P, I64, P, F32, P, I64, P, F32, P, F32, P, I32, P, I64, I64, I64, P, SZ, P], I32),
+    "q35_quantize_rows_i8": ([P, I64, I32, P, P, I64, I64, P], I32),
+    "q35_add_rmsnorm_i8": ([P, I64, P, I64, P, P, P, I64, I64, F32, P], I32),
+    "q35_gemm_i8": ([P, I64, P, P, P, P, I64, I64, I64, I64, I32, P, I64, I64, P, I64, I64, P], I32),
 }
 
 

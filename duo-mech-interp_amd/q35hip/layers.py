@@ -297,14 +297,16 @@ def gated_attention_layer(x, p, k_cache, v_cache, pos, *, rope_theta=1e7, partia
 
 
 def gated_attention_layer_paged(x, p, pages, table, pos, *, lens=None, rope_theta=1e7, partial_rotary_factor=0.25,
-                                eps=1e-6, prenorm=None, residual=None, fixed_order=False):
+                                eps=1e-6, prenorm=None, residual=None, fixed_order=False, shared_blocks=0):
     """gated_attention_layer over a paged KV cache in bf16 or 4 bits (ops.kv_pages; head dim 256): a decode step (T = 1),
     the check of drafted tokens (a few), a chunk of a prompt (many). x: [B, T, H] fp32; token t < lens[b] of row b (lens
     [B] int32 on the device, None: all T) sits at position pos[b] + t ([B] int32 on the device); its key and value go into
     the pages that table ([B, blocks] int32) names, and it attends to positions 0 .. pos[b] + t. Tokens past lens, or past
     the table, leave the pages alone and give 0 (residual: itself). A HIP graph that holds the call follows table, pos and
     lens. The first call stacks the weights, and the first over a table of more positions than any before waits for the
-    rotation tables (rope_tables), so make one of each ahead of a capture; other calls synchronise with nothing. prenorm, residual, fixed_order: see gated_attention_layer."""
+    rotation tables (rope_tables), so make one of each ahead of a capture; other calls synchronise with nothing. shared_blocks: how
+    many of the table's first blocks name the same pages in every row (several continuations of one prompt): their keys are
+    read once for all rows (ops.gated_attention_paged_shared). prenorm, residual, fixed_order: see gated_attention_layer."""
     B, T, _ = x.shape
     D = p["q_norm"].numel()
     Hq = p["q_proj"].shape[0] // (2 * D)
@@ -318,9 +320,12 @@ def gated_attention_layer_paged(x, p, pages, table, pos, *, lens=None, rope_thet
     # as the dense layer: fp32 for the GEMV of a few rows, bf16 for the int8 GEMM
     wq_o, ws_o = _q8(p, "o_proj")
     half = B * T > 8 and wq_o is not None
-    o = ops.gated_attention_paged(q[..., :D], q[..., D:], pages, table, pos, cos, sin, lens=lens,
-                                  q_norm_w=p["q_norm"].float().contiguous(), eps=eps, scale=1.0 / math.sqrt(D),
-                                  out_dtype=torch.bfloat16 if half else torch.float32)
+    args = dict(lens=lens, q_norm_w=p["q_norm"].float().contiguous(), eps=eps, scale=1.0 / math.sqrt(D),
+                out_dtype=torch.bfloat16 if half else torch.float32)
+    if shared_blocks:
+        o = ops.gated_attention_paged_shared(q[..., :D], q[..., D:], pages, table, pos, cos, sin, shared_blocks, **args)
+    else:
+        o = ops.gated_attention_paged(q[..., :D], q[..., D:], pages, table, pos, cos, sin, **args)
     return linear(o, p["o_proj"], wq_o, ws_o, residual=residual, fixed_order=fixed_order)
 
 

@@ -123,6 +123,17 @@ _LIB.define("gated_attn_paged(Tensor q, Tensor? gate, Tensor k_pages, Tensor v_p
             "float eps, float scale, int splits, bool f32_out) -> Tensor")
 _LIB.define("verify_drafts(Tensor logits, Tensor draft_ids, Tensor? draft_probs, Tensor u, Tensor? lens, "
             "Tensor? temperatures, float temperature) -> (Tensor, Tensor)")
+_LIB.define("gated_attn_paged_shared(Tensor q, Tensor? gate, Tensor k_pages, Tensor v_pages, Tensor? k_scale, "
+            "Tensor? v_scale, Tensor table, Tensor pos, Tensor? lens, Tensor cos, Tensor sin, Tensor? q_norm_w, "
+            "float eps, float scale, bool f32_out, int shared_blocks) -> Tensor")
+_CUTS = ("Tensor? temperatures, float temperature, Tensor? top_ks, int top_k, Tensor? top_ps, float top_p, "
+         "Tensor? min_ps, float min_p")
+_LIB.define(f"sample_tokens(Tensor logits, Tensor u, {_CUTS}, bool want_probs) -> (Tensor, Tensor)")
+_LIB.define(f"filter_logits(Tensor logits, {_CUTS}) -> Tensor")
+_LIB.define("quantize_rows_i8(Tensor x) -> (Tensor, Tensor)")
+_LIB.define("add_rmsnorm_i8_(Tensor(a!) x, Tensor? y, Tensor w, float eps) -> (Tensor, Tensor)")
+_LIB.define("gemm_i8_(Tensor q, Tensor q_scale, Tensor W, Tensor w_scale, Tensor(a!) y, int epilogue, Tensor? pushes, int T, "
+            "Tensor(b!)? cap=None) -> ()")
 
 
 # ---------------------------------------------------------------- gated delta rule
@@ -366,6 +377,9 @@ def _paged_host():
                   *(ctypes.cast(getattr(lib, f), ctypes.c_void_p).value for f in (
                       "q35_paged_kv_append", "q35_paged_kv_rows", "q35_gated_attn_paged_workspace_bytes",
                       "q35_gated_attn_paged", "q35_verify_drafts_workspace_bytes", "q35_verify_drafts")))
+        host.bind_sampling(*(ctypes.cast(getattr(lib, f), ctypes.c_void_p).value for f in (
+            "q35_gated_attn_paged_shared_workspace_bytes", "q35_gated_attn_paged_shared", "q35_sample_tokens_workspace_bytes",
+            "q35_sample_tokens", "q35_quantize_rows_i8", "q35_add_rmsnorm_i8", "q35_gemm_i8")))
         _HOST = host
     return _HOST
 
@@ -384,6 +398,30 @@ def _attn_paged_impl(*args):
 
 def _verify_drafts_impl(*args):
     return _paged_host().verify_drafts(*args)
+
+
+def _attn_paged_shared_impl(*args):
+    return _paged_host().gated_attn_paged_shared(*args)
+
+
+def _sample_tokens_impl(*args):
+    return _paged_host().sample_tokens(*args)
+
+
+def _filter_logits_impl(*args):
+    return _paged_host().filter_logits(*args)
+
+
+def _quantize_rows_i8_impl(x):
+    return _paged_host().quantize_rows_i8(x)
+
+
+def _add_rmsnorm_i8_impl(*args):
+    return _paged_host().add_rmsnorm_i8_(*args)
+
+
+def _gemm_i8_impl(q, q_scale, W, w_scale, y, epilogue, pushes, T, cap=None):
+    _paged_host().gemm_i8_(q, q_scale, W, w_scale, y, epilogue, pushes, T, cap)
 
 
 def _resid_add_impl(x, vecs, vec_of_row):
@@ -806,7 +844,10 @@ for _name, _impl in [("gdn_recurrent", _gdn_recurrent_impl), ("gdn_decode_step_"
                      ("gdn_chunk_prefill_conv_", _gdn_chunk_prefill_conv_impl),
                      ("gemv_norm_conv_", _gemv_norm_conv_impl), ("gemv_gated_norm_", _gemv_gated_norm_impl),
                      ("paged_kv_append_", _paged_kv_append_impl), ("paged_kv_rows", _paged_kv_rows_impl),
-                     ("gated_attn_paged", _attn_paged_impl), ("verify_drafts", _verify_drafts_impl)]:
+                     ("gated_attn_paged", _attn_paged_impl), ("verify_drafts", _verify_drafts_impl),
+                     ("gated_attn_paged_shared", _attn_paged_shared_impl), ("sample_tokens", _sample_tokens_impl),
+                     ("filter_logits", _filter_logits_impl), ("quantize_rows_i8", _quantize_rows_i8_impl),
+                     ("add_rmsnorm_i8_", _add_rmsnorm_i8_impl), ("gemm_i8_", _gemm_i8_impl)]:
     _LIB.impl(_name, _impl, "CUDA")
     _LIB.impl(_name, _no_cpu(_name), "CPU")
 
@@ -895,6 +936,16 @@ _LIB.impl("gated_attn_paged", lambda q, g, kp, vp, ks, vs, tb, pos, lens, cos, s
                       dtype=torch.float32 if f32_out else torch.bfloat16), "Meta")
 _LIB.impl("verify_drafts", lambda x, ids, q, u, lens, ts, t:
           (ids.new_empty(ids.shape[0]), ids.new_empty(ids.shape[0], ids.shape[1] + 1)), "Meta")
+_LIB.impl("gated_attn_paged_shared", lambda q, g, kp, vp, ks, vs, tb, pos, lens, cos, sin, w, eps, scale, f32_out, shared:
+          q.new_empty(q.shape[0], q.shape[1], q.shape[2] * q.shape[3],
+                      dtype=torch.float32 if f32_out else torch.bfloat16), "Meta")
+_LIB.impl("sample_tokens", lambda x, u, ts, t, ks, k, ps, p, ms, m, want:
+          (x.new_empty(x.shape[0], dtype=torch.int32), x.new_empty(x.shape if want else (0,))), "Meta")
+_LIB.impl("filter_logits", lambda x, ts, t, ks, k, ps, p, ms, m: x.new_empty(x.shape), "Meta")
+_LIB.impl("quantize_rows_i8", lambda x: (x.new_empty(x.shape, dtype=torch.int8),
+                                         x.new_empty(x.shape[:-1], dtype=torch.float32)), "Meta")
+_LIB.impl("add_rmsnorm_i8_", lambda x, y, w, eps: (x.new_empty(x.shape, dtype=torch.int8), x.new_empty(x.shape[:-1])), "Meta")
+_LIB.impl("gemm_i8_", lambda q, qs, W, ws, y, e, pushes, T, cap=None: None, "Meta")
 _LIB.impl("gdn_conv", _meta_gdn_conv, "Meta")
 _LIB.impl("attn_prep", _meta_attn_prep, "Meta")
 
@@ -1254,6 +1305,82 @@ def gated_attention_paged(q, gate, pages, table, pos, cos, sin, *, lens=None, q_
     return _call("try_gated_attn_paged", torch.ops.q35.gated_attn_paged, q, gate, *_four(pages), table, pos, lens, cos, sin,
                  q_norm_w, float(eps), q.shape[-1] ** -0.5 if scale is None else float(scale), int(splits),
                  out_dtype == torch.float32)
+
+
+def gated_attention_paged_shared(q, gate, pages, table, pos, cos, sin, shared_blocks, *, lens=None, q_norm_w=None, eps=1e-6,
+                                 scale=None, out_dtype=torch.bfloat16):
+    """gated_attention_paged for sequences that share their first shared_blocks pages (several continuations of one prompt, many
+    questions about one document): the first shared_blocks entries of every row of the table name the same pages, as row 0's
+    do (those are the ones read), and their keys are read once for the rows of all sequences. The result is that of
+    gated_attention_paged up to the order of its sums. shared_blocks is a host number: a captured call keeps it."""
+    _require(out_dtype in (torch.bfloat16, torch.float32), "out_dtype: bf16 or fp32")
+    return _call("try_gated_attn_paged_shared", torch.ops.q35.gated_attn_paged_shared, q, gate, *_four(pages), table, pos, lens,
+                 cos, sin, q_norm_w, float(eps), q.shape[-1] ** -0.5 if scale is None else float(scale),
+                 out_dtype == torch.float32, int(shared_blocks))
+
+
+def _cuts(temperature, top_k, top_p, min_p):
+    """Each setting as (per-row tensor or None, the one value)."""
+    return (*((temperature, 1.0) if torch.is_tensor(temperature) else (None, float(temperature))),
+            *((top_k, 0) if torch.is_tensor(top_k) else (None, int(top_k))),
+            *((top_p, 1.0) if torch.is_tensor(top_p) else (None, float(top_p))),
+            *((min_p, 0.0) if torch.is_tensor(min_p) else (None, float(min_p))))
+
+
+def sample_tokens(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, want_probs=False):
+    """One token per row from softmax(logits / temperature) cut by top_k, top_p and min_p (the sampling form of argmax_rows).
+    logits: [B, V] fp32 with dense rows; u: [B] fp32 random numbers in [0, 1); each setting a number or a tensor [B] (fp32,
+    top_k int32). In the order of the logits, ties by index: the first top_k tokens (0: all); of these while the
+    probabilities ahead of a token sum to less than top_p of all of these; of these the ones of at least min_p times the first
+    one's probability. The first always stays; temperature 0 is the argmax. The token is the first kept one, in this order,
+    whose running sum exceeds u of the kept ones' sum. Returns tokens [B] int32; with want_probs also the probabilities that
+    the draw is from, [B, V] fp32 (0 where cut): what verify_drafts takes as draft_probs."""
+    tokens, probs = _call("try_sample_tokens", torch.ops.q35.sample_tokens, logits, u, *_cuts(temperature, top_k, top_p, min_p),
+                          bool(want_probs))
+    return (tokens, probs) if want_probs else tokens
+
+
+def filter_logits(logits, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """The logits [B, V] or [B, P, V] (P positions share their row's settings) with what sample_tokens cuts at -inf:
+    verify_drafts(filter_logits(x, ...), ..., temperature=the same) checks drafts against the cut distribution."""
+    return _call("try_filter_logits", torch.ops.q35.filter_logits, logits, *_cuts(temperature, top_k, top_p, min_p))
+
+
+class RowsI8(NamedTuple):
+    """Rows in 8 bits: q [..., K] int8 codes, s [...] fp32 scales, standing for q s."""
+    q: torch.Tensor
+    s: torch.Tensor
+
+
+def quantize_rows(x):
+    """x [..., K] fp32 or bf16 (dense rows, evenly strided; K a multiple of 4, at most 16384) as RowsI8: s = fp32(max |x| / 127),
+    q = rint(x / s). A row that holds a value that is not finite gets codes 0 and the scale NaN."""
+    return RowsI8(*_call("try_quantize_rows_i8", torch.ops.q35.quantize_rows_i8, x))
+
+
+def add_rmsnorm_i8_(x, y, w, eps=1e-6):
+    """add_rmsnorm_ with the normed rows as RowsI8 (norm and quotients in 64 bits): x += y in place (y None: no add), then
+    quantize_rows of x * rsqrt(mean x^2 + eps) * (1 + w). x, y: [..., K] fp32, rows dense and evenly strided."""
+    return RowsI8(*_call("try_add_rmsnorm_i8_", torch.ops.q35.add_rmsnorm_i8_, x, y, w.float().contiguous(), float(eps)))
+
+
+def gemm_i8(x, W, w_scale, out=None, epilogue="store", pushes=None, T=1, capture=None):
+    """The product in 8-bit integers of RowsI8 x (q [..., K], K a multiple of 64) with W [N, K] int8, one scale per row of x
+    and per row of W (w_scale [N]): (sum_k q W) s w_scale, the sum exact. Any number of rows. epilogue "store" returns
+    [..., N] fp32 (in out when it is given), "add" accumulates into out, "swiglu" treats W's rows as interleaved (gate, up)
+    pairs and returns silu(gate) * up [..., N / 2] with the neuron pushes (pack_pushes) applied; T and capture as for gemm_q8."""
+    e = _EPI.get(epilogue, -1)
+    _require(e in (0, 1, 2), "gemm_i8: epilogue 'store', 'add' or 'swiglu'")
+    _require(e != 1 or out is not None, "gemm_i8: the add epilogue needs out")
+    q, s = x
+    if not torch.compiler.is_compiling() and isinstance(q, torch.Tensor) and q.is_cuda:
+        y = (_HOST or _paged_host()).try_gemm_i8_(q, s, W, w_scale, out, e, pushes, int(T), capture)
+        if y is not NotImplemented:
+            return y if out is None else out
+    if out is None:
+        out = torch.empty(*q.shape[:-1], W.shape[0] // (2 if e == 2 else 1), dtype=torch.float32, device=q.device)
+    torch.ops.q35.gemm_i8_(q, s, W, w_scale, out, e, pushes, int(T), capture)
+    return out
 
 
 def _four(pages):

@@ -583,6 +583,22 @@ int q35_gated_attn_paged(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh
                          int64_t splits, void* workspace, size_t workspace_bytes, q35_stream_t stream);
 
 /*
+ * q35_gated_attn_paged for sequences whose tables begin with the same pages: the first shared_blocks entries of every row of
+ * the table name the pages that row 0's do (only row 0's are read), and their keys are read once for the rows of all
+ * sequences. The result is that of q35_gated_attn_paged up to the order of its sums; a sequence may also end inside the
+ * shared part. shared_blocks 0 is q35_gated_attn_paged. B T Hq / Hkv up to 2^24, in at most 65535 / Hkv blocks of 32 rows.
+ */
+size_t q35_gated_attn_paged_shared_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t n_blocks,
+                                                   int64_t page_size, int64_t shared_blocks);
+int q35_gated_attn_paged_shared(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* gate, int64_t g_sb,
+                                int64_t g_st, int64_t g_sh, int dtype, const float* q_norm_w, float eps, const float* cos,
+                                const float* sin, int64_t rot, const void* k_pages, const void* v_pages, const void* k_scale,
+                                const void* v_scale, int fmt, int64_t n_pages, int64_t page_size, const int32_t* table,
+                                int64_t ld_table, int64_t n_blocks, int64_t shared_blocks, const int32_t* pos,
+                                const int32_t* lens, void* out, int out_dtype, int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
+                                int64_t D, float scale, void* workspace, size_t workspace_bytes, q35_stream_t stream);
+
+/*
  * Drafted tokens kept or refused against the target's probabilities, and one token drawn behind the kept ones.
  *   logits: [B, K + 1, V] fp32 (strides l_sb, l_sp): position i the target's logits behind i drafts
  *   draft_ids: [B, K] int32 (row stride d_sb); draft_probs: [B, K, V] fp32 (strides p_sb, p_sp), the probabilities each
@@ -605,6 +621,54 @@ int q35_verify_drafts(const float* logits, int64_t l_sb, int64_t l_sp, const int
                       const int32_t* lens, const float* temperatures, float temperature, int32_t* n_accept,
                       int32_t* tokens, int64_t B, int64_t K, int64_t V, void* workspace, size_t workspace_bytes,
                       q35_stream_t stream);
+
+/*
+ * Tokens drawn from softmax(logits / temperature) cut by top-k, top-p and min-p, from given random numbers, and the cut itself.
+ *   logits: [B, P, V] fp32 (strides l_sb, l_sp): P positions a row share the row's settings
+ *   temperatures, top_ks (int32), top_ps, min_ps: [B] on the device, or NULL for the one value on every row
+ * Tokens in the order of their logits, ties by index: of these the first top_k (0 or less: all); of them those whose weights
+ * ahead sum to less than top_p of all of theirs (1 or more: all); of them those of at least min_p of the first one's weight (0
+ * or less: all). The first always stays. Temperature 0 (on the device also less) is top-k 1. Weights exp((x - max) /
+ * temperature) and their sums are formed in 64 bits, as whole numbers of 2^-44 of the largest weight for 2^18 tokens (2^-40
+ * for 2^22).
+ *   tokens: [B] int32 (P = 1) or NULL: the first kept token whose running sum exceeds u[b] (fp32, stride u_sb, in [0, 1)) of
+ *   the kept ones' sum
+ *   out: [B, P, V] fp32 dense: out_kind 1 the probabilities that the draw is from, 2 the logits with what is cut at -inf
+ *   (what q35_verify_drafts takes, at the same temperature); out_kind 0: none (NULL)
+ * A NaN logit counts as -inf; a row with no logit above -inf gives token 0 and probabilities 0. B P <= 65535, V <= 4,194,304.
+ * Needs q35_sample_tokens_workspace_bytes(B, P, V) bytes of workspace, 16-byte aligned.
+ */
+size_t q35_sample_tokens_workspace_bytes(int64_t B, int64_t P, int64_t V);
+int q35_sample_tokens(const float* logits, int64_t l_sb, int64_t l_sp, const float* u, int64_t u_sb, const float* temperatures,
+                      float temperature, const int32_t* top_ks, int64_t top_k, const float* top_ps, float top_p,
+                      const float* min_ps, float min_p, int32_t* tokens, int out_kind, float* out, int64_t B, int64_t P,
+                      int64_t V, void* workspace, size_t workspace_bytes, q35_stream_t stream);
+
+/*
+ * Rows in 8 bits with one scale a row: s[m] = fp32(max_k |x[m, k]| / 127), q[m, k] = rint(x[m, k] / s[m]), half to even, the
+ * quotient of the exact x (a row of zeros, or of values so small that s is 0: codes 0). A row that holds a value that is not
+ * finite gets codes 0 and the scale NaN, and its products are NaN.
+ *   x: [M, ldx] in dtype (Q35_F32, 16-byte aligned, or Q35_BF16, 8-byte); q: [M, K] int8, rows dense; s: [M] fp32.
+ *   K and ldx multiples of 4, K <= 16384.
+ * q35_add_rmsnorm_i8: x += y (y may be NULL) in place as q35_add_rmsnorm, and the rows x * rsqrt(mean x^2 + eps) * (1 + w),
+ * formed in 64 bits, as codes and scales.
+ */
+int q35_quantize_rows_i8(const void* x, int64_t ldx, int dtype, int8_t* q, float* s, int64_t M, int64_t K,
+                         q35_stream_t stream);
+int q35_add_rmsnorm_i8(float* x, int64_t ldx, const float* y, int64_t ldy, const float* w, int8_t* q, float* s, int64_t M,
+                       int64_t K, float eps, q35_stream_t stream);
+
+/*
+ * Product in 8-bit integers: v[m, n] = (sum_k q[m, k] W[n, k]) q_scale[m] w_scale[n], the sum exact in 32 bits.
+ *   q: [M, ldq] int8 (16-byte aligned, ldq a multiple of 16); W: [N, K] int8 (16-byte aligned); q_scale [M], w_scale [N] fp32;
+ *   K a multiple of 64, at most 65536
+ *   epilogue 0: y[m, n] = v (y: [M, ldy] fp32, ldy >= N); 1: y[m, n] += v; 2: SwiGLU over interleaved (gate, up) rows of W,
+ *   y[m, j] = silu(v_2j) v_2j+1 then the pushes in order (N even, ldy >= N / 2); pushes, npush <= 64, T and the capture as for
+ *   q35_gemm_q8.
+ */
+int q35_gemm_i8(const int8_t* q, int64_t ldq, const float* q_scale, const int8_t* W, const float* w_scale, float* y,
+                int64_t ldy, int64_t M, int64_t N, int64_t K, int epilogue, const q35_push* pushes, int64_t npush, int64_t T,
+                float* cap, int64_t ld_cap, int64_t ld_cap_row, q35_stream_t stream);
 
 #ifdef __cplusplus
 }
