@@ -8,16 +8,18 @@
 // and the draw is the first kept token whose running sum exceeds u of the kept ones' sum. So all that is ever asked is where in
 // one order a running count or sum reaches a target. The first token always stays; temperature 0 is top-k 1.
 //
-// Weights w = exp((x - max) / T) are formed in 64 bits and held as whole numbers of 2^-S (S = 62 - log2 V: the sum fits), so
-// that sums depend on no order and a border lies where 64 bits put it: 2^-44 of the largest weight for 150 K tokens.
+// Weights w = exp((x - max) / T) are formed in 64 bits and held as whole numbers of 2^-S (S = 62 - log2 V, at most 50: the sum
+// fits), so that sums depend on no order and a border lies where 64 bits put it: 2^-44 of the largest weight for 150 K tokens.
 //
-//   sample_max_kernel    the row's maximum, by chunks of 4096
-//   sample_hist_kernel   counts and sums of weights of the row in 2048 bins by distance from the maximum (1/50 nat of the
-//                        scaled logit for 30.7 nats, 1/2 nat behind them), from LDS into the row's bins by integer atomics
-//   sample_pick_kernel   one block a row: the bins' running sums give the bin of each border; its few tokens are fetched and
-//                        ordered
+//   sample_max_kernel    the largest value of each group of 16 and of each chunk of 4096
+//   sample_hist_kernel   counts and sums of weights of the row in 2048 bins by distance from the maximum, from LDS into the
+//                        row's bins by integer atomics. Rows of a small top-k need none of it
+//   sample_pick_kernel   one block a row: the bins' running sums give the bin of each border; the groups whose largest value
+//                        reaches that bin are fetched, and the bin's few tokens put in order. For a small top-k it forms the
+//                        bins itself, of the groups that reach the k-th largest group's bin: all larger tokens are in them
 //   sample_write_kernel  probabilities or cut logits, where they are asked for
 #include <algorithm>
+#include <type_traits>
 
 #include "token_weights.h"
 
@@ -25,19 +27,22 @@ namespace q35 {
 
 typedef unsigned long long u64;
 constexpr int kSBins = 2048, kSFine = 1536;
-constexpr int kSChunk = 1024;  // quads of a block of the maximum and the write kernel
-constexpr int kSList = 2048;   // tokens of a bin that are held in LDS
+constexpr int kSChunk = 1024;    // quads of a block of the maximum and the write kernel: 256 groups of 4
+constexpr int kSFew = 1024;      // the largest top-k whose rows need no histogram
+constexpr int kSThreads = 1024;  // of the pick kernel
+constexpr int kSHeld = 10;       // groups' maxima that one of its threads holds
+constexpr int kSSort = kSThreads;  // tokens that it sorts
+constexpr int kSWaves = kSThreads / 64, kSSeg = 512;  // tokens that each of its waves can list
 constexpr int64_t kSMaxV = 1 << 22;
 
 enum SampleOut : int { kSampleNone = 0, kSampleProbs = 1, kSampleLogits = 2 };
 
-// What is kept of a row: bins below b, and of bin b the tokens up to (key, idx) in the order.
+// What is kept of a row: the tokens up to (x, idx) in the order; none where idx is -1 and x infinite.
 struct SampleCut {
   double scale;  // probability of a weight of 1
-  float max;
-  int b;
-  uint32_t key;
+  float max, x;
   int idx;
+  int pad;
 };
 struct SampleArgs {
   const float* x;
@@ -50,8 +55,9 @@ struct SampleArgs {
   const float* u;
   int64_t ub;
   int V, C, R;  // chunks of the maximum kernel, blocks per row of the histogram kernel
-  double unit;  // 2^S
+  int S;        // weights are whole numbers of 2^-S
   float* cmax;  // [rows][C]
+  float* gmax;  // [rows][C 256]
   u64* mass;    // [rows][kSBins]
   uint32_t* count;
   SampleCut* cut;
@@ -62,9 +68,9 @@ struct SampleArgs {
 struct SampleRow {
   const float* x;
   double inv_t;  // 32 log2(e) / T
-  float bins;    // bins per unit of the logit
   float t, p, m;
-  int k;  // 0: all
+  int k;     // 0: all
+  bool few;  // a small top-k
 };
 __device__ __forceinline__ float s_setting(const float* v, float one, int b) {
   return v ? __int_as_float(load_uniform(reinterpret_cast<const int32_t*>(v) + b)) : one;
@@ -82,20 +88,34 @@ __device__ __forceinline__ SampleRow s_row(const SampleArgs& a, int row) {
     r.k = 1;
   }
   if (r.k <= 0 || r.k >= a.V) r.k = 0;
+  r.few = r.k > 0 && r.k <= kSFew;
   r.inv_t = fmax(32.0 * 1.4426950408889634074 / (double)r.t, 1e-300);
-  r.bins = 50.f / r.t;
   return r;
 }
 
-// The bin of x under the maximum M: the same in every kernel (no contraction), never larger for a larger x.
-__device__ __forceinline__ int s_bin(float x, float M, float bins) {
-#pragma clang fp contract(off)
-  if (x == M) return 0;
-  const float y = (M - x) * bins;
-  if (y < (float)kSFine) return (int)y;
-  const float z = (y - (float)kSFine) * 0.04f;
-  return z < (float)(kSBins - 1 - kSFine) ? kSFine + (int)z : kSBins - 1;  // (NaN: an infinite temperature and -inf)
+// The distance of x from the maximum M in 1/32 octaves of the weight, rounded, and the weight in units of 2^-S: 2^(z / 32) as in
+// exp2_neg, with S in the exponent and the conversion to a whole number by adding 2^52 (fp64 has no other short one).
+constexpr double kSFar = 1100.0 * kVTab;  // 0 from there on, also for -inf
+struct SampleWeight {
+  int n;
+  u64 w;
+};
+__device__ __forceinline__ double s_z(float x, float M, double inv_t) {
+  return x == M ? 0.0 : fmin(((double)M - (double)x) * inv_t, kSFar);
 }
+__device__ __forceinline__ SampleWeight s_weight(float x, float M, double inv_t, int S, const double* tab) {
+  constexpr double c1 = -0.69314718055994530942 / kVTab, c2 = c1 * c1 / 2.0, c3 = c1 * c2 / 3.0, c4 = c1 * c3 / 4.0;
+  const double z = s_z(x, M, inv_t), n = __builtin_rint(z), r = z - n;
+  const int k = -(int)n;
+  const double e = __builtin_fma(__builtin_fma(__builtin_fma(__builtin_fma(c4, r, c3), r, c2), r, c1), r, 1.0);
+  const double w = __builtin_ldexp(e * tab[k & (kVTab - 1)], (k >> 5) + S) + 0x1p52;
+  return {-k, __builtin_bit_cast(u64, w) & 0xFFFFFFFFFFFFFull};
+}
+// The bin of a distance: 1/32 octave each for 48 octaves, then an octave each. Never larger for a larger x.
+__device__ __forceinline__ int s_bin(int n) {
+  return n < kSFine ? n : min(kSFine + ((n - kSFine) >> 5), kSBins - 1);
+}
+__device__ __forceinline__ int s_bin(float x, float M, double inv_t) { return s_bin((int)__builtin_rint(s_z(x, M, inv_t))); }
 // Order-preserving bits (-0 as +0; no NaN).
 __device__ __forceinline__ uint32_t s_key(float x) {
   const uint32_t b = __float_as_uint(x == 0.f ? 0.f : x);
@@ -103,9 +123,6 @@ __device__ __forceinline__ uint32_t s_key(float x) {
 }
 __device__ __forceinline__ float s_unkey(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
-}
-__device__ __forceinline__ u64 s_mass(float x, float M, double inv_t, double unit, const double* tab) {
-  return (u64)(v_weight(x, M, inv_t, tab) * unit + 0.5);
 }
 
 // A row in quads that lie on 16 bytes: quad q holds elements 4 q - ahead .. + 3 (ahead < 4: how far the row's start is past 16
@@ -118,6 +135,15 @@ struct SampleQuads {
     base = row - ahead;
   }
   __device__ __forceinline__ int n() const { return (ahead + V + 3) >> 2; }
+  // the quads that lie in the row whole
+  __device__ __forceinline__ int whole_first() const { return ahead ? 1 : 0; }
+  __device__ __forceinline__ int whole_last() const { return (ahead + V) >> 2; }
+  __device__ __forceinline__ f32x4 whole(int q) const {
+    f32x4 v = *reinterpret_cast<const f32x4*>(base + 4 * (int64_t)q);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = v_clean(v[e]);
+    return v;
+  }
   __device__ __forceinline__ f32x4 load(int q) const {
     const int i = 4 * q - ahead;
     f32x4 v;
@@ -132,25 +158,33 @@ struct SampleQuads {
     return v;
   }
 };
-// f(index, value) of the row's quads first, first + step, ... below last; elements outside the row are left out.
+// f(value) of the row's quads first, first + step, ... below last.
 template <typename F>
 __device__ __forceinline__ void s_for_row(const SampleQuads& s, int first, int step, int last, F&& f) {
-  constexpr int U = 4;
-  for (int q = first; q < last; q += U * step) {
+  constexpr int U = 2;
+  const int w0 = s.whole_first(), w1 = min(last, s.whole_last());
+  int q = first < w0 ? first + step : first;
+  for (; q + (U - 1) * step < w1; q += U * step) {
     f32x4 v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      v[u] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      if (q + u * step < last) v[u] = s.load(q + u * step);
-    }
+    for (int u = 0; u < U; ++u) v[u] = s.whole(q + u * step);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (q + u * step >= last) break;
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = 4 * (q + u * step) - s.ahead + e;
-        if (i >= 0 && i < s.V) f(i, v[u][e]);
-      }
+      for (int e = 0; e < 4; ++e) f(v[u][e]);
+  }
+  for (; q < w1; q += step) {
+    const f32x4 v = s.whole(q);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f(v[e]);
+  }
+  // the row's ends, in quads that others share
+  for (int e = 0; e < 2; ++e) {
+    const int k = e ? s.whole_last() : 0;
+    if (k < last && k >= first && (k - first) % step == 0 && (e ? s.n() > s.whole_last() && (k > 0 || w0 == 0) : w0 == 1)) {
+      const f32x4 v = s.load(k);
+      for (int i = 0; i < 4; ++i)
+        if (4 * k - s.ahead + i >= 0 && 4 * k - s.ahead + i < s.V) f(v[i]);
     }
   }
 }
@@ -159,11 +193,12 @@ __global__ __launch_bounds__(256) void sample_max_kernel(SampleArgs a) {
   const int tid = threadIdx.x, row = blockIdx.y, c = blockIdx.x;
   const SampleRow r = s_row(a, row);
   const SampleQuads s(r.x, a.V);
-  // the row's bins, cleared for the next kernel
-  const int per = (kSBins + a.C - 1) / a.C;
-  for (int i = c * per + tid; i < min((c + 1) * per, kSBins); i += 256) {
-    a.mass[(size_t)row * kSBins + i] = 0;
-    a.count[(size_t)row * kSBins + i] = 0;
+  if (!r.few) {  // the row's bins, cleared for the next kernel
+    const int per = (kSBins + a.C - 1) / a.C;
+    for (int i = c * per + tid; i < min((c + 1) * per, kSBins); i += 256) {
+      a.mass[(size_t)row * kSBins + i] = 0;
+      a.count[(size_t)row * kSBins + i] = 0;
+    }
   }
   const int last = min((c + 1) * kSChunk, s.n());
   float m = -INFINITY;
@@ -175,6 +210,7 @@ __global__ __launch_bounds__(256) void sample_max_kernel(SampleArgs a) {
       m = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), m);
     }
   }
+  a.gmax[((size_t)row * a.C + c) * 256 + tid] = m;
   m = wave_max_f32(m);
   __shared__ float sm[4];
   if ((tid & 63) == 0) sm[tid >> 6] = m;
@@ -192,6 +228,7 @@ __device__ __forceinline__ float s_max(const SampleArgs& a, int row) {
 __global__ __launch_bounds__(256) void sample_hist_kernel(SampleArgs a) {
   const int tid = threadIdx.x, row = blockIdx.y;
   const SampleRow r = s_row(a, row);
+  if (r.few) return;
   const SampleQuads s(r.x, a.V);
   __shared__ u64 mass[kSBins];
   __shared__ uint32_t count[kSBins];
@@ -204,12 +241,14 @@ __global__ __launch_bounds__(256) void sample_hist_kernel(SampleArgs a) {
   const float M = s_max(a, row);
   __syncthreads();
   const int nq = s.n(), per = (nq + a.R - 1) / a.R, first = blockIdx.x * per;
-  s_for_row(s, first + tid, 256, min(first + per, nq), [&](int, float x) {
-    const int b = s_bin(x, M, r.bins);
-    const u64 w = s_mass(x, M, r.inv_t, a.unit, tab);
-    atomicAdd(&count[b], 1u);
-    if (w) atomicAdd(&mass[b], w);
-  });
+  auto add = [&](float x, bool counts) {
+    const SampleWeight w = s_weight(x, M, r.inv_t, a.S, tab);
+    const int b = s_bin(w.n);
+    if (counts) atomicAdd(&count[b], 1u);
+    atomicAdd(&mass[b], w.w);
+  };
+  if (r.k > 0) s_for_row(s, first + tid, 256, min(first + per, nq), [&](float x) { add(x, true); });
+  else s_for_row(s, first + tid, 256, min(first + per, nq), [&](float x) { add(x, false); });
   __syncthreads();
   for (int i = tid; i < kSBins; i += 256) {
     if (count[i]) __hip_atomic_fetch_add(a.count + (size_t)row * kSBins + i, count[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -218,45 +257,90 @@ __global__ __launch_bounds__(256) void sample_hist_kernel(SampleArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int kSThreads = 1024;
-
 struct SamplePick {
-  u64 mass[kSBins];  // sums up to and with each bin
+  u64 mass[kSBins];  // of each bin, then sums up to and with it
   uint32_t count[kSBins];
-  float lx[kSList];  // the tokens of a bin
-  int li[kSList];
+  u64 list[kSWaves][kSSeg];  // tokens, each wave's own: bits that sort as the order, above the index
+  u64 sort[kSSort];
+  uint16_t group[kSHeld * kSThreads];  // groups that reach a value, from a first one on
   u64 hmass[256];
   uint32_t hcount[256];
-  u64 wmass[16];
-  uint32_t wcount[16];
+  u64 wmass[kSWaves];
+  uint32_t wcount[kSWaves];
   double tab[kVTab];
-  int n;            // tokens of the bin
-  int bin;          // of a target
-  uint32_t key;     // the border: key, index, and count and mass up to and with it
-  int idx;
-  u64 to_mass, sum;
+  int groups;  // of the list
+  int n;       // tokens to be sorted
+  int full;    // whether a wave's list was
+  int bin;     // of a target
+  u64 sum, to_mass;
   uint32_t digit;
 };
 
-__device__ __forceinline__ u64 s_wave_scan(u64 v, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const u64 w = __shfl_up(v, o);
-    if (lane >= o) v += w;
-  }
+// Lane exchanges on the vector ALU. A ds_bpermute takes 100 cycles, a scan or a step of a sort of 64-bit values two of them: the
+// pick of three rows of top-k 20 16.2 -> PICK us.
+template <int CTRL, int ROWS> __device__ __forceinline__ u64 s_dpp_or_0(u64 v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (uint32_t)v, CTRL, ROWS, 0xF, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (uint32_t)(v >> 32), CTRL, ROWS, 0xF, true);
+  return ((u64)hi << 32) | lo;
+}
+// Sums up to and with each lane.
+__device__ __forceinline__ u64 s_wave_scan(u64 v) {
+  v += s_dpp_or_0<0x111, 0xF>(v);  // row_shr:1
+  v += s_dpp_or_0<0x112, 0xF>(v);
+  v += s_dpp_or_0<0x114, 0xF>(v);
+  v += s_dpp_or_0<0x118, 0xF>(v);
+  v += s_dpp_or_0<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+  v += s_dpp_or_0<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
   return v;
 }
-
-// What is in the row, kept by a cut, as f(index, value).
-struct SampleKept {
-  int b;
-  uint32_t key;
-  int idx;
-  __device__ __forceinline__ bool has(int bin, float x, int i) const {
-    if (bin != b) return bin < b;
-    const uint32_t k = s_key(x);
-    return k > key || (k == key && i <= idx);
+__device__ __forceinline__ uint32_t s_wave_scan(uint32_t v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, true);
+  return v;
+}
+__device__ __forceinline__ u64 s_lane(u64 v, int lane) {  // of a uniform lane
+  return ((u64)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(v >> 32), lane) << 32) |
+         (uint32_t)__builtin_amdgcn_readlane((uint32_t)v, lane);
+}
+// The value J lanes apart (lane ^ J).
+template <int J> __device__ __forceinline__ uint32_t s_xor(uint32_t v, int lane) {
+  if constexpr (J == 1) return __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, false);        // quad_perm [1,0,3,2]
+  else if constexpr (J == 2) return __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, false);   // quad_perm [2,3,0,1]
+  else if constexpr (J == 4) {  // row_shl:4 into banks 0 and 2, row_shr:4 into banks 1 and 3
+    const uint32_t up = __builtin_amdgcn_update_dpp(v, v, 0x104, 0xF, 0x5, false);
+    return __builtin_amdgcn_update_dpp(up, v, 0x114, 0xF, 0xA, false);
+  } else if constexpr (J == 8) return __builtin_amdgcn_mov_dpp(v, 0x128, 0xF, 0xF, false);  // row_ror:8
+  else if constexpr (J == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return lane & 16 ? r[0] : r[1];
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return lane & 32 ? r[0] : r[1];
   }
+}
+// One step of a bitonic sort over J lanes: the smaller of the two stays in the lower lane where `up`.
+template <int J> __device__ __forceinline__ u64 s_sort_step(u64 v, bool up, int lane) {
+  const u64 o = ((u64)s_xor<J>((uint32_t)(v >> 32), lane) << 32) | s_xor<J>((uint32_t)v, lane);
+  return (o < v) == (((lane & J) == 0) == up) ? o : v;
+}
+__device__ __forceinline__ u64 s_sort_steps(u64 v, int from, bool up, int lane) {
+  if (from >= 32) v = s_sort_step<32>(v, up, lane);
+  if (from >= 16) v = s_sort_step<16>(v, up, lane);
+  if (from >= 8) v = s_sort_step<8>(v, up, lane);
+  if (from >= 4) v = s_sort_step<4>(v, up, lane);
+  if (from >= 2) v = s_sort_step<2>(v, up, lane);
+  return s_sort_step<1>(v, up, lane);
+}
+
+// Whether a token is kept: up to (x, idx) in the order.
+struct SampleKept {
+  float x;
+  uint32_t idx;
+  __device__ __forceinline__ bool has(float v, int i) const { return v > x || (v == x && (uint32_t)i <= idx); }
 };
 
 __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
@@ -264,46 +348,241 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
   const SampleRow r = s_row(a, row);
   const SampleQuads s(r.x, a.V);
   __shared__ SamplePick g;
+  const int G = a.C * 256;
+  const float* gmax = a.gmax + (size_t)row * G;
+  float held[kSHeld];  // the maxima of groups tid + 1024 i
+#pragma unroll
+  for (int i = 0; i < kSHeld; ++i) held[i] = tid + kSThreads * i < G ? gmax[tid + kSThreads * i] : -INFINITY;
   exp2_table(g.tab, tid);
   const float M = s_max(a, row);
   if (!(M > -INFINITY)) {  // nothing above -inf: token 0, nothing kept
     if (tid == 0) {
-      a.cut[row] = {0.0, M, -1, 0, 0};
+      a.cut[row] = {0.0, M, INFINITY, -1, 0};
       if (a.tokens) a.tokens[row] = 0;
     }
     return;
   }
-  // ---- running sums of the bins: two a thread
-  {
+  // ---- f(in, index, value) by whole waves, for the row's tokens, `in` for those of lo to hi: of the groups whose maximum reaches
+  // lo, or, where most of them do, of all. False, and not all of them seen, as soon as more than `most` groups do.
+  // Loads in flight of a wave: D in a pass over all (150 K tokens are otherwise a chain of their latencies), L of listed groups.
+  auto traverse = [&](auto loads, auto still_held, float lo, float hi, int most, auto&& f) __attribute__((always_inline)) -> bool {
+    constexpr int D = decltype(loads)::value, L = D > 1 ? 4 : 1;
+    auto quad = [&](bool there, int q, const f32x4& v) __attribute__((always_inline)) {
+      const int i = 4 * q - s.ahead;
+      bool in[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) in[e] = there && v[e] >= lo && v[e] <= hi && i + e >= 0 && i + e < a.V;
+      if (__builtin_amdgcn_ballot_w64(in[0] | in[1] | in[2] | in[3]) == 0) return;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f(in[e], i + e, v[e]);
+    };
+    int seen = 0;
+    for (int g0 = 0; g0 < G; g0 += kSHeld * kSThreads) {
+      if (tid == 0) g.groups = 0;
+      __syncthreads();
+      uint32_t mine = 0;
+#pragma unroll
+      for (int i = 0; i < kSHeld; ++i) {
+        const int at = g0 + tid + kSThreads * i;
+        const float m = decltype(still_held)::value && g0 == 0 ? held[i] : at < G ? gmax[at] : -INFINITY;
+        mine |= (at < G && m >= lo ? 1u : 0u) << i;
+      }
+      const uint32_t sum = s_wave_scan((uint32_t)__builtin_popcount(mine));
+      int base = 0;
+      if (lane == 63 && sum) base = atomicAdd(&g.groups, (int)sum);
+      int put = __builtin_amdgcn_readlane(base, 63) + (int)sum - __builtin_popcount(mine);
+#pragma unroll
+      for (int i = 0; i < kSHeld; ++i)
+        if (mine >> i & 1) g.group[put++] = (uint16_t)(tid + kSThreads * i);
+      __syncthreads();
+      const int listed = g.groups, nq = s.n(), here = min(G - g0, kSHeld * kSThreads);
+      seen += listed;
+      if (seen > most) {
+        __syncthreads();
+        return false;
+      }
+      if (4 * listed < here) {
+        for (int k0 = 64 * wave; k0 < 4 * listed; k0 += L * kSThreads) {
+          f32x4 v[L];
+          int q[L];
+#pragma unroll
+          for (int u = 0; u < L; ++u) {
+            const int k = k0 + lane + u * kSThreads, gr = k < 4 * listed ? g0 + g.group[k >> 2] : 0;
+            q[u] = k < 4 * listed ? (gr >> 8) * kSChunk + (gr & 255) + 256 * (k & 3) : nq;
+            v[u] = q[u] < nq ? s.load(q[u]) : zero4();
+          }
+#pragma unroll
+          for (int u = 0; u < L; ++u) quad(q[u] < nq, q[u], v[u]);
+        }
+      } else {
+        const int last = min(4 * (g0 + here), nq);
+        for (int q0 = 4 * g0 + 64 * wave; q0 < last; q0 += D * kSThreads) {
+          f32x4 v[D];
+          if (q0 >= s.whole_first() && q0 + 63 + (D - 1) * kSThreads < min(last, s.whole_last())) {
+#pragma unroll
+            for (int u = 0; u < D; ++u) v[u] = s.whole(q0 + lane + u * kSThreads);
+          } else {
+#pragma unroll
+            for (int u = 0; u < D; ++u) v[u] = q0 + lane + u * kSThreads < last ? s.load(q0 + lane + u * kSThreads) : zero4();
+          }
+#pragma unroll
+          for (int u = 0; u < D; ++u) quad(q0 + lane + u * kSThreads < last, q0 + lane + u * kSThreads, v[u]);
+        }
+      }
+      __syncthreads();
+    }
+    return true;
+  };
+  // The tokens of lo to hi whose bits are first to last into the waves' lists (mine_n of this one's); false where they do not
+  // fit, or traverse() gave up.
+  int mine_n = 0;
+  auto collect = [&](auto still_held, float lo, float hi, u64 first, u64 last, int most) __attribute__((always_inline)) -> bool {
+    mine_n = 0;
+    if (tid == 0) g.full = 0;
+    const bool all = traverse(std::integral_constant<int, 4>{}, still_held, lo, hi, most, [&](bool in, int i, float x) __attribute__((always_inline)) {
+      const u64 bits = ((u64)~s_key(x) << 32) | (uint32_t)i;
+      const bool ours = in && bits >= first && bits <= last;
+      const u64 mask = __builtin_amdgcn_ballot_w64(ours);
+      if (mask == 0) return;
+      const int to = mine_n + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+      if (ours && to < kSSeg) g.list[wave][to] = bits;
+      mine_n += __popcll(mask);
+    });
+    if (lane == 0 && mine_n > kSSeg) g.full = 1;
+    __syncthreads();
+    const bool fits = all && !g.full;
+    __syncthreads();
+    return fits;
+  };
+  // Of the waves' lists those whose bits are first to last, together, to be sorted: how many (the first kSSort are there).
+  auto gather = [&](u64 first, u64 last) __attribute__((always_inline)) -> int {
+    if (tid == 0) g.n = 0;
+    __syncthreads();
+    for (int l0 = 0; l0 < mine_n; l0 += 64) {
+      const u64 bits = l0 + lane < mine_n ? g.list[wave][l0 + lane] : 0;
+      const bool in = l0 + lane < mine_n && bits >= first && bits <= last;
+      const u64 mask = __builtin_amdgcn_ballot_w64(in);
+      int base = 0;
+      if (lane == 0 && mask) base = atomicAdd(&g.n, __popcll(mask));
+      const int to = __builtin_amdgcn_readfirstlane(base) +
+                     __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+      if (in && to < kSSort) g.sort[to] = bits;
+    }
+    __syncthreads();
+    const int n = g.n;
+    __syncthreads();
+    return n;
+  };
+  // ---- the list (n tokens of it, up to kSSort) sorted, and its running sum of weights, token i in thread i; up to 64 tokens by
+  // every wave for itself
+  u64 v = 0, run = 0;
+  int at = 0;       // this thread's place
+  bool one = true;  // (every wave for itself)
+  auto sort = [&](int n) __attribute__((always_inline)) {
+    one = n <= 64;
+    at = one ? lane : tid;
+    v = at < n ? g.sort[at] : ~0ull;
+    int P = 2;
+    while (P < n) P <<= 1;
+    for (int k = 2; k <= P; k <<= 1) {
+      const bool up = (at & k) == 0;
+      for (int j = k >> 1; j >= 64; j >>= 1) {
+        __syncthreads();
+        g.sort[tid] = v;
+        __syncthreads();
+        const u64 o = g.sort[tid ^ j];
+        v = (o < v) == (((tid & j) == 0) == up) ? o : v;
+      }
+      v = s_sort_steps(v, min(k >> 1, 32), up, lane);
+    }
+    run = s_wave_scan(at < n ? s_weight(s_unkey(~(uint32_t)(v >> 32)), M, r.inv_t, a.S, g.tab).w : 0ull);
+    if (!one) {
+      __syncthreads();
+      if (lane == 63) g.wmass[wave] = run;
+      __syncthreads();
+      const u64 w = s_wave_scan(lane < 16 ? g.wmass[lane] : 0ull);
+      if (wave) run += s_lane(w, wave - 1);
+    }
+  };
+  // what thread i of the sorted list holds; the first place of it whose running sum reaches a target (or the last asked)
+  auto of_place = [&](u64 mine, int i) __attribute__((always_inline)) -> u64 {
+    if (one) return s_lane(mine, i);
+    __syncthreads();
+    if (tid == i) g.sum = mine;
+    __syncthreads();
+    return g.sum;
+  };
+  auto place_of = [&](u64 target, int most) __attribute__((always_inline)) -> int {
+    const u64 in = __builtin_amdgcn_ballot_w64(at < most && run >= target);
+    if (one) return in ? __builtin_ctzll(in) : most - 1;
+    if (tid == 0) g.bin = most - 1;
+    __syncthreads();
+    if (in && lane == __builtin_ctzll(in)) atomicMin(&g.bin, tid);
+    __syncthreads();
+    const int i = g.bin;
+    __syncthreads();
+    return i;
+  };
+  const float u = a.tokens ? a.u[(int64_t)(row / a.P) * a.ub] : 0.f;
+  auto p_target = [&](u64 Z) __attribute__((always_inline)) -> u64 {
+    const double goal = ceil((double)fmaxf(r.p, 0.f) * (double)Z);
+    return goal < 1.0 ? 1 : min((u64)goal, Z);
+  };
+  auto u_target = [&](u64 Z) __attribute__((always_inline)) -> u64 {
+    const double goal = floor(fmax((double)u, 0.0) * (double)Z);
+    return goal >= (double)Z ? Z : min((u64)goal + 1, Z);
+  };
+  // the smallest value of weight m or more: next to max + T ln m, found among its neighbours (more than 1: the largest value)
+  float least = -INFINITY;
+  if (r.m > 0.f) {
+    const float guess = fminf((float)((double)M + log((double)r.m) * (double)r.t), M);
+    if (!(fabsf(M) < INFINITY)) {
+      least = M;
+    } else if (guess > -INFINITY) {
+      least = M;
+      const uint32_t mine = min(s_key(guess) + (uint32_t)lane - 32u, s_key(M));
+      const u64 in = __builtin_amdgcn_ballot_w64(v_weight(s_unkey(mine), M, r.inv_t, g.tab) >= (double)r.m);
+      if (in) least = s_unkey(__builtin_amdgcn_readlane(mine, __builtin_ctzll(in)));
+    }
+  }
+  // ---- the row's bins, and their running sums: two a thread
+  auto clear = [&]() __attribute__((always_inline)) {
+    for (int i = tid; i < kSBins; i += kSThreads) {
+      g.mass[i] = 0;
+      g.count[i] = 0;
+    }
+    __syncthreads();
+  };
+  auto scan = [&](bool from_row) __attribute__((always_inline)) {
     u64 m[2];
     uint32_t c[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      m[i] = a.mass[(size_t)row * kSBins + 2 * tid + i];
-      c[i] = a.count[(size_t)row * kSBins + 2 * tid + i];
+      m[i] = from_row ? a.mass[(size_t)row * kSBins + 2 * tid + i] : g.mass[2 * tid + i];
+      c[i] = from_row ? a.count[(size_t)row * kSBins + 2 * tid + i] : g.count[2 * tid + i];
     }
-    const u64 im = s_wave_scan(m[0] + m[1], lane);
-    const uint32_t ic = (uint32_t)s_wave_scan(c[0] + c[1], lane);
+    u64 im = s_wave_scan(m[0] + m[1]);
+    uint32_t ic = s_wave_scan(c[0] + c[1]);
     if (lane == 63) {
       g.wmass[wave] = im;
       g.wcount[wave] = ic;
     }
     __syncthreads();
-    u64 bm = 0;
-    uint32_t bc = 0;
-    for (int w = 0; w < wave; ++w) {
-      bm += g.wmass[w];
-      bc += g.wcount[w];
+    const u64 wm = s_wave_scan(lane < 16 ? g.wmass[lane] : 0ull);
+    const uint32_t wc = s_wave_scan(lane < 16 ? g.wcount[lane] : 0u);
+    if (wave) {
+      im += s_lane(wm, wave - 1);
+      ic += __builtin_amdgcn_readlane(wc, wave - 1);
     }
-    g.mass[2 * tid + 1] = bm + im;
-    g.mass[2 * tid] = bm + im - m[1];
-    g.count[2 * tid + 1] = bc + ic;
-    g.count[2 * tid] = bc + ic - c[1];
+    g.mass[2 * tid + 1] = im;
+    g.mass[2 * tid] = im - m[1];
+    g.count[2 * tid + 1] = ic;
+    g.count[2 * tid] = ic - c[1];
     __syncthreads();
-  }
-  auto mass_below = [&](int b) -> u64 { return b > 0 ? g.mass[b - 1] : 0; };
-  auto count_below = [&](int b) -> uint32_t { return b > 0 ? g.count[b - 1] : 0; };
-  auto bin_of_mass = [&](u64 target) -> int {
+  };
+  auto mass_below = [&](int b) __attribute__((always_inline)) -> u64 { return b > 0 ? g.mass[b - 1] : 0; };
+  auto count_below = [&](int b) __attribute__((always_inline)) -> uint32_t { return b > 0 ? g.count[b - 1] : 0; };
+  auto bin_of_mass = [&](u64 target) __attribute__((always_inline)) -> int {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
       if (g.mass[2 * tid + i] >= target && mass_below(2 * tid + i) < target) g.bin = 2 * tid + i;
@@ -312,7 +591,7 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
     __syncthreads();
     return b;
   };
-  auto bin_of_count = [&](uint32_t target) -> int {
+  auto bin_of_count = [&](uint32_t target) __attribute__((always_inline)) -> int {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
       if (g.count[2 * tid + i] >= target && count_below(2 * tid + i) < target) g.bin = 2 * tid + i;
@@ -321,82 +600,191 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
     __syncthreads();
     return b;
   };
-  // ---- the tokens of bin b that a cut keeps: into the list; their number (the list holds the first kSList that came)
-  auto collect = [&](int b, const SampleKept& kept) -> int {
-    if (tid == 0) g.n = 0;
-    __syncthreads();
-    s_for_row(s, tid, kSThreads, s.n(), [&](int i, float x) {
-      if (s_bin(x, M, r.bins) == b && kept.has(b, x, i)) {
-        const int at = atomicAdd(&g.n, 1);
-        if (at < kSList) {
-          g.lx[at] = x;
-          g.li[at] = i;
-        }
-      }
-    });
-    __syncthreads();
-    return g.n;
+  // no token of the bins up to b is smaller (d: its distance in 1/32 octaves)
+  auto bound = [&](int b) __attribute__((always_inline)) -> float {
+    if (b >= kSBins - 1) return -INFINITY;
+    if (!(fabsf(M) < INFINITY)) return M;
+    const double d = b < kSFine ? b + 1.0 : kSFine + 32.0 * (b - kSFine + 1) + 1.0;
+    return (float)((double)M - d / r.inv_t - 1e-6 * fabs((double)M)) - 1e-37f;
   };
-  // f(index, value) of these n tokens, from the list or, where it does not hold them, from the row
-  auto for_bin = [&](int b, int n, const SampleKept& kept, auto&& f) {
-    if (n <= kSList) {
-      for (int i = tid; i < n; i += kSThreads) f(g.li[i], g.lx[i]);
-    } else {
-      s_for_row(s, tid, kSThreads, s.n(), [&](int i, float x) {
-        if (s_bin(x, M, r.bins) == b && kept.has(b, x, i)) f(i, x);
-      });
-    }
-  };
-  // ---- the token of bin b at which the running count or mass reaches target: (g.key, g.idx), with the bin's mass up to and
-  // with it in g.to_mass
-  auto border = [&](int b, const SampleKept& kept, u64 target, bool by_mass) {
-    const int n = collect(b, kept);
-    if (n <= 64) {
-      if (wave == 0) {
-        const bool there = lane < n;
-        const float x = there ? g.lx[lane] : 0.f;
-        const u64 me = there ? ((u64)~s_key(x) << 32) | (uint32_t)g.li[lane] : ~0ull;
-        const u64 w = there ? s_mass(x, M, r.inv_t, a.unit, g.tab) : 0, t = by_mass ? w : (there ? 1 : 0);
-        u64 run = 0, runw = 0;
-        for (int j = 0; j < n; ++j) {
-          const bool le = __shfl(me, j) <= me;
-          const u64 wj = __shfl(w, j);
-          run += le ? (by_mass ? wj : 1) : 0;
-          runw += le ? wj : 0;
-        }
-        if (there && run >= target && run - t < target) {
-          g.key = s_key(x);
-          g.idx = g.li[lane];
-          g.to_mass = runw;
-        }
-      }
+
+  // ---- Where all that is kept is among few tokens: these are sorted, and the rest is looked up in the running sum. For a small
+  // top-k the k-th largest token is no further than the k-th largest group's bin (fewer groups than k: than any), in bins of
+  // its own that take no 64-bit operations.
+  float floor_x = -INFINITY;
+  bool bounded = true;
+  u64 Z_row = 0;
+  if (r.few) {
+    for (int i = tid; i < kSBins; i += kSThreads) g.count[i] = 0;
+    __syncthreads();
+    const float per = fminf((float)r.inv_t, 1e30f);
+    auto bin = [&](float x) __attribute__((always_inline)) {
+      const float y = (M - x) * per;
+      return x == M ? 0 : y < (float)(kSBins - 1) ? (int)y : kSBins - 1;
+    };
+#pragma unroll
+    for (int i = 0; i < kSHeld; ++i)
+      if (tid + kSThreads * i < G) atomicAdd(&g.count[bin(held[i])], 1u);
+    for (int i = tid + kSHeld * kSThreads; i < G; i += kSThreads) atomicAdd(&g.count[bin(gmax[i])], 1u);
+    __syncthreads();
+    if (G >= r.k) {
+      const uint32_t c0 = g.count[2 * tid], c1 = g.count[2 * tid + 1];
+      uint32_t ic = s_wave_scan(c0 + c1);
+      if (lane == 63) g.wcount[wave] = ic;
       __syncthreads();
+      const uint32_t wc = s_wave_scan(lane < 16 ? g.wcount[lane] : 0u);
+      if (wave) ic += __builtin_amdgcn_readlane(wc, wave - 1);
+      if (ic >= (uint32_t)r.k && ic - c0 - c1 < (uint32_t)r.k) g.bin = ic - c1 >= (uint32_t)r.k ? 2 * tid : 2 * tid + 1;
+      __syncthreads();
+      const int b = g.bin;
+      if (b < kSBins - 1)
+        floor_x = fabsf(M) < INFINITY ? (float)((double)M - (b + 1.001) / (double)per - 1e-6 * fabs((double)M)) - 1e-37f : M;
+      __syncthreads();
+    }
+  } else {
+    scan(true);
+    Z_row = g.mass[kSBins - 1];
+    if (r.k > 0) floor_x = bound(bin_of_count((uint32_t)r.k));
+    else if (r.p < 1.f) floor_x = bound(bin_of_mass(p_target(Z_row)));
+    else bounded = false;
+  }
+  if (least > floor_x && !(r.k > 0 && r.p < 1.f)) {  // (top-p of top-k takes all of top-k's sum)
+    floor_x = least;
+    bounded = true;
+  }
+  if (bounded) {
+    const int n = collect(std::true_type{}, floor_x, M, 0, ~0ull, kSSort) ? gather(0, ~0ull) : kSSort + 1;
+    if (n <= kSSort) {
+      sort(n);
+      int K = r.k > 0 ? min(r.k, n) : n;
+      if (r.p < 1.f) K = place_of(p_target(r.k > 0 ? of_place(run, K - 1) : Z_row), K) + 1;
+      if (r.m > 0.f) {  // (sorted: those of at least `least` come first)
+        int c = __popcll(__builtin_amdgcn_ballot_w64(at < K && s_unkey(~(uint32_t)(v >> 32)) >= least));
+        if (!one) {
+          if (tid == 0) g.n = 0;
+          __syncthreads();
+          if (lane == 0) atomicAdd(&g.n, c);
+          __syncthreads();
+          c = g.n;
+        }
+        K = max(c, 1);
+      }
+      const u64 Z = of_place(run, K - 1);
+      if (tid == K - 1) a.cut[row] = {__builtin_ldexp(1.0, a.S) / (double)Z, M, s_unkey(~(uint32_t)(v >> 32)), (int)(uint32_t)v, 0};
+      if (a.tokens) {
+        const int i = place_of(u_target(Z), K);
+        if (tid == i) a.tokens[row] = (int)(uint32_t)v;
+      }
       return;
     }
-    // digits of 8 bits: four of the key, from the largest, then three of the index, from the smallest
-    u64 ahead = 0, aheadw = 0;
-    uint32_t key = 0, idx = 0;
-    for (int level = 0; level < 7; ++level) {
+    if (r.few) {  // many tokens of about one value: the bins, of the tokens themselves
+      clear();
+      traverse(std::integral_constant<int, 1>{}, std::false_type{}, floor_x, M, G, [&](bool in, int, float x) __attribute__((always_inline)) {
+        if (!in) return;
+        const SampleWeight w = s_weight(x, M, r.inv_t, a.S, g.tab);
+        const int b = s_bin(w.n);
+        atomicAdd(&g.count[b], 1u);
+        atomicAdd(&g.mass[b], w.w);
+      });
+      scan(false);
+    }
+  }
+
+  // ---- Otherwise the bin of each border, and its tokens. The smallest value of a bin up to b: six bits a step, a lane each
+  auto smallest = [&](int b) __attribute__((always_inline)) -> float {
+    uint32_t key = s_key(-INFINITY);  // the largest known to be below
+    const uint32_t top = s_key(M);
+    if (s_bin(-INFINITY, M, r.inv_t) <= b) return -INFINITY;
+    for (int sh = 26; sh > -6; sh -= 6) {
+      const uint32_t step = sh >= 0 ? 1u << sh : 1u;
+      const u64 at64 = (u64)key + (u64)(lane + 1) * step;
+      const uint32_t to = (uint32_t)(at64 < top ? at64 : top);
+      const u64 in = __builtin_amdgcn_ballot_w64(s_bin(s_unkey(to), M, r.inv_t) <= b);
+      const u64 below = (u64)key + (u64)__builtin_ctzll(in) * step;  // (the last lane's value is inside)
+      key = (uint32_t)(below < top ? below : top - 1);
+    }
+    return s_unkey(key + 1);
+  };
+  float lo = 0.f, hi = 0.f;  // bin b's smallest and largest value
+  auto in_bin = [&](int b) __attribute__((always_inline)) {
+    lo = smallest(b);
+    hi = b > 0 ? s_unkey(s_key(smallest(b - 1)) - 1) : M;
+  };
+  auto value_of = [&](u64 bits) __attribute__((always_inline)) -> float { return s_unkey(~(uint32_t)(bits >> 32)); };
+  // What is kept so far: the tokens up to these bits (as listed), and their mass. Top-k, top-p, then (behind min-p) the draw: each
+  // the token of a bin at which the running count or mass reaches a target.
+  u64 kept = ~0ull, Z = g.mass[kSBins - 1];
+  // (three copies: as a loop it held what they share in registers, more than there are)
+  auto cut = [&](auto step_of) __attribute__((always_inline)) {
+    constexpr int step = decltype(step_of)::value;
+    int b;
+    u64 target;
+    const bool by_mass = step > 0;
+    if (step == 0) {
+      if (r.k <= 0 || g.count[kSBins - 1] < (uint32_t)r.k) return;  // (fewer than that are of weight m)
+      b = bin_of_count((uint32_t)r.k);
+      target = (uint32_t)r.k - count_below(b);
+    } else if (step == 1) {
+      if (!(r.p < 1.f)) return;
+      target = p_target(Z);
+      b = bin_of_mass(target);
+      target -= mass_below(b);
+    } else {
+      const u64 enough = least > -INFINITY ? ((u64)~s_key(least) << 32) | 0xFFFFFFFFu : ~0ull;  // all of weight m
+      if (enough < kept) {
+        b = s_bin(least, M, r.inv_t);
+        if (tid == 0) g.to_mass = 0;
+        in_bin(b);
+        traverse(std::integral_constant<int, 1>{}, std::false_type{}, fmaxf(lo, least), hi, G, [&](bool in, int, float x) __attribute__((always_inline)) {
+          if (in) atomicAdd(&g.to_mass, s_weight(x, M, r.inv_t, a.S, g.tab).w);
+        });
+        kept = enough;
+        Z = mass_below(b) + g.to_mass;
+        __syncthreads();
+      }
+      if (tid == 0)
+        a.cut[row] = {__builtin_ldexp(1.0, a.S) / (double)Z, M, kept == ~0ull ? -INFINITY : value_of(kept), (int)(uint32_t)kept, 0};
+      if (!a.tokens) return;
+      target = u_target(Z);
+      b = bin_of_mass(target);
+      target -= mass_below(b);
+    }
+    u64 token = 0;
+    in_bin(b);
+    u64 first = (u64)~s_key(hi) << 32, last = min(((u64)~s_key(lo) << 32) | 0xFFFFFFFFu, kept), ahead = 0, aheadw = 0;
+    bool lists = false;  // whether the waves' lists hold what is first to last
+    // (each turn takes 8 of the 64 bits, and 512 neighbouring ones fit any list: done in 9 turns, and bounded in any case)
+    for (int turn = 0; turn < 10; ++turn) {
+      // narrowed by 256 (a digit's running sums; ahead, aheadw: count or mass, and mass, in front) until the rest can be sorted
+      if (!lists) lists = collect(std::false_type{}, value_of(last), value_of(first), first, last, G);
+      const int n = lists ? gather(first, last) : kSSort + 1;
+      if (n <= kSSort) {
+        sort(n);
+        const int i = by_mass ? place_of(target - ahead, n) : (int)(target - ahead) - 1;
+        token = of_place(v, i);
+        Z = mass_below(b) + aheadw + of_place(run, i);
+        __syncthreads();
+        break;
+      }
+      const int shift = max(56 - __builtin_clzll((last - first) | 1), 0);
       for (int i = tid; i < 256; i += kSThreads) {
         g.hmass[i] = 0;
         g.hcount[i] = 0;
       }
       __syncthreads();
-      for_bin(b, n, kept, [&](int i, float x) {
-        const uint32_t d = ~s_key(x);
-        uint32_t at;
-        if (level < 4) {
-          if (level > 0 && (d >> (32 - 8 * level)) != key) return;
-          at = (d >> (24 - 8 * level)) & 255;
-        } else {
-          const int l = level - 4;
-          if (d != key || (l > 0 && ((uint32_t)i >> (24 - 8 * l)) != idx)) return;
-          at = ((uint32_t)i >> (16 - 8 * l)) & 255;
-        }
-        atomicAdd(&g.hcount[at], 1u);
-        atomicAdd(&g.hmass[at], s_mass(x, M, r.inv_t, a.unit, g.tab));
-      });
-      __syncthreads();
+      auto count = [&](u64 bits) __attribute__((always_inline)) {
+        if (bits < first || bits > last) return;
+        atomicAdd(&g.hcount[(bits - first) >> shift], 1u);
+        atomicAdd(&g.hmass[(bits - first) >> shift], s_weight(value_of(bits), M, r.inv_t, a.S, g.tab).w);
+      };
+      if (lists) {
+        for (int l = lane; l < mine_n; l += 64) count(g.list[wave][l]);
+        __syncthreads();
+      } else {
+        traverse(std::integral_constant<int, 1>{}, std::false_type{}, value_of(last), value_of(first), G, [&](bool in, int i, float x) __attribute__((always_inline)) {
+          if (in) count(((u64)~s_key(x) << 32) | (uint32_t)i);
+        });
+      }
       if (wave == 0) {
         u64 t[4], w[4], st = 0, sw = 0;
 #pragma unroll
@@ -406,94 +794,31 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
           st += t[e];
           sw += w[e];
         }
-        u64 run = ahead + s_wave_scan(st, lane) - st, runw = aheadw + s_wave_scan(sw, lane) - sw;
+        u64 upto = ahead + s_wave_scan(st) - st, uptow = aheadw + s_wave_scan(sw) - sw;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if (run < target && run + t[e] >= target) {
+          if (upto < target && upto + t[e] >= target) {
             g.digit = 4 * lane + e;
-            g.sum = run;
-            g.to_mass = level == 6 ? runw + w[e] : runw;
+            g.sum = upto;
+            g.to_mass = uptow;
           }
-          run += t[e];
-          runw += w[e];
+          upto += t[e];
+          uptow += w[e];
         }
       }
       __syncthreads();
       ahead = g.sum;
       aheadw = g.to_mass;
-      if (level < 4) key = (key << 8) | g.digit;
-      else idx = (idx << 8) | g.digit;
+      first = min(first + ((u64)(g.digit & 255) << shift), last);
+      last = min(last, first + (((u64)1 << shift) - 1));
       __syncthreads();
     }
-    if (tid == 0) {
-      g.key = ~key;
-      g.idx = (int)idx;
-    }
-    __syncthreads();
+    if (step == 2 && tid == 0) a.tokens[row] = (int)(uint32_t)token;
+    kept = token;
   };
-
-  SampleKept kept{kSBins - 1, 0, 0x7fffffff};
-  u64 Z = g.mass[kSBins - 1];
-  if (r.k > 0) {
-    const int b = bin_of_count((uint32_t)r.k);
-    if (g.count[b] == (uint32_t)r.k) {
-      kept.b = b;
-      Z = g.mass[b];
-    } else {
-      border(b, kept, (uint32_t)r.k - count_below(b), false);
-      kept = {b, g.key, g.idx};
-      Z = mass_below(b) + g.to_mass;
-      __syncthreads();
-    }
-  }
-  if (r.p < 1.f) {
-    const double goal = ceil((double)fmaxf(r.p, 0.f) * (double)Z);
-    const u64 target = goal < 1.0 ? 1 : min((u64)goal, Z);
-    const int b = bin_of_mass(target);
-    if (b < kept.b && count_below(b) + 1 == g.count[b]) {
-      kept = {b, 0, 0x7fffffff};
-      Z = g.mass[b];
-    } else {
-      border(b, kept, target - mass_below(b), true);
-      kept = {b, g.key, g.idx};
-      Z = mass_below(b) + g.to_mass;
-      __syncthreads();
-    }
-  }
-  if (r.m > 0.f) {
-    // the smallest value of weight m or more: next to max + T ln m, found among its neighbours (more than 1: the largest value)
-    const float guess = fminf((float)((double)M + log((double)r.m) * (double)r.t), M);
-    uint32_t key = s_key(M);
-    if (fabsf(M) < INFINITY && guess > -INFINITY) {
-      const uint32_t mine = min(s_key(guess) + (uint32_t)lane - 32u, key);
-      const u64 in = __builtin_amdgcn_ballot_w64(v_weight(s_unkey(mine), M, r.inv_t, g.tab) >= (double)r.m);
-      if (in) key = __shfl(mine, __builtin_ctzll(in));
-    } else if (fabsf(M) < INFINITY) {
-      key = 0;
-    }
-    const int b = key ? s_bin(s_unkey(key), M, r.bins) : kSBins;
-    if (b < kept.b || (b == kept.b && key > kept.key)) {
-      const int n = g.count[b] == count_below(b) ? 0 : collect(b, kept);
-      if (tid == 0) g.sum = 0;
-      __syncthreads();
-      if (n)
-        for_bin(b, n, kept, [&](int, float x) {
-          if (s_key(x) >= key) atomicAdd(&g.sum, s_mass(x, M, r.inv_t, a.unit, g.tab));
-        });
-      __syncthreads();
-      kept = {b, key, b == kept.b && key == kept.key ? kept.idx : 0x7fffffff};
-      Z = mass_below(b) + g.sum;
-      __syncthreads();
-    }
-  }
-  if (tid == 0) a.cut[row] = {a.unit / (double)Z, M, kept.b, kept.key, kept.idx};
-  if (!a.tokens) return;
-  const float u = a.u[(int64_t)(row / a.P) * a.ub];
-  const double goal = floor(fmax((double)u, 0.0) * (double)Z);
-  const u64 target = goal >= (double)Z ? Z : min((u64)goal + 1, Z);
-  const int b = bin_of_mass(target);
-  border(b, kept, target - mass_below(b), true);
-  if (tid == 0) a.tokens[row] = g.idx;
+  cut(std::integral_constant<int, 0>{});
+  cut(std::integral_constant<int, 1>{});
+  cut(std::integral_constant<int, 2>{});
 }
 
 template <int OUT>
@@ -502,10 +827,12 @@ __global__ __launch_bounds__(256) void sample_write_kernel(SampleArgs a) {
   const SampleRow r = s_row(a, row);
   const SampleQuads s(r.x, a.V);
   const SampleCut c = a.cut[row];
-  const SampleKept kept{c.b, c.key, c.idx};
+  const SampleKept kept{c.x, (uint32_t)c.idx};
   __shared__ double tab[kVTab];
-  exp2_table(tab, tid);
-  __syncthreads();
+  if (OUT == kSampleProbs) {
+    exp2_table(tab, tid);
+    __syncthreads();
+  }
   float* o = a.out + (int64_t)row * a.V;
   const bool vec = (((uintptr_t)o - 4 * (uintptr_t)s.ahead) & 15) == 0;
 #pragma unroll
@@ -514,12 +841,20 @@ __global__ __launch_bounds__(256) void sample_write_kernel(SampleArgs a) {
     if (q >= s.n()) continue;
     const f32x4 x = s.load(q);
     const int i = 4 * q - s.ahead;
-    f32x4 y;
+    bool in[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const bool in = kept.has(s_bin(x[e], c.max, r.bins), x[e], i + e);
-      if (OUT == kSampleLogits) y[e] = in ? x[e] : -INFINITY;
-      else y[e] = in ? (float)(v_weight(x[e], c.max, r.inv_t, tab) * c.scale) : 0.f;
+    for (int e = 0; e < 4; ++e) in[e] = kept.has(x[e], i + e);
+    f32x4 y;
+    if constexpr (OUT == kSampleLogits) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = in[e] ? x[e] : -INFINITY;
+    } else {
+      y = zero4();
+      if (in[0] || in[1] || in[2] || in[3]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (in[e]) y[e] = (float)(v_weight(x[e], c.max, r.inv_t, tab) * c.scale);
+      }
     }
     if (vec && i >= 0 && i + 3 < a.V) {
       *reinterpret_cast<f32x4*>(o + i) = y;
@@ -539,7 +874,7 @@ extern "C" size_t q35_sample_tokens_workspace_bytes(int64_t B, int64_t P, int64_
   using namespace q35;
   if (B <= 0 || P <= 0 || V <= 0 || B > 65535 || P > 65535 || B * P > 65535 || V > kSMaxV) return 0;
   const size_t rows = (size_t)B * P;
-  return rows * (kSBins * (sizeof(u64) + sizeof(uint32_t)) + sizeof(SampleCut) + ((s_chunks(V) + 3) & ~3) * sizeof(float));
+  return rows * (kSBins * (sizeof(u64) + sizeof(uint32_t)) + sizeof(SampleCut) + s_chunks(V) * 257 * sizeof(float));
 }
 
 extern "C" int q35_sample_tokens(const float* logits, int64_t l_sb, int64_t l_sp, const float* u, int64_t u_sb,
@@ -564,18 +899,22 @@ extern "C" int q35_sample_tokens(const float* logits, int64_t l_sb, int64_t l_sp
   a.u = u, a.ub = u_sb, a.V = (int)V, a.C = (int)s_chunks(V);
   int bits = 0;
   while (((int64_t)1 << bits) < V) ++bits;
-  a.unit = __builtin_ldexp(1.0, 62 - bits);
+  a.S = std::min(62 - bits, 50);
   a.mass = (u64*)workspace;
   a.count = (uint32_t*)(a.mass + rows * kSBins);
   a.cut = (SampleCut*)(a.count + rows * kSBins);
   a.cmax = (float*)(a.cut + rows);
+  a.gmax = a.cmax + rows * a.C;
   a.tokens = tokens, a.out = out;
   const int64_t nq = (V + 3) / 4 + 1;
   a.R = (int)std::max<int64_t>(1, std::min<int64_t>((1024 + rows - 1) / rows, (nq + 1023) / 1024));
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const dim3 chunks(a.C, (unsigned)rows);
   hipLaunchKernelGGL(sample_max_kernel, chunks, dim3(256), 0, st, a);
-  hipLaunchKernelGGL(sample_hist_kernel, dim3(a.R, (unsigned)rows), dim3(256), 0, st, a);
+  // (none of its blocks has work where one small top-k holds for all rows, or the argmax)
+  const int64_t k = temperature > 0.f ? top_k : 1;  // (as s_row has it)
+  if (temperatures || top_ks || k <= 0 || k >= V || k > kSFew)
+    hipLaunchKernelGGL(sample_hist_kernel, dim3(a.R, (unsigned)rows), dim3(256), 0, st, a);
   hipLaunchKernelGGL(sample_pick_kernel, dim3((unsigned)rows), dim3(kSThreads), 0, st, a);
   if (out_kind == kSampleProbs) hipLaunchKernelGGL(sample_write_kernel<kSampleProbs>, chunks, dim3(256), 0, st, a);
   else if (out_kind == kSampleLogits) hipLaunchKernelGGL(sample_write_kernel<kSampleLogits>, chunks, dim3(256), 0, st, a);
