@@ -277,7 +277,7 @@ struct SamplePick {
 };
 
 // Lane exchanges on the vector ALU. A ds_bpermute takes 100 cycles, a scan or a step of a sort of 64-bit values two of them: the
-// pick of three rows of top-k 20 16.2 -> PICK us.
+// pick of three rows of top-k 20 16.2 -> 12.7 us.
 template <int CTRL, int ROWS> __device__ __forceinline__ u64 s_dpp_or_0(u64 v) {
   const uint32_t lo = __builtin_amdgcn_update_dpp(0, (uint32_t)v, CTRL, ROWS, 0xF, true);
   const uint32_t hi = __builtin_amdgcn_update_dpp(0, (uint32_t)(v >> 32), CTRL, ROWS, 0xF, true);
@@ -336,6 +336,9 @@ __device__ __forceinline__ u64 s_sort_steps(u64 v, int from, bool up, int lane) 
   return s_sort_step<1>(v, up, lane);
 }
 
+// x[e] of four in registers
+template <typename X> __device__ __forceinline__ auto pick4(const X& x, int e) { return e < 2 ? (e ? x[1] : x[0]) : e == 2 ? x[2] : x[3]; }
+
 // Whether a token is kept: up to (x, idx) in the order.
 struct SampleKept {
   float x;
@@ -362,19 +365,20 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
     }
     return;
   }
-  // ---- f(in, index, value) by whole waves, for the row's tokens, `in` for those of lo to hi: of the groups whose maximum reaches
+  // ---- f(in, index, values) by whole waves, for quads of the row, in[e] for tokens of lo to hi: of the groups whose maximum reaches
   // lo, or, where most of them do, of all. False, and not all of them seen, as soon as more than `most` groups do.
   // Loads in flight of a wave: D in a pass over all (150 K tokens are otherwise a chain of their latencies), L of listed groups.
   auto traverse = [&](auto loads, auto still_held, float lo, float hi, int most, auto&& f) __attribute__((always_inline)) -> bool {
     constexpr int D = decltype(loads)::value, L = D > 1 ? 4 : 1;
-    auto quad = [&](bool there, int q, const f32x4& v) __attribute__((always_inline)) {
+    auto quad = [&](auto whole, bool there, int q, const f32x4& v) __attribute__((always_inline)) {
       const int i = 4 * q - s.ahead;
       bool in[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) in[e] = there && v[e] >= lo && v[e] <= hi && i + e >= 0 && i + e < a.V;
-      if (__builtin_amdgcn_ballot_w64(in[0] | in[1] | in[2] | in[3]) == 0) return;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) f(in[e], i + e, v[e]);
+      for (int e = 0; e < 4; ++e) {
+        in[e] = v[e] >= lo && v[e] <= hi;
+        if constexpr (!decltype(whole)::value) in[e] = in[e] && there && i + e >= 0 && i + e < a.V;
+      }
+      if (__builtin_amdgcn_ballot_w64(in[0] | in[1] | in[2] | in[3])) f(in, i, v);
     };
     int seen = 0;
     for (int g0 = 0; g0 < G; g0 += kSHeld * kSThreads) {
@@ -412,7 +416,7 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
             v[u] = q[u] < nq ? s.load(q[u]) : zero4();
           }
 #pragma unroll
-          for (int u = 0; u < L; ++u) quad(q[u] < nq, q[u], v[u]);
+          for (int u = 0; u < L; ++u) quad(std::false_type{}, q[u] < nq, q[u], v[u]);
         }
       } else {
         const int last = min(4 * (g0 + here), nq);
@@ -421,32 +425,42 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
           if (q0 >= s.whole_first() && q0 + 63 + (D - 1) * kSThreads < min(last, s.whole_last())) {
 #pragma unroll
             for (int u = 0; u < D; ++u) v[u] = s.whole(q0 + lane + u * kSThreads);
+#pragma unroll
+            for (int u = 0; u < D; ++u) quad(std::true_type{}, true, q0 + lane + u * kSThreads, v[u]);
           } else {
-#pragma unroll
-            for (int u = 0; u < D; ++u) v[u] = q0 + lane + u * kSThreads < last ? s.load(q0 + lane + u * kSThreads) : zero4();
+#pragma unroll 1
+            for (int u = 0; u < D; ++u) {
+              const int q = q0 + lane + u * kSThreads;
+              quad(std::false_type{}, q < last, q, q < last ? s.load(q) : zero4());
+            }
           }
-#pragma unroll
-          for (int u = 0; u < D; ++u) quad(q0 + lane + u * kSThreads < last, q0 + lane + u * kSThreads, v[u]);
         }
       }
       __syncthreads();
     }
     return true;
   };
-  // The tokens of lo to hi whose bits are first to last into the waves' lists (mine_n of this one's); false where they do not
-  // fit, or traverse() gave up.
+  // The tokens of lo to hi into the waves' lists (mine_n of this one's), only those whose bits are first to last where `exact`;
+  // false where they do not fit, or traverse() gave up.
   int mine_n = 0;
-  auto collect = [&](auto still_held, float lo, float hi, u64 first, u64 last, int most) __attribute__((always_inline)) -> bool {
+  auto collect = [&](auto still_held, float lo, float hi, bool exact, u64 first, u64 last, int most) __attribute__((always_inline)) -> bool {
     mine_n = 0;
     if (tid == 0) g.full = 0;
-    const bool all = traverse(std::integral_constant<int, 4>{}, still_held, lo, hi, most, [&](bool in, int i, float x) __attribute__((always_inline)) {
-      const u64 bits = ((u64)~s_key(x) << 32) | (uint32_t)i;
-      const bool ours = in && bits >= first && bits <= last;
-      const u64 mask = __builtin_amdgcn_ballot_w64(ours);
-      if (mask == 0) return;
-      const int to = mine_n + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
-      if (ours && to < kSSeg) g.list[wave][to] = bits;
-      mine_n += __popcll(mask);
+    const bool all = traverse(std::integral_constant<int, 6>{}, still_held, lo, hi, most, [&](bool (&in)[4], int i, const f32x4& v) __attribute__((always_inline)) {
+      if (!decltype(still_held)::value && exact) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const u64 bits = ((u64)~s_key(v[e]) << 32) | (uint32_t)(i + e);
+          in[e] = in[e] && bits >= first && bits <= last;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const u64 mask = __builtin_amdgcn_ballot_w64(in[e]);
+        const int to = __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, mine_n));
+        if (in[e] && to < kSSeg) g.list[wave][to] = ((u64)__float_as_uint(v[e]) << 32) | (uint32_t)(i + e);
+        mine_n += __popcll(mask);
+      }
     });
     if (lane == 0 && mine_n > kSSeg) g.full = 1;
     __syncthreads();
@@ -454,12 +468,16 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
     __syncthreads();
     return fits;
   };
+  auto listed = [&](int l) __attribute__((always_inline)) -> u64 {
+    const u64 t = g.list[wave][l];
+    return ((u64)~s_key(__uint_as_float((uint32_t)(t >> 32))) << 32) | (uint32_t)t;
+  };
   // Of the waves' lists those whose bits are first to last, together, to be sorted: how many (the first kSSort are there).
   auto gather = [&](u64 first, u64 last) __attribute__((always_inline)) -> int {
     if (tid == 0) g.n = 0;
     __syncthreads();
     for (int l0 = 0; l0 < mine_n; l0 += 64) {
-      const u64 bits = l0 + lane < mine_n ? g.list[wave][l0 + lane] : 0;
+      const u64 bits = l0 + lane < mine_n ? listed(l0 + lane) : 0;
       const bool in = l0 + lane < mine_n && bits >= first && bits <= last;
       const u64 mask = __builtin_amdgcn_ballot_w64(in);
       int base = 0;
@@ -653,7 +671,7 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
     bounded = true;
   }
   if (bounded) {
-    const int n = collect(std::true_type{}, floor_x, M, 0, ~0ull, kSSort) ? gather(0, ~0ull) : kSSort + 1;
+    const int n = collect(std::true_type{}, floor_x, M, false, 0, ~0ull, kSSort) ? gather(0, ~0ull) : kSSort + 1;
     if (n <= kSSort) {
       sort(n);
       int K = r.k > 0 ? min(r.k, n) : n;
@@ -679,12 +697,15 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
     }
     if (r.few) {  // many tokens of about one value: the bins, of the tokens themselves
       clear();
-      traverse(std::integral_constant<int, 1>{}, std::false_type{}, floor_x, M, G, [&](bool in, int, float x) __attribute__((always_inline)) {
-        if (!in) return;
-        const SampleWeight w = s_weight(x, M, r.inv_t, a.S, g.tab);
-        const int b = s_bin(w.n);
-        atomicAdd(&g.count[b], 1u);
-        atomicAdd(&g.mass[b], w.w);
+      traverse(std::integral_constant<int, 1>{}, std::false_type{}, floor_x, M, G, [&](bool (&in)[4], int, const f32x4& x) __attribute__((always_inline)) {
+#pragma unroll 1
+        for (int e = 0; e < 4; ++e) {
+          if (!pick4(in, e)) continue;
+          const SampleWeight w = s_weight(pick4(x, e), M, r.inv_t, a.S, g.tab);
+          const int b = s_bin(w.n);
+          atomicAdd(&g.count[b], 1u);
+          atomicAdd(&g.mass[b], w.w);
+        }
       });
       scan(false);
     }
@@ -735,8 +756,10 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
         b = s_bin(least, M, r.inv_t);
         if (tid == 0) g.to_mass = 0;
         in_bin(b);
-        traverse(std::integral_constant<int, 1>{}, std::false_type{}, fmaxf(lo, least), hi, G, [&](bool in, int, float x) __attribute__((always_inline)) {
-          if (in) atomicAdd(&g.to_mass, s_weight(x, M, r.inv_t, a.S, g.tab).w);
+        traverse(std::integral_constant<int, 1>{}, std::false_type{}, fmaxf(lo, least), hi, G, [&](bool (&in)[4], int, const f32x4& x) __attribute__((always_inline)) {
+#pragma unroll 1
+          for (int e = 0; e < 4; ++e)
+            if (pick4(in, e)) atomicAdd(&g.to_mass, s_weight(pick4(x, e), M, r.inv_t, a.S, g.tab).w);
         });
         kept = enough;
         Z = mass_below(b) + g.to_mass;
@@ -756,7 +779,7 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
     // (each turn takes 8 of the 64 bits, and 512 neighbouring ones fit any list: done in 9 turns, and bounded in any case)
     for (int turn = 0; turn < 10; ++turn) {
       // narrowed by 256 (a digit's running sums; ahead, aheadw: count or mass, and mass, in front) until the rest can be sorted
-      if (!lists) lists = collect(std::false_type{}, value_of(last), value_of(first), first, last, G);
+      if (!lists) lists = collect(std::false_type{}, value_of(last), value_of(first), turn > 0, first, last, G);
       const int n = lists ? gather(first, last) : kSSort + 1;
       if (n <= kSSort) {
         sort(n);
@@ -778,11 +801,13 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
         atomicAdd(&g.hmass[(bits - first) >> shift], s_weight(value_of(bits), M, r.inv_t, a.S, g.tab).w);
       };
       if (lists) {
-        for (int l = lane; l < mine_n; l += 64) count(g.list[wave][l]);
+        for (int l = lane; l < mine_n; l += 64) count(listed(l));
         __syncthreads();
       } else {
-        traverse(std::integral_constant<int, 1>{}, std::false_type{}, value_of(last), value_of(first), G, [&](bool in, int i, float x) __attribute__((always_inline)) {
-          if (in) count(((u64)~s_key(x) << 32) | (uint32_t)i);
+        traverse(std::integral_constant<int, 1>{}, std::false_type{}, value_of(last), value_of(first), G, [&](bool (&in)[4], int i, const f32x4& x) __attribute__((always_inline)) {
+#pragma unroll 1
+          for (int e = 0; e < 4; ++e)
+            if (pick4(in, e)) count(((u64)~s_key(pick4(x, e)) << 32) | (uint32_t)(i + e));
         });
       }
       if (wave == 0) {
