@@ -13,7 +13,8 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 // ---------------------------------------------------------------------------------------------------------------
-// Rows in 8 bits, one block a row, held in registers: PER quads of values a thread.
+// Rows in 8 bits, one block a row, held in registers: PER quads of values a thread, so that memory is passed over once. 16384
+// rows of 3584 fp32 values take 60 us, 4.9 TB/s of the 294 MB read and written (a large copy reaches 5.2).
 
 // rint(x / s), half to even: x, s exact, |x / s| <= 127.5. The remainder settles what the product with 1 / s left undecided.
 __device__ __forceinline__ int i8_code(double x, double s, double inv) {
@@ -129,9 +130,15 @@ static int rows_i8_launch(Tx* x, int64_t ldx, const float* y, int64_t ldy, const
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Tiles of BM x BN outputs, a wave 32 MT x 32 NT of them. Rows of q and W go to LDS by DMA in stages of 64 inputs (rows of 64
-// bytes, 16-byte chunk c at c ^ ((row >> 2) & 3): 16 consecutive lanes of a fragment read fall in distinct slots).
-constexpr int kIK = 64, kINS = 4;
+// Tiles of BM x BN outputs, a wave 32 MT x 32 NT of them. Rows of q and W go to LDS by DMA in stages of 128 inputs, whole cache
+// lines (rows of 128 bytes, 16-byte chunk c at c ^ ((row >> 1) & 7): 16 consecutive lanes of a fragment read fall in distinct
+// slots). Stages of 64 inputs fetched half lines and took 1.4 times as long.
+//
+// 16384 rows of 3584 inputs by 1024 outputs, tiles of 256 x 256 (8 waves of 128 x 64): 63 us alone, 1.9 P operations a second (a
+// library product of 8192^3 reaches 2.05); the matrix units bound it, then the 64 MB of results, which leave at the end as all
+// blocks run in step. 6144 rows of 1024 inputs by 7168 outputs with SwiGLU: 73 us, 1.23 P; 672 tiles are 2.6 a CU, and 88 MB
+// leave. 333 rows of 3584 by 1024 (352 tiles of 32): 7.2 us; 32 rows of 1024 by 5120 3.2 us: latency of a stage from memory.
+constexpr int kIK = 128;  // inputs of a stage
 
 struct GemmI8Args {
   const int8_t* q;
@@ -147,49 +154,107 @@ struct GemmI8Args {
   GemmCap cap;
 };
 
-// lane of a 1 KB copy of 16 rows -> its row and 16-byte chunk
-__device__ __forceinline__ int i8_copy_row(int lane) { return lane >> 2; }
-__device__ __forceinline__ int i8_copy_chunk(int lane) { return (lane & 3) ^ ((lane >> 4) & 3); }
+// What becomes of CL scaled sums of row m from column n on (CL even columns are CL / 2 gate and up pairs).
+template <int EPI, int CL>
+__device__ __forceinline__ void gemm_i8_finish(const GemmI8Args& p, int m, int n, const float (&v)[CL], bool vec, bool pushes_here) {
+  if constexpr (EPI == kGemmSwiglu) {
+    constexpr int NA = CL / 2;
+    typedef float fvec __attribute__((ext_vector_type(NA)));
+    const int neuron = n >> 1, I = p.N >> 1;
+    fvec a;
+#pragma unroll
+    for (int e = 0; e < NA; ++e) a[e] = silu_f(v[2 * e]) * v[2 * e + 1];
+    if (pushes_here) {
+      const int row = gemm_push_row(m, p.T);
+      for (int k = 0; k < p.npush; ++k)
+#pragma unroll
+        for (int e = 0; e < NA; ++e) a[e] = gemm_push(p.pushes + k, neuron + e, row, a[e]);
+    }
+    float* dst = p.y + (int64_t)m * p.ldy + neuron;
+    if (vec && neuron + NA <= I) {
+      *reinterpret_cast<fvec*>(dst) = a;
+    } else {
+#pragma unroll
+      for (int e = 0; e < NA; ++e)
+        if (neuron + e < I) dst[e] = a[e];
+    }
+#pragma unroll
+    for (int e = 0; e < NA; ++e)
+      if (neuron + e < I) gemm_capture(p.cap, m, p.T, neuron + e, a[e]);
+  } else {
+    static_assert(CL == 4, "one store");
+    float* dst = p.y + (int64_t)m * p.ldy + n;
+    if (vec && n + 4 <= p.N) {
+      f32x4 o = {v[0], v[1], v[2], v[3]};
+      if constexpr (EPI == kGemmAccumulate) {
+        const f32x4 old = *reinterpret_cast<const f32x4*>(dst);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += old[e];
+      }
+      *reinterpret_cast<f32x4*>(dst) = o;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < p.N) dst[e] = EPI == kGemmAccumulate ? dst[e] + v[e] : v[e];
+    }
+  }
+}
 
-template <int MT, int NT, int WR, int WC, int EPI>
-__global__ __launch_bounds__(64 * WR * WC) void gemm_i8_kernel(GemmI8Args p) {
+// The tile of a block: each XCD takes a run of neighbouring tiles, down the rows of q where these are the fewer bytes, else along
+// W's, so that its L2 holds the smaller operand and a run of the other.
+__device__ __forceinline__ void gemm_i8_tile(const GemmI8Args& p, int nbm, int nbn, int& bm, int& bn) {
+  const int ntiles = nbm * nbn, xj = (int)(blockIdx.x & 7), xq = ntiles >> 3, xr = ntiles & 7;
+  const int tile = xj * xq + min(xj, xr) + (int)(blockIdx.x >> 3);
+  if (p.M < p.N) {
+    bn = tile / nbm;
+    bm = tile - bn * nbm;
+  } else {
+    bm = tile / nbn;
+    bn = tile - bm * nbn;
+  }
+}
+
+template <int MT, int NT, int WR, int WC, int NS, int EPI>
+__global__ __launch_bounds__(64 * WR * WC, MT * NT > 8 ? 1 : 2) void gemm_i8_kernel(GemmI8Args p) {
   constexpr int BM = 32 * MT * WR, BN = 32 * NT * WC, NW = WR * WC;
-  constexpr int UA = BM / 16, U = (BM + BN) / 16 / NW;  // copies of a stage's q, copies per wave
+  constexpr int UA = BM / 8, U = (BM + BN) / 8 / NW;  // 1 KB copies (8 rows) of a stage's q, copies per wave
   constexpr int SB = (BM + BN) * kIK;
-  static_assert((BM + BN) / 16 % NW == 0, "copies are dealt evenly");
-  __shared__ __attribute__((aligned(16))) char smem[kINS * SB];
+  static_assert((BM + BN) / 8 % NW == 0, "copies are dealt evenly");
+  __shared__ __attribute__((aligned(16))) char smem[NS * SB];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wr = wv / WC, wc = wv % WC, l32 = lane & 31, lh = lane >> 5;
-  const int nbn = (p.N + BN - 1) / BN, ntiles = nbn * ((p.M + BM - 1) / BM);
-  const int xj = (int)(blockIdx.x & 7), xq = ntiles >> 3, xr = ntiles & 7;
-  const int tile = xj * xq + min(xj, xr) + (int)(blockIdx.x >> 3);
-  const int bm = tile / nbn, bn = tile - bm * nbn;
-  const int m0 = bm * BM, n0 = bn * BN, KT = p.K / kIK;
+  int bm, bn;
+  gemm_i8_tile(p, (p.M + BM - 1) / BM, (p.N + BN - 1) / BN, bm, bn);
+  const int m0 = bm * BM, n0 = bn * BN, KT = (p.K + kIK - 1) / kIK;
 
   const int8_t* qb = p.q + (int64_t)m0 * p.ldq;
   const int8_t* wb = p.W + (int64_t)n0 * p.K;
-  uint32_t src[U];
+  // a copy's lane: row lane / 8 of its eight, slot lane % 8. K may end in the middle of a stage: then no more than its first half
+  // is multiplied, and the other half's lanes copy that again.
+  const int half_end = p.K % kIK ? KT - 1 : KT;
+  uint32_t src[U], tail[U];
 #pragma unroll
   for (int i = 0; i < U; ++i) {
-    const int u = wv + NW * i, row = 16 * (u < UA ? u : u - UA) + i8_copy_row(lane);
-    src[i] = (u < UA ? (uint32_t)min(row, p.M - 1 - m0) * (uint32_t)p.ldq : (uint32_t)min(row, p.N - 1 - n0) * (uint32_t)p.K) +
-             16 * i8_copy_chunk(lane);
+    const int u = wv + NW * i, row = 8 * (u < UA ? u : u - UA) + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
+    const uint32_t at = u < UA ? (uint32_t)min(row, p.M - 1 - m0) * (uint32_t)p.ldq : (uint32_t)min(row, p.N - 1 - n0) * (uint32_t)p.K;
+    src[i] = at + 16 * c;
+    tail[i] = at + 16 * (c & 3);
   }
   const uint32_t lds0 = gemm_lds_u32(smem);
   auto issue = [&](int s) {
-    const uint32_t base = lds0 + (s % kINS) * SB;
+    const uint32_t base = lds0 + (s % NS) * SB;
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int u = wv + NW * i;
-      gemm_dma16s((u < UA ? qb : wb) + (int64_t)s * kIK, src[i], base + u * 1024);
+      gemm_dma16s((u < UA ? qb : wb) + (int64_t)s * kIK, s < half_end ? src[i] : tail[i], base + u * 1024);
     }
   };
   const int ra = wr * 32 * MT + l32, rb = wc * 32 * NT + l32;
-  uint32_t ao[2], bo[2];
+  uint32_t ao[4], bo[4];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int ch = ((2 * lh + j) ^ ((l32 >> 2) & 3)) << 4;
+  for (int j = 0; j < 4; ++j) {
+    const int ch = ((2 * j + lh) ^ ((l32 >> 1) & 7)) << 4;
     ao[j] = ra * kIK + ch;
     bo[j] = (BM + rb) * kIK + ch;
   }
@@ -201,34 +266,59 @@ __global__ __launch_bounds__(64 * WR * WC) void gemm_i8_kernel(GemmI8Args p) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
 
-  for (int s = 0; s < kINS - 1; ++s)
-    if (s < KT) issue(s);
-  for (int s = 0; s < KT; ++s) {
-    const int ahead = min(KT - 1 - s, kINS - 2);
-    if (ahead >= 2) gemm_wait_vm<2 * U>();
-    else if (ahead == 1) gemm_wait_vm<U>();
+  // The fragments of 32 inputs are read ahead of the products of the 32 before, so that the one runs beside the other: the
+  // barrier that hands a stage's buffer on stands before its last products, when all of it has been read.
+  i32x4 fa[2][MT], fb[2][NT];
+  auto read = [&](int s, int j) {
+    const char* st = smem + (s % NS) * SB;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) fa[j & 1][i] = *reinterpret_cast<const i32x4*>(st + ao[j] + i * 32 * kIK);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) fb[j & 1][i] = *reinterpret_cast<const i32x4*>(st + bo[j] + i * 32 * kIK);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto multiply = [&](int j) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int k = 0; k < NT; ++k)
+        acc[i][k] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[j & 1][i], fb[j & 1][k], acc[i][k], 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto wait = [&](int s) {  // stage s has landed, with up to NS - 2 behind it in flight; all waves are past their earlier reads
+    const int behind = min(KT - 1 - s, NS - 2);
+    if (NS == 4 && behind >= 2) gemm_wait_vm<2 * U>();
+    else if (NS == 4 && behind == 1) gemm_wait_vm<U>();
     else gemm_wait_vm<0>();
     lds_barrier();
-    if (s + kINS - 1 < KT) issue(s + kINS - 1);
-    const char* st = smem + (s % kINS) * SB;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      i32x4 a[MT], b[NT];
-#pragma unroll
-      for (int i = 0; i < MT; ++i) a[i] = *reinterpret_cast<const i32x4*>(st + ao[j] + i * 32 * kIK);
-#pragma unroll
-      for (int i = 0; i < NT; ++i) b[i] = *reinterpret_cast<const i32x4*>(st + bo[j] + i * 32 * kIK);
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int k = 0; k < NT; ++k) acc[i][k] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[i], b[k], acc[i][k], 0, 0, 0);
+  };
+  static_assert(NS == 2 || NS == 4, "wait()");
+  for (int s = 0; s < NS - 1; ++s)
+    if (s < KT) issue(s);
+  wait(0);
+  if (NS - 1 < KT) issue(NS - 1);
+  read(0, 0);
+  for (int s = 0; s < KT; ++s) {
+    read(s, 1);
+    multiply(0);
+    if (s < half_end) {
+      read(s, 2);
+      multiply(1);
+      read(s, 3);
+      multiply(2);
     }
+    if (s + 1 < KT) {
+      wait(s + 1);
+      if (s + NS < KT) issue(s + NS);
+      read(s + 1, 0);
+    }
+    multiply(1);
   }
 
   // The results leave through LDS, a wave's 32 rows at a time in an area of its own, so that a store holds whole runs of a row:
   // a lane takes CL columns of a row (gate and up of a neuron meet in it).
   constexpr int CW = 32 * NT, LD = CW + 4, CL = EPI == kGemmSwiglu ? 8 : 4, LR = CW / CL, RS = 64 / LR;
-  static_assert(NW * 32 * LD * 4 <= kINS * SB, "the stages hold the waves' areas");
+  static_assert(NW * 32 * LD * 4 <= NS * SB, "the stages hold the waves' areas");
   lds_barrier();  // every wave has read its last fragments
   float* t = reinterpret_cast<float*>(smem) + wv * 32 * LD;
   const int c = CL * (lane % LR), n = n0 + wc * CW + c;
@@ -237,6 +327,12 @@ __global__ __launch_bounds__(64 * WR * WC) void gemm_i8_kernel(GemmI8Args p) {
   for (int e = 0; e < CL; ++e) sn[e] = p.ws[min(n + e, p.N - 1)];
   const bool pushes_here = EPI == kGemmSwiglu && gemm_pushes_touch(p.pushes, p.npush, n0 >> 1, (n0 + BN) >> 1);
   const bool vec = (p.ldy & 3) == 0 && ((uintptr_t)p.y & 15) == 0;
+  // (all rows' scales at once: a load for each row's turn was a third of the time of a tile of 1024 inputs)
+  float sm[MT][32 / RS];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int k = 0; k < 32 / RS; ++k) sm[i][k] = p.qs[min(m0 + (wr * MT + i) * 32 + lane / LR + RS * k, p.M - 1)];
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
 #pragma unroll
@@ -247,55 +343,18 @@ __global__ __launch_bounds__(64 * WR * WC) void gemm_i8_kernel(GemmI8Args p) {
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     const int mb = m0 + (wr * MT + i) * 32 + lane / LR;
+#pragma unroll
     for (int k = 0; k < 32 / RS; ++k) {
       const int m = mb + RS * k;
-      if (m >= p.M) break;
-      const float sm = p.qs[m];
+      if (m >= p.M) continue;
       float v[CL];
 #pragma unroll
       for (int q = 0; q < CL / 4; ++q) {
         const f32x4 x = *reinterpret_cast<const f32x4*>(t + (lane / LR + RS * k) * LD + c + 4 * q);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[4 * q + e] = x[e] * sm * sn[4 * q + e];
+        for (int e = 0; e < 4; ++e) v[4 * q + e] = x[e] * sm[i][k] * sn[4 * q + e];
       }
-      if constexpr (EPI == kGemmSwiglu) {
-        const int neuron = n >> 1, I = p.N >> 1;
-        f32x4 a;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) a[e] = silu_f(v[2 * e]) * v[2 * e + 1];
-        if (pushes_here) {
-          const int row = gemm_push_row(m, p.T);
-          for (int k2 = 0; k2 < p.npush; ++k2)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) a[e] = gemm_push(p.pushes + k2, neuron + e, row, a[e]);
-        }
-        float* dst = p.y + (int64_t)m * p.ldy + neuron;
-        if (vec && neuron + 4 <= I) {
-          *reinterpret_cast<f32x4*>(dst) = a;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (neuron + e < I) dst[e] = a[e];
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (neuron + e < I) gemm_capture(p.cap, m, p.T, neuron + e, a[e]);
-      } else {
-        float* dst = p.y + (int64_t)m * p.ldy + n;
-        if (vec && n + 4 <= p.N) {
-          f32x4 o = {v[0], v[1], v[2], v[3]};
-          if constexpr (EPI == kGemmAccumulate) {
-            const f32x4 old = *reinterpret_cast<const f32x4*>(dst);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] += old[e];
-          }
-          *reinterpret_cast<f32x4*>(dst) = o;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n + e < p.N) dst[e] = EPI == kGemmAccumulate ? dst[e] + v[e] : v[e];
-        }
-      }
+      gemm_i8_finish<EPI, CL>(p, m, n, v, vec, pushes_here);
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -303,13 +362,90 @@ __global__ __launch_bounds__(64 * WR * WC) void gemm_i8_kernel(GemmI8Args p) {
   }
 }
 
-template <int MT, int NT, int WR, int WC>
+// Few tiles: 32 x 32 outputs a block, its four waves a quarter of the stages each (wave w takes w, w + 4, ...), with no barrier
+// between them before the four sums meet in LDS.
+template <int EPI>
+__global__ __launch_bounds__(256, 2) void gemm_i8_few_kernel(GemmI8Args p) {
+  constexpr int SB = 64 * kIK, NS = 2, LD = 36;  // a stage's 32 rows of q, then of W; LD: a row of sums
+  __shared__ __attribute__((aligned(16))) char smem[4 * NS * SB];
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, lh = lane >> 5;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int bm, bn;
+  gemm_i8_tile(p, (p.M + 31) / 32, (p.N + 31) / 32, bm, bn);
+  const int m0 = bm * 32, n0 = bn * 32, KT = (p.K + kIK - 1) / kIK, half_end = p.K % kIK ? KT - 1 : KT;
+  const int8_t* qb = p.q + (int64_t)m0 * p.ldq;
+  const int8_t* wb = p.W + (int64_t)n0 * p.K;
+  uint32_t src[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = 8 * (i & 3) + (lane >> 3);
+    src[i] = i < 4 ? (uint32_t)min(row, p.M - 1 - m0) * (uint32_t)p.ldq : (uint32_t)min(row, p.N - 1 - n0) * (uint32_t)p.K;
+  }
+  const uint32_t lds0 = gemm_lds_u32(smem) + wv * NS * SB;
+  auto issue = [&](int s) {  // the last stage may be half a one, as above
+    const uint32_t base = lds0 + ((s >> 2) % NS) * SB;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int c = (lane & 7) ^ (((8 * (i & 3) + (lane >> 3)) >> 1) & 7);
+      gemm_dma16s((i < 4 ? qb : wb) + (int64_t)s * kIK, src[i] + 16 * (s < half_end ? c : c & 3), base + i * 1024);
+    }
+  };
+  i32x16 acc;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) acc[r] = 0;
+  if (wv < KT) issue(wv);
+  if (wv + 4 < KT) issue(wv + 4);
+  for (int s = wv; s < KT; s += 4) {
+    if (s + 4 < KT) gemm_wait_vm<8>();
+    else gemm_wait_vm<0>();
+    const char* st = smem + (wv * NS + (s >> 2) % NS) * SB;
+    i32x4 a[4], b[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int at = l32 * kIK + (((2 * j + lh) ^ ((l32 >> 1) & 7)) << 4);
+      a[j] = *reinterpret_cast<const i32x4*>(st + at);
+      b[j] = *reinterpret_cast<const i32x4*>(st + 32 * kIK + at);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage has been read
+    if (s + 8 < KT) issue(s + 8);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < 2 || s < half_end) acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[j], b[j], acc, 0, 0, 0);
+  }
+  // the sums of a wave to where its first stage was: nobody else reads or writes there
+  int* t = reinterpret_cast<int*>(smem);
+  constexpr int AW = NS * SB / 4;
+  static_assert(AW >= 32 * LD, "an area each");
+#pragma unroll
+  for (int r = 0; r < 16; ++r) t[wv * AW + (8 * (r >> 2) + (r & 3) + 4 * lh) * LD + l32] = acc[r];
+  __syncthreads();
+  const int row = tid >> 3, c = 4 * (tid & 7), m = m0 + row, n = n0 + c;
+  if (m >= p.M || n >= p.N) return;
+  const bool pushes_here = EPI == kGemmSwiglu && gemm_pushes_touch(p.pushes, p.npush, n0 >> 1, (n0 + 32) >> 1);
+  constexpr int al = EPI == kGemmSwiglu ? 2 : 4;
+  const bool vec = (p.ldy & (al - 1)) == 0 && ((uintptr_t)p.y & (4 * al - 1)) == 0;
+  i32x4 sum = {0, 0, 0, 0};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const i32x4 x = *reinterpret_cast<const i32x4*>(t + k * AW + row * LD + c);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] += x[e];
+  }
+  const float sm = p.qs[m];
+  float v[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = (float)sum[e] * sm * p.ws[min(n + e, p.N - 1)];
+  gemm_i8_finish<EPI, 4>(p, m, n, v, vec, pushes_here);
+}
+
+template <int MT, int NT, int WR, int WC, int NS>
 static void gemm_i8_launch(const GemmI8Args& a, int epilogue, hipStream_t st) {
   constexpr int BM = 32 * MT * WR, BN = 32 * NT * WC;
   const dim3 grid((unsigned)(((a.M + (int64_t)BM - 1) / BM) * ((a.N + (int64_t)BN - 1) / BN))), block(64 * WR * WC);
-  if (epilogue == kGemmStore) hipLaunchKernelGGL((gemm_i8_kernel<MT, NT, WR, WC, kGemmStore>), grid, block, 0, st, a);
-  else if (epilogue == kGemmAccumulate) hipLaunchKernelGGL((gemm_i8_kernel<MT, NT, WR, WC, kGemmAccumulate>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((gemm_i8_kernel<MT, NT, WR, WC, kGemmSwiglu>), grid, block, 0, st, a);
+  if (epilogue == kGemmStore) hipLaunchKernelGGL((gemm_i8_kernel<MT, NT, WR, WC, NS, kGemmStore>), grid, block, 0, st, a);
+  else if (epilogue == kGemmAccumulate)
+    hipLaunchKernelGGL((gemm_i8_kernel<MT, NT, WR, WC, NS, kGemmAccumulate>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((gemm_i8_kernel<MT, NT, WR, WC, NS, kGemmSwiglu>), grid, block, 0, st, a);
 }
 
 }  // namespace q35
@@ -347,14 +483,29 @@ extern "C" int q35_gemm_i8(const int8_t* q, int64_t ldq, const float* q_scale, c
   if (epilogue == kGemmSwiglu ? (N % 2 != 0 || ldy < N / 2) : ldy < N) return Q35_EINVAL;
   if (cap && (epilogue != kGemmSwiglu || ld_cap < N / 2 || ld_cap_row < N / 2 || ((uintptr_t)cap & 3))) return Q35_EINVAL;
   if (ldq < K) return Q35_EINVAL;
-  if (K % kIK || K > 65536 || ldq % 16 || ldq > (1 << 23) || ((uintptr_t)q | (uintptr_t)W) & 15) return Q35_EUNSUPPORTED;
+  if (K % 64 || K > 65536 || ldq % 16 || ldq > (1 << 23) || ((uintptr_t)q | (uintptr_t)W) & 15) return Q35_EUNSUPPORTED;
   if (M > (1 << 30) || N > (1 << 30) || T > 0x7fffffff) return Q35_EUNSUPPORTED;
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const GemmI8Args a{q, ldq, q_scale, W, w_scale, y, ldy, (int)M, (int)N, (int)K, pushes, (int)npush, (int)T, {cap, ld_cap, ld_cap_row}};
   const int64_t cus = device_cus();
-  if (((M + 63) / 64) * ((N + 63) / 64) > 0x7fffffff) return Q35_EUNSUPPORTED;
-  if (((M + 255) / 256) * ((N + 255) / 256) >= cus) gemm_i8_launch<4, 2, 2, 4>(a, epilogue, st);
-  else if (((M + 127) / 128) * ((N + 127) / 128) >= cus) gemm_i8_launch<2, 2, 2, 2>(a, epilogue, st);
-  else gemm_i8_launch<1, 1, 2, 2>(a, epilogue, st);
+  const auto tiles = [&](int64_t b) { return ((M + b - 1) / b) * ((N + b - 1) / b); };
+  if (tiles(256) > 0x7fffffff) return Q35_EUNSUPPORTED;
+  // The smallest tile of which the chip takes all blocks at once, two to a CU; a larger one beyond, which reads each operand
+  // less often. Where the next larger has few tiles, its CUs wait for their own reads: 1024 outputs of 3584 inputs take, in us,
+  // with tiles of 32 / 64 / 128 / 256, 4.3 / 10.4 / 18.6 / 42 for 32 rows, 8.0 / 11.2 / 19.9 / 44 for 512 (512 tiles of 32), 23.4
+  // / 16.1 / 23.1 / 46 for 2048 (512 of 64), 43 / 29 / 26 / 48 for 4096; 7168 outputs of 1024 inputs 32 / 21 / 15 / 22 for 1024
+  // rows (448 of 128), 150 / 79 / 48 / 44 for 4096.
+  if (tiles(32) <= 2 * cus) {
+    const dim3 grid((unsigned)tiles(32)), block(256);
+    if (epilogue == kGemmStore) hipLaunchKernelGGL((gemm_i8_few_kernel<kGemmStore>), grid, block, 0, st, a);
+    else if (epilogue == kGemmAccumulate) hipLaunchKernelGGL((gemm_i8_few_kernel<kGemmAccumulate>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((gemm_i8_few_kernel<kGemmSwiglu>), grid, block, 0, st, a);
+  } else if (tiles(64) <= 2 * cus) {
+    gemm_i8_launch<1, 1, 2, 2, 4>(a, epilogue, st);
+  } else if (tiles(128) <= 2 * cus) {
+    gemm_i8_launch<2, 2, 2, 2, 2>(a, epilogue, st);
+  } else {
+    gemm_i8_launch<4, 2, 2, 4, 2>(a, epilogue, st);
+  }
   return hipGetLastError() == hipSuccess ? Q35_OK : Q35_ELAUNCH;
 }
