@@ -59,11 +59,13 @@ struct PagedAttnArgs {
   // sequences whose tables begin with the same n_sh keys: the runs of these (Sp) and of a sequence's own keys (S) leave their
   // parts in part and ml [B T Hq][Sp + S]
   int B, n_sh, Sp;
+  uint32_t inv_g, inv_t;  // (2^32 - 1) / G and / T
+  int n_pre;  // blocks of the shared keys, which come before those of the rows' own
 };
 
-// What a block's keys are: a row's; or, of sequences that share their first keys, these, for the rows of all of them, or a
-// row's own.
-enum PagedKeys : int { kAllKeys = 0, kSharedKeys = 1, kOwnKeys = 2 };
+// What a block's keys are: a row's; or, of sequences that share their first keys, either these, for the rows of all of them, or
+// a row's own behind them.
+enum PagedKeys : int { kAllKeys = 0, kSplitKeys = 1 };
 
 typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
 typedef __attribute__((__vector_size__(8 * sizeof(_Float16)))) _Float16 f16x8;
@@ -76,6 +78,11 @@ constexpr int kORow = kPgD + 4; // LDS row of a wave's result
 __device__ __forceinline__ int keys_seen(const PagedAttnArgs& p, int64_t pos, int len, int t) {
   const int64_t at = pos + t;
   return t < len && at >= 0 && at < p.pt.capacity() ? (int)at + 1 : 0;
+}
+// n / d for n >= 0, inv = (2^32 - 1) / d: the product's high half is the quotient or one below it.
+__device__ __forceinline__ int div_by(int n, int d, uint32_t inv) {
+  const int q = (int)__umulhi((uint32_t)n, inv);
+  return q + (n - q * d >= d);
 }
 // Keys of row b's run over S blocks, from the keys its last token sees: a multiple of a round.
 __device__ __forceinline__ int run_keys(int n, int S) {
@@ -216,12 +223,25 @@ __device__ __forceinline__ void out_store(const PagedAttnArgs& p, const f32x4& O
 
 template <bool I4, int NR, int W, int KEYS_OF = kAllKeys>
 __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(PagedAttnArgs p) {
-  constexpr bool kPre = KEYS_OF == kSharedKeys, kOwn = KEYS_OF == kOwnKeys;
+  constexpr bool kSplit = KEYS_OF == kSplitKeys;
   constexpr int ROWS = 16 * NR, KEYS = 32 * W, QP = I4 ? 1 : 2, QF = 8 * 64;  // parts of Q, 16-byte operands of one
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, a = lane >> 4;
-  const int s = blockIdx.x, kvh = blockIdx.y % p.Hkv, rb = blockIdx.y / p.Hkv, b = blockIdx.z;
-  const int R = (kPre ? p.B : 1) * p.T * p.G, r0 = rb * ROWS;
+  int s = blockIdx.x, by = blockIdx.y, b = blockIdx.z;
+  bool pre = false;  // the shared keys
+  if constexpr (kSplit) {
+    pre = (int)blockIdx.x < p.n_pre;
+    const int i = pre ? (int)blockIdx.x : (int)blockIdx.x - p.n_pre, S = pre ? p.Sp : p.S;
+    by = __builtin_amdgcn_readfirstlane(i / S);
+    s = i - by * S;
+    b = 0;
+    if (!pre) {
+      b = __builtin_amdgcn_readfirstlane(by / (p.Hkv * p.RB));
+      by -= b * p.Hkv * p.RB;
+    }
+  }
+  const int kvh = by % p.Hkv, rb = by / p.Hkv;
+  const int R = (kSplit && pre ? p.B : 1) * p.T * p.G, r0 = rb * ROWS;
 
   constexpr int kQBytes = NR * QP * QF * 16, kOBytes = W * 16 * kORow * 4;
   __shared__ __attribute__((aligned(16))) char lds[kQBytes > kOBytes ? kQBytes : kOBytes];
@@ -229,6 +249,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(PagedAttnArgs p) 
   __shared__ float qfac[ROWS];           // the power of two taken out of a row of Q
   __shared__ float mls[W][16][2];
   __shared__ __attribute__((aligned(16))) float sbuf[I4 ? W : 1][2][kPgNG][32];  // scales of a wave's keys and values
+  __shared__ int seen_s[kSplit ? ROWS : 1];
   __shared__ u32x4 m24[7];  // -24 eight times between zeros
   u32x4* qf = reinterpret_cast<u32x4*>(lds);  // [NR][hi, lo][8 steps][64 lanes]
   float* ob = reinterpret_cast<float*>(lds);  // [W waves][16][kORow], once Q has been used
@@ -240,13 +261,24 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(PagedAttnArgs p) 
   constexpr int QT = W == 4 ? NR : 1;  // tiles that a wave prepares: all, or tile wave / 4 where there is one
   const int q0 = W == 4 ? 0 : wave >> 2;
   u32x4 qx[QT][4], qp[QT][4];
+  int at_q[kSplit ? QT : 1], seen_q[kSplit ? QT : 1];  // the rows' positions, and how many of the keys they see
   f32x4 wx[4], wp[4];
   auto pair_of = [&](int d) { return d >= p.rot ? d : d < half ? d + half : d - half; };
 #pragma unroll
   for (int i = 0; i < QT; ++i) {
-    const int r = r0 + 16 * (q0 + i) + qcol, t = r / p.G, h = kvh * p.G + r - t * p.G;
+    const int r = r0 + 16 * (q0 + i) + qcol, t = kSplit ? div_by(r, p.G, p.inv_g) : r / p.G, h = kvh * p.G + r - t * p.G;
     int64_t o = b * p.qb + t * p.qt + h * p.qh;
-    if constexpr (kPre) o = (t / p.T) * p.qb + (t % p.T) * p.qt + h * p.qh;
+    if constexpr (kSplit) {
+      const int br = pre ? div_by(t, p.T, p.inv_t) : b, tr = pre ? t - br * p.T : t;
+      o = br * p.qb + tr * p.qt + h * p.qh;
+      at_q[i] = seen_q[i] = 0;
+      if (r < R && q0 + i < NR) {
+        const int64_t at = p.pos[br];
+        const int n = keys_seen(p, at, p.lens ? min(max(p.lens[br], 0), p.T) : p.T, tr);
+        at_q[i] = (int)(at + tr);  // (a position that is there fits)
+        seen_q[i] = pre ? min(n, p.n_sh) : n;
+      }
+    }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       qx[i][q] = qp[i][q] = u32x4{0, 0, 0, 0};
@@ -267,18 +299,8 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(PagedAttnArgs p) 
   }
   __builtin_amdgcn_sched_barrier(0);
 
-  const int64_t pos = kPre ? 0 : load_uniform(p.pos + b);
-  const int len = kPre ? 0 : p.lens ? min(max(load_uniform(p.lens + b), 0), p.T) : p.T;
-  // of the rows of all sequences: the position of row r's token, and how many of the shared keys it sees
-  struct Place {
-    int64_t at;
-    int seen;
-  };
-  auto place = [&](int r) -> Place {
-    const int tt = r / p.G, br = tt / p.T, t = tt - br * p.T;
-    const int64_t at = p.pos[br];
-    return {at + t, min(keys_seen(p, at, p.lens ? min(max(p.lens[br], 0), p.T) : p.T, t), p.n_sh)};
-  };
+  const int64_t pos = load_uniform(p.pos + b);
+  const int len = p.lens ? min(max(load_uniform(p.lens + b), 0), p.T) : p.T;
   // the row's keys: those of its last token that is there (a later one sees more)
   int n_row = 0;
   if (len > 0) n_row = (int)min(max(pos + len, (int64_t)0), p.pt.capacity());
@@ -286,15 +308,20 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(PagedAttnArgs p) 
   // what this block's rows see at most and at least
   int n_max = 0;
   if (t0 < len) n_max = (int)min(max(pos + min(t1, len - 1) + 1, (int64_t)0), p.pt.capacity());
-  if constexpr (kPre) n_max = p.n_sh;
-  const int kb = kOwn ? p.n_sh : 0;
-  const int run = kPre ? __builtin_amdgcn_readfirstlane(run_keys(p.n_sh, p.Sp)) : run_keys(kOwn ? max(n_row - kb, 0) : n_row, p.S);
+  int kb = 0, run = 0;
+  if constexpr (kSplit) {
+    if (pre) n_max = p.n_sh;
+    else kb = p.n_sh;
+    run = __builtin_amdgcn_readfirstlane(run_keys(pre ? p.n_sh : max(n_row - kb, 0), pre ? p.Sp : p.S));
+  } else {
+    run = run_keys(n_row, p.S);
+  }
   const int k0 = kb + s * run, k1 = min(k0 + run, n_max);
   const bool work = k0 < k1;
-  if (!work && (KEYS_OF != kAllKeys || p.S > 1)) return;  // the merge does not read empty runs' slots
+  if (!work && (kSplit || p.S > 1)) return;  // the merge does not read empty runs' slots
 
   int n_min = keys_seen(p, pos, len, t0);
-  if constexpr (kPre) n_min = p.n_sh;  // (less where a row is inside the shared part: below)
+  if constexpr (kSplit) n_min = n_max;  // (less where a row sees less: below)
   const int n_last = n_max - 1, pmask = (1 << p.pt.shift) - 1;
   // 16 keys from key0 on: the page (that of the last key for a tile past it, whose keys are masked) and the row in it.
   // Bases are scalar, a lane's part of the address 32 bits.
@@ -381,14 +408,12 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(PagedAttnArgs p) 
   constexpr int kAngles = kTurns ? 1 : QT;
   f32x4 co[kAngles][4], si[kAngles][4];
   auto angles = [&](int i, f32x4 (&co)[4], f32x4 (&si)[4]) {
-    const int tk = (r0 + 16 * (q0 + i) + qcol) / p.G;
+    const int tk = kSplit ? 0 : (r0 + 16 * (q0 + i) + qcol) / p.G;
     bool there = r0 + 16 * (q0 + i) + qcol < R && q0 + i < NR && keys_seen(p, pos, len, tk) > 0;
     int64_t at = pos + tk;
-    if constexpr (kPre) {
-      const int r = r0 + 16 * (q0 + i) + qcol;
-      const Place pl = place(min(r, R - 1));
-      there = r < R && q0 + i < NR && pl.seen > 0;
-      at = pl.at;
+    if constexpr (kSplit) {
+      there = seen_q[i] > 0;
+      at = at_q[i];
     }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -440,9 +465,12 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(PagedAttnArgs p) 
   if (work && q0 < NR) {
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
-      const int tk = (r0 + 16 * (q0 + i) + qcol) / p.G, ia = i < kAngles ? i : 0;
+      const int tk = kSplit ? 0 : (r0 + 16 * (q0 + i) + qcol) / p.G, ia = i < kAngles ? i : 0;
       bool there = r0 + 16 * (q0 + i) + qcol < R && keys_seen(p, pos, len, tk) > 0;
-      if constexpr (kPre) there = r0 + 16 * (q0 + i) + qcol < R && place(min(r0 + 16 * (q0 + i) + qcol, R - 1)).seen > 0;
+      if constexpr (kSplit) {
+        there = seen_q[i] > 0;
+        if (qj == 0) seen_s[16 * (q0 + i) + qcol] = r0 + 16 * (q0 + i) + qcol < R ? seen_q[i] : n_max;
+      }
       if (i >= kAngles) angles(i, co[0], si[0]);
       f32x4 x[4], px[4];
 #pragma unroll
@@ -475,18 +503,13 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(PagedAttnArgs p) 
   }
 
   int seen[NR];
+  if constexpr (!kSplit) {
 #pragma unroll
-  for (int i = 0; i < NR; ++i) {
-    // rows that are not there are not stored: let them see what the others do, so that they ask for no mask
-    const int r = r0 + 16 * i + c;
-    seen[i] = r < R ? keys_seen(p, pos, len, r / p.G) : n_max;
-    if constexpr (kPre) seen[i] = r < R ? place(min(r, R - 1)).seen : n_max;
-  }
-  if constexpr (kPre) {
-    bool less = false;
-#pragma unroll
-    for (int i = 0; i < NR; ++i) less |= seen[i] < n_max;
-    if (__builtin_amdgcn_ballot_w64(less) != 0) n_min = 0;
+    for (int i = 0; i < NR; ++i) {
+      // rows that are not there are not stored: let them see what the others do, so that they ask for no mask
+      const int r = r0 + 16 * i + c;
+      seen[i] = r < R ? keys_seen(p, pos, len, r / p.G) : n_max;
+    }
   }
   f32x4 acc[NR][16];
   f32x4 corr[NR];  // 4 bits: -24 times the sum of the weights, of groups 0 .. 3
@@ -506,6 +529,15 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(PagedAttnArgs p) 
   lds_barrier();
 #pragma unroll
   for (int i = 0; i < NR; ++i) fac[i] = I4 ? qfac[16 * i + c] : 1.f;
+  if constexpr (kSplit) {
+    bool less = false;
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      seen[i] = seen_s[16 * i + c];
+      less |= seen[i] < n_max;
+    }
+    if (__builtin_amdgcn_ballot_w64(less) != 0) n_min = 0;
+  }
   // 16 rows against codes: Q's operands and the offsets stay in registers
   constexpr bool kQReg = I4 && NR == 1;
   u32x4 qreg[kQReg ? 8 : 1];
@@ -836,27 +868,35 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_kernel(PagedAttnArgs p) 
     for (int jj = 0; jj < 16 / W; ++jj) {
       const int j = W * jj + wave;
       if (r0 + 16 * i + j >= R) break;
-      const int r = r0 + 16 * i + j, t = r / p.G, h = kvh * p.G + r - t * p.G;
+      const int r = r0 + 16 * i + j, t = kSplit ? div_by(r, p.G, p.inv_g) : r / p.G, h = kvh * p.G + r - t * p.G;
       float M = -INFINITY;
 #pragma unroll
       for (int w = 0; w < W; ++w) M = fmaxf(M, mls[w][j][0]);
       float L = 0.f;
       f32x4 O = zero4();
       if (M > -INFINITY) {
+        // (selects, so that all waves' reads are in flight together; a wave that has seen nothing may have left anything)
+        f32x4 v[W];
+        float m[W], l[W];
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-          if (mls[w][j][0] == -INFINITY) continue;  // nothing seen
-          const float f = __builtin_amdgcn_exp2f(mls[w][j][0] - M);
-          L += mls[w][j][1] * f;
-          const f32x4 v = *reinterpret_cast<const f32x4*>(ob + ((size_t)w * 16 + j) * kORow + de);
+          v[w] = *reinterpret_cast<const f32x4*>(ob + ((size_t)w * 16 + j) * kORow + de);
+          m[w] = mls[w][j][0];
+          l[w] = mls[w][j][1];
+        }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) O[e] += v[e] * f;
+        for (int w = 0; w < W; ++w) {
+          const bool in = m[w] > -INFINITY;
+          const float f = __builtin_amdgcn_exp2f(m[w] - M);
+          L = in ? L + l[w] * f : L;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) O[e] = in ? O[e] + v[w][e] * f : O[e];
         }
       }
-      if (KEYS_OF != kAllKeys || p.S > 1) {
+      if (kSplit || p.S > 1) {
         size_t slot = (((size_t)b * p.Hkv + kvh) * R + r) * p.S + s;
-        if constexpr (KEYS_OF != kAllKeys)
-          slot = (((size_t)(kPre ? 0 : b) * p.T + t) * p.Hkv * p.G + h) * (p.Sp + p.S) + (kPre ? s : p.Sp + s);
+        if constexpr (kSplit)  // (b is 0 where t counts the tokens of all sequences)
+          slot = (((size_t)b * p.T + t) * p.Hkv * p.G + h) * (p.Sp + p.S) + (pre ? s : p.Sp + s);
         *reinterpret_cast<f32x4*>(p.part + slot * kPgD + de) = O;
         if (le < 2) p.ml[2 * slot + le] = le ? L : M;
       } else {
@@ -955,11 +995,14 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs p) 
   out_store(p, O, L, true, g, b, t, h, d0);
 }
 
-// A query row's runs over the shared and over its own keys joined, one wave a row.
+// A query row's runs over the shared and over its own keys joined, by one wave or, of many runs, by the block's four, wave w
+// folding runs w, w + 4, ...
+template <int W>
 __global__ __launch_bounds__(256) void paged_attn_shared_merge_kernel(PagedAttnArgs p) {
   constexpr int U = 8;
-  const int lane = threadIdx.x & 63, d0 = 4 * lane;
-  const int64_t row = 4 * (int64_t)blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, d0 = 4 * lane, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = W == 1 ? 4 * (int64_t)blockIdx.x + wave : (int64_t)blockIdx.x;
+  const int w0 = W == 1 ? 0 : wave;
   const int Hq = p.Hkv * p.G;
   if (row >= (int64_t)p.B * p.T * Hq) return;
   const int h = (int)(row % Hq), tt = (int)(row / Hq), b = tt / p.T, t = tt - b * p.T;
@@ -976,12 +1019,12 @@ __global__ __launch_bounds__(256) void paged_attn_shared_merge_kernel(PagedAttnA
   float M = -INFINITY, L = 0.f;
   f32x4 O = zero4();
   const f32x4 g = gate_load(p, b, t, h, d0);
-  for (int s0 = 0; s0 < n; s0 += U) {
+  for (int s0 = w0; s0 < n; s0 += W * U) {
     f32x4 pv[U];
     float m[U], l[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = min(s0 + u, n - 1);
+      const int i = min(s0 + W * u, n - 1);
       const size_t s = base + (i < n0 ? i : p.Sp + i - n0);
       pv[u] = *reinterpret_cast<const f32x4*>(p.part + s * kPgD + d0);
       m[u] = p.ml[2 * s];
@@ -990,7 +1033,7 @@ __global__ __launch_bounds__(256) void paged_attn_shared_merge_kernel(PagedAttnA
     float mn = M;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      m[u] = s0 + u < n ? m[u] : -INFINITY;
+      m[u] = s0 + W * u < n ? m[u] : -INFINITY;
       mn = fmaxf(mn, m[u]);
     }
     const float c0 = M > -INFINITY ? __builtin_amdgcn_exp2f(M - mn) : 0.f;
@@ -1006,6 +1049,27 @@ __global__ __launch_bounds__(256) void paged_attn_shared_merge_kernel(PagedAttnA
       for (int e = 0; e < 4; ++e) O[e] += in ? pv[u][e] * c1 : 0.f;
     }
     M = mn;
+  }
+  if constexpr (W > 1) {
+    __shared__ float gm[4], gl[4];
+    __shared__ f32x4 go[4][64];
+    if (lane == 0) {
+      gm[wave] = M;
+      gl[wave] = L;
+    }
+    go[wave][lane] = O;
+    __syncthreads();
+    if (wave) return;
+    M = fmaxf(fmaxf(gm[0], gm[1]), fmaxf(gm[2], gm[3]));
+    L = 0.f;
+    O = zero4();
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = gm[w] > -INFINITY ? __builtin_amdgcn_exp2f(gm[w] - M) : 0.f;
+      L += gm[w] > -INFINITY ? gl[w] * f : 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) O[e] += gm[w] > -INFINITY ? go[w][lane][e] * f : 0.f;
+    }
   }
   out_store(p, O, L, true, g, b, t, h, d0);
 }
@@ -1079,21 +1143,22 @@ static int paged_attn_args(PagedAttnArgs& a, const void* q, int64_t q_sb, int64_
   return Q35_OK;
 }
 
-// Of sequences that share their first n_sh keys: tiles and runs of these for the rows of all, and of each one's own keys.
+// Of sequences that share their first n_sh keys: 16s of rows a block, tiles of the rows of all and of a sequence's, runs over the
+// shared and over a sequence's own keys.
 struct SharedPlan {
-  int NP, RBP, SP;  // 16s of rows, tiles and runs over the shared keys
-  PagedPlan own;
+  int NR, RBP, RB, SP, S;
 };
-static int shared_runs(int64_t base, int64_t keys) {
-  const int64_t most = (keys + kRound - 1) / kRound;
-  int64_t S = (512 + base - 1) / base;
-  if (most <= 2 * S) S = (256 + base - 1) / base;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({S, most, 1024}));
-}
 static SharedPlan shared_plan(int64_t B, int64_t T, int64_t Hkv, int64_t G, int64_t n_sh, int64_t n_own) {
-  const int64_t R = B * T * G, NP = R <= 16 ? 1 : 2, RBP = (R + 16 * NP - 1) / (16 * NP);
-  const int64_t own = T * G, NR = own <= 16 ? 1 : 2, RB = (own + 16 * NR - 1) / (16 * NR);
-  return {(int)NP, (int)RBP, shared_runs(Hkv * RBP, n_sh), {(int)NR, (int)RB, shared_runs(B * Hkv * RB, n_own), 4}};
+  const int64_t NR = B * T * G <= 16 ? 1 : 2, RBP = (B * T * G + 16 * NR - 1) / (16 * NR), RB = (T * G + 16 * NR - 1) / (16 * NR);
+  const int64_t np = Hkv * RBP, no = B * Hkv * RB, mp = (n_sh + kRound - 1) / kRound, mo = (n_own + kRound - 1) / kRound;
+  // Runs of as many rounds as make 512 blocks of them all, two a CU (32 rows of one token, 8192 shared and up to 500 own bf16 keys:
+  // runs of two rounds 29 us, of one 40, of four 31). Own keys' blocks that find the shared ones' on every CU run behind them: one
+  // a CU then (64 rows of four tokens, 32768 shared and up to 1000 own 4-bit keys: own keys in one run 131 us, two 123, four 133).
+  const int64_t rr = std::max<int64_t>({1, (np * mp + no * mo + 511) / 512, (std::max(mp, mo) + 1023) / 1024});
+  const int64_t SP = (mp + rr - 1) / rr;
+  int64_t S = std::max<int64_t>(1, (mo + rr - 1) / rr);
+  if (np * SP >= 512) S = std::max(S, std::min(mo, 256 / no));
+  return {(int)NR, (int)RBP, (int)RB, (int)SP, (int)S};
 }
 
 }  // namespace q35
@@ -1162,7 +1227,7 @@ extern "C" size_t q35_gated_attn_paged_shared_workspace_bytes(int64_t B, int64_t
   const size_t all = q35_gated_attn_paged_workspace_bytes(B, T, Hq, Hkv, D, n_blocks, page_size, 0);
   if (all == 0 || shared_blocks == 0) return all;
   const SharedPlan pl = shared_plan(B, T, Hkv, Hq / Hkv, shared_blocks * page_size, (n_blocks - shared_blocks) * page_size);
-  return (size_t)B * T * Hq * (pl.SP + pl.own.S) * (kPgD + 2) * sizeof(float);
+  return (size_t)B * T * Hq * (pl.SP + pl.S) * (kPgD + 2) * sizeof(float);
 }
 
 extern "C" int q35_gated_attn_paged_shared(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* gate, int64_t g_sb,
@@ -1186,25 +1251,29 @@ extern "C" int q35_gated_attn_paged_shared(const void* q, int64_t q_sb, int64_t 
   if (chk != Q35_OK) return chk;
   const SharedPlan pl = shared_plan(B, T, Hkv, Hq / Hkv, shared_blocks * page_size, (n_blocks - shared_blocks) * page_size);
   const int64_t rows = B * T * Hq;
-  if (B * T * (Hq / Hkv) > (1 << 24) || Hkv * pl.RBP > 65535 || Hkv * pl.own.RB > 65535 || rows > 0x7fffffff)
+  if (B * T * (Hq / Hkv) > (1 << 24) || rows > 0x7fffffff)
     return Q35_EUNSUPPORTED;
-  const size_t slots = (size_t)rows * (pl.SP + pl.own.S);
+  const size_t slots = (size_t)rows * (pl.SP + pl.S);
   if (!workspace || workspace_bytes < slots * (kPgD + 2) * sizeof(float) || (uintptr_t)workspace & 15) return Q35_EWORKSPACE;
   a.part = (float*)workspace;
   a.ml = a.part + slots * kPgD;
-  a.S = pl.own.S, a.RB = pl.own.RB;
+  a.S = pl.S, a.RB = pl.RB;
   a.B = (int)B, a.n_sh = (int)(shared_blocks * page_size), a.Sp = pl.SP;
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const bool i4 = fmt == Q35_I4_G64;
-#define Q35_SHARED(I4, NR, KEYS, GRID) hipLaunchKernelGGL((paged_attn_kernel<I4, NR, 4, KEYS>), GRID, dim3(256), 0, st, a)
-  const dim3 gp(pl.SP, (unsigned)(Hkv * pl.RBP)), go(pl.own.S, (unsigned)(Hkv * pl.own.RB), (unsigned)B);
-  if (pl.NP == 1) { if (i4) Q35_SHARED(true, 1, kSharedKeys, gp); else Q35_SHARED(false, 1, kSharedKeys, gp); }
-  else { if (i4) Q35_SHARED(true, 2, kSharedKeys, gp); else Q35_SHARED(false, 2, kSharedKeys, gp); }
-  if (n_blocks > shared_blocks) {
-    if (pl.own.NR == 1) { if (i4) Q35_SHARED(true, 1, kOwnKeys, go); else Q35_SHARED(false, 1, kOwnKeys, go); }
-    else { if (i4) Q35_SHARED(true, 2, kOwnKeys, go); else Q35_SHARED(false, 2, kOwnKeys, go); }
+  const int64_t n_pre = (int64_t)pl.SP * Hkv * pl.RBP, n_own = n_blocks > shared_blocks ? (int64_t)pl.S * Hkv * pl.RB * B : 0;
+  if (n_pre + n_own > 0x7fffffff) return Q35_EUNSUPPORTED;
+  a.n_pre = (int)n_pre;
+  a.inv_g = (uint32_t)(0xFFFFFFFFu / (uint32_t)a.G), a.inv_t = (uint32_t)(0xFFFFFFFFu / (uint32_t)T);
+  const dim3 grid((unsigned)(n_pre + n_own)), block(256);
+  if (pl.NR == 1) {
+    if (i4) hipLaunchKernelGGL((paged_attn_kernel<true, 1, 4, kSplitKeys>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((paged_attn_kernel<false, 1, 4, kSplitKeys>), grid, block, 0, st, a);
+  } else {
+    if (i4) hipLaunchKernelGGL((paged_attn_kernel<true, 2, 4, kSplitKeys>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((paged_attn_kernel<false, 2, 4, kSplitKeys>), grid, block, 0, st, a);
   }
-#undef Q35_SHARED
-  hipLaunchKernelGGL(paged_attn_shared_merge_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
+  if (pl.SP + pl.S > 8 && rows <= 1024) hipLaunchKernelGGL((paged_attn_shared_merge_kernel<4>), dim3((unsigned)rows), block, 0, st, a);
+  else hipLaunchKernelGGL((paged_attn_shared_merge_kernel<1>), dim3((unsigned)((rows + 3) / 4)), block, 0, st, a);
   return hipGetLastError() == hipSuccess ? Q35_OK : Q35_ELAUNCH;
 }
