@@ -68,7 +68,7 @@ def rmsnorm_1p(x, w, eps=1e-6):
 
 
 def gated_deltanet_layer(x, p, conv_state, rec_state, head_scale=None, *, num_k_heads=None, head_k_dim=None,
-                         eps=1e-6, prefill="chunk", prenorm=None, residual=None, fixed_order=False):
+                         eps=1e-6, prefill="chunk", prenorm=None, residual=None, fixed_order=False, act_int8=False):
     """Gated DeltaNet mixer of one decoder layer (Qwen3_5GatedDeltaNet.forward, HF:432-543; the WGSL conv + delta
     kernels, engine/kernels_qwen35.js:127-247). x: [B, T, H] fp32 (the input-normed residual). A call with T == 1
     is one recurrent decode step (HF:505-517). T > 1 runs from rec_state either the chunked prefill (HF:518-530;
@@ -80,8 +80,9 @@ def gated_deltanet_layer(x, p, conv_state, rec_state, head_scale=None, *, num_k_
     the residual and the layer's input norm runs inside the input projection). Returns y [B, T, H], or with
     residual [B, T, H] given, residual + y computed in place by the output projection (then returned). For T > 1,
     x may be the int32 words of the normed rows already split for the int8 GEMM (add_rmsnorm_(..., split=True);
-    the layer must then have int8 input projections). fixed_order: the decode step's residual add sums every output
-    in one fixed order (repeatable bits; see linear())."""
+    the layer must then have int8 input projections), or RowsI8 (weights with one scale per row). fixed_order: the decode
+    step's residual add sums every output in one fixed order (repeatable bits; see linear()). act_int8: the two
+    projections of more than 8 rows as products in 8-bit integers (see linear())."""
     if prefill not in ("chunk", "recurrent"):
         raise ValueError(f"gated_deltanet_layer: prefill must be 'chunk' or 'recurrent', not {prefill!r}")
     B, T, _ = x.shape
@@ -109,7 +110,7 @@ def gated_deltanet_layer(x, p, conv_state, rec_state, head_scale=None, *, num_k_
         ops.gemv_gated_norm(o, y2[:, C:], p["norm"], wq_out, ws_out, out, head_scale=head_scale, eps=eps,
                             epilogue="store" if residual is None else ("add_fixed" if fixed_order else "add"))
         return residual if residual is not None else out.view(B, 1, N)
-    y = linear(x, w_in, wq_in, ws_in, prenorm=prenorm)
+    y = linear(x, w_in, wq_in, ws_in, prenorm=prenorm, act_int8=act_int8)
     if T == 1 and Hk == Hv and dk == dv == 128 and x.dtype == torch.float32:
         # the decode step's conv, recurrent rule and gated norm in one launch (the same arithmetic as the three
         # kernels below)
@@ -117,7 +118,7 @@ def gated_deltanet_layer(x, p, conv_state, rec_state, head_scale=None, *, num_k_
                                   rec_state, p["norm"], b_off=C + Vd, a_off=C + Vd + Hv, z_off=C,
                                   head_scale=head_scale, eps=eps)
         return linear(o.view(B, 1, Vd), p["out_proj"], *_q8(p, "out_proj"), residual=residual,
-                      fixed_order=fixed_order)
+                      fixed_order=fixed_order, act_int8=act_int8)
     if (T > 1 and prefill == "chunk" and _act_dtype(x) == torch.float32 and dk == dv == 128
             and p["conv1d"].shape[-1] == 4 and rec_state.is_contiguous()):
         # the conv + SiLU, l2 norms and gate terms in the chunk kernel's load phase (q, k, v, g, beta never written
@@ -136,14 +137,14 @@ def gated_deltanet_layer(x, p, conv_state, rec_state, head_scale=None, *, num_k_
             rec_state.copy_(S)
     # gated RMSNorm: plain w, norm before the silu(z) gate (HF:168-184; engine/kernels_qwen35.js:237-243)
     # (fp32 o before an int8 output projection: the result already split for the int8 GEMM)
-    split = T > 1 and o.dtype == torch.float32 and wq_out is not None and Vd % 64 == 0
+    split = T > 1 and o.dtype == torch.float32 and wq_out is not None and Vd % 64 == 0 and not act_int8
     o = ops.gated_rmsnorm(o, y[..., C:C + Vd], p["norm"], head_scale, eps, split=split)
-    return linear(o, p["out_proj"], wq_out, ws_out, residual=residual)
+    return linear(o, p["out_proj"], wq_out, ws_out, residual=residual, act_int8=act_int8)
 
 
 def _act_dtype(x):
-    """The value dtype of a layer input: fp32 for the int32 words of split activations."""
-    return torch.float32 if x.dtype == torch.int32 else x.dtype
+    """The value dtype of a layer input: fp32 for the int32 words of split activations and for rows in 8 bits."""
+    return torch.float32 if x.dtype == torch.int32 or isinstance(x, ops.RowsI8) else x.dtype
 
 
 def prenorm_torch(x, prenorm):
@@ -156,7 +157,29 @@ def prenorm_torch(x, prenorm):
     return ops.add_rmsnorm_(s, None, nw, eps)
 
 
-def linear(x, w, wq=None, ws=None, prenorm=None, residual=None, conv=None, fixed_order=False):
+def rows_int8(x, prenorm=None):
+    """x [..., K] fp32 or bf16 as RowsI8 [M, K]; prenorm (see linear()): the normed rows, x fp32."""
+    x = x.reshape(-1, x.shape[-1])
+    if prenorm is None:
+        return ops.quantize_rows(x)
+    x_add, nw, eps, x_out = prenorm
+    if x_add is None:
+        if x_out is not None:
+            x_out.view(x.shape).copy_(x)
+        return ops.add_rmsnorm_i8_(x, None, nw, eps)
+    s = x + x_add.reshape(x.shape)
+    if x_out is not None:
+        x_out.view(x.shape).copy_(s)
+    return ops.add_rmsnorm_i8_(s, None, nw, eps)
+
+
+def int8_rows_ok(wq, ws):
+    """Whether products with the weight wq, ws can take their rows in 8 bits: int8 with one scale per row, K a multiple of 64
+    up to 16384."""
+    return wq is not None and ws.dim() == 1 and wq.shape[1] % 64 == 0 and wq.shape[1] <= 16384
+
+
+def linear(x, w, wq=None, ws=None, prenorm=None, residual=None, conv=None, fixed_order=False, act_int8=False):
     """x [..., K] @ w[N, K]^T in fp32: the HIP GEMV for a few rows (decode), on the int8 weights wq with scales ws
     ([N, K / 128] per group or [N] per row; w their dequantised values) when given, else on w; for more rows the HIP
     int8 GEMM on wq (fp32-accurate) when given, else a torch GEMM on w. prenorm = (x_add, norm_w, eps, x_out): x is
@@ -168,9 +191,22 @@ def linear(x, w, wq=None, ws=None, prenorm=None, residual=None, conv=None, fixed
     int32 words of split activations (ops.split_activations) when wq is given: the int8 GEMM reads them as they are.
     fixed_order (with residual): the decode GEMV sums every output in one fixed order (the "add_fixed" epilogue:
     repeatable bits) instead of splitting K over blocks that add with atomics; the GEMM's sums are always in a fixed
-    order."""
+    order. act_int8: more than 8 rows against wq with one scale per row (K a multiple of 64, at most 16384) are taken in 8
+    bits, with one scale per row, and multiplied as integers (ops.quantize_rows, ops.gemm_i8): half the GEMM's operations and
+    less, for activations of 8 bits; other products are as without it. x may be RowsI8 itself."""
     K = x.shape[-1]
-    M = x.numel() // K
+    M = math.prod(x.shape[:-1])
+    rows = x.flat() if isinstance(x, ops.RowsI8) else None
+    if rows is not None and (prenorm is not None or not int8_rows_ok(wq, ws)):
+        raise ValueError("linear: rows in 8 bits need int8 weights with one scale per row, and take no prenorm")
+    if rows is None and act_int8 and M > 8 and conv is None and int8_rows_ok(wq, ws) and \
+            x.dtype in (torch.float32, torch.bfloat16) and (prenorm is None or x.dtype == torch.float32):
+        rows = rows_int8(x, prenorm)
+    if rows is not None and conv is None:
+        if residual is not None:
+            ops.gemm_i8(rows, wq, ws, out=residual.view(M, wq.shape[0]), epilogue="add")
+            return residual
+        return ops.gemm_i8(rows, wq, ws).view(*x.shape[:-1], wq.shape[0])
     N = (wq if wq is not None else w).shape[0]
     out, epi = (None, "store") if residual is None else (residual.view(M, N), "add_fixed" if fixed_order else "add")
     if M <= 8 and K % 256 == 0 and x.dtype == torch.float32 and (wq is not None or w.dtype == torch.float32):
@@ -227,7 +263,7 @@ def attn_in_weight(p):
 
 
 def gated_attention_layer(x, p, k_cache, v_cache, pos, *, rope_theta=1e7, partial_rotary_factor=0.25, eps=1e-6,
-                          cache_len=None, prenorm=None, residual=None, fixed_order=False):
+                          cache_len=None, prenorm=None, residual=None, fixed_order=False, act_int8=False):
     """Gated softmax attention mixer of one decoder layer (Qwen3_5Attention.forward, HF:656-701; WGSL attnPrep +
     attention, engine/kernels_qwen35.js:18-123). x: [B, T, H] fp32; the T tokens sit at positions pos..pos+T-1,
     pos a Python int or a [B] int32 device tensor (per row; a device tensor keeps the call capturable in a HIP
@@ -238,9 +274,9 @@ def gated_attention_layer(x, p, k_cache, v_cache, pos, *, rope_theta=1e7, partia
     of 64; for an fp32 y with the front end in its pre-pass, q35_gated_attn_prefill_cached_proj); T == 1 the split-K
     decode over cache positions 0..pos (cache_len: optional [B] int32 per-row lengths, default pos + 1; without it
     the q / k norms, RoPE and the cache append run inside the decode kernels, q35_gated_attn_decode_proj, instead of
-    a front-end launch). prenorm: see linear(). For T > 1, x may be the int32 words of split activations (see
+    a front-end launch). prenorm: see linear(). For T > 1, x may be the int32 words of split activations or RowsI8 (see
     gated_deltanet_layer). Returns y [B, T, H], or with residual [B, T, H] given,
-    residual + y computed in place by o_proj (then returned). fixed_order: see linear()."""
+    residual + y computed in place by o_proj (then returned). fixed_order, act_int8: see linear()."""
     B, T, _ = x.shape
     D = p["q_norm"].numel()
     Hq = p["q_proj"].shape[0] // (2 * D)
@@ -256,21 +292,21 @@ def gated_attention_layer(x, p, k_cache, v_cache, pos, *, rope_theta=1e7, partia
         pos_t = torch.full((B,), int(pos), dtype=torch.int32, device=x.device)
         own_keys = pos == 0
     cos, sin = rope_tables(max_len, rot, rope_theta, x.device)
-    y = linear(x, attn_in_weight(p), *_q8(p, "_in_fused"), prenorm=prenorm)
+    y = linear(x, attn_in_weight(p), *_q8(p, "_in_fused"), prenorm=prenorm, act_int8=act_int8)
     if T == 1 and cache_len is None and y.dtype == torch.float32 and y.shape[-1] % 4 == 0:
         # one token: the front end (q / k norms, RoPE, cache append) runs inside the decode kernels, reading y
         o = ops.gated_attention_decode_proj(y, p["q_norm"], p["k_norm"], k_cache, v_cache, pos_t, cos, sin,
                                             num_heads=Hq, eps=eps, scale=1.0 / math.sqrt(D),
                                             out_dtype=torch.float32).view(B, 1, Hq * D)
         wq_o, ws_o = _q8(p, "o_proj")
-        return linear(o, p["o_proj"], wq_o, ws_o, residual=residual, fixed_order=fixed_order)
+        return linear(o, p["o_proj"], wq_o, ws_o, residual=residual, fixed_order=fixed_order, act_int8=act_int8)
     if T > 1 and own_keys and y.dtype == torch.float32 and y.shape[-1] % 4 == 0:
         # the call's own tokens: the front end runs in the prefill's pre-pass, reading y (q35_gated_attn_prefill_proj)
         o = ops.gated_attention_prefill_proj(y, p["q_norm"], p["k_norm"], k_cache, v_cache, cos, sin, num_heads=Hq,
                                              pos0=0, eps=eps, scale=1.0 / math.sqrt(D))
         wq_o, ws_o = _q8(p, "o_proj")
         xo = o if (wq_o is not None and o.shape[-1] % 64 == 0) else o.float()
-        return linear(xo, p["o_proj"], wq_o, ws_o, residual=residual, fixed_order=fixed_order)
+        return linear(xo, p["o_proj"], wq_o, ws_o, residual=residual, fixed_order=fixed_order, act_int8=act_int8)
     if T > 1 and not own_keys and y.dtype == torch.float32 and y.shape[-1] % 4 == 0 and max_len % 64 == 0:
         # the same over the cache (tokens at per-row positions), the front end in the pre-pass
         # (q35_gated_attn_prefill_cached_proj)
@@ -278,7 +314,7 @@ def gated_attention_layer(x, p, k_cache, v_cache, pos, *, rope_theta=1e7, partia
                                                     num_heads=Hq, eps=eps, scale=1.0 / math.sqrt(D))
         wq_o, ws_o = _q8(p, "o_proj")
         xo = o if (wq_o is not None and o.shape[-1] % 64 == 0) else o.float()
-        return linear(xo, p["o_proj"], wq_o, ws_o, residual=residual, fixed_order=fixed_order)
+        return linear(xo, p["o_proj"], wq_o, ws_o, residual=residual, fixed_order=fixed_order, act_int8=act_int8)
     q, gate, k, v = ops.attn_prep(y, p["q_norm"], p["k_norm"], cos, sin, pos_t, k_cache, v_cache, num_heads=Hq,
                                   num_kv_heads=Hkv, eps=eps, want_kv=T > 1 and own_keys)
     if T > 1 and own_keys:
@@ -293,11 +329,12 @@ def gated_attention_layer(x, p, k_cache, v_cache, pos, *, rope_theta=1e7, partia
     wq_o, ws_o = _q8(p, "o_proj")
     # bf16 o straight into the int8 GEMM (the product of o.float(), bitwise); fp32 for the other forms
     xo = o if (T > 1 and wq_o is not None and o.shape[-1] % 64 == 0) else o.float()
-    return linear(xo, p["o_proj"], wq_o, ws_o, residual=residual, fixed_order=fixed_order)
+    return linear(xo, p["o_proj"], wq_o, ws_o, residual=residual, fixed_order=fixed_order, act_int8=act_int8)
 
 
 def gated_attention_layer_paged(x, p, pages, table, pos, *, lens=None, rope_theta=1e7, partial_rotary_factor=0.25,
-                                eps=1e-6, prenorm=None, residual=None, fixed_order=False, shared_blocks=0):
+                                eps=1e-6, prenorm=None, residual=None, fixed_order=False, shared_blocks=0,
+                                act_int8=False):
     """gated_attention_layer over a paged KV cache in bf16 or 4 bits (ops.kv_pages; head dim 256): a decode step (T = 1),
     the check of drafted tokens (a few), a chunk of a prompt (many). x: [B, T, H] fp32; token t < lens[b] of row b (lens
     [B] int32 on the device, None: all T) sits at position pos[b] + t ([B] int32 on the device); its key and value go into
@@ -306,27 +343,28 @@ def gated_attention_layer_paged(x, p, pages, table, pos, *, lens=None, rope_thet
     lens. The first call stacks the weights, and the first over a table of more positions than any before waits for the
     rotation tables (rope_tables), so make one of each ahead of a capture; other calls synchronise with nothing. shared_blocks: how
     many of the table's first blocks name the same pages in every row (several continuations of one prompt): their keys are
-    read once for all rows (ops.gated_attention_paged_shared). prenorm, residual, fixed_order: see gated_attention_layer."""
+    read once for all rows (ops.gated_attention_paged_shared). prenorm, residual, fixed_order, act_int8: see
+    gated_attention_layer."""
     B, T, _ = x.shape
     D = p["q_norm"].numel()
     Hq = p["q_proj"].shape[0] // (2 * D)
     Hkv = p["k_proj"].shape[0] // D
     cos, sin = _rope_tables_over(table.shape[1] * pages[0].shape[2], int(D * partial_rotary_factor), rope_theta, x.device)
-    y = linear(x, attn_in_weight(p), *_q8(p, "_in_fused"), prenorm=prenorm)
+    y = linear(x, attn_in_weight(p), *_q8(p, "_in_fused"), prenorm=prenorm, act_int8=act_int8)
     q, k, v = y.split([2 * Hq * D, Hkv * D, Hkv * D], -1)
     q = q.unflatten(-1, (Hq, 2 * D))
     ops.paged_kv_append_(k.unflatten(-1, (Hkv, D)), v.unflatten(-1, (Hkv, D)), pages, table, pos, cos, sin, lens=lens,
                          k_norm_w=p["k_norm"].float().contiguous(), eps=eps)
-    # as the dense layer: fp32 for the GEMV of a few rows, bf16 for the int8 GEMM
+    # as the dense layer: fp32 for the GEMV of a few rows, bf16 for the int8 GEMM (fp32 again for rows in 8 bits: one rounding)
     wq_o, ws_o = _q8(p, "o_proj")
-    half = B * T > 8 and wq_o is not None
+    half = B * T > 8 and wq_o is not None and not (act_int8 and int8_rows_ok(wq_o, ws_o))
     args = dict(lens=lens, q_norm_w=p["q_norm"].float().contiguous(), eps=eps, scale=1.0 / math.sqrt(D),
                 out_dtype=torch.bfloat16 if half else torch.float32)
     if shared_blocks:
         o = ops.gated_attention_paged_shared(q[..., :D], q[..., D:], pages, table, pos, cos, sin, shared_blocks, **args)
     else:
         o = ops.gated_attention_paged(q[..., :D], q[..., D:], pages, table, pos, cos, sin, **args)
-    return linear(o, p["o_proj"], wq_o, ws_o, residual=residual, fixed_order=fixed_order)
+    return linear(o, p["o_proj"], wq_o, ws_o, residual=residual, fixed_order=fixed_order, act_int8=act_int8)
 
 
 def residual_steer_add(x, vecs, rows=None):

@@ -7,6 +7,8 @@ SwiGLU MLP -> + residual -> [steering add]. The mixers and the steering add are 
 q35hip.layers; the model owns their states (GDN conv / recurrent states, bf16 KV caches) and mutates them in place
 (engine/model.js:308-342).
 """
+import math
+
 import torch
 
 from . import layers, ops
@@ -55,6 +57,7 @@ def mlp_weights(p):
 _GDN_IN = ("in_proj_qkv", "in_proj_z", "in_proj_b", "in_proj_a")
 _ATTN_IN = ("q_proj", "k_proj", "v_proj")
 _MLP_IN = ("gate_proj", "up_proj")
+_MLP = (*_MLP_IN, "down_proj")
 
 
 def _split_ok(p, names, x):
@@ -63,7 +66,12 @@ def _split_ok(p, names, x):
     return x.shape[-1] % 64 == 0 and all(n + ".q" in p for n in names)
 
 
-def mlp(p, h, x, prenorm=None, capture=None, fixed_order=False):
+def _rows8_ok(p, names):
+    """Whether the products `names` of a layer can take their rows in 8 bits (layers.int8_rows_ok)."""
+    return all(layers.int8_rows_ok(p.get(n + ".q"), p.get(n + ".s")) for n in names)
+
+
+def mlp(p, h, x, prenorm=None, capture=None, fixed_order=False, act_int8=False):
     """x += SwiGLU MLP (HF:704-717) of h, in place, with the layer's neuron pushes at the down_proj input
     (engine/model.js:7-9, engine/kernels_qwen35.js:250-279). Decode (at most 8 rows, int8 weights present): one GEMV
     over the interleaved int8 gate/up rows with the SwiGLU + push epilogue, and one int8 GEMV accumulating down_proj
@@ -75,13 +83,22 @@ def mlp(p, h, x, prenorm=None, capture=None, fixed_order=False):
     the layer has int8 weights: the gate/up GEMM reads them as they are. capture: an fp32 view [rows, T, I] (unit
     neuron stride) that receives the post-push activations, the down_proj input (the engine's capture hook,
     engine/model.js:9, :451-453), written by the SwiGLU epilogue itself. fixed_order: the decode down_proj sums
-    every output in one fixed order (repeatable bits; layers.linear). Returns x."""
+    every output in one fixed order (repeatable bits; layers.linear). act_int8: both products of more than 8 rows in 8-bit
+    integers, where the weights have one scale per row (layers.linear), the activations between them in 8 bits too; h may then
+    be RowsI8. Returns x."""
     mlp_weights(p)
     H = h.shape[-1]
-    M = h.numel() // H
-    T = h.shape[1] if h.dim() == 3 else 1
+    M = math.prod(h.shape[:-1])
+    T = h.shape[1] if len(h.shape) == 3 else 1
     # h + y_add is written to x when x is another buffer; with x = h and no y_add the norm reads h as it is
     pn = None if prenorm is None else (prenorm[0], prenorm[1], prenorm[2], None if x is h else x)
+    if isinstance(h, ops.RowsI8) or (act_int8 and M > 8 and _rows8_ok(p, _MLP) and h.dtype == torch.float32):
+        if not _rows8_ok(p, _MLP):
+            raise ValueError("mlp: rows in 8 bits need int8 weights with one scale per row")
+        rows = h.flat() if isinstance(h, ops.RowsI8) else layers.rows_int8(h, pn)
+        a = ops.gemm_i8(rows, p["_gu_q8"], p["_gu_s"], epilogue="swiglu", pushes=p["_pushes"], T=T, capture=capture)
+        ops.gemm_i8(ops.quantize_rows(a), p["down_proj.q"], p["down_proj.s"], out=x.view(M, H), epilogue="add")
+        return x
     if M <= 8 and "_gu_q8" in p and H % 256 == 0 and p["down_proj.q"].shape[1] % 256 == 0 and \
             h.dtype == torch.float32:
         pn2 = None if pn is None else (None if pn[0] is None else pn[0].reshape(M, H), pn[1], pn[2],
@@ -126,17 +143,22 @@ class HybridModel:
     deterministic: the decode step's residual adds (the mixers' output projections and down_proj) sum every output
     in one fixed order, so that two runs give identical logits bit for bit; by default these N = hidden products
     split K over four blocks that add with fp32 atomics (faster; the last bits of a step may vary between runs).
-    Prefill is deterministic either way."""
+    Prefill is deterministic either way.
+
+    act_int8: the layers' products of more than 8 rows (prefill, and steps of more rows) whose weights are int8 with one
+    scale per row take their rows in 8 bits, one scale per token, and multiply integers (layers.linear, mlp): faster than
+    the fp32-accurate products, with activations rounded to 8 bits. Products of other weights, of few rows and the LM head
+    are as without it; a model none of whose weights can raises."""
 
     MAX_VECS = 4  # vector rows of the steering buffer (the WGSL resAdd clamps its row index to 3, engine/kernels.js:201)
 
     def __init__(self, cfg, W, device, max_len=4096, rows=3, steer_layer=12, gdn_prefill="chunk",
-                 deterministic=False):
+                 deterministic=False, act_int8=False):
         if gdn_prefill not in ("chunk", "recurrent"):
             raise ValueError(f"HybridModel: gdn_prefill must be 'chunk' or 'recurrent', not {gdn_prefill!r}")
         self.cfg, self.device, self.steer_layer = cfg, device, steer_layer
         self.gdn_prefill = gdn_prefill
-        self.deterministic = bool(deterministic)
+        self.deterministic, self.act_int8 = bool(deterministic), bool(act_int8)
         self.W = W if isinstance(W, Q35Weights) else Q35Weights(W, device)
         # the KV caches hold a multiple of 64 positions (the multi-token attention over the cache reads 64-key tiles)
         self.max_len, self.rows = (max_len + 63) // 64 * 64, rows
@@ -153,6 +175,8 @@ class HybridModel:
                 # the engine's per-head output scale (engine/model.js:362-368): 1 for every head until set
                 p["_head_scale"] = torch.ones(cfg.lin_v_heads, device=device)
             mlp_weights(p)
+        if self.act_int8 and not any(_rows8_ok(p, names) for p in self.params for names in (("_in_fused",), _MLP)):
+            raise ValueError("HybridModel: act_int8 needs int8 weights with one scale per row, inputs a multiple of 64 up to 16384")
         self.states = []
         for l in range(cfg.layers):
             if cfg.is_attention(l):
@@ -267,7 +291,7 @@ class HybridModel:
                 res_buf[l, :, res_t0:res_t0 + T].copy_(x.view(res_buf.shape[1], T, -1))
         pos_dev, vec_rows = self.pos_dev[rs], self.vec_rows[rs]
         if T == 1:
-            fx = self.deterministic
+            fx, i8 = self.deterministic, self.act_int8
             for l in range(last + 1):
                 p = self.params[l]
                 st = {n: t[rs] for n, t in self.states[l].items()}
@@ -275,14 +299,15 @@ class HybridModel:
                 if cfg.is_attention(l):
                     layers.gated_attention_layer(x, p, st["k"], st["v"], pos_dev, rope_theta=cfg.rope_theta,
                                                  partial_rotary_factor=cfg.partial_rotary, eps=cfg.eps,
-                                                 prenorm=pre, residual=x, fixed_order=fx)
+                                                 prenorm=pre, residual=x, fixed_order=fx, act_int8=i8)
                 else:
                     layers.gated_deltanet_layer(x, p, st["conv"], st["rec"], p["_head_scale"],
                                                 num_k_heads=cfg.lin_k_heads, head_k_dim=cfg.lin_dk, eps=cfg.eps,
-                                                prefill=self.gdn_prefill, prenorm=pre, residual=x, fixed_order=fx)
+                                                prefill=self.gdn_prefill, prenorm=pre, residual=x, fixed_order=fx,
+                                                act_int8=i8)
                 snap(l, "mixer")
                 mlp(p, x, x, prenorm=(None, p["post_attention_layernorm"], cfg.eps), capture=cap_view(l),
-                    fixed_order=fx)
+                    fixed_order=fx, act_int8=i8)
                 if l == self.steer_layer and steer:
                     layers.residual_steer_add(x, self.vec_buf, vec_rows)
                 snap(l, "layer")
@@ -290,20 +315,26 @@ class HybridModel:
                     collected = x.clone()
             return x, collected
         y = None  # the previous mixer's output, added to x by the next norm
+
+        def normed(y, w, names):
+            # the norms hand the int8 GEMMs their rows already split (bf16 hi + lo), or in 8 bits, when the layer's products
+            # are int8
+            if self.act_int8 and _rows8_ok(p, names):
+                return ops.add_rmsnorm_i8_(x, y, w, cfg.eps)
+            return ops.add_rmsnorm_(x, y, w, cfg.eps, split=_split_ok(p, _MLP_IN if names is _MLP else names, x))
         for l in range(last + 1):
             p = self.params[l]
             st = {n: t[rs] for n, t in self.states[l].items()}
-            # the norms hand the int8 GEMMs their rows already split (bf16 hi + lo) when the layer's products are int8
-            mixer = _ATTN_IN if cfg.is_attention(l) else _GDN_IN
-            h = ops.add_rmsnorm_(x, y, p["input_layernorm"], cfg.eps, split=_split_ok(p, mixer, x))
+            h = normed(y, p["input_layernorm"], _ATTN_IN if cfg.is_attention(l) else _GDN_IN)
             if cfg.is_attention(l):
                 y = layers.gated_attention_layer(h, p, st["k"], st["v"], attn_pos, rope_theta=cfg.rope_theta,
-                                                 partial_rotary_factor=cfg.partial_rotary, eps=cfg.eps)
+                                                 partial_rotary_factor=cfg.partial_rotary, eps=cfg.eps,
+                                                 act_int8=self.act_int8)
             else:
                 y = layers.gated_deltanet_layer(h, p, st["conv"], st["rec"], p["_head_scale"],
                                                 num_k_heads=cfg.lin_k_heads, head_k_dim=cfg.lin_dk, eps=cfg.eps,
-                                                prefill=self.gdn_prefill)
-            h = ops.add_rmsnorm_(x, y, p["post_attention_layernorm"], cfg.eps, split=_split_ok(p, _MLP_IN, x))
+                                                prefill=self.gdn_prefill, act_int8=self.act_int8)
+            h = normed(y, p["post_attention_layernorm"], _MLP if self.act_int8 else _MLP_IN)
             y = None
             snap(l, "mixer")
             mlp(p, h, x, capture=cap_view(l))
@@ -484,6 +515,25 @@ def greedy(model, prompt_ids, steps):
         margins.append(top2.values[:, 0] - top2.values[:, 1])
         logits = model.decode_step(nxt)
     return torch.stack(toks, 1).cpu(), torch.stack(margins, 1).cpu()
+
+
+@torch.no_grad()
+def sampled(model, prompt_ids, steps, *, u=None, generator=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """Prefill prompt_ids [B, T], then `steps` tokens drawn with ops.sample_tokens (temperature, top_k, top_p, min_p: numbers, or
+    one per row [B] on the device). u: the draws' random numbers [B, steps] fp32 in [0, 1) on the device (None: torch.rand
+    with `generator`). The host waits for nothing between the steps. Returns tokens [B, steps] on the CPU."""
+    logits, _ = model.forward(prompt_ids)
+    if u is None:
+        u = torch.rand(logits.shape[0], steps, generator=generator, device=logits.device)
+    if tuple(u.shape) != (logits.shape[0], steps):
+        raise ValueError(f"sampled: u must be [{logits.shape[0]}, {steps}]")
+    toks = []
+    for i in range(steps):
+        nxt = ops.sample_tokens(logits, u[:, i].contiguous(), temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        toks.append(nxt)
+        if i + 1 < steps:
+            logits = model.decode_step(nxt)
+    return torch.stack(toks, 1).long().cpu()
 
 
 def median_resid_norm(resid_row):

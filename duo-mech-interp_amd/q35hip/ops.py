@@ -1351,6 +1351,22 @@ class RowsI8(NamedTuple):
     q: torch.Tensor
     s: torch.Tensor
 
+    @property
+    def shape(self):
+        return self.q.shape
+
+    @property
+    def dtype(self):
+        return self.q.dtype
+
+    @property
+    def device(self):
+        return self.q.device
+
+    def flat(self):
+        """The same rows as [M, K] and [M]."""
+        return RowsI8(self.q.reshape(-1, self.q.shape[-1]), self.s.reshape(-1))
+
 
 def quantize_rows(x):
     """x [..., K] fp32 or bf16 (dense rows, evenly strided; K a multiple of 4, at most 16384) as RowsI8: s = fp32(max |x| / 127),
