@@ -14,7 +14,7 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 // ---------------------------------------------------------------------------------------------------------------
 // Rows in 8 bits, one block a row, held in registers: PER quads of values a thread, so that memory is passed over once. 16384
-// rows of 3584 fp32 values take 60 us, 4.9 TB/s of the 294 MB read and written (a large copy reaches 5.2).
+// rows of 3584 fp32 values take 54 us, 5.4 TB/s of the 294 MB read and written (a large copy reaches 5.2).
 
 // rint(x / s), half to even: x, s exact, |x / s| <= 127.5. The remainder settles what the product with 1 / s left undecided.
 __device__ __forceinline__ int i8_code(double x, double s, double inv) {
@@ -24,93 +24,151 @@ __device__ __forceinline__ int i8_code(double x, double s, double inv) {
   return (int)fmin(fmax(t, -127.0), 127.0);
 }
 
-template <typename Tx, bool NORM, int PER>
-__global__ __launch_bounds__(256) void rows_i8_kernel(Tx* __restrict__ x, int64_t ldx, const float* __restrict__ y,
+// Values and quotients are formed in fp32 first, 2^-21 of themselves: an element whose quotient is then within 2^-12 of a half,
+// or whose factors leave fp32's middle range, is formed again in 64 bits, and so are those within 2^-19 of the largest, for
+// the scale. A row whose scale is far from 1 is formed in 64 bits as a whole. (All elements in 64 bits: three times the
+// operations, 68 us for those 16384 rows.)
+constexpr float kI8Far = 0x1p100f;
+
+template <typename Tx, bool NORM, int NW, int PER>
+__global__ __launch_bounds__(64 * NW) void rows_i8_kernel(Tx* __restrict__ x, int64_t ldx, const float* __restrict__ y,
                                                       int64_t ldy, const float* __restrict__ w, int8_t* __restrict__ q,
                                                       float* __restrict__ s, int K, float eps) {
   const int64_t m = blockIdx.x;
   const int tid = threadIdx.x;
   Tx* xr = x + m * ldx;
-  double v[PER][4];
+  f32x4 f[PER], v[NORM ? PER : 1], w1;
   double ss = 0.0;
-  float mx = 0.f;
-  bool odd = false;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int c = 4 * (tid + 256 * i);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[i][e] = 0.0;
+    const int c = 4 * (tid + 64 * NW * i);
+    f[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (c < K) {
-      f32x4 f;
       if constexpr (sizeof(Tx) == 4) {
-        f = *reinterpret_cast<const f32x4*>(xr + c);
+        f[i] = *reinterpret_cast<const f32x4*>(xr + c);
       } else {
         const u32x2 r = *reinterpret_cast<const u32x2*>(xr + c);
-        f = f32x4{bf16lo(r.x), bf16hi(r.x), bf16lo(r.y), bf16hi(r.y)};
+        f[i] = f32x4{bf16lo(r.x), bf16hi(r.x), bf16lo(r.y), bf16hi(r.y)};
       }
       if constexpr (NORM) {
+        v[i] = w1 = *reinterpret_cast<const f32x4*>(w + c);
         if (y) {
           const f32x4 a = *reinterpret_cast<const f32x4*>(y + m * ldy + c);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) f[e] += a[e];
-          *reinterpret_cast<f32x4*>(xr + c) = f;
+          for (int e = 0; e < 4; ++e) f[i][e] += a[e];
+          *reinterpret_cast<f32x4*>(xr + c) = f[i];
         }
-      }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[i][e] = f[e];
-        if constexpr (NORM) ss += v[i][e] * v[i][e];
+        for (int e = 0; e < 4; ++e) ss = __builtin_fma((double)f[i][e], (double)f[i][e], ss);
       }
     }
   }
-  __shared__ double red[4];
-  __shared__ float redm[4];
-  __shared__ int redo[4];
+  __shared__ double red[NW];
+  __shared__ float redm[2][NW];
+  __shared__ int redo[NW];
+  const int wave = tid >> 6;
+  double r = 1.0;
   if constexpr (NORM) {
     ss = wave_sum64(ss);
-    if ((tid & 63) == 0) red[tid >> 6] = ss;
-    __syncthreads();
-    const double r = 1.0 / sqrt((red[0] + red[1] + red[2] + red[3]) / (double)K + (double)eps);
+    if constexpr (NW > 1) {
+      if ((tid & 63) == 0) red[wave] = ss;
+      __syncthreads();
+      ss = red[0] + red[1] + red[2] + red[3];
+    }
+    r = 1.0 / sqrt(ss / (double)K + (double)eps);
+  }
+  // one quad a thread: all of them in 64 bits for the scale, for one barrier less (32 rows of 1024: 3.3 us, 4.1 with it)
+  constexpr bool kAll = NORM && NW > 1 && PER == 1;
+  auto exact = [&](int i, int e) -> double {
+    if constexpr (!NORM) return (double)f[i][e];
+    return (double)f[i][e] * r * (1.0 + (double)(PER == 1 ? w1[e] : w[4 * (tid + 64 * NW * i) + e]));
+  };
+  // v: the values in fp32, NaN where these cannot be relied on
+  bool odd = false;
+  float mx = 0.f;
+  if constexpr (NORM) {
+    const float rf = (float)r;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int c = 4 * (tid + 256 * i);
-      if (c < K) {
-        const f32x4 wv = *reinterpret_cast<const f32x4*>(w + c);
+      const bool in = 4 * (tid + 64 * NW * i) < K;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[i][e] = v[i][e] * r * (1.0 + (double)wv[e]);
+      for (int e = 0; e < 4; ++e) {
+        const float g = rf * (1.f + v[i][e]), t = f[i][e] * g;
+        const bool good = fabsf(g) > 1.f / kI8Far && fabsf(g) < kI8Far && fabsf(t) < kI8Far;
+        v[i][e] = in ? (good ? t : NAN) : 0.f;
+        mx = fmaxf(mx, v[i][e] == v[i][e] ? fabsf(v[i][e]) : 0.f);
       }
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        odd |= !(fabsf(f[i][e]) < INFINITY);
+        mx = fmaxf(mx, fabsf(f[i][e]));
+      }
   }
-  double md = 0.0;
-#pragma unroll
-  for (int i = 0; i < PER; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      odd |= !(fabs(v[i][e]) < INFINITY);
-      md = fmax(md, fabs(v[i][e]));
+  if constexpr (!kAll) mx = wave_max_f32(mx);
+  if constexpr (NORM) {
+    if constexpr (!kAll && NW > 1) {
+      if ((tid & 63) == 0) redm[0][wave] = mx;
+      __syncthreads();
+      mx = fmaxf(fmaxf(redm[0][0], redm[0][1]), fmaxf(redm[0][2], redm[0][3]));
     }
-  // the scale of the largest: fp32(max / 127) is monotone, so the maximum of the rounded quotients
-  mx = wave_max_f32((float)(md / 127.0));
-  const bool any = __builtin_amdgcn_ballot_w64(odd) != 0;
-  if ((tid & 63) == 0) {
-    redm[tid >> 6] = mx;
-    redo[tid >> 6] = any;
+    const float near = !kAll && mx > 1.f / kI8Far ? mx * (1.f - 0x1p-19f) : 0.f;
+    double md = 0.0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      bool any = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) any |= !(fabsf(v[i][e]) < near);
+      if (any && 4 * (tid + 64 * NW * i) < K) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const double d = fabs(exact(i, e));
+          odd |= !(d < INFINITY);
+          md = fmax(md, d);
+        }
+      }
+    }
+    // the scale of the largest: fp32(max / 127) is monotone, so the maximum of the rounded quotients
+    mx = wave_max_f32((float)(md / 127.0));
   }
-  __syncthreads();
+  bool bad = __builtin_amdgcn_ballot_w64(odd) != 0;
+  if constexpr (NW > 1) {
+    if ((tid & 63) == 0) {
+      redm[1][wave] = mx;
+      redo[wave] = bad;
+    }
+    __syncthreads();
+    mx = fmaxf(fmaxf(redm[1][0], redm[1][1]), fmaxf(redm[1][2], redm[1][3]));
+    bad = redo[0] | redo[1] | redo[2] | redo[3];
+  }
   // a row that holds a value that is not finite has the scale NaN, and its products are NaN
-  const float sc = fmaxf(fmaxf(redm[0], redm[1]), fmaxf(redm[2], redm[3]));
-  const bool bad = redo[0] | redo[1] | redo[2] | redo[3] || !(sc < INFINITY);
+  const float sc = NORM ? mx : (float)((double)mx / 127.0);
+  bad |= !(sc < INFINITY);
   if (tid == 0) s[m] = bad ? __int_as_float(0x7fc00000) : sc;
-  const bool none = bad || !(sc > 0.f);
+  const bool none = bad || !(sc > 0.f), all = !(sc > 1.f / kI8Far && sc < kI8Far);
   const double sd = none ? 1.0 : (double)sc, inv = 1.0 / sd;
+  const float invf = (float)inv;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int c = 4 * (tid + 256 * i);
+    const int c = 4 * (tid + 64 * NW * i);
     if (c < K) {
       uint32_t o = 0;
+      bool again = false;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o |= (uint32_t)(uint8_t)(none ? 0 : i8_code(v[i][e], sd, inv)) << (8 * e);
-      *reinterpret_cast<uint32_t*>(q + m * K + c) = o;
+      for (int e = 0; e < 4; ++e) {
+        const float t = (NORM ? v[i][e] : f[i][e]) * invf, n = __builtin_rintf(t);
+        again |= !(fabsf(t - n) < 0.5f - 0x1p-12f);
+        o |= (uint32_t)(uint8_t)(int)n << (8 * e);
+      }
+      if (again || all) {
+        o = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o |= (uint32_t)(uint8_t)i8_code(exact(i, e), sd, inv) << (8 * e);
+      }
+      *reinterpret_cast<uint32_t*>(q + m * K + c) = none ? 0 : o;
     }
   }
 }
@@ -118,13 +176,19 @@ __global__ __launch_bounds__(256) void rows_i8_kernel(Tx* __restrict__ x, int64_
 template <typename Tx, bool NORM>
 static int rows_i8_launch(Tx* x, int64_t ldx, const float* y, int64_t ldy, const float* w, int8_t* q, float* s, int64_t M,
                           int64_t K, float eps, hipStream_t st) {
-#define Q35_ROWS(PER)                                                                                                   \
-  hipLaunchKernelGGL((rows_i8_kernel<Tx, NORM, PER>), dim3((unsigned)M), dim3(256), 0, st, x, ldx, y, ldy, w, q, s, (int)K, eps)
-  if (K <= 1024) Q35_ROWS(1);
-  else if (K <= 2048) Q35_ROWS(2);
-  else if (K <= 4096) Q35_ROWS(4);
-  else if (K <= 8192) Q35_ROWS(8);
-  else Q35_ROWS(16);
+#define Q35_ROWS(NW, PER)                                                                                                \
+  hipLaunchKernelGGL((rows_i8_kernel<Tx, NORM, NW, PER>), dim3((unsigned)M), dim3(64 * NW), 0, st, x, ldx, y, ldy, w, q, s, \
+                     (int)K, eps)
+  // one wave a row of up to 1024 values where there are rows for all CUs to hold eight (normed rows of 1024 by one wave and by
+  // four: 6144 rows 10.8 and 14.1 us, 2048 6.6 and 6.9, 1024 6.2 and 4.8, 32 4.9 and 3.3)
+  if (K <= 256) Q35_ROWS(1, 1);
+  else if (K <= 512) Q35_ROWS(1, 2);
+  else if (K <= 1024 && M >= 2048) Q35_ROWS(1, 4);
+  else if (K <= 1024) Q35_ROWS(4, 1);
+  else if (K <= 2048) Q35_ROWS(4, 2);
+  else if (K <= 4096) Q35_ROWS(4, 4);
+  else if (K <= 8192) Q35_ROWS(4, 8);
+  else Q35_ROWS(4, 16);
 #undef Q35_ROWS
   return hipGetLastError() == hipSuccess ? Q35_OK : Q35_ELAUNCH;
 }
