@@ -1394,7 +1394,7 @@ def gemm_i8(x, W, w_scale, out=None, epilogue="store", pushes=None, T=1, capture
         if y is not NotImplemented:
             return y if out is None else out
     if out is None:
-        out = torch.empty(*q.shape[:-1], W.shape[0] // (2 if e == 2 else 1), dtype=torch.float32, device=q.device)
+        out = s.new_empty(*q.shape[:-1], W.shape[0] // (2 if e == 2 else 1))
     torch.ops.q35.gemm_i8_(q, s, W, w_scale, out, e, pushes, int(T), capture)
     return out
 
