@@ -19,6 +19,7 @@
 //                        bins itself, of the groups that reach the k-th largest group's bin: all larger tokens are in them
 //   sample_write_kernel  probabilities or cut logits, where they are asked for
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "token_weights.h"
@@ -27,7 +28,7 @@ namespace q35 {
 
 typedef unsigned long long u64;
 constexpr int kSBins = 2048, kSFine = 1536;
-constexpr int kSChunk = 1024;    // quads of a block of the maximum and the write kernel: 256 groups of 4
+constexpr int kSChunk = 1024;    // quads of a block of the maximum and the write kernel: 256 groups of 4 neighbouring ones
 constexpr int kSFew = 1024;      // the largest top-k whose rows need no histogram
 constexpr int kSThreads = 1024;  // of the pick kernel
 constexpr int kSHeld = 10;       // groups' maxima that one of its threads holds
@@ -65,6 +66,7 @@ struct SampleArgs {
   float* out;  // [rows][V]
 };
 
+constexpr double kSFar = 1100.0 * kVTab;  // 1/32 octaves from where on a weight is 0
 struct SampleRow {
   const float* x;
   double inv_t;  // 32 log2(e) / T
@@ -93,29 +95,37 @@ __device__ __forceinline__ SampleRow s_row(const SampleArgs& a, int row) {
   return r;
 }
 
-// The distance of x from the maximum M in 1/32 octaves of the weight, rounded, and the weight in units of 2^-S: 2^(z / 32) as in
-// exp2_neg, with S in the exponent and the conversion to a whole number by adding 2^52 (fp64 has no other short one).
-constexpr double kSFar = 1100.0 * kVTab;  // 0 from there on, also for -inf
+// The distance of x from the maximum M in 1/32 octaves of the weight, and the weight in units of 2^-S: 2^(-z / 32) by the series
+// of exp2_neg, with S in the exponent, and both conversions to whole numbers by adding a power of two (fp64 has no other short
+// one): 25 operations a token where rint, conversions and a comparison with an infinite maximum took 34 (256 rows of 151,936
+// 49 -> 43 us).
 struct SampleWeight {
   int n;
   u64 w;
 };
-__device__ __forceinline__ double s_z(float x, float M, double inv_t) {
-  return x == M ? 0.0 : fmin(((double)M - (double)x) * inv_t, kSFar);
+struct SampleDistance {
+  int n;
+  double r;  // distance less n
+};
+__device__ __forceinline__ SampleDistance s_distance(float x, float M, const SampleRow& r) {
+  constexpr double kRound = 0x1.8p52;
+  // (an infinite maximum is the largest number, from which the finite ones are as far as from any)
+  const double m = fmin((double)M, DBL_MAX), z = fmin((m - fmin((double)x, DBL_MAX)) * r.inv_t, kSFar), t = z + kRound;
+  return {(int)(uint32_t)__builtin_bit_cast(u64, t), z - (t - kRound)};
 }
-__device__ __forceinline__ SampleWeight s_weight(float x, float M, double inv_t, int S, const double* tab) {
+__device__ __forceinline__ SampleWeight s_weight(float x, float M, const SampleRow& row, int S, const double* tab) {
   constexpr double c1 = -0.69314718055994530942 / kVTab, c2 = c1 * c1 / 2.0, c3 = c1 * c2 / 3.0, c4 = c1 * c3 / 4.0;
-  const double z = s_z(x, M, inv_t), n = __builtin_rint(z), r = z - n;
-  const int k = -(int)n;
-  const double e = __builtin_fma(__builtin_fma(__builtin_fma(__builtin_fma(c4, r, c3), r, c2), r, c1), r, 1.0);
+  const SampleDistance z = s_distance(x, M, row);
+  const double e = __builtin_fma(__builtin_fma(__builtin_fma(__builtin_fma(c4, z.r, c3), z.r, c2), z.r, c1), z.r, 1.0);
+  const int k = -z.n;
   const double w = __builtin_ldexp(e * tab[k & (kVTab - 1)], (k >> 5) + S) + 0x1p52;
-  return {-k, __builtin_bit_cast(u64, w) & 0xFFFFFFFFFFFFFull};
+  return {z.n, __builtin_bit_cast(u64, w) & 0xFFFFFFFFFFFFFull};
 }
 // The bin of a distance: 1/32 octave each for 48 octaves, then an octave each. Never larger for a larger x.
 __device__ __forceinline__ int s_bin(int n) {
-  return n < kSFine ? n : min(kSFine + ((n - kSFine) >> 5), kSBins - 1);
+  return min(min(n, kSFine - (kSFine >> 5) + (n >> 5)), kSBins - 1);
 }
-__device__ __forceinline__ int s_bin(float x, float M, double inv_t) { return s_bin((int)__builtin_rint(s_z(x, M, inv_t))); }
+__device__ __forceinline__ int s_bin(float x, float M, const SampleRow& r) { return s_bin(s_distance(x, M, r).n); }
 // Order-preserving bits (-0 as +0; no NaN).
 __device__ __forceinline__ uint32_t s_key(float x) {
   const uint32_t b = __float_as_uint(x == 0.f ? 0.f : x);
@@ -201,16 +211,22 @@ __global__ __launch_bounds__(256) void sample_max_kernel(SampleArgs a) {
     }
   }
   const int last = min((c + 1) * kSChunk, s.n());
-  float m = -INFINITY;
+  float m = -INFINITY, mine = -INFINITY;
 #pragma unroll
-  for (int u = 0; u < kSChunk / 256; ++u) {
+  for (int u = 0; u < 4; ++u) {
     const int q = c * kSChunk + tid + 256 * u;
+    float mq = -INFINITY;
     if (q < last) {
       const f32x4 v = s.load(q);
-      m = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), m);
+      mq = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
     }
+    m = fmaxf(mq, m);
+    // a group's quads lie in four lanes, of which lane u keeps the u-th one's
+    mq = fmaxf(mq, __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(mq), 0xB1, 0xF, 0xF, false)));
+    mq = fmaxf(mq, __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(mq), 0x4E, 0xF, 0xF, false)));
+    if ((tid & 3) == u) mine = mq;
   }
-  a.gmax[((size_t)row * a.C + c) * 256 + tid] = m;
+  a.gmax[((size_t)row * a.C + c) * 256 + 64 * (tid & 3) + (tid >> 2)] = mine;
   m = wave_max_f32(m);
   __shared__ float sm[4];
   if ((tid & 63) == 0) sm[tid >> 6] = m;
@@ -242,7 +258,7 @@ __global__ __launch_bounds__(256) void sample_hist_kernel(SampleArgs a) {
   __syncthreads();
   const int nq = s.n(), per = (nq + a.R - 1) / a.R, first = blockIdx.x * per;
   auto add = [&](float x, bool counts) {
-    const SampleWeight w = s_weight(x, M, r.inv_t, a.S, tab);
+    const SampleWeight w = s_weight(x, M, r, a.S, tab);
     const int b = s_bin(w.n);
     if (counts) atomicAdd(&count[b], 1u);
     atomicAdd(&mass[b], w.w);
@@ -412,7 +428,7 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
 #pragma unroll
           for (int u = 0; u < L; ++u) {
             const int k = k0 + lane + u * kSThreads, gr = k < 4 * listed ? g0 + g.group[k >> 2] : 0;
-            q[u] = k < 4 * listed ? (gr >> 8) * kSChunk + (gr & 255) + 256 * (k & 3) : nq;
+            q[u] = k < 4 * listed ? 4 * gr + (k & 3) : nq;
             v[u] = q[u] < nq ? s.load(q[u]) : zero4();
           }
 #pragma unroll
@@ -513,7 +529,7 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
       }
       v = s_sort_steps(v, min(k >> 1, 32), up, lane);
     }
-    run = s_wave_scan(at < n ? s_weight(s_unkey(~(uint32_t)(v >> 32)), M, r.inv_t, a.S, g.tab).w : 0ull);
+    run = s_wave_scan(at < n ? s_weight(s_unkey(~(uint32_t)(v >> 32)), M, r, a.S, g.tab).w : 0ull);
     if (!one) {
       __syncthreads();
       if (lane == 63) g.wmass[wave] = run;
@@ -701,7 +717,7 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
 #pragma unroll 1
         for (int e = 0; e < 4; ++e) {
           if (!pick4(in, e)) continue;
-          const SampleWeight w = s_weight(pick4(x, e), M, r.inv_t, a.S, g.tab);
+          const SampleWeight w = s_weight(pick4(x, e), M, r, a.S, g.tab);
           const int b = s_bin(w.n);
           atomicAdd(&g.count[b], 1u);
           atomicAdd(&g.mass[b], w.w);
@@ -715,12 +731,12 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
   auto smallest = [&](int b) __attribute__((always_inline)) -> float {
     uint32_t key = s_key(-INFINITY);  // the largest known to be below
     const uint32_t top = s_key(M);
-    if (s_bin(-INFINITY, M, r.inv_t) <= b) return -INFINITY;
+    if (s_bin(-INFINITY, M, r) <= b) return -INFINITY;
     for (int sh = 26; sh > -6; sh -= 6) {
       const uint32_t step = sh >= 0 ? 1u << sh : 1u;
       const u64 at64 = (u64)key + (u64)(lane + 1) * step;
       const uint32_t to = (uint32_t)(at64 < top ? at64 : top);
-      const u64 in = __builtin_amdgcn_ballot_w64(s_bin(s_unkey(to), M, r.inv_t) <= b);
+      const u64 in = __builtin_amdgcn_ballot_w64(s_bin(s_unkey(to), M, r) <= b);
       const u64 below = (u64)key + (u64)__builtin_ctzll(in) * step;  // (the last lane's value is inside)
       key = (uint32_t)(below < top ? below : top - 1);
     }
@@ -753,13 +769,13 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
     } else {
       const u64 enough = least > -INFINITY ? ((u64)~s_key(least) << 32) | 0xFFFFFFFFu : ~0ull;  // all of weight m
       if (enough < kept) {
-        b = s_bin(least, M, r.inv_t);
+        b = s_bin(least, M, r);
         if (tid == 0) g.to_mass = 0;
         in_bin(b);
         traverse(std::integral_constant<int, 1>{}, std::false_type{}, fmaxf(lo, least), hi, G, [&](bool (&in)[4], int, const f32x4& x) __attribute__((always_inline)) {
 #pragma unroll 1
           for (int e = 0; e < 4; ++e)
-            if (pick4(in, e)) atomicAdd(&g.to_mass, s_weight(pick4(x, e), M, r.inv_t, a.S, g.tab).w);
+            if (pick4(in, e)) atomicAdd(&g.to_mass, s_weight(pick4(x, e), M, r, a.S, g.tab).w);
         });
         kept = enough;
         Z = mass_below(b) + g.to_mass;
@@ -798,7 +814,7 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
       auto count = [&](u64 bits) __attribute__((always_inline)) {
         if (bits < first || bits > last) return;
         atomicAdd(&g.hcount[(bits - first) >> shift], 1u);
-        atomicAdd(&g.hmass[(bits - first) >> shift], s_weight(value_of(bits), M, r.inv_t, a.S, g.tab).w);
+        atomicAdd(&g.hmass[(bits - first) >> shift], s_weight(value_of(bits), M, r, a.S, g.tab).w);
       };
       if (lists) {
         for (int l = lane; l < mine_n; l += 64) count(listed(l));
