@@ -34,6 +34,14 @@
 // 49 us (2.8 TB/s), bf16 104 (4.7 TB/s); 512 tokens of one row behind 16 K 4-bit keys 115 us (528 TFLOP/s), bf16 165; one token
 // of three rows of 8192 4-bit keys 14 us.
 //
+// Sequences that share their first keys (several continuations of one prompt): these keys are read once for the rows of all,
+// tiles of whose rows hold tokens of several sequences, and each sequence's own keys once for it, by blocks of one launch (two
+// launches and a merge took 21.5 us where one and a merge take 13.1: one token of three rows, 2048 shared 4-bit keys and up to
+// 64 own). Both leave (max, sum, acc) of their runs to a merge. What bounds it: few rows, the chain of dependent loads (positions,
+// table, keys, parts); one token of 32 rows, 8192 shared bf16 keys and up to 500 own, 29 us, of which a block's two rounds take 8,
+// the queries' preparation 8 and the join of its waves 5; four tokens of 64 rows, 32768 shared 4-bit keys, 121 to 126 us (560
+// TFLOP/s), the vector ALU as above: 650 operations beside 72 products for 32 rows x 32 keys.
+//
 // A row's keys are dealt over S blocks in runs of whole 128-key rounds by the row's own length, read on the device: the
 // grid is sized by the table's capacity, the work by what is cached. With S > 1 the blocks leave (max, sum, acc) and a
 // second kernel merges them; blocks whose run is empty leave nothing and are not read.

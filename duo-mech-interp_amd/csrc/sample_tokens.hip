@@ -18,6 +18,12 @@
 //                        reaches that bin are fetched, and the bin's few tokens put in order. For a small top-k it forms the
 //                        bins itself, of the groups that reach the k-th largest group's bin: all larger tokens are in them
 //   sample_write_kernel  probabilities or cut logits, where they are asked for
+//
+// Rows of 151,936 logits (a copy runs at 5.2 TB/s): three of top-k 20 13.4 us, a chain of two launches and, in the second, of
+// a dozen dependent steps of one block; 256 of top-p 0.9 124 us: the maximum 29 (5.4 TB/s), the histogram 44 (26 operations a
+// token, most of 64 bits, and an atomic in LDS), the pick 53, whose one block a row reads what reaches the border's bin at a CU's
+// 50 GB/s, most of the row where the nucleus is large; 160 of top-k 50 and top-p 0.95 cut into logits 94 us: 22, 33, 12, and 29
+// for the write.
 #include <algorithm>
 #include <cfloat>
 #include <type_traits>

@@ -1377,7 +1377,9 @@ def quantize_rows(x):
 def add_rmsnorm_i8_(x, y, w, eps=1e-6):
     """add_rmsnorm_ with the normed rows as RowsI8 (norm and quotients in 64 bits): x += y in place (y None: no add), then
     quantize_rows of x * rsqrt(mean x^2 + eps) * (1 + w). x, y: [..., K] fp32, rows dense and evenly strided."""
-    return RowsI8(*_call("try_add_rmsnorm_i8_", torch.ops.q35.add_rmsnorm_i8_, x, y, w.float().contiguous(), float(eps)))
+    if w.dtype is not torch.float32 or not w.is_contiguous():
+        w = w.float().contiguous()
+    return RowsI8(*_call("try_add_rmsnorm_i8_", torch.ops.q35.add_rmsnorm_i8_, x, y, w, float(eps)))
 
 
 def gemm_i8(x, W, w_scale, out=None, epilogue="store", pushes=None, T=1, capture=None):
