@@ -177,7 +177,7 @@ struct SampleQuads {
 // f(value) of the row's quads first, first + step, ... below last.
 template <typename F>
 __device__ __forceinline__ void s_for_row(const SampleQuads& s, int first, int step, int last, F&& f) {
-  constexpr int U = 2;
+  constexpr int U = 4;
   const int w0 = s.whole_first(), w1 = min(last, s.whole_last());
   int q = first < w0 ? first + step : first;
   for (; q + (U - 1) * step < w1; q += U * step) {
