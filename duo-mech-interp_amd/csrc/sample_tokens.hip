@@ -479,6 +479,7 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const u64 mask = __builtin_amdgcn_ballot_w64(in[e]);
+        if (!mask) continue;
         const int to = __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, mine_n));
         if (in[e] && to < kSSeg) g.list[wave][to] = ((u64)__float_as_uint(v[e]) << 32) | (uint32_t)(i + e);
         mine_n += __popcll(mask);
