@@ -319,7 +319,7 @@ class HybridModel:
         def normed(y, w, names):
             # the norms hand the int8 GEMMs their rows already split (bf16 hi + lo), or in 8 bits, when the layer's products
             # are int8
-            if self.act_int8 and _rows8_ok(p, names):
+            if self.act_int8 and x.shape[0] * T > 8 and _rows8_ok(p, names):
                 return ops.add_rmsnorm_i8_(x, y, w, cfg.eps)
             return ops.add_rmsnorm_(x, y, w, cfg.eps, split=_split_ok(p, _MLP_IN if names is _MLP else names, x))
         for l in range(last + 1):
@@ -533,7 +533,7 @@ def sampled(model, prompt_ids, steps, *, u=None, generator=None, temperature=1.0
         toks.append(nxt)
         if i + 1 < steps:
             logits = model.decode_step(nxt)
-    return torch.stack(toks, 1).long().cpu()
+    return torch.stack(toks, 1).long().cpu() if toks else torch.empty(logits.shape[0], 0, dtype=torch.int64)
 
 
 def median_resid_norm(resid_row):

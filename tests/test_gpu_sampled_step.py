@@ -217,6 +217,18 @@ def test_model(rows, T, mlp_only, monkeypatch):
         assert not torch.equal(a, f)  # the 8-bit operators ran
 
 
+@pytest.mark.parametrize("rows,T", [(2, 4), (1, 8), (8, 1)])
+def test_few_rows_are_as_without(rows, T):
+    """Up to 8 rows in all: the same bits as a model without act_int8, in prefill and steps."""
+    announce(f"model act_int8, few rows {rows} T{T}")
+    cfg = config()
+    W = workloads.init_weights(cfg, seed=3, group=0)
+    ids = torch.randint(0, cfg.vocab, (rows, T), generator=torch.Generator().manual_seed(5))
+    a, b = (gm.HybridModel(cfg, W, device(), max_len=64, rows=rows, deterministic=True, act_int8=i) for i in (True, False))
+    assert torch.equal(a.forward(ids)[0], b.forward(ids)[0])
+    assert torch.equal(a.decode_step(ids[:, 0].to(device())), b.decode_step(ids[:, 0].to(device())))
+
+
 def test_model_refuses():
     W = workloads.init_weights(config(), seed=3)
     with pytest.raises(ValueError, match="act_int8"):
@@ -251,6 +263,8 @@ def test_sampled(graph):
     m.reset()
     again = gm.sampled(m, ids, steps, temperature=0.0)
     assert torch.equal(again, greedy)
+    m.reset()
+    assert gm.sampled(m, ids, 0).shape == (rows, 0)
     m.reset()
     gen = torch.Generator(device=device()).manual_seed(8)
     a = gm.sampled(m, ids, steps, generator=gen, temperature=5.0)
