@@ -1009,11 +1009,11 @@ template <int W>
 __global__ __launch_bounds__(256) void paged_attn_shared_merge_kernel(PagedAttnArgs p) {
   constexpr int U = 8;
   const int lane = threadIdx.x & 63, d0 = 4 * lane, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row = W == 1 ? 4 * (int64_t)blockIdx.x + wave : (int64_t)blockIdx.x;
+  const uint32_t row = W == 1 ? 4 * blockIdx.x + wave : blockIdx.x;
   const int w0 = W == 1 ? 0 : wave;
-  const int Hq = p.Hkv * p.G;
-  if (row >= (int64_t)p.B * p.T * Hq) return;
-  const int h = (int)(row % Hq), tt = (int)(row / Hq), b = tt / p.T, t = tt - b * p.T;
+  const uint32_t Hq = (uint32_t)(p.Hkv * p.G);
+  if (row >= (uint32_t)(p.B * p.T) * Hq) return;
+  const int tt = (int)(row / Hq), h = (int)(row - tt * Hq), b = div_by(tt, p.T, p.inv_t), t = tt - b * p.T;
   const int64_t pos = load_uniform(p.pos + b);
   const int len = p.lens ? min(max(load_uniform(p.lens + b), 0), p.T) : p.T;
   const int seen = keys_seen(p, pos, len, t);

@@ -20,8 +20,8 @@
 //   sample_write_kernel  probabilities or cut logits, where they are asked for
 //
 // Rows of 151,936 logits (a copy runs at 5.2 TB/s): three of top-k 20 13.4 us, a chain of two launches and, in the second, of
-// a dozen dependent steps of one block; 256 of top-p 0.9 124 us: the maximum 29 (5.4 TB/s), the histogram 44 (26 operations a
-// token, most of 64 bits, and an atomic in LDS), the pick 53, whose one block a row reads what reaches the border's bin at a CU's
+// a dozen dependent steps of one block; 256 of top-p 0.9 120 us: the maximum 29 (5.4 TB/s), the histogram 43 (26 operations a
+// token, most of 64 bits, and an atomic in LDS), the pick 51, whose one block a row reads what reaches the border's bin at a CU's
 // 50 GB/s, most of the row where the nucleus is large; 160 of top-k 50 and top-p 0.95 cut into logits 94 us: 22, 33, 12, and 29
 // for the write.
 #include <algorithm>
@@ -103,7 +103,7 @@ __device__ __forceinline__ SampleRow s_row(const SampleArgs& a, int row) {
 
 // The distance of x from the maximum M in 1/32 octaves of the weight, and the weight in units of 2^-S: 2^(-z / 32) by the series
 // of exp2_neg, with S in the exponent, and both conversions to whole numbers by adding a power of two (fp64 has no other short
-// one): 25 operations a token where rint, conversions and a comparison with an infinite maximum took 34 (256 rows of 151,936
+// one): 26 operations a token where rint, conversions and a comparison with an infinite maximum took 34 (256 rows of 151,936
 // 49 -> 43 us).
 struct SampleWeight {
   int n;
