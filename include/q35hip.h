@@ -586,7 +586,8 @@ int q35_gated_attn_paged(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh
  * q35_gated_attn_paged for sequences whose tables begin with the same pages: the first shared_blocks entries of every row of
  * the table name the pages that row 0's do (only row 0's are read), and their keys are read once for the rows of all
  * sequences. The result is that of q35_gated_attn_paged up to the order of its sums; a sequence may also end inside the
- * shared part. shared_blocks 0 is q35_gated_attn_paged. B T Hq / Hkv up to 2^24, in at most 65535 / Hkv blocks of 32 rows.
+ * shared part. shared_blocks 0 is q35_gated_attn_paged. B up to 65535, B T Hq / Hkv up to 2^24. The workspace is sized
+ * for the table's capacity.
  */
 size_t q35_gated_attn_paged_shared_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t n_blocks,
                                                    int64_t page_size, int64_t shared_blocks);

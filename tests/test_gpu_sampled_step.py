@@ -270,3 +270,25 @@ def test_sampled(graph):
     a = gm.sampled(m, ids, steps, generator=gen, temperature=5.0)
     m.reset()
     assert torch.equal(a, gm.sampled(m, ids, steps, generator=gen.manual_seed(8), temperature=5.0))
+
+
+def test_many_rows_in_a_decode_graph():
+    """12 rows with act_int8: the captured step's replays, with eager work between, against the eager steps of another model, and
+    sampled() through the graph against sampled() without."""
+    announce("model act_int8, decode graph of 12 rows")
+    cfg, rows = config(), 12
+    W = workloads.init_weights(cfg, seed=9, group=0)
+    eager, graph = (gm.HybridModel(cfg, W, device(), max_len=64, rows=rows, deterministic=True, act_int8=True) for _ in range(2))
+    graph.enable_decode_graph()
+    ids = torch.randint(0, cfg.vocab, (rows, 7), generator=torch.Generator().manual_seed(2))
+    a, b = eager.forward(ids)[0], graph.forward(ids)[0]
+    assert torch.equal(a, b)
+    for step in range(6):
+        nxt = ops.sample_tokens(a, torch.full((rows,), 0.1 * step + 0.05, device=device()), top_k=40)
+        a, b = eager.decode_step(nxt).clone(), graph.decode_step(nxt).clone()
+        torch.cuda.synchronize()
+        assert torch.equal(a, b), step
+    u = torch.rand(rows, 5, generator=torch.Generator().manual_seed(3)).to(device())
+    eager.reset()
+    graph.reset()
+    assert torch.equal(gm.sampled(eager, ids, 5, u=u, top_p=0.9), gm.sampled(graph, ids, 5, u=u, top_p=0.9))
