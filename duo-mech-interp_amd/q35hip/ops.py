@@ -1371,7 +1371,7 @@ class RowsI8(NamedTuple):
 def quantize_rows(x):
     """x [..., K] fp32 or bf16 (dense rows, evenly strided; K a multiple of 4, at most 16384) as RowsI8: s = fp32(max |x| / 127),
     q = rint(x / s). A row that holds a value that is not finite gets codes 0 and the scale NaN."""
-    return RowsI8(*_call("try_quantize_rows_i8", torch.ops.q35.quantize_rows_i8, x))
+    return tuple.__new__(RowsI8, _call("try_quantize_rows_i8", torch.ops.q35.quantize_rows_i8, x))
 
 
 def add_rmsnorm_i8_(x, y, w, eps=1e-6):
@@ -1379,7 +1379,7 @@ def add_rmsnorm_i8_(x, y, w, eps=1e-6):
     quantize_rows of x * rsqrt(mean x^2 + eps) * (1 + w). x, y: [..., K] fp32, rows dense and evenly strided."""
     if w.dtype is not torch.float32 or not w.is_contiguous():
         w = w.float().contiguous()
-    return RowsI8(*_call("try_add_rmsnorm_i8_", torch.ops.q35.add_rmsnorm_i8_, x, y, w, float(eps)))
+    return tuple.__new__(RowsI8, _call("try_add_rmsnorm_i8_", torch.ops.q35.add_rmsnorm_i8_, x, y, w, float(eps)))
 
 
 def gemm_i8(x, W, w_scale, out=None, epilogue="store", pushes=None, T=1, capture=None):
