@@ -431,7 +431,7 @@ void sample(const Tensor& x, const Logits& l, const Tensor* u, const Cuts& c, co
   });
 }
 
-// logits, u, temperatures, temperature, top_ks, top_k, top_ps, top_p, min_ps, min_p, want_probs -> (tokens, probs or empty)
+// logits, u, temperatures, temperature, top_ks, top_k, top_ps, top_p, min_ps, min_p, want_probs -> (tokens, probs), or tokens
 PyObject* sample_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded(n, 11, [&]() -> PyObject* {
     const Tensor &x = tensor(a[0]), &u = tensor(a[1]);
@@ -443,8 +443,9 @@ PyObject* sample_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Cuts c = cuts_of(a + 2, d, l.B);
     const int want = PyObject_IsTrue(a[10]);
     if (want < 0) throw PyFailed{};
-    const Tensor tokens = make({l.B}, at::kInt, x), probs = want ? make({l.B, l.V}, at::kFloat, x) : make({0}, at::kFloat, x);
+    const Tensor tokens = make({l.B}, at::kInt, x), probs = want ? make({l.B, l.V}, at::kFloat, x) : Tensor();
     if (l.B) sample(x, l, &u, c, &tokens, want, want ? &probs : nullptr);
+    if (!want) return THPVariable_Wrap(tokens);
     return Py_BuildValue("(NN)", THPVariable_Wrap(tokens), THPVariable_Wrap(probs));
   });
 }

@@ -404,8 +404,9 @@ def _attn_paged_shared_impl(*args):
     return _paged_host().gated_attn_paged_shared(*args)
 
 
-def _sample_tokens_impl(*args):
-    return _paged_host().sample_tokens(*args)
+def _sample_tokens_impl(logits, u, *args):
+    out = _paged_host().sample_tokens(logits, u, *args)
+    return out if args[-1] else (out, logits.new_empty(0))
 
 
 def _filter_logits_impl(*args):
@@ -1335,9 +1336,9 @@ def sample_tokens(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
     one's probability. The first always stays; temperature 0 is the argmax. The token is the first kept one, in this order,
     whose running sum exceeds u of the kept ones' sum. Returns tokens [B] int32; with want_probs also the probabilities that
     the draw is from, [B, V] fp32 (0 where cut): what verify_drafts takes as draft_probs."""
-    tokens, probs = _call("try_sample_tokens", torch.ops.q35.sample_tokens, logits, u, *_cuts(temperature, top_k, top_p, min_p),
-                          bool(want_probs))
-    return (tokens, probs) if want_probs else tokens
+    out = _call("try_sample_tokens", torch.ops.q35.sample_tokens, logits, u, *_cuts(temperature, top_k, top_p, min_p),
+                bool(want_probs))
+    return out if want_probs or isinstance(out, torch.Tensor) else out[0]
 
 
 def filter_logits(logits, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
