@@ -17,6 +17,7 @@
 //   sample_pick_kernel   one block a row: the bins' running sums give the bin of each border; the groups whose largest value
 //                        reaches that bin are fetched, and the bin's few tokens put in order. For a small top-k it forms the
 //                        bins itself, of the groups that reach the k-th largest group's bin: all larger tokens are in them
+//                        Of rows of up to 16 K tokens it is also what the two above are
 //   sample_write_kernel  probabilities or cut logits, where they are asked for
 //
 // Rows of 151,936 logits (a copy runs at 5.2 TB/s): three of top-k 20 13.4 us, a chain of two launches and, in the second, of
@@ -37,6 +38,7 @@ constexpr int kSBins = 2048, kSFine = 1536;
 constexpr int kSChunk = 1024;    // quads of a block of the maximum and the write kernel: 256 groups of 4 neighbouring ones
 constexpr int kSFew = 1024;      // the largest top-k whose rows need no histogram
 constexpr int kSThreads = 1024;  // of the pick kernel
+constexpr int kSShort = 4;       // chunks of a row that the pick kernel takes alone
 constexpr int kSHeld = 10;       // groups' maxima that one of its threads holds
 constexpr int kSSort = kSThreads;  // tokens that it sorts
 constexpr int kSWaves = kSThreads / 64, kSSeg = 512;  // tokens that each of its waves can list
@@ -289,6 +291,7 @@ struct SamplePick {
   uint32_t hcount[256];
   u64 wmass[kSWaves];
   uint32_t wcount[kSWaves];
+  float wmax[kSWaves];
   double tab[kVTab];
   int groups;  // of the list
   int n;       // tokens to be sorted
@@ -368,18 +371,42 @@ struct SampleKept {
   __device__ __forceinline__ bool has(float v, int i) const { return v > x || (v == x && (uint32_t)i <= idx); }
 };
 
+// SHORT: a row of up to 1024 groups, whose maxima and bins the block forms as well.
+template <bool SHORT>
 __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x;
   const SampleRow r = s_row(a, row);
   const SampleQuads s(r.x, a.V);
   __shared__ SamplePick g;
   const int G = a.C * 256;
-  const float* gmax = a.gmax + (size_t)row * G;
+  float* gmax = a.gmax + (size_t)row * G;
+  exp2_table(g.tab, tid);
+  float M = -INFINITY;
+  if constexpr (SHORT) {
+#pragma unroll
+    for (int j = 0; j < kSShort; ++j) {
+      const int q = tid + kSThreads * j;
+      float m = -INFINITY;
+      if (q < s.n()) {
+        const f32x4 v = s.load(q);
+        m = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+      }
+      M = fmaxf(M, m);
+      m = fmaxf(m, __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(m), 0xB1, 0xF, 0xF, false)));
+      m = fmaxf(m, __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(m), 0x4E, 0xF, 0xF, false)));
+      if (j < a.C && (tid & 3) == 0) gmax[q >> 2] = m;
+    }
+    M = wave_max_f32(M);
+    if (lane == 0) g.wmax[wave] = M;
+    __syncthreads();
+    M = wave_max_f32(g.wmax[lane & (kSWaves - 1)]);
+  } else {
+    M = s_max(a, row);
+  }
   float held[kSHeld];  // the maxima of groups tid + 1024 i
 #pragma unroll
-  for (int i = 0; i < kSHeld; ++i) held[i] = tid + kSThreads * i < G ? gmax[tid + kSThreads * i] : -INFINITY;
-  exp2_table(g.tab, tid);
-  const float M = s_max(a, row);
+  for (int i = 0; i < kSHeld; ++i)
+    held[i] = (i == 0 || !SHORT) && tid + kSThreads * i < G ? gmax[tid + kSThreads * i] : -INFINITY;
   if (!(M > -INFINITY)) {  // nothing above -inf: token 0, nothing kept
     if (tid == 0) {
       a.cut[row] = {0.0, M, INFINITY, -1, 0};
@@ -683,7 +710,25 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
       __syncthreads();
     }
   } else {
-    scan(true);
+    if constexpr (SHORT) {
+      clear();
+#pragma unroll 1
+      for (int j = 0; j < kSShort; ++j) {
+        const int q = tid + kSThreads * j, i = 4 * q - s.ahead;
+        if (q >= s.n()) break;
+        const f32x4 x = s.load(q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (i + e < 0 || i + e >= a.V) continue;
+          const SampleWeight w = s_weight(x[e], M, r, a.S, g.tab);
+          const int b = s_bin(w.n);
+          if (r.k > 0) atomicAdd(&g.count[b], 1u);
+          atomicAdd(&g.mass[b], w.w);
+        }
+      }
+      __syncthreads();
+    }
+    scan(!SHORT);
     Z_row = g.mass[kSBins - 1];
     if (r.k > 0) floor_x = bound(bin_of_count((uint32_t)r.k));
     else if (r.p < 1.f) floor_x = bound(bin_of_mass(p_target(Z_row)));
@@ -958,12 +1003,16 @@ extern "C" int q35_sample_tokens(const float* logits, int64_t l_sb, int64_t l_sp
   a.R = (int)std::max<int64_t>(1, std::min<int64_t>((1024 + rows - 1) / rows, (nq + 1023) / 1024));
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const dim3 chunks(a.C, (unsigned)rows);
-  hipLaunchKernelGGL(sample_max_kernel, chunks, dim3(256), 0, st, a);
+  // A short row's maximum and bins take its one block less than the launches of the two kernels (top-p 0.9, with them and
+  // without: one row of 4000 21.4 and 15.5 us, 256 of 2000 21.2 and 15.3, of 16000 30.9 and 20.1, 1024 of 16000 87 and 76)
+  const bool brief = a.C <= kSShort;
+  if (!brief) hipLaunchKernelGGL(sample_max_kernel, chunks, dim3(256), 0, st, a);
   // (none of its blocks has work where one small top-k holds for all rows, or the argmax)
   const int64_t k = temperature > 0.f ? top_k : 1;  // (as s_row has it)
-  if (temperatures || top_ks || k <= 0 || k >= V || k > kSFew)
+  if (!brief && (temperatures || top_ks || k <= 0 || k >= V || k > kSFew))
     hipLaunchKernelGGL(sample_hist_kernel, dim3(a.R, (unsigned)rows), dim3(256), 0, st, a);
-  hipLaunchKernelGGL(sample_pick_kernel, dim3((unsigned)rows), dim3(kSThreads), 0, st, a);
+  if (brief) hipLaunchKernelGGL(sample_pick_kernel<true>, dim3((unsigned)rows), dim3(kSThreads), 0, st, a);
+  else hipLaunchKernelGGL(sample_pick_kernel<false>, dim3((unsigned)rows), dim3(kSThreads), 0, st, a);
   if (out_kind == kSampleProbs) hipLaunchKernelGGL(sample_write_kernel<kSampleProbs>, chunks, dim3(256), 0, st, a);
   else if (out_kind == kSampleLogits) hipLaunchKernelGGL(sample_write_kernel<kSampleLogits>, chunks, dim3(256), 0, st, a);
   return hipGetLastError() == hipSuccess ? Q35_OK : Q35_ELAUNCH;
