@@ -190,3 +190,24 @@ def test_products_past_32_bits():
     q, s = ops.quantize_rows(x[:, 100:164])
     assert bool((q.float() == torch.where(s[:, None] > 0, 127.0, 0.0)).all())
     assert torch.equal(s, (x[:, 100].double() / 127).float())
+
+
+@pytest.mark.parametrize("V", [4092, 4093, 16379, 16380, 16381, 16385])
+def test_where_short_rows_end(V):
+    """Around the longest row that one block takes, at each distance from 16 bytes; first and last tokens kept and drawn."""
+    announce(f"sample short rows V{V}")
+    g = torch.Generator().manual_seed(V)
+    for off in range(4):
+        wide = torch.full((3, V + 8), 90.0)
+        x = torch.randn(3, V, generator=g) * 3
+        x[0, 0], x[1, V - 1], x[2, [0, V - 1]] = 12.0, 12.0, 11.0
+        wide[:, off:off + V] = x
+        view = wide.to(device())[:, off:off + V]
+        u = torch.tensor([0.1, 0.5, 0.9])
+        for cuts in (dict(), dict(top_k=30), dict(top_k=2000, top_p=0.99), dict(top_p=0.97, min_p=1e-3)):
+            tok, pr = ops.sample_tokens(view, u.to(device()), want_probs=True, **cuts)
+            want, wp = sampling.sample_tokens(x, u, **cuts)
+            assert torch.equal(tok.cpu(), want)
+            assert torch.equal(pr.cpu() > 0, wp > 0)
+            kept = ops.filter_logits(view, **cuts).cpu()
+            assert torch.equal(kept, sampling.filter_logits(x, **cuts))
