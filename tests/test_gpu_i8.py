@@ -239,3 +239,32 @@ def test_captured_and_replayed():
     a = block()
     torch.cuda.synchronize()
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("M,N,K", [(700, 1000, 64), (700, 1002, 192), (1000, 3000, 64), (1001, 2998, 448), (2500, 5000, 64),
+                                   (2600, 8222, 320), (4100, 8200, 128)])
+@pytest.mark.parametrize("epilogue", ["store", "swiglu"])
+def test_each_tile(M, N, K, epilogue):
+    """Sizes at which tiles of 64, 128 and 256 are chosen, inputs of one stage or less and those that end inside one."""
+    W, ws = weights(N, K, seed=N)
+    q, s = int8.quantize_rows(rows(M, K, seed=M))
+    dev = device()
+    announce(f"gemm_i8 tiles M{M} N{N} K{K} {epilogue}")
+    y = ops.gemm_i8((q.to(dev), s.to(dev)), W.to(dev), ws.to(dev), epilogue=epilogue).double().cpu()
+    v = int8.product(q, s, W, ws)
+    if epilogue == "store":
+        check(y, v)
+        return
+    gate, up = v[:, 0::2], v[:, 1::2]
+    want = gate * torch.sigmoid(gate) * up
+    assert bool(((y - want).abs() <= (12 + 8 * gate.abs()) * H * want.abs() + 1e-37).all())
+
+
+@pytest.mark.parametrize("M,N", [(600, 900), (1100, 2100), (2500, 5000)])
+def test_largest_sums_of_each_tile(M, N):
+    K = 4096
+    W, ws = weights(N, K, extremes=True)
+    q, s = torch.full((M, K), -127, dtype=torch.int8), torch.rand(M, generator=torch.Generator().manual_seed(1)) + 0.5
+    dev = device()
+    announce(f"gemm_i8 largest sums M{M} N{N} K{K}")
+    check(ops.gemm_i8((q.to(dev), s.to(dev)), W.to(dev), ws.to(dev)), int8.product(q, s, W, ws))
