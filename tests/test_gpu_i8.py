@@ -268,3 +268,30 @@ def test_largest_sums_of_each_tile(M, N):
     dev = device()
     announce(f"gemm_i8 largest sums M{M} N{N} K{K}")
     check(ops.gemm_i8((q.to(dev), s.to(dev)), W.to(dev), ws.to(dev)), int8.product(q, s, W, ws))
+
+
+@pytest.mark.parametrize("M,K", [(2100, 516), (2048, 1000), (2300, 1024), (40, 1024), (40, 300), (12, 4096), (5, 8196)])
+def test_codes_far_from_one(M, K):
+    """Rows and gains over the whole range: what fp32 alone would lose is formed in 64 bits. Many rows of up to 1024 values are a
+    wave's each, others a block's."""
+    g = torch.Generator().manual_seed(M + K)
+    x = torch.randn(M, K, generator=g)
+    x[0::7] *= 1e-30
+    x[1::7] *= 1e30
+    x[2::7] *= torch.logspace(-20, 20, K)
+    x[3::7, ::3] = 0.0
+    x[4::7] = (torch.randint(-254, 255, (x[4::7].shape[0], K), generator=g).float() * 0.5)  # codes and halves
+    x[4::7, 0] = 127.0
+    w = torch.randn(K, generator=g) * 0.1
+    w[:6] = torch.tensor([-1.0, -1.0000001, -0.99999994, 1e30, 1e-30, -1e25])
+    dev = device()
+    announce(f"rows in 8 bits far from one M{M} K{K}")
+    q, s = ops.quantize_rows(x.to(dev))
+    wq, ws = int8.quantize_rows(x)
+    assert torch.equal(q.cpu(), wq) and torch.equal(s.cpu(), ws)
+    for gain in (w, torch.cat([w[:3], w[6:9], w[6:]])[:K]):
+        xd = x.to(dev)
+        q, s = ops.add_rmsnorm_i8_(xd, None, gain.to(dev))
+        wq, ws = int8.quantize_rows(int8.norm_rows(x, gain, torch.tensor(1e-6).item()))  # (eps is an fp32 argument)
+        assert torch.equal(xd.cpu(), x)
+        assert torch.equal(s.cpu(), ws) and torch.equal(q.cpu(), wq)
