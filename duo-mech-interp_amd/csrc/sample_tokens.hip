@@ -402,6 +402,7 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
     M = wave_max_f32(g.wmax[lane & (kSWaves - 1)]);
   } else {
     M = s_max(a, row);
+    __syncthreads();  // (the table; above, the barrier of the maxima)
   }
   float held[kSHeld];  // the maxima of groups tid + 1024 i
 #pragma unroll
