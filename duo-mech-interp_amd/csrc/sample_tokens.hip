@@ -601,17 +601,17 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
     const double goal = floor(fmax((double)u, 0.0) * (double)Z);
     return goal >= (double)Z ? Z : min((u64)goal + 1, Z);
   };
-  // the smallest value of weight m or more: next to max + T ln m, found among its neighbours (more than 1: the largest value)
+  // The smallest value of weight m or more: exp((x - max) / T) >= m where x >= max + T ln m, in 64 bits. (Looked for by the weights of
+  // values next to it, it was off by their series' 2e-12 T, which around 0 is more than any number of neighbouring values. 2^-54
+  // less: what rounds to 1 weighs 1, at an infinite temperature every finite logit.)
   float least = -INFINITY;
   if (r.m > 0.f) {
-    const float guess = fminf((float)((double)M + log((double)r.m) * (double)r.t), M);
+    const double border = fmin(__builtin_fma(log((double)r.m) - 0x1p-54, (double)r.t, (double)M), (double)M);
     if (!(fabsf(M) < INFINITY)) {
       least = M;
-    } else if (guess > -INFINITY) {
-      least = M;
-      const uint32_t mine = min(s_key(guess) + (uint32_t)lane - 32u, s_key(M));
-      const u64 in = __builtin_amdgcn_ballot_w64(v_weight(s_unkey(mine), M, r.inv_t, g.tab) >= (double)r.m);
-      if (in) least = s_unkey(__builtin_amdgcn_readlane(mine, __builtin_ctzll(in)));
+    } else if (border >= -(double)FLT_MAX) {
+      least = (float)border;
+      if ((double)least < border) least = s_unkey(s_key(least) + 1);
     }
   }
   // ---- the row's bins, and their running sums: two a thread

@@ -39,3 +39,67 @@ def test_long_rows_behind_kernels_that_use_all_of_lds(V):
         tok = ops.sample_tokens(xd, ud, **up)
         assert torch.equal(tok.cpu(), want)
     same(x, u, **cuts)
+
+
+def border_rows(V, temps, ps, seed):
+    """Rows whose largest logit M lies 0 to 2 steps of fp32 beside -T ln m, so that the border of min-p lies next to 0, where fp32
+    is finest; the others on both sides of 0 from 1e-9 on, and anywhere. Returns logits, temperatures, min-ps."""
+    g = torch.Generator().manual_seed(seed)
+    t, m = (a.flatten() for a in torch.meshgrid(torch.tensor(temps), torch.tensor(ps), indexing="ij"))
+    t, m = t.repeat(5), m.repeat(5)
+    top = -t.double() * m.double().log()
+    top = top.float()
+    for i, steps in enumerate((-2, -1, 0, 1, 2)):
+        at = slice(i * len(temps) * len(ps), (i + 1) * len(temps) * len(ps))
+        for _ in range(abs(steps)):
+            top[at] = torch.nextafter(top[at], torch.tensor(float("inf") if steps > 0 else -float("inf")))
+    x = torch.rand(t.numel(), V, generator=g) * 1.5 * t[:, None] - t[:, None]
+    x[1::2] -= 0.6 * t[1::2, None]  # (every other row: the border's own tokens alone)
+    near = torch.cat([torch.zeros(1), 10.0 ** -torch.arange(3, 10)])
+    x[:, 1:1 + near.numel()] = near
+    x[:, 10:10 + near.numel()] = -near
+    x = torch.minimum(x, top[:, None])
+    x[:, 20] = top
+    # nothing lies so near a border that 64 bits could not tell
+    w = torch.exp((x.double() - top[:, None].double()) / t[:, None].double()) / m[:, None].double()
+    assert float((w - 1).abs().min()) > 1e-13
+    return x, t, m
+
+
+TEMPS = [0.05, 0.3, 0.5, 0.6, 0.7, 0.8, 0.9, 1.0, 1.2, 1.5, 2.0, 5.0]
+MINS = [1e-4, 1e-3, 0.005, 0.01, 0.02, 0.03, 0.05, 0.1, 0.2, 0.3, 0.5, 0.9]
+
+
+@pytest.mark.parametrize("V", [33, 5000])
+@pytest.mark.parametrize("cuts", [dict(), dict(top_k=30), dict(top_k=1500), dict(top_p=0.98), dict(top_k=40, top_p=0.9)], ids=str)
+def test_min_p_whose_border_is_next_to_zero(V, cuts):
+    x, t, m = border_rows(V, TEMPS, MINS, V)
+    announce(f"min-p next to 0, V{V} {cuts}")
+    same(x, torch.linspace(0, 0.999, x.shape[0]), temperature=t, min_p=m, **cuts)
+
+
+@pytest.mark.parametrize("cuts", [dict(), dict(top_k=30), dict(top_p=0.98)], ids=str)
+def test_min_p_of_long_rows_next_to_zero(cuts):
+    x, t, m = border_rows(20011, [0.5, 0.7, 1.0, 1.2], [0.01, 0.02, 0.1, 0.3], 1)
+    announce(f"min-p next to 0, long rows {cuts}")
+    same(x, torch.linspace(0, 0.999, x.shape[0]), temperature=t, min_p=m, **cuts)
+
+
+def test_min_p_of_one_number():
+    """The plain settings, as numbers: 0.01 of the largest keeps what is above 0 here."""
+    announce("min-p numbers")
+    for m, t, top in ((0.01, 1.0, 4.60517025), (0.01, 0.5, 2.30258512), (0.02, 0.7, 2.73841596)):
+        x = torch.full((1, 100), -0.5)
+        x[0, 7], x[0, 50:60], x[0, 60:70] = top, 0.25, -0.25
+        same(x, torch.tensor([0.98]), temperature=t, min_p=m)
+        assert sampling.filter_logits(x, temperature=t, min_p=m).isfinite().sum() == 11
+
+
+@pytest.mark.parametrize("V", [50, 20000])
+def test_min_p_at_infinite_temperature(V):
+    """Every finite logit weighs 1, which is at least any min-p up to 1."""
+    x = logits(3, V, seed=V)
+    x[1, ::3], x[2, 1::2] = -float("inf"), float("nan")
+    announce(f"min-p at an infinite temperature V{V}")
+    for m in (0.5, 1.0):
+        same(x, torch.tensor([0.1, 0.6, 0.9]), temperature=float("inf"), min_p=m)
