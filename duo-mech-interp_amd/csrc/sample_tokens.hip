@@ -97,6 +97,10 @@ __device__ __forceinline__ SampleRow s_row(const SampleArgs& a, int row) {
     r.t = 1.f;
     r.k = 1;
   }
+  if (r.m > 1.f) {  // more than any weight: the first token alone, whatever equals it
+    r.m = 0.f;
+    r.k = 1;
+  }
   if (r.k <= 0 || r.k >= a.V) r.k = 0;
   r.few = r.k > 0 && r.k <= kSFew;
   r.inv_t = fmax(32.0 * 1.4426950408889634074 / (double)r.t, 1e-300);
@@ -606,7 +610,7 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
   // less: what rounds to 1 weighs 1, at an infinite temperature every finite logit.)
   float least = -INFINITY;
   if (r.m > 0.f) {
-    const double border = fmin(__builtin_fma(log((double)r.m) - 0x1p-54, (double)r.t, (double)M), (double)M);
+    const double border = __builtin_fma(log((double)r.m) - 0x1p-54, (double)r.t, (double)M);
     if (!(fabsf(M) < INFINITY)) {
       least = M;
     } else if (border >= -(double)FLT_MAX) {
@@ -1009,7 +1013,7 @@ extern "C" int q35_sample_tokens(const float* logits, int64_t l_sb, int64_t l_sp
   const bool brief = a.C <= kSShort;
   if (!brief) hipLaunchKernelGGL(sample_max_kernel, chunks, dim3(256), 0, st, a);
   // (none of its blocks has work where one small top-k holds for all rows, or the argmax)
-  const int64_t k = temperature > 0.f ? top_k : 1;  // (as s_row has it)
+  const int64_t k = temperature > 0.f && (min_ps || !(min_p > 1.f)) ? top_k : 1;  // (as s_row has it)
   if (!brief && (temperatures || top_ks || k <= 0 || k >= V || k > kSFew))
     hipLaunchKernelGGL(sample_hist_kernel, dim3(a.R, (unsigned)rows), dim3(256), 0, st, a);
   if (brief) hipLaunchKernelGGL(sample_pick_kernel<true>, dim3((unsigned)rows), dim3(kSThreads), 0, st, a);

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+import q35hip
 from gpu_util import announce, device
 from oracle import sampling
 from q35hip import ops
@@ -103,3 +104,42 @@ def test_min_p_at_infinite_temperature(V):
     announce(f"min-p at an infinite temperature V{V}")
     for m in (0.5, 1.0):
         same(x, torch.tensor([0.1, 0.6, 0.9]), temperature=float("inf"), min_p=m)
+
+
+@pytest.mark.parametrize("V", [40, 5000, 20000])
+def test_min_p_above_one_keeps_the_first_token(V):
+    """No weight is more than the first one's: it alone stays, also where others equal it."""
+    x = torch.zeros(4, V)
+    x[1, V // 2:V // 2 + 9] = 1.0
+    x[2] = float("inf")
+    x[3, ::2] = -0.0
+    u = torch.tensor([0.9, 0.95, 0.99, 0.5])
+    announce(f"min-p above 1 V{V}")
+    for cuts in (dict(min_p=1.5), dict(min_p=float("inf")), dict(min_p=3.0, top_k=5), dict(min_p=3.0, top_k=3000), dict(min_p=2.0, top_p=0.9),
+                 dict(min_p=1.0, top_k=12), dict(min_p=torch.tensor([1.1, 0.5, 4.0, 0.0])),
+                 dict(min_p=2.0, temperature=torch.tensor([0.0, 5.0, 0.1, float("inf")]))):
+        same(x, u, **cuts)
+
+
+def test_numbers_beside_tensors_are_not_read():
+    """From C: where a row has its own settings the one number says nothing, also not which kernels run."""
+    dev = device()
+    B, V = 3, 20000
+    x, u = logits(B, V, seed=5), torch.tensor([0.2, 0.7, 0.95])
+    own = dict(temperature=torch.tensor([1.0, 0.8, 1.2]), top_k=torch.tensor([0, 5, 2000], dtype=torch.int32),
+               top_p=torch.tensor([0.9, 1.0, 0.95]), min_p=torch.tensor([0.0, 0.1, 0.01]))
+    one = dict(temperature=0.0, top_k=1, top_p=0.0, min_p=9.0)
+    L = q35hip.lib()
+    size = L.q35_sample_tokens_workspace_bytes(B, 1, V)
+    ws, tok = torch.empty(size, dtype=torch.uint8, device=dev), torch.full((B,), -1, dtype=torch.int32, device=dev)
+    xd, ud, up = x.to(dev), u.to(dev), {n: t.to(dev) for n, t in own.items()}
+    for names in (("temperature", "top_k", "top_p", "min_p"), ("min_p",), ("top_k", "min_p"), ("temperature",), ("top_k", "top_p")):
+        args = []
+        for n in ("temperature", "top_k", "top_p", "min_p"):
+            # (a number of no effect where the rows have none of their own)
+            plain = dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0)[n]
+            args += [up[n].data_ptr() if n in names else None, one[n] if n in names else plain]
+        announce(f"sample from C, {names}")
+        assert L.q35_sample_tokens(xd.data_ptr(), V, V, ud.data_ptr(), 1, *args, tok.data_ptr(), 0, None, B, 1, V, ws.data_ptr(),
+                                   size, torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(tok.cpu(), sampling.sample_tokens(x, u, **{n: own[n] for n in names})[0])
