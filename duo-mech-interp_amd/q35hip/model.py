@@ -85,7 +85,7 @@ def mlp(p, h, x, prenorm=None, capture=None, fixed_order=False, act_int8=False):
     engine/model.js:9, :451-453), written by the SwiGLU epilogue itself. fixed_order: the decode down_proj sums
     every output in one fixed order (repeatable bits; layers.linear). act_int8: both products of more than 8 rows in 8-bit
     integers, where the weights have one scale per row (layers.linear), the activations between them in 8 bits too; h may then
-    be RowsI8. Returns x."""
+    be RowsI8 (without prenorm). Returns x."""
     mlp_weights(p)
     H = h.shape[-1]
     M = math.prod(h.shape[:-1])
@@ -93,8 +93,8 @@ def mlp(p, h, x, prenorm=None, capture=None, fixed_order=False, act_int8=False):
     # h + y_add is written to x when x is another buffer; with x = h and no y_add the norm reads h as it is
     pn = None if prenorm is None else (prenorm[0], prenorm[1], prenorm[2], None if x is h else x)
     if isinstance(h, ops.RowsI8) or (act_int8 and M > 8 and _rows8_ok(p, _MLP) and h.dtype == torch.float32):
-        if not _rows8_ok(p, _MLP):
-            raise ValueError("mlp: rows in 8 bits need int8 weights with one scale per row")
+        if not _rows8_ok(p, _MLP) or (pn is not None and isinstance(h, ops.RowsI8)):
+            raise ValueError("mlp: rows in 8 bits need int8 weights with one scale per row, and take no prenorm")
         rows = h.flat() if isinstance(h, ops.RowsI8) else layers.rows_int8(h, pn)
         a = ops.gemm_i8(rows, p["_gu_q8"], p["_gu_s"], epilogue="swiglu", pushes=p["_pushes"], T=T, capture=capture)
         ops.gemm_i8(ops.quantize_rows(a), p["down_proj.q"], p["down_proj.s"], out=x.view(M, H), epilogue="add")
