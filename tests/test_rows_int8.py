@@ -23,3 +23,14 @@ def test_mlp_of_rows_in_8_bits_takes_no_prenorm():
         with pytest.raises(ValueError, match="prenorm"):
             model.mlp(p, rows(2, 6, 64), x, prenorm=(y, torch.zeros(64), 1e-6))
     assert bool((x == 0).all())
+
+
+def test_linear_of_rows_in_8_bits_takes_no_prenorm_and_no_conv():
+    w, q, s = torch.zeros(256, 64), torch.zeros(256, 64, dtype=torch.int8), torch.ones(256)
+    for M in (1, 3, 20):
+        with pytest.raises(ValueError, match="prenorm"):
+            layers.linear(rows(M, 1, 64), w, q, s, prenorm=(None, torch.zeros(64), 1e-6, None))
+        with pytest.raises(ValueError, match="conv"):
+            layers.linear(rows(M, 1, 64), w, q, s, conv=(torch.zeros(128, 4), None, torch.zeros(M, 128, 3)))
+        with pytest.raises(ValueError, match="one scale per row"):
+            layers.linear(rows(M, 1, 64), w, q, torch.ones(256, 2))
