@@ -8,8 +8,10 @@
 // and the draw is the first kept token whose running sum exceeds u of the kept ones' sum. So all that is ever asked is where in
 // one order a running count or sum reaches a target. The first token always stays; temperature 0 is top-k 1.
 //
-// Weights w = exp((x - max) / T) are formed in 64 bits and held as whole numbers of 2^-S (S = 62 - log2 V, at most 50: the sum
-// fits), so that sums depend on no order and a border lies where 64 bits put it: 2^-44 of the largest weight for 150 K tokens.
+// Weights w = exp((x - max) / T) are formed in 64 bits, to 2e-12 of themselves, and held as whole numbers of 2^-S of the largest (S =
+// 62 - log2 V, at most 50: the sum fits), so that sums depend on no order. Half a unit a token: a sum, and with it a border of top-p
+// or a draw, is known to V 2^-(S + 1) of the largest weight and 2e-12 of itself (150 K tokens: 2^-28, and fp32's own step next to 1 is
+// 2^-24; 2^22 tokens: 2^-19, where a tail of weights below 2^-41 each counts as nothing). min-p is a border of logits, to 64 bits.
 //
 //   sample_max_kernel    the largest value of each group of 16 and of each chunk of 4096
 //   sample_hist_kernel   counts and sums of weights of the row in 2048 bins by distance from the maximum, from LDS into the

@@ -1334,7 +1334,8 @@ def sample_tokens(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
     top_k int32). In the order of the logits, ties by index: the first top_k tokens (0: all); of these while the
     probabilities ahead of a token sum to less than top_p of all of these; of these the ones of at least min_p times the first
     one's probability. The first always stays; temperature 0 is the argmax. The token is the first kept one, in this order,
-    whose running sum exceeds u of the kept ones' sum. Returns tokens [B] int32; with want_probs also the probabilities that
+    whose running sum exceeds u of the kept ones' sum (sums to 2^-27 of the largest weight for up to 2^18 tokens, 2^-19 for
+    2^22). Returns tokens [B] int32; with want_probs also the probabilities that
     the draw is from, [B, V] fp32 (0 where cut): what verify_drafts takes as draft_probs."""
     out = _call("try_sample_tokens", torch.ops.q35.sample_tokens, logits, u, *_cuts(temperature, top_k, top_p, min_p),
                 bool(want_probs))

@@ -630,8 +630,9 @@ int q35_verify_drafts(const float* logits, int64_t l_sb, int64_t l_sp, const int
  * Tokens in the order of their logits, ties by index: of these the first top_k (0 or less: all); of them those whose weights
  * ahead sum to less than top_p of all of theirs (1 or more: all); of them those of at least min_p of the first one's weight (0
  * or less: all). The first always stays. Temperature 0 (on the device also less) is top-k 1. Weights exp((x - max) /
- * temperature) and their sums are formed in 64 bits, as whole numbers of 2^-44 of the largest weight for 2^18 tokens (2^-40
- * for 2^22).
+ * temperature) are formed in 64 bits, to 2e-12 of themselves, and summed as whole numbers of 2^-S of the largest (S = 62 - log2 V,
+ * at most 50): the sums behind top-p and the draw are exact to V 2^-(S + 1) of the largest weight (2^-27 for 2^18 tokens, 2^-19 for
+ * 2^22) and 2e-12 of themselves.
  *   tokens: [B] int32 (P = 1) or NULL: the first kept token whose running sum exceeds u[b] (fp32, stride u_sb, in [0, 1)) of
  *   the kept ones' sum
  *   out: [B, P, V] fp32 dense: out_kind 1 the probabilities that the draw is from, 2 the logits with what is cut at -inf

@@ -1,4 +1,6 @@
 """Truncated sampling where a border can go wrong, against oracle/sampling.py in 64 bits: what is kept and drawn is equal."""
+import math
+
 import pytest
 import torch
 
@@ -143,3 +145,31 @@ def test_numbers_beside_tensors_are_not_read():
         assert L.q35_sample_tokens(xd.data_ptr(), V, V, ud.data_ptr(), 1, *args, tok.data_ptr(), 0, None, B, 1, V, ws.data_ptr(),
                                    size, torch.cuda.current_stream().cuda_stream) == 0
         assert torch.equal(tok.cpu(), sampling.sample_tokens(x, u, **{n: own[n] for n in names})[0])
+
+
+@pytest.mark.parametrize("bits", [9, 16, 18, 22])
+def test_borders_behind_a_flat_tail(bits):
+    """One token and a flat tail of 2^bits - 1 whose weights are about half of 2^-S, the unit of the sums (S = min(62 - bits, 50)).
+    Each weight is off by half a unit and 2e-12 of itself, so a sum by e = 2^bits 2^-(S + 1) + 2e-12 of it, and the border of
+    top-p and the draw lie where sums within 2 e (the whole's and the running one's) put them: a place in the tail is not
+    known better than that, and what is kept is a first part of the order in any case."""
+    V, S = 1 << bits, min(62 - bits, 50)
+    u = torch.tensor([0.5, 1 - 2.0 ** -24])
+    for halves in (0.5, 0.98, 1.02, 1.5, 3.0, 1000.0):  # of a weight in units of 2^-(S + 1)
+        x = torch.full((2, V), math.log(halves) - (S + 1) * math.log(2.0))
+        x[:, V // 3] = 0.0
+        w = math.exp(float(x[0, 0]))  # (of the logit in fp32)
+        Z = 1 + (V - 1) * w
+        e = 2 * (V * 2.0 ** -(S + 1) + 2e-12 * Z) + 2.0 ** -S
+        for p in (0.999, 1 - 2.0 ** -20, 1 - 2.0 ** -22, 1 - 2.0 ** -24):
+            announce(f"flat tail V{V}, {halves} halves of a unit, top-p {p}")
+            cut = ops.filter_logits(x.to(device()), top_p=p).cpu()
+            kept = (cut > -math.inf).nonzero()[:, 1].view(2, -1)[0]
+            n = kept.numel() - 1  # of the tail
+            order = torch.cat([torch.tensor([V // 3]), torch.arange(V - 1) + (torch.arange(V - 1) >= V // 3)])
+            assert torch.equal(kept, order[:n + 1].sort().values)
+            assert 1 + n * w >= p * Z - e and (n == 0 or 1 + (n - 1) * w <= p * Z + e)
+        tok = ops.sample_tokens(x.to(device()), u.to(device())).cpu()
+        assert int(tok[0]) == V // 3
+        at = int((order == tok[1]).nonzero())
+        assert 1 + at * w >= float(u[1]) * Z - e and (at == 0 or 1 + (at - 1) * w <= float(u[1]) * Z + e)
