@@ -1,6 +1,6 @@
 // Products in 8-bit integers with one scale per token and one per output channel, and the rows in 8 bits that they take.
 //
-//   s[m] = fp32(max_k |x[m, k]| / 127), q[m, k] = rint(x[m, k] / s[m]) (half to even)
+//   s[m] = fp32(max_k |x[m, k]| / 127), q[m, k] = rint(x[m, k] / s[m]) (half to even), -127 .. 127
 //   y[m, n] = (sum_k q[m, k] W[n, k]) s[m] ws[n]
 //
 // The sum is exact (int32, K up to 65536), so it depends on no order and every kernel here gives the same bits. A code is a
@@ -16,7 +16,9 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 // Rows in 8 bits, one block a row, held in registers: PER quads of values a thread, so that memory is passed over once. 16384
 // rows of 3584 fp32 values take 54 us, 5.4 TB/s of the 294 MB read and written (a large copy reaches 5.2).
 
-// rint(x / s), half to even: x, s exact, |x / s| <= 127.5. The remainder settles what the product with 1 / s left undecided.
+// rint(x / s), half to even, in -127 .. 127: x, s exact. The remainder settles what the product with 1 / s left undecided. |x / s| is
+// 127 to fp32's rounding of s; where s is subnormal that rounding is up to a third of it (190 2^-149 / 127 is 2^-149 then: a quotient
+// of 190), and the largest code stands for less than the value.
 __device__ __forceinline__ int i8_code(double x, double s, double inv) {
   double t = __builtin_rint(x * inv);
   const double r = __builtin_fma(-t, s, x), a = fabs(r) * 2.0;  // exact: t has 8 bits, s 24

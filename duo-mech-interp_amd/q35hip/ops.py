@@ -1372,7 +1372,7 @@ class RowsI8(NamedTuple):
 
 def quantize_rows(x):
     """x [..., K] fp32 or bf16 (dense rows, evenly strided; K a multiple of 4, at most 16384) as RowsI8: s = fp32(max |x| / 127),
-    q = rint(x / s). A row that holds a value that is not finite gets codes 0 and the scale NaN."""
+    q = rint(x / s), -127 .. 127. A row that holds a value that is not finite gets codes 0 and the scale NaN."""
     return tuple.__new__(RowsI8, _call("try_quantize_rows_i8", torch.ops.q35.quantize_rows_i8, x))
 
 

@@ -648,7 +648,8 @@ int q35_sample_tokens(const float* logits, int64_t l_sb, int64_t l_sp, const flo
 
 /*
  * Rows in 8 bits with one scale a row: s[m] = fp32(max_k |x[m, k]| / 127), q[m, k] = rint(x[m, k] / s[m]), half to even, the
- * quotient of the exact x (a row of zeros, or of values so small that s is 0: codes 0). A row that holds a value that is not
+ * quotient of the exact x, held to -127 .. 127 (which matters where s is subnormal and so rounded by as much as a third; a row of
+ * zeros, or of values so small that s is 0: codes 0). A row that holds a value that is not
  * finite gets codes 0 and the scale NaN, and its products are NaN.
  *   x: [M, ldx] in dtype (Q35_F32, 16-byte aligned, or Q35_BF16, 8-byte); q: [M, K] int8, rows dense; s: [M] fp32.
  *   K and ldx multiples of 4, K <= 16384.
