@@ -39,8 +39,10 @@
 // launches and a merge took 21.5 us where one and a merge take 13.1: one token of three rows, 2048 shared 4-bit keys and up to
 // 64 own). Both leave (max, sum, acc) of their runs to a merge. What bounds it: few rows, the chain of dependent loads (positions,
 // table, keys, parts); one token of 32 rows, 8192 shared bf16 keys and up to 500 own, 29 us, of which a block's two rounds take 8,
-// the queries' preparation 8 and the join of its waves 5; four tokens of 64 rows, 32768 shared 4-bit keys, 121 to 126 us (560
-// TFLOP/s), the vector ALU as above: 650 operations beside 72 products for 32 rows x 32 keys.
+// the queries' preparation 8 and the join of its waves 5 (4-bit keys 27); up to four tokens of 64 rows, 32768 shared 4-bit keys, 121
+// to 129 us, the vector ALU as above: 650 operations beside 72 products for 32 rows x 32 keys (bf16 keys 202 to 206). That is 340 to 363
+// TFLOP/s of the tokens that are there, 5 of 8; the others take rows of the shared blocks' tiles as well, see nothing, and so have every
+// round of them masked. An own-keys block has as many 16s of rows as a shared one, whether its sequence fills them or not.
 //
 // A row's keys are dealt over S blocks in runs of whole 128-key rounds by the row's own length, read on the device: the
 // grid is sized by the table's capacity, the work by what is cached. With S > 1 the blocks leave (max, sum, acc) and a

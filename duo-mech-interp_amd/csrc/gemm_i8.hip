@@ -14,7 +14,8 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 // ---------------------------------------------------------------------------------------------------------------
 // Rows in 8 bits, one block a row, held in registers: PER quads of values a thread, so that memory is passed over once. 16384
-// rows of 3584 fp32 values take 54 us, 5.4 TB/s of the 294 MB read and written (a large copy reaches 5.2).
+// rows of 3584 fp32 values take 54 us, 5.4 TB/s of the 294 MB read and written (a large copy reaches 5.2), of bf16 values 40 to 45
+// (176 MB). 6144 rows of 1024 normed take 11.4 to 13.3 us (31 MB; 32 % of the vector ALU, in 64 bits), with an added y 18 (82 MB).
 
 // rint(x / s), half to even, in -127 .. 127: x, s exact. The remainder settles what the product with 1 / s left undecided. |x / s| is
 // 127 to fp32's rounding of s; where s is subnormal that rounding is up to a third of it (190 2^-149 / 127 is 2^-149 then: a quotient
@@ -200,10 +201,10 @@ static int rows_i8_launch(Tx* x, int64_t ldx, const float* y, int64_t ldy, const
 // lines (rows of 128 bytes, 16-byte chunk c at c ^ ((row >> 1) & 7): 16 consecutive lanes of a fragment read fall in distinct
 // slots). Stages of 64 inputs fetched half lines and took 1.4 times as long.
 //
-// 16384 rows of 3584 inputs by 1024 outputs, tiles of 256 x 256 (8 waves of 128 x 64): 63 us alone, 1.9 P operations a second (a
-// library product of 8192^3 reaches 2.05); the matrix units bound it, then the 64 MB of results, which leave at the end as all
-// blocks run in step. 6144 rows of 1024 inputs by 7168 outputs with SwiGLU: 73 us, 1.23 P; 672 tiles are 2.6 a CU, and 88 MB
-// leave. 333 rows of 3584 by 1024 (352 tiles of 32): 7.2 us; 32 rows of 1024 by 5120 3.2 us: latency of a stage from memory.
+// 16384 rows of 3584 inputs by 1024 outputs, tiles of 256 x 256 (8 waves of 128 x 64): 65 us alone, 1.86 P operations a second (a
+// library product of 8192^3 reaches 2.07), 71 behind the rows' kernel, 73 added to what is there; the matrix units bound it, then the
+// 64 MB of results, which leave at the end as all blocks run in step. 6144 rows of 1024 inputs by 7168 outputs with SwiGLU: 70 us,
+// 1.29 P; 672 tiles are 2.6 a CU, and 88 MB leave. 333 rows of 3584 by 1024 (352 tiles of 32): 7.2 us; 32 rows of 1024 by 5120 3.2 us: latency of a stage from memory.
 constexpr int kIK = 128;  // inputs of a stage
 
 struct GemmI8Args {

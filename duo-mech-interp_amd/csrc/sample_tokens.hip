@@ -25,8 +25,10 @@
 // Rows of 151,936 logits (a copy runs at 5.2 TB/s): three of top-k 20 13.4 us, a chain of two launches and, in the second, of
 // a dozen dependent steps of one block; 256 of top-p 0.9 120 us: the maximum 29 (5.4 TB/s), the histogram 43 (26 operations a
 // token, most of 64 bits, and an atomic in LDS), the pick 51, whose one block a row reads what reaches the border's bin at a CU's
-// 50 GB/s, most of the row where the nucleus is large; 160 of top-k 50 and top-p 0.95 cut into logits 94 us: 22, 33, 12, and 29
-// for the write.
+// 50 GB/s, most of the row where the nucleus is large; 160 of top-p 0.95 and min-p 0.02 cut into logits 94 us: 22, 33, 12, and 29
+// for the write; the same of top-k 50 and top-p 0.95, which need no histogram, 63. 250,000 logits: three rows of top-k 20 18.0 us, 32 of
+// top-p 0.9 80 (8, 19, 55; 151,936: 59). 1024 rows of 16,000 take one block each, one a CU for its LDS, four turns of them: 76 us with
+// logits that fall with rank^-1.5, 100 where every row falls with a power of its own, from 1.1 to 3.
 #include <algorithm>
 #include <cfloat>
 #include <type_traits>
@@ -41,7 +43,7 @@ constexpr int kSChunk = 1024;    // quads of a block of the maximum and the writ
 constexpr int kSFew = 1024;      // the largest top-k whose rows need no histogram
 constexpr int kSThreads = 1024;  // of the pick kernel
 constexpr int kSShort = 4;       // chunks of a row that the pick kernel takes alone
-constexpr int kSHeld = 10;       // groups' maxima that one of its threads holds
+constexpr int kSHeld = 10;       // groups' maxima that one of its threads holds: rows of up to 163,840 tokens; further ones are read again
 constexpr int kSSort = kSThreads;  // tokens that it sorts
 constexpr int kSWaves = kSThreads / 64, kSSeg = 512;  // tokens that each of its waves can list
 constexpr int64_t kSMaxV = 1 << 22;
