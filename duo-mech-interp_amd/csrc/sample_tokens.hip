@@ -609,9 +609,9 @@ __global__ __launch_bounds__(kSThreads) void sample_pick_kernel(SampleArgs a) {
     const double goal = floor(fmax((double)u, 0.0) * (double)Z);
     return goal >= (double)Z ? Z : min((u64)goal + 1, Z);
   };
-  // The smallest value of weight m or more: exp((x - max) / T) >= m where x >= max + T ln m, in 64 bits. (Looked for by the weights of
-  // values next to it, it was off by their series' 2e-12 T, which around 0 is more than any number of neighbouring values. 2^-54
-  // less: what rounds to 1 weighs 1, at an infinite temperature every finite logit.)
+  // The smallest value of weight m or more: exp((x - max) / T) >= m where x >= max + T ln m, in 64 bits. (Not by the weights of values
+  // next to it: their series is 2e-12 off, and next to 0 fp32 has any number of values within 2e-12 T. 2^-54 less: what rounds to 1
+  // weighs 1, at an infinite temperature every finite logit.)
   float least = -INFINITY;
   if (r.m > 0.f) {
     const double border = __builtin_fma(log((double)r.m) - 0x1p-54, (double)r.t, (double)M);
